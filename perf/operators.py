@@ -201,8 +201,8 @@ def prepare(case, seed):
         elif op == "append":
             state["bound"] = kv.KvAppend.bind(
                 stream, kv.KvCache(state["k_cache"], state["v_cache"]), 0, state["q"], state["k"], state["v"], state["positions"],
-                state["frequencies"], state["sections"], state["table"], state["lengths"], state["starts"], tokens=case["tokens"],
-                interleaved=case["interleaved"], q_out=state["q_out"], q_norm=state["q_norm"], k_norm=state["k_norm"], epsilon=EPSILON)
+                state["frequencies"], state["sections"], state["table"], state["lengths"], state["starts"], interleaved=case["interleaved"],
+                q_out=state["q_out"], q_norm=state["q_norm"], k_norm=state["k_norm"], epsilon=EPSILON)
         else:
             query, heads, size = HEADS[case["heads"]]
             plan = state["plan"] = host.Plan(stream, kv.paged_attention_scratch_bytes(query, heads, size, case["tokens"]))
