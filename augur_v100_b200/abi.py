@@ -38,6 +38,10 @@ MAX_SMALL_TOKENS = 8
 SCALE_COMPRESSED_TENSORS = 0
 SCALE_MODELOPT = 1
 STATIC_SCRATCH_BYTES = 4 << 20
+MAX_SEQUENCES = 1024
+MAX_ALTERNATIVES = 32
+LOGITS_F32 = 0
+LOGITS_BF16 = 1
 
 
 class Result(Structure):
@@ -169,8 +173,64 @@ class GemmSwigluQuantArgs(Structure):
                 ("destination_global_scale", c_float), ("destination_terms", c_uint32), ("reserved", c_uint32)]
 
 
+class KvLayer(Structure):
+    _fields_ = [("keys", c_uint64), ("values", c_uint64), ("len_bytes", c_uint64),
+                ("pages", c_uint32), ("kv_heads", c_uint32), ("page_tokens", c_uint32), ("head_dim", c_uint32)]
+
+
+class KvBatch(Structure):
+    _fields_ = [("page_table", c_uint64), ("page_table_len_bytes", c_uint64),
+                ("lengths", c_uint64), ("lengths_len_bytes", c_uint64),
+                ("token_starts", c_uint64), ("token_starts_len_bytes", c_uint64),
+                ("sequences", c_uint32), ("table_pages", c_uint32), ("rows", c_uint32), ("reserved", c_uint32)]
+
+
+class KvAppendArgs(Structure):
+    _fields_ = [("abi_version", c_uint32), ("struct_size", c_uint32),
+                ("layer", KvLayer), ("batch", KvBatch),
+                ("query", c_uint64), ("query_len_bytes", c_uint64),
+                ("key", c_uint64), ("key_len_bytes", c_uint64),
+                ("value", c_uint64), ("value_len_bytes", c_uint64),
+                ("query_row_stride", c_uint64), ("query_head_stride", c_uint64),
+                ("key_row_stride", c_uint64), ("key_head_stride", c_uint64),
+                ("value_row_stride", c_uint64), ("value_head_stride", c_uint64),
+                ("positions", c_uint64), ("positions_len_bytes", c_uint64),
+                ("inv_freq_f32", c_uint64), ("inv_freq_len_bytes", c_uint64),
+                ("query_norm_f32", c_uint64), ("key_norm_f32", c_uint64), ("norm_len_bytes", c_uint64),
+                ("query_out", c_uint64), ("query_out_len_bytes", c_uint64),
+                ("query_heads", c_uint32), ("rotary_dim", c_uint32), ("sections", c_uint32 * 3), ("interleaved", c_uint32),
+                ("epsilon", c_float), ("reserved", c_uint32)]
+
+
+class PagedAttentionArgs(Structure):
+    _fields_ = [("abi_version", c_uint32), ("struct_size", c_uint32),
+                ("layer", KvLayer), ("batch", KvBatch),
+                ("query", c_uint64), ("query_len_bytes", c_uint64),
+                ("output", c_uint64), ("output_len_bytes", c_uint64),
+                ("query_heads", c_uint32), ("max_new_tokens", c_uint32), ("scale", c_float), ("reserved", c_uint32)]
+
+
+class KvPageCopyArgs(Structure):
+    _fields_ = [("abi_version", c_uint32), ("struct_size", c_uint32),
+                ("keys", c_uint64), ("values", c_uint64), ("len_bytes", c_uint64), ("page_bytes", c_uint64),
+                ("layers", c_uint32), ("pages", c_uint32)]
+
+
+class TokenLogprobsArgs(Structure):
+    _fields_ = [("abi_version", c_uint32), ("struct_size", c_uint32),
+                ("logits", c_uint64), ("logits_len_bytes", c_uint64),
+                ("targets", c_uint64), ("targets_len_bytes", c_uint64),
+                ("logprobs", c_uint64), ("logprobs_len_bytes", c_uint64),
+                ("entropy", c_uint64), ("entropy_len_bytes", c_uint64),
+                ("ids", c_uint64), ("ids_len_bytes", c_uint64),
+                ("alternative_logprobs", c_uint64), ("alternative_logprobs_len_bytes", c_uint64),
+                ("row_stride", c_uint64),
+                ("rows", c_uint32), ("vocabulary", c_uint32), ("alternatives", c_uint32), ("logits_type", c_uint32)]
+
+
 # Every symbol the header declares: name -> (restype, argtypes).
 _U8P = POINTER(c_uint8)
+_U32P = POINTER(c_uint32)
 EXPORTS = {
     "augur_cuda_nvfp4_sm100_abi_version": (c_uint32, []),
     "augur_cuda_nvfp4_sm100_build_capability_v1": (c_uint32, []),
@@ -226,6 +286,16 @@ EXPORTS = {
     "augur_cuda_nvfp4_sm100_gemm_swiglu_quant_preflight_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(GemmSwigluQuantArgs)]),
     "augur_cuda_nvfp4_sm100_gemm_swiglu_quant_prevalidated_submit_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(GemmSwigluQuantArgs)]),
     "augur_cuda_nvfp4_sm100_interleave_gate_up_host_v1": (Result, [c_uint32, c_uint32, _U8P, _U8P, _U8P, _U8P, _U8P, _U8P]),
+    "augur_cuda_nvfp4_sm100_kv_append_preflight_v1": (Result, [c_int32, c_void_p, POINTER(KvAppendArgs)]),
+    "augur_cuda_nvfp4_sm100_kv_append_prevalidated_submit_v1": (Result, [c_int32, c_void_p, POINTER(KvAppendArgs)]),
+    "augur_cuda_nvfp4_sm100_paged_attention_scratch_extent_host_v1": (Result, [c_uint32, c_uint32, c_uint32, c_uint32, c_uint32, POINTER(c_uint64)]),
+    "augur_cuda_nvfp4_sm100_paged_attention_preflight_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(PagedAttentionArgs)]),
+    "augur_cuda_nvfp4_sm100_paged_attention_prevalidated_submit_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(PagedAttentionArgs)]),
+    "augur_cuda_nvfp4_sm100_kv_page_copy_preflight_v1": (Result, [c_int32, c_void_p, POINTER(KvPageCopyArgs)]),
+    "augur_cuda_nvfp4_sm100_kv_page_copy_prevalidated_submit_v1": (Result, [c_int32, c_void_p, POINTER(KvPageCopyArgs), _U32P, _U32P, c_uint32]),
+    "augur_cuda_nvfp4_sm100_token_logprobs_scratch_extent_host_v1": (Result, [c_uint32, c_uint32, c_uint32, POINTER(c_uint64)]),
+    "augur_cuda_nvfp4_sm100_token_logprobs_preflight_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(TokenLogprobsArgs)]),
+    "augur_cuda_nvfp4_sm100_token_logprobs_prevalidated_submit_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(TokenLogprobsArgs)]),
     "augur_cuda_nvfp4_sm100_diagnostic_inject_submit_fault_v1": (None, [c_uint32]),
     "augur_cuda_nvfp4_sm100_allocation_snapshot_v1": (None, [POINTER(c_uint64), POINTER(c_uint64)]),
     "augur_cuda_nvfp4_sm100_launch_count_v1": (c_uint64, []),

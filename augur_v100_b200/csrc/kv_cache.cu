@@ -1,0 +1,326 @@
+// Writing and moving the pages of a key-value cache on sm_100a: rotary positions with the cache write of a step's tokens, and page copies.
+#include <cstdlib>
+
+#include "kv_cache.cuh"
+
+namespace augur_sm100 {
+namespace {
+
+static_assert(sizeof(augur_cuda_nvfp4_sm100_kv_layer_v1) == 40 && sizeof(augur_cuda_nvfp4_sm100_kv_batch_v1) == 64, "cache ABI");
+static_assert(sizeof(augur_cuda_nvfp4_sm100_kv_append_args_v1) == 312, "append ABI");
+static_assert(sizeof(augur_cuda_nvfp4_sm100_kv_page_copy_args_v1) == 48, "page copy ABI");
+
+// ---- rotary positions and the cache write ---------------------------------------------------------
+
+struct AppendParams {
+    const __nv_bfloat16 *query, *key, *value;
+    uint64_t query_row_stride, query_head_stride, key_row_stride, key_head_stride, value_row_stride, value_head_stride;
+    const int32_t *positions, *page_table, *lengths, *token_starts;
+    const float *inv_freq, *query_norm, *key_norm;
+    __nv_bfloat16 *query_out, *keys, *values;
+    uint32_t rows, sequences, table_pages, pages, query_heads, kv_heads, page_shift;
+    uint32_t half;                       // rotary pairs
+    uint32_t sections[3], interleaved;
+    float epsilon;
+    uint32_t parts;                      // CTAs that share a row's heads
+};
+
+constexpr uint32_t kAppendThreads = 256;
+
+// A CTA turns some of the heads of one row, head_dim / 8 neighbouring lanes to a head with eight elements (one 16-byte access) each. The
+// sines and cosines of the row are formed once per CTA. What the rotation pairs lies rotary_dim / 16 lanes away: a shuffle.
+template <uint32_t kHeadDim>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
+    constexpr uint32_t kLanes = kHeadDim / 8, kGroups = kAppendThreads / kLanes;
+    __shared__ float cosine[kHeadDim / 2], sine[kHeadDim / 2];
+    __shared__ int32_t sequence_at, slot_page, slot_offset;
+    const uint32_t row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+    const uint32_t group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+    if (threadIdx.x == 0) sequence_at = -1;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __syncthreads();
+    for (uint32_t b = threadIdx.x; b < p.sequences; b += kAppendThreads) {
+        const int32_t from = p.token_starts[b], to = p.token_starts[b + 1];
+        if (static_cast<int32_t>(row) >= from && static_cast<int32_t>(row) < to) {
+            const int64_t position = static_cast<int64_t>(p.lengths[b]) - to + row;   // in the cache
+            const int64_t page = position >> p.page_shift;
+            int32_t at = -1;
+            if (position >= 0 && page < p.table_pages) at = p.page_table[static_cast<uint64_t>(b) * p.table_pages + page];
+            sequence_at = static_cast<int32_t>(b);
+            slot_page = at >= 0 && static_cast<uint32_t>(at) < p.pages ? at : -1;
+            slot_offset = static_cast<int32_t>(position & ((int64_t(1) << p.page_shift) - 1));
+        }
+    }
+    if (threadIdx.x < p.half) {
+        const uint32_t i = threadIdx.x;
+        uint32_t axis;
+        if (p.interleaved) {
+            axis = i % 3;
+            if (i >= 3 * p.sections[axis]) axis = 0;
+        } else {
+            axis = (i >= p.sections[0] ? 1u : 0u) + (i >= p.sections[0] + p.sections[1] ? 1u : 0u);
+        }
+        // In turns, in 64 bits: a position of 2^20 leaves 2^-33 of a turn, where the F32 product would have lost 2^-7.
+        const double turns = static_cast<double>(p.positions[static_cast<uint64_t>(axis) * p.rows + row]) * static_cast<double>(p.inv_freq[i]) * 0.15915494309189535;
+        const float part_turn = static_cast<float>(turns - rint(turns));
+        sincospif(2.0f * part_turn, &sine[i], &cosine[i]);
+    }
+    __syncthreads();
+    if (sequence_at < 0) return;
+    const int32_t page = slot_page;
+    const uint32_t heads = p.query_heads + 2 * p.kv_heads, half_lanes = p.half / 8;
+    for (uint32_t h = part * kGroups + group; h < heads; h += p.parts * kGroups) {   // the lanes of a head stay together
+        const __nv_bfloat16* from;
+        __nv_bfloat16* to;
+        const float* norm = nullptr;
+        bool turn = true;
+        if (h < p.query_heads) {
+            from = p.query + row * p.query_row_stride + h * p.query_head_stride;
+            to = p.query_out + (static_cast<uint64_t>(row) * p.query_heads + h) * kHeadDim;
+            norm = p.query_norm;
+        } else {
+            const bool is_key = h < p.query_heads + p.kv_heads;
+            const uint32_t head = h - p.query_heads - (is_key ? 0 : p.kv_heads);
+            if (page < 0) continue;
+            const uint64_t slot = ((static_cast<uint64_t>(page) * p.kv_heads + head) << p.page_shift) + slot_offset;
+            from = is_key ? p.key + row * p.key_row_stride + head * p.key_head_stride : p.value + row * p.value_row_stride + head * p.value_head_stride;
+            to = (is_key ? p.keys : p.values) + slot * kHeadDim;
+            norm = is_key ? p.key_norm : nullptr;
+            turn = is_key;
+        }
+        uint4 raw = *reinterpret_cast<const uint4*>(from + 8 * lane);
+        if (turn) {
+            const unsigned mask = kLanes == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
+            float x[8];
+            const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                x[2 * i] = __uint_as_float(word[i] << 16);
+                x[2 * i + 1] = __uint_as_float(word[i] & 0xffff0000u);
+            }
+            if (norm) {
+                float sum = 0.0f;
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+#pragma unroll
+                for (uint32_t step = kLanes / 2; step; step /= 2) sum += __shfl_xor_sync(mask, sum, step);
+                const float scale = __frsqrt_rn(sum * (1.0f / kHeadDim) + p.epsilon);
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) x[i] = x[i] * scale * norm[8 * lane + i];
+            }
+            const bool upper = lane >= half_lanes;
+            const uint32_t partner = lane >= 2 * half_lanes ? lane : upper ? lane - half_lanes : lane + half_lanes;
+            const uint32_t pair = 8 * (upper ? lane - half_lanes : lane);
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const float other = __shfl_sync(mask, x[i], partner, kLanes);
+                if (lane < 2 * half_lanes) x[i] = fmaf(x[i], cosine[pair + i], (upper ? other : -other) * sine[pair + i]);
+            }
+            uint32_t packed[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const __nv_bfloat162 two = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                packed[i] = *reinterpret_cast<const uint32_t*>(&two);
+            }
+            raw = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+        }
+        *reinterpret_cast<uint4*>(to + 8 * lane) = raw;
+    }
+}
+
+bool check_append(int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm100_kv_append_args_v1* a, bool full, augur_cuda_result_v1* failure) {
+    *failure = invalid();
+    if (!header_ok(d, s, a)) {
+        if (a && s && d >= 0 && s->ordinal == d && a->abi_version != AUGUR_CUDA_ABI_VERSION_V1) *failure = make_result(AUGUR_CUDA_STATUS_ABI_VERSION_MISMATCH);
+        return false;
+    }
+    if (!kv_layer_ok(a->layer) || !kv_batch_ok(a->batch) || a->reserved != 0 || a->interleaved > 1) return false;
+    const uint32_t head_dim = a->layer.head_dim, kv_heads = a->layer.kv_heads, rows = a->batch.rows;
+    if (!a->query_heads || a->query_heads > 1024 || a->rotary_dim > head_dim || a->rotary_dim % 16 != 0 || a->rotary_dim == 0) return false;
+    if (!(std::isfinite(a->epsilon) && a->epsilon >= 0.0f)) return false;
+    const uint64_t pairs = static_cast<uint64_t>(a->sections[0]) + a->sections[1] + a->sections[2];
+    if (pairs != a->rotary_dim / 2) return false;
+    const uint64_t strides[6] = {a->query_row_stride, a->query_head_stride, a->key_row_stride, a->key_head_stride, a->value_row_stride, a->value_head_stride};
+    for (const uint64_t stride : strides) {
+        if (stride % 8 != 0 || stride < head_dim) return false;
+    }
+    if (a->query_len_bytes != 2 * strided_elements(rows, a->query_heads, head_dim, strides[0], strides[1])) return false;
+    if (a->key_len_bytes != 2 * strided_elements(rows, kv_heads, head_dim, strides[2], strides[3])) return false;
+    if (a->value_len_bytes != 2 * strided_elements(rows, kv_heads, head_dim, strides[4], strides[5])) return false;
+    if (a->positions_len_bytes != static_cast<uint64_t>(rows) * 12 || a->inv_freq_len_bytes != a->rotary_dim * UINT64_C(2)) return false;
+    if (a->query_out_len_bytes != static_cast<uint64_t>(rows) * a->query_heads * head_dim * 2) return false;
+    if (a->norm_len_bytes != (a->query_norm_f32 || a->key_norm_f32 ? head_dim * UINT64_C(4) : 0)) return false;
+    // What is written is disjoint from everything; what is read may share memory (q, k and v of one projection, one norm weight for both).
+    Range written[3] = {{a->query_out, a->query_out_len_bytes, 16}, {a->layer.keys, a->layer.len_bytes, 16}, {a->layer.values, a->layer.len_bytes, 16}};
+    Range read[10] = {{a->query, a->query_len_bytes, 16}, {a->key, a->key_len_bytes, 16}, {a->value, a->value_len_bytes, 16},
+                      {a->positions, a->positions_len_bytes, 4}, {a->inv_freq_f32, a->inv_freq_len_bytes, 4},
+                      {a->batch.page_table, a->batch.page_table_len_bytes, 4}, {a->batch.lengths, a->batch.lengths_len_bytes, 4},
+                      {a->batch.token_starts, a->batch.token_starts_len_bytes, 4}, {}, {}};
+    size_t count = 8;
+    if (a->query_norm_f32) read[count++] = {a->query_norm_f32, a->norm_len_bytes, 4};
+    if (a->key_norm_f32) read[count++] = {a->key_norm_f32, a->norm_len_bytes, 4};
+    if (!all_disjoint(written, 3)) return false;
+    for (size_t i = 0; i < count; ++i) {
+        for (size_t j = 0; j < 3; ++j) {
+            if (!disjoint(read[i], written[j])) return false;
+        }
+    }
+    return !full || (inspect_device_ranges(d, written, 3, failure) && inspect_device_ranges(d, read, count, failure));
+}
+
+// ---- page copies ---------------------------------------------------------------------------------
+
+constexpr uint32_t kPairsPerLaunch = 1000;   // the page numbers travel as launch parameters: nothing to copy ahead, nothing to keep
+constexpr uint32_t kCopyThreads = 256, kCopyPiece = kCopyThreads * 16 * 4;
+struct PagePairs {
+    uint32_t source[kPairsPerLaunch], destination[kPairsPerLaunch];
+};
+
+__global__ void __launch_bounds__(kCopyThreads) kv_page_copy_kernel(const __grid_constant__ PagePairs pairs, uint8_t* keys, uint8_t* values, uint64_t page_bytes,
+                                                                    uint32_t pages, uint32_t layers, uint32_t pieces) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    uint32_t at = blockIdx.x;
+    const uint32_t piece = at % pieces;
+    at /= pieces;
+    const uint32_t tensor = at & 1;
+    at >>= 1;
+    const uint32_t layer = at % layers, pair = at / layers;
+    uint8_t* base = (tensor ? values : keys) + static_cast<uint64_t>(layer) * pages * page_bytes;
+    const uint64_t first = static_cast<uint64_t>(piece) * kCopyPiece;
+    const uint8_t* from = base + pairs.source[pair] * page_bytes + first;
+    uint8_t* to = base + pairs.destination[pair] * page_bytes + first;
+    const uint64_t bytes = page_bytes - first < kCopyPiece ? page_bytes - first : kCopyPiece;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    uint4 v[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t offset = (i * kCopyThreads + threadIdx.x) * 16;
+        if (offset < bytes) v[i] = *reinterpret_cast<const uint4*>(from + offset);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t offset = (i * kCopyThreads + threadIdx.x) * 16;
+        if (offset < bytes) *reinterpret_cast<uint4*>(to + offset) = v[i];
+    }
+}
+
+bool check_page_copy(int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm100_kv_page_copy_args_v1* a, bool full, augur_cuda_result_v1* failure) {
+    *failure = invalid();
+    if (!header_ok(d, s, a)) {
+        if (a && s && d >= 0 && s->ordinal == d && a->abi_version != AUGUR_CUDA_ABI_VERSION_V1) *failure = make_result(AUGUR_CUDA_STATUS_ABI_VERSION_MISMATCH);
+        return false;
+    }
+    if (!a->layers || a->layers > 1024 || !a->pages || a->pages > (1u << 27) || !a->page_bytes || a->page_bytes % 16 != 0 || a->page_bytes > (1u << 30)) return false;
+    if (a->len_bytes / a->layers / a->pages != a->page_bytes || a->len_bytes != a->page_bytes * a->pages * a->layers) return false;
+    const Range r[2] = {{a->keys, a->len_bytes, 16}, {a->values, a->len_bytes, 16}};
+    if (!all_disjoint(r, 2)) return false;
+    return !full || inspect_device_ranges(d, r, 2, failure);
+}
+
+// Destinations distinct, none of them a source, all inside the cache.
+bool pairs_ok(uint32_t pages, const uint32_t* sources, const uint32_t* destinations, uint32_t count, bool* out_of_memory) {
+    *out_of_memory = false;
+    if (!sources || !destinations || count > pages) return false;
+    for (uint32_t i = 0; i < count; ++i) {
+        if (sources[i] >= pages || destinations[i] >= pages) return false;
+    }
+    if (count == 1) return sources[0] != destinations[0];
+    uint8_t* taken = static_cast<uint8_t*>(std::calloc((pages + 7) / 8, 1));
+    if (!taken) {
+        *out_of_memory = true;
+        return false;
+    }
+    bool fine = true;
+    for (uint32_t i = 0; i < count && fine; ++i) {
+        const uint32_t page = destinations[i];
+        fine = (taken[page >> 3] >> (page & 7) & 1) == 0;
+        taken[page >> 3] |= static_cast<uint8_t>(1u << (page & 7));
+    }
+    for (uint32_t i = 0; i < count && fine; ++i) fine = (taken[sources[i] >> 3] >> (sources[i] & 7) & 1) == 0;
+    std::free(taken);
+    return fine;
+}
+
+}  // namespace
+}  // namespace augur_sm100
+
+using namespace augur_sm100;
+
+extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append_preflight_v1(int32_t d, augur_cuda_stream_t s,
+                                                                                            const augur_cuda_nvfp4_sm100_kv_append_args_v1* a) {
+    augur_cuda_result_v1 failure;
+    return check_append(d, s, a, true, &failure) ? ok() : failure;
+}
+
+extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append_prevalidated_submit_v1(
+    int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm100_kv_append_args_v1* a) {
+    augur_cuda_result_v1 failure;
+    if (!check_append(d, s, a, false, &failure)) return failure;
+    if (consume_injected_fault()) return make_result(AUGUR_CUDA_STATUS_DIAGNOSTIC_FAULT_INJECTED);
+    const cudaError_t e = cudaSetDevice(d);
+    if (e != cudaSuccess) return make_result(AUGUR_CUDA_STATUS_RUNTIME_FAILURE, e);
+    AppendParams p{};
+    p.query = reinterpret_cast<const __nv_bfloat16*>(a->query);
+    p.key = reinterpret_cast<const __nv_bfloat16*>(a->key);
+    p.value = reinterpret_cast<const __nv_bfloat16*>(a->value);
+    p.query_row_stride = a->query_row_stride, p.query_head_stride = a->query_head_stride;
+    p.key_row_stride = a->key_row_stride, p.key_head_stride = a->key_head_stride;
+    p.value_row_stride = a->value_row_stride, p.value_head_stride = a->value_head_stride;
+    p.positions = reinterpret_cast<const int32_t*>(a->positions);
+    p.page_table = reinterpret_cast<const int32_t*>(a->batch.page_table);
+    p.lengths = reinterpret_cast<const int32_t*>(a->batch.lengths);
+    p.token_starts = reinterpret_cast<const int32_t*>(a->batch.token_starts);
+    p.inv_freq = reinterpret_cast<const float*>(a->inv_freq_f32);
+    p.query_norm = reinterpret_cast<const float*>(a->query_norm_f32);
+    p.key_norm = reinterpret_cast<const float*>(a->key_norm_f32);
+    p.query_out = reinterpret_cast<__nv_bfloat16*>(a->query_out);
+    p.keys = reinterpret_cast<__nv_bfloat16*>(a->layer.keys);
+    p.values = reinterpret_cast<__nv_bfloat16*>(a->layer.values);
+    p.rows = a->batch.rows, p.sequences = a->batch.sequences, p.table_pages = a->batch.table_pages, p.pages = a->layer.pages;
+    p.query_heads = a->query_heads, p.kv_heads = a->layer.kv_heads, p.page_shift = static_cast<uint32_t>(__builtin_ctz(a->layer.page_tokens));
+    p.half = a->rotary_dim / 2;
+    for (uint32_t i = 0; i < 3; ++i) p.sections[i] = a->sections[i];
+    p.interleaved = a->interleaved, p.epsilon = a->epsilon;
+    p.parts = 1;
+    if (a->layer.head_dim == 256) {
+        launch_dependent(s->stream, kv_append_kernel<256>, p.rows * p.parts, kAppendThreads, 0, p);
+    } else {
+        launch_dependent(s->stream, kv_append_kernel<128>, p.rows * p.parts, kAppendThreads, 0, p);
+    }
+    count_launch();
+    return submitted();
+}
+
+extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_copy_preflight_v1(
+    int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm100_kv_page_copy_args_v1* a) {
+    augur_cuda_result_v1 failure;
+    return check_page_copy(d, s, a, true, &failure) ? ok() : failure;
+}
+
+extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_copy_prevalidated_submit_v1(
+    int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm100_kv_page_copy_args_v1* a, const uint32_t* sources, const uint32_t* destinations,
+    uint32_t count) {
+    augur_cuda_result_v1 failure;
+    if (!check_page_copy(d, s, a, false, &failure)) return failure;
+    bool out_of_memory = false;
+    if (count && !pairs_ok(a->pages, sources, destinations, count, &out_of_memory)) return out_of_memory ? make_result(AUGUR_CUDA_STATUS_OUT_OF_MEMORY) : invalid();
+    if (consume_injected_fault()) return make_result(AUGUR_CUDA_STATUS_DIAGNOSTIC_FAULT_INJECTED);
+    if (!count) return ok();
+    const cudaError_t e = cudaSetDevice(d);
+    if (e != cudaSuccess) return make_result(AUGUR_CUDA_STATUS_RUNTIME_FAILURE, e);
+    const uint32_t pieces = static_cast<uint32_t>((a->page_bytes + kCopyPiece - 1) / kCopyPiece);
+    const uint64_t per_pair = static_cast<uint64_t>(pieces) * 2 * a->layers;        // below 2^28
+    const uint32_t most = static_cast<uint32_t>(per_pair * kPairsPerLaunch < INT32_MAX ? kPairsPerLaunch : INT32_MAX / per_pair);
+    PagePairs pairs;
+    for (uint32_t at = 0; at < count;) {
+        const uint32_t take = count - at < most ? count - at : most;
+        for (uint32_t i = 0; i < take; ++i) pairs.source[i] = sources[at + i], pairs.destination[i] = destinations[at + i];
+        for (uint32_t i = take; i < kPairsPerLaunch; ++i) pairs.source[i] = pairs.destination[i] = 0;
+        launch_dependent(s->stream, kv_page_copy_kernel, static_cast<uint32_t>(per_pair * take), kCopyThreads, 0, pairs, reinterpret_cast<uint8_t*>(a->keys),
+                         reinterpret_cast<uint8_t*>(a->values), a->page_bytes, a->pages, a->layers, pieces);
+        count_launch();
+        at += take;
+    }
+    return submitted();
+}

@@ -105,6 +105,10 @@ def gemv_scratch_bytes(rows: int, cols: int, tokens: int = 8) -> int:
     return int(out.value)
 
 
+def sm_count() -> int:
+    return torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
+
+
 def gemm_plan_scratch_bytes(sm_count: int = 0) -> int:
     """Plan scratch with which the prefill GEMM can cut its leftover tiles along k (0: this device's SM count)."""
     if not sm_count:
@@ -697,6 +701,60 @@ class Bf16Head:
     def submit(self) -> None:
         _check("bf16_head_submit", abi.lib().augur_cuda_nvfp4_sm100_bf16_head_prevalidated_submit_v1(
             self.stream.ordinal, self.stream.handle, byref(self.args)))
+
+
+def logprobs_scratch_bytes(rows: int, alternatives: int, sms: int = 0) -> int:
+    """Plan scratch of a `TokenLogprobs` (`sms` 0: of this device), whatever the vocabulary."""
+    out = c_uint64()
+    _check("token_logprobs_scratch_extent", abi.lib().augur_cuda_nvfp4_sm100_token_logprobs_scratch_extent_host_v1(
+        rows, alternatives, sms or sm_count(), byref(out)))
+    return int(out.value)
+
+
+class TokenLogprobs:
+    """Log probabilities of given tokens, entropy and the best alternatives of rows of logits: what stands behind the
+    head. `logits` [rows, vocabulary] F32 (`Bf16Head.out`) or BF16, rows strided; `targets` int32 [rows] (one outside the
+    vocabulary gives NaN). Results: `logprobs` and `entropy` F32 [rows], `ids` int32 and `alternative_logprobs` F32
+    [rows, alternatives], the largest first, the lowest index first where logits are equal."""
+
+    def __init__(self, plan: Plan, logits: torch.Tensor, targets: torch.Tensor, alternatives: int):
+        rows, vocabulary = logits.shape
+        if logits.dtype not in (torch.float32, torch.bfloat16) or (logits.stride(1) != 1 and vocabulary > 1):
+            raise ValueError("F32 or BF16 logits with contiguous rows")
+        if targets.dtype != torch.int32 or tuple(targets.shape) != (rows,) or not targets.is_contiguous() or targets.device != logits.device:
+            raise ValueError("an int32 target for every row, on the logits' device")
+        if not 0 <= alternatives <= abi.MAX_ALTERNATIVES:
+            raise ValueError(f"0 to {abi.MAX_ALTERNATIVES} alternatives")
+        self.plan, self.logits, self.targets = plan, logits, targets
+        empty = functools.partial(torch.empty, device=logits.device)
+        self.logprobs, self.entropy = empty(rows, dtype=torch.float32), empty(rows, dtype=torch.float32)
+        self.ids = empty((rows, alternatives), dtype=torch.int32)
+        self.alternative_logprobs = empty((rows, alternatives), dtype=torch.float32)
+        a = abi.header(abi.TokenLogprobsArgs)
+        a.row_stride = logits.stride(0) if rows > 1 else vocabulary
+        a.logits, a.logits_len_bytes = _ptr(logits), ((rows - 1) * a.row_stride + vocabulary) * logits.element_size()
+        a.targets, a.targets_len_bytes = _ptr(targets), _nbytes(targets)
+        a.logprobs, a.logprobs_len_bytes = _ptr(self.logprobs), _nbytes(self.logprobs)
+        a.entropy, a.entropy_len_bytes = _ptr(self.entropy), _nbytes(self.entropy)
+        if alternatives:
+            a.ids, a.ids_len_bytes = _ptr(self.ids), _nbytes(self.ids)
+            a.alternative_logprobs, a.alternative_logprobs_len_bytes = _ptr(self.alternative_logprobs), _nbytes(self.alternative_logprobs)
+        a.rows, a.vocabulary, a.alternatives = rows, vocabulary, alternatives
+        a.logits_type = abi.LOGITS_F32 if logits.dtype == torch.float32 else abi.LOGITS_BF16
+        self.args = a
+
+    @classmethod
+    def bind(cls, plan: Plan, logits: torch.Tensor, targets: torch.Tensor, alternatives: int = 0):
+        self = cls(plan, logits, targets, alternatives)
+        s = plan.stream
+        _check("token_logprobs_preflight", abi.lib().augur_cuda_nvfp4_sm100_token_logprobs_preflight_v1(
+            s.ordinal, s.handle, plan.handle, byref(self.args)))
+        return self
+
+    def submit_for_plan(self) -> None:
+        s = self.plan.stream
+        _check("token_logprobs_submit", abi.lib().augur_cuda_nvfp4_sm100_token_logprobs_prevalidated_submit_v1(
+            s.ordinal, s.handle, self.plan.handle, byref(self.args)))
 
 
 SHAPE_SMALL_BATCH = "small-batch"

@@ -657,6 +657,188 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_interleave_gate_up_h
     uint32_t rows, uint32_t cols, const uint8_t* gate_codes, const uint8_t* gate_scales,
     const uint8_t* up_codes, const uint8_t* up_scales, uint8_t* out_codes, uint8_t* out_scales);
 
+/* ---- paged key-value cache: what a decoding step does between the projections ------------------ */
+/* The reference keeps one contiguous cache per session (its attention and cache kernels are sm_70 code outside the
+ * quantised linear); the entries below have no counterpart of the same form there. One layer of the cache is two BF16
+ * tensors [pages][kv_heads][page_tokens][head_dim]; a sequence's tokens fill the pages of its page-table row in order.
+ * page_tokens: a power of two, 16..1024. head_dim: 128 or 256. pages * kv_heads * page_tokens below 2^31. */
+typedef struct augur_cuda_nvfp4_sm100_kv_layer_v1 {
+    augur_cuda_device_ptr_t keys;
+    augur_cuda_device_ptr_t values;
+    uint64_t len_bytes;                     /* of each of the two */
+    uint32_t pages;
+    uint32_t kv_heads;
+    uint32_t page_tokens;
+    uint32_t head_dim;
+} augur_cuda_nvfp4_sm100_kv_layer_v1;
+
+/* The sequences of one step, all in device memory, so that a captured program can be replayed with new contents:
+ * sequence b owns the token rows [token_starts[b], token_starts[b + 1]) of the step, which are the last tokens of the
+ * lengths[b] that its cache holds with them. Sequences without new tokens are allowed (idle slots); rows outside every
+ * sequence are neither read nor written. Contents that do not fit (a page outside the cache, a length beyond the table,
+ * row numbers outside `rows`) never lead to an access out of bounds; each entry says what it does with them. */
+#define AUGUR_NVFP4_SM100_MAX_SEQUENCES 1024
+typedef struct augur_cuda_nvfp4_sm100_kv_batch_v1 {
+    augur_cuda_device_ptr_t page_table;     /* [sequences][table_pages] int32 */
+    uint64_t page_table_len_bytes;
+    augur_cuda_device_ptr_t lengths;        /* [sequences] int32 */
+    uint64_t lengths_len_bytes;
+    augur_cuda_device_ptr_t token_starts;   /* [sequences + 1] int32, not decreasing */
+    uint64_t token_starts_len_bytes;
+    uint32_t sequences;                     /* 1..MAX_SEQUENCES */
+    uint32_t table_pages;
+    uint32_t rows;                          /* token rows of the step's tensors */
+    uint32_t reserved;
+} augur_cuda_nvfp4_sm100_kv_batch_v1;
+
+/* Rotary positions and the cache write of a step's tokens. For every row of a sequence and every head:
+ *   query_out[row][h] = R N_q(query[row][h]),  keys[slot][h] = R N_k(key[row][h]),  values[slot][h] = value[row][h]
+ * N(x) = x * weight / sqrt(mean(x^2) + epsilon), or x where the weight is 0 (none). R turns the pairs (i, i + rotary_dim / 2) of
+ * the first rotary_dim elements by positions[axis(i)][row] * inv_freq[i]. axis(i): sections one behind the other (time,
+ * height, width; they add up to rotary_dim / 2) or, `interleaved`, i mod 3 while i < 3 * sections[i mod 3], else 0. With text
+ * all three axes hold the same positions. The angle is formed in 64 bits and reduced to one turn there, so that positions of
+ * millions lose nothing; the rest is F32, rounded once. Inputs are BF16 with strides (in elements, multiples of 8;
+ * a head's elements are contiguous), so that q may be the query half of a query|gate projection: query_len_bytes and its
+ * like are the bytes from the first to the last element. A row whose page is not in the table or outside the cache is rotated
+ * into query_out, and its key and value are not written. Any number of rows per sequence (a chunk of a prompt too). */
+typedef struct augur_cuda_nvfp4_sm100_kv_append_args_v1 {
+    uint32_t abi_version;
+    uint32_t struct_size;
+    augur_cuda_nvfp4_sm100_kv_layer_v1 layer;
+    augur_cuda_nvfp4_sm100_kv_batch_v1 batch;
+    augur_cuda_device_ptr_t query;
+    uint64_t query_len_bytes;
+    augur_cuda_device_ptr_t key;
+    uint64_t key_len_bytes;
+    augur_cuda_device_ptr_t value;
+    uint64_t value_len_bytes;
+    uint64_t query_row_stride, query_head_stride;
+    uint64_t key_row_stride, key_head_stride;
+    uint64_t value_row_stride, value_head_stride;
+    augur_cuda_device_ptr_t positions;      /* [3][rows] int32 */
+    uint64_t positions_len_bytes;
+    augur_cuda_device_ptr_t inv_freq_f32;   /* [rotary_dim / 2] radians per position */
+    uint64_t inv_freq_len_bytes;
+    augur_cuda_device_ptr_t query_norm_f32; /* [head_dim], or 0 */
+    augur_cuda_device_ptr_t key_norm_f32;   /* [head_dim], or 0 */
+    uint64_t norm_len_bytes;                /* of each that is given, else 0 */
+    augur_cuda_device_ptr_t query_out;      /* [rows][query_heads][head_dim] BF16 */
+    uint64_t query_out_len_bytes;
+    uint32_t query_heads;
+    uint32_t rotary_dim;                    /* a multiple of 16, up to head_dim */
+    uint32_t sections[3];
+    uint32_t interleaved;
+    float epsilon;
+    uint32_t reserved;
+} augur_cuda_nvfp4_sm100_kv_append_args_v1;
+
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append_preflight_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, const augur_cuda_nvfp4_sm100_kv_append_args_v1* args);
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append_prevalidated_submit_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, const augur_cuda_nvfp4_sm100_kv_append_args_v1* args);
+
+/* Attention of up to max_new_tokens (1..8) new tokens per sequence over its cache, their own keys and values included:
+ *   output[row][h] = sum_j p_j values[j],  p = softmax over j of scale * query[row][h] . keys[j]
+ * for all cached j up to the row's own token. query_heads is a multiple of kv_heads; query_heads / kv_heads * max_new_tokens
+ * is at most 64. Products of BF16 are exact, sums, maxima and exponentials F32; a weight p is rounded to BF16 for the product with the values (and
+ * counted in the denominator as rounded). A row that sees no token gets zeros. What the pages hold
+ * behind a sequence's length is never used, infinities and NaN included; a value that is not finite among the sequence's own
+ * new tokens may reach all of that sequence's rows. A page outside the cache counts as not there and sets the plan's status word to
+ * 0x401, as does a length beyond the table; rows outside the tensors or more than max_new_tokens rows set 0x402, and such a
+ * sequence is left out. A wait that runs out sets 0x411..0x417. The results of a call depend on its inputs
+ * and on the device's SM count alone, not on the order in which CTAs finish. */
+typedef struct augur_cuda_nvfp4_sm100_paged_attention_args_v1 {
+    uint32_t abi_version;
+    uint32_t struct_size;
+    augur_cuda_nvfp4_sm100_kv_layer_v1 layer;
+    augur_cuda_nvfp4_sm100_kv_batch_v1 batch;
+    augur_cuda_device_ptr_t query;          /* [rows][query_heads][head_dim] BF16 */
+    uint64_t query_len_bytes;
+    augur_cuda_device_ptr_t output;         /* [rows][query_heads][head_dim] BF16 */
+    uint64_t output_len_bytes;
+    uint32_t query_heads;
+    uint32_t max_new_tokens;
+    float scale;                            /* finite, usually 1 / sqrt(head_dim) */
+    uint32_t reserved;
+} augur_cuda_nvfp4_sm100_paged_attention_args_v1;
+
+/* Bytes of plan scratch for a device with `sm_count` SMs: the parts of sequences that several CTAs share. */
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_paged_attention_scratch_extent_host_v1(
+    uint32_t query_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_new_tokens, uint32_t sm_count, uint64_t* out_bytes);
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_paged_attention_preflight_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, augur_cuda_nvfp4_sm100_plan_v1* plan,
+    const augur_cuda_nvfp4_sm100_paged_attention_args_v1* args);
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_paged_attention_prevalidated_submit_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, augur_cuda_nvfp4_sm100_plan_v1* plan,
+    const augur_cuda_nvfp4_sm100_paged_attention_args_v1* args);
+
+/* Copies pages in all layers of a cache: keys[l][destinations[i]] = keys[l][sources[i]], values likewise, for every layer l
+ * and i < count (a fork's partly filled page, a compaction's moves). The two lists are host memory, read during the
+ * call; destinations are distinct and none is a source (one source may have several destinations); anything else, or a page
+ * outside the cache, is INVALID_ARGUMENT with nothing enqueued. count = 0 does nothing. */
+typedef struct augur_cuda_nvfp4_sm100_kv_page_copy_args_v1 {
+    uint32_t abi_version;
+    uint32_t struct_size;
+    augur_cuda_device_ptr_t keys;           /* [layers][pages][page_bytes] */
+    augur_cuda_device_ptr_t values;
+    uint64_t len_bytes;                     /* of each of the two */
+    uint64_t page_bytes;                    /* a multiple of 16 */
+    uint32_t layers;
+    uint32_t pages;
+} augur_cuda_nvfp4_sm100_kv_page_copy_args_v1;
+
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_copy_preflight_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, const augur_cuda_nvfp4_sm100_kv_page_copy_args_v1* args);
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_copy_prevalidated_submit_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, const augur_cuda_nvfp4_sm100_kv_page_copy_args_v1* args,
+    const uint32_t* sources, const uint32_t* destinations, uint32_t count);
+
+/* ---- log probabilities behind the vocabulary head -------------------------------------------------- */
+/* For every row x of logits, with m = max x, L = sum e^(x - m):
+ *   logprobs[row] = x[targets[row]] - m - ln L       (NaN where targets[row] is outside the vocabulary)
+ *   entropy[row]  = ln L - sum e^(x - m) (x - m) / L  (a logit of -infinity adds nothing)
+ *   ids[row], alternative_logprobs[row]: the `alternatives` largest logits in order, the lowest index first where they are
+ *   equal (+0 and -0 are), and their log probabilities.
+ * The reference selects on the host or with its own top-k kernels behind the same head; there is no counterpart of this
+ * form. F32 logits (bf16_head) or BF16 ones (a linear's output); sums and statistics F32. A row of -infinities has entropy 0 and
+ * log probabilities -infinity; a NaN or +infinity in a row gives what the formulas give (NaN), NaN ordered above all
+ * numbers. row_stride in elements, at least `vocabulary`, vocabulary up to 2^24, alternatives 0..32 (and at most
+ * vocabulary; 0: ids and alternative_logprobs are 0, with 0 bytes). */
+#define AUGUR_NVFP4_SM100_MAX_ALTERNATIVES 32
+#define AUGUR_NVFP4_SM100_LOGITS_F32 UINT32_C(0)
+#define AUGUR_NVFP4_SM100_LOGITS_BF16 UINT32_C(1)
+typedef struct augur_cuda_nvfp4_sm100_token_logprobs_args_v1 {
+    uint32_t abi_version;
+    uint32_t struct_size;
+    augur_cuda_device_ptr_t logits;         /* [rows][row_stride] */
+    uint64_t logits_len_bytes;              /* ((rows - 1) * row_stride + vocabulary) elements */
+    augur_cuda_device_ptr_t targets;        /* [rows] int32 */
+    uint64_t targets_len_bytes;
+    augur_cuda_device_ptr_t logprobs;       /* [rows] F32 */
+    uint64_t logprobs_len_bytes;
+    augur_cuda_device_ptr_t entropy;        /* [rows] F32 */
+    uint64_t entropy_len_bytes;
+    augur_cuda_device_ptr_t ids;            /* [rows][alternatives] int32 */
+    uint64_t ids_len_bytes;
+    augur_cuda_device_ptr_t alternative_logprobs; /* [rows][alternatives] F32 */
+    uint64_t alternative_logprobs_len_bytes;
+    uint64_t row_stride;
+    uint32_t rows;
+    uint32_t vocabulary;
+    uint32_t alternatives;
+    uint32_t logits_type;
+} augur_cuda_nvfp4_sm100_token_logprobs_args_v1;
+
+/* Bytes of plan scratch: partial statistics and candidates of rows that several CTAs share, whatever the vocabulary. */
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_token_logprobs_scratch_extent_host_v1(
+    uint32_t rows, uint32_t alternatives, uint32_t sm_count, uint64_t* out_bytes);
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_token_logprobs_preflight_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, augur_cuda_nvfp4_sm100_plan_v1* plan,
+    const augur_cuda_nvfp4_sm100_token_logprobs_args_v1* args);
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_token_logprobs_prevalidated_submit_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, augur_cuda_nvfp4_sm100_plan_v1* plan,
+    const augur_cuda_nvfp4_sm100_token_logprobs_args_v1* args);
+
 /* ---- diagnostics ------------------------------------------------------------ */
 /* Host-side fault injection (the reference injects with a device trap,
  * native augur_m306_k14_async_fault_sm70.cu:7-9,61; here nothing touches the GPU):
