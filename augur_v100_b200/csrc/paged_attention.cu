@@ -1,84 +1,681 @@
-// Attention of a step's new tokens over a paged key-value cache on sm_100a.
+// Attention of a step's 1..8 new tokens per sequence over a paged key-value cache on sm_100a.
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(s_j - m),  s_j = scale log2(e) q . k_j
+//
+// The cache is read once (4 kv_heads head_dim bytes a token) and that is the bound: for up to 64 queries per key-value head (new tokens x query
+// heads that share it) the products are small change for the tensor cores. So no thread touches a key or a value: TMA brings pages
+// into a ring in shared memory, and tcgen05.mma reads them there as the 128-row operand, the queries as the narrow one:
+//
+//   S^T[key][query]   = K Q^T          K as it lies in the pages (rows of head_dim: K-major), 128 keys a tile
+//   O^T[dim][query]  += V^T P^T        V as it lies in the pages (the key is the k dimension: MN-major)
+//
+// A thread of the four softmax warps holds one key and all queries of S^T. The running maximum is a reference that only
+// moves when a score passes it by more than 2^8: then O^T is scaled down in tensor memory; otherwise a tile costs a thread one comparison, one
+// exponential and one 2-byte store per query. p is rounded to BF16 for the second product (its relative error of 2^-9 averages
+// out over the keys and stays below the output's own rounding) and counted in the denominator as rounded.
+//
+// Work: the cached tokens of all (sequence, key-value head) pairs in units of 64, dealt out evenly as one span of units per SM. A pair
+// that lies in several spans leaves an unnormalised part per span in the plan's scratch, and a second launch joins those, in
+// the order of the spans. The spans follow from the lengths alone (read on the device, so that a captured call can be replayed).
 #include "kv_cache.cuh"
+#include "nvfp4_gemm.cuh"
 
 namespace augur_sm100 {
 namespace {
+using namespace tc;
 
 static_assert(sizeof(augur_cuda_nvfp4_sm100_paged_attention_args_v1) == 160, "attention ABI");
 
 constexpr uint32_t kMaxQueries = 64;   // new tokens x query heads of a key-value head
+constexpr uint32_t kMaxCtas = 256;     // spans that a launch deals out
+constexpr uint32_t kUnit = 64;         // tokens of a unit of work
+constexpr uint32_t kTile = 128;        // tokens of an MMA tile
+constexpr uint32_t kSlotBytes = kTile * 128;   // 64 dims of a tile
+constexpr uint32_t kMaxSequences = AUGUR_NVFP4_SM100_MAX_SEQUENCES;
+constexpr uint32_t kMaxTokensLog2 = 24;   // of a sequence
+constexpr float kSlack = 8.0f;            // how far, in powers of two, a score may pass the reference maximum
 constexpr uint32_t kStatusPage = 0x401, kStatusRows = 0x402;
+constexpr uint32_t kStatusLoad = 0x411, kStatusMma = 0x412, kStatusScores = 0x413, kStatusValues = 0x414, kStatusQuery = 0x415, kStatusGroup = 0x416, kStatusProduct = 0x417;
+constexpr uint32_t kThreads = 256;        // warp 0 loads, 1 MMA, 2 and 3 queries, 4..7 softmax
+constexpr uint32_t kSmemLimit = 227 * 1024;
+constexpr uint32_t kInfos = 8;            // tiles that the loader is ahead of the softmax at most, rounded up
 
 struct AttentionParams {
-    const __nv_bfloat16 *query, *keys, *values;
+    const __nv_bfloat16* query;
     __nv_bfloat16* output;
     const int32_t *page_table, *lengths, *token_starts;
     uint32_t* status_word;
-    uint32_t rows, sequences, table_pages, pages, query_heads, kv_heads, page_shift, max_new;
-    float scale_log2;   // scale * log2(e)
+    struct JoinRecord* records;   // [spans]
+    float* parts;                 // [spans][2][kN][head_dim], then [spans][2][kN] (reference maximum, denominator)
+    uint32_t rows, sequences, table_pages, pages, query_heads, kv_heads, page_shift, max_new, spans;
+    float scale_log2;             // scale * log2(e)
 };
 
-// One CTA per token row and query head, a warp per key, online softmax in registers.
-template <uint32_t kHeadDim>
-__global__ void __launch_bounds__(256) attention_simple_kernel(const AttentionParams p) {
-    constexpr uint32_t kPer = kHeadDim / 32, kWarps = 8;
-    __shared__ float part[kWarps][kHeadDim], tops[kWarps], sums[kWarps];
-    __shared__ int32_t sequence_at;
-    const uint32_t row = blockIdx.x / p.query_heads, head = blockIdx.x % p.query_heads, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (threadIdx.x == 0) sequence_at = -1;
+// What the join has to know of the pair whose first part span `c` holds (tokens 0: none).
+struct JoinRecord {
+    uint32_t row, tokens, head, last;   // first token row, new tokens, key-value head, last span
+    uint32_t reserved[4];
+};
+
+// Small state of a CTA, behind the ring, the queries and the weights.
+struct State {
+    uint64_t full[16], empty[16];
+    uint64_t scores_full[2], scores_empty[2], weights_full[2], weights_empty[2], query_full[2], query_empty[2], group;
+    uint32_t tmem, abort[1 + kThreads / 32];
+    uint32_t needs[2];                 // a byte per softmax warp: a reference has to move
+    uint32_t info[kInfos];             // of a tile: pages that are there, a bit per box; bit 31: the last tile
+    uint32_t scan[kThreads / 32];
+    float reference[kMaxQueries], factor[kMaxQueries];
+    float wide[4][kMaxQueries];        // a value per softmax warp and query
+    int32_t limit[kMaxQueries];        // keys that a query sees
+    uint32_t units[kMaxSequences + 1]; // before sequence b, of one head
+    uint32_t length[kMaxSequences];    // | new tokens << 25
+};
+
+template <uint32_t kHeadDim, uint32_t kN>
+struct Shape {
+    static constexpr uint32_t kChunks = kHeadDim / 64, kHalves = kHeadDim / 128;
+    static constexpr uint32_t kQueryBytes = kN * kHeadDim * 2, kQueryBuffers = kQueryBytes > 24 * 1024 ? 1 : 2;
+    static constexpr uint32_t kWeightBytes = kN * kTile * 2;
+    static constexpr uint32_t kRoom = kSmemLimit - 1024 - sizeof(State) - kQueryBuffers * kQueryBytes - 2 * kWeightBytes;
+    static constexpr uint32_t kSlots = kRoom / kSlotBytes / 2 * 2 > 16 ? 16 : kRoom / kSlotBytes / 2 * 2;
+    static constexpr uint32_t kSmem = 1024 + kSlots * kSlotBytes + kQueryBuffers * kQueryBytes + 2 * kWeightBytes + sizeof(State);
+    static constexpr uint32_t kColumns = (2 + kHalves) * kN, kTmem = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : 256;
+    static_assert(kSlots >= 2 * kChunks && kSmem <= kSmemLimit && kColumns <= 256, "a CTA's memory");
+};
+
+// A CTA's way through its span: one (sequence, head) after the other, in each the keys [key, key_end).
+struct Walk {
+    uint64_t unit, end;
+    uint32_t sequence, head, key, key_end, length, tokens;
+    bool starts, ends;   // the pair's first and last key are in the span
+
+    __device__ void open(const State* st, const AttentionParams& p, uint64_t from, uint64_t to) {
+        unit = from, end = to;
+        uint32_t low = 0, high = p.sequences;   // the last sequence whose units start at or before `from`
+        while (high - low > 1) {
+            const uint32_t middle = (low + high) / 2;
+            if (static_cast<uint64_t>(st->units[middle]) * p.kv_heads <= from) low = middle;
+            else high = middle;
+        }
+        sequence = low;
+    }
+    __device__ bool next(const State* st, const AttentionParams& p) {
+        if (unit >= end) return false;
+        while (unit >= static_cast<uint64_t>(st->units[sequence + 1]) * p.kv_heads) ++sequence;
+        const uint32_t count = st->units[sequence + 1] - st->units[sequence];
+        const uint32_t at = static_cast<uint32_t>(unit - static_cast<uint64_t>(st->units[sequence]) * p.kv_heads);
+        head = at / count;
+        const uint32_t first = at - head * count;
+        const uint32_t take = static_cast<uint32_t>(end - unit < count - first ? end - unit : count - first);
+        length = st->length[sequence] & ((1u << (kMaxTokensLog2 + 1)) - 1), tokens = st->length[sequence] >> (kMaxTokensLog2 + 1);
+        starts = first == 0, ends = first + take == count;
+        key = first * kUnit;
+        const uint32_t stop = (first + take) * kUnit;
+        key_end = stop < length ? stop : length;
+        unit += take;
+        return true;
+    }
+};
+// The same, tile by tile (pairs without keys are passed over).
+struct Tiles {
+    Walk walk;
+    uint32_t key;
+    bool valid;
+    __device__ void open(const State* st, const AttentionParams& p, uint64_t from, uint64_t to) {
+        walk.open(st, p, from, to);
+        seek(st, p);
+    }
+    __device__ void seek(const State* st, const AttentionParams& p) {
+        do {
+            valid = walk.next(st, p);
+        } while (valid && walk.key >= walk.key_end);
+        key = walk.key;
+    }
+    __device__ void advance(const State* st, const AttentionParams& p) {
+        key += kTile;
+        if (key >= walk.key_end) seek(st, p);
+    }
+    __device__ bool first() const { return key == walk.key; }
+    __device__ bool last() const { return key + kTile >= walk.key_end; }
+    __device__ uint32_t keys() const { return walk.key_end - key < kTile ? walk.key_end - key : kTile; }
+};
+
+__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+// V as the 128-row operand: 128-byte rows of 64 dims, one per key, so the rows are the k dimension; 8 keys are 1024 bytes, the next 64 dims
+// lie one ring slot further.
+__device__ __forceinline__ uint64_t value_desc(uint32_t smem_addr) {
+    return static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4) | (static_cast<uint64_t>(kSlotBytes >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
+           (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+__device__ __forceinline__ void load_columns16(uint32_t taddr, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                   "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void store_columns16(uint32_t taddr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+                   "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float warp_max(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <uint32_t kHeadDim, uint32_t kN>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __grid_constant__ CUtensorMap map_values, const __grid_constant__ AttentionParams p) {
+    using S = Shape<kHeadDim, kN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* const query_smem = smem + S::kSlots * kSlotBytes;
+    uint8_t* const weight_smem = query_smem + S::kQueryBuffers * S::kQueryBytes;
+    State* const st = reinterpret_cast<State*>(weight_smem + 2 * S::kWeightBytes);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t full = smem_u32(st->full), empty = smem_u32(st->empty), scores_full = smem_u32(st->scores_full), scores_empty = smem_u32(st->scores_empty);
+    const uint32_t weights_full = smem_u32(st->weights_full), weights_empty = smem_u32(st->weights_empty);
+    const uint32_t query_full = smem_u32(st->query_full), query_empty = smem_u32(st->query_empty), group_bar = smem_u32(&st->group);
+    volatile uint32_t* abort_flag = st->abort;
+    uint32_t* const status = p.status_word;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < S::kSlots; ++s) mbar_init(full + 8 * s, 1), mbar_init(empty + 8 * s, 1);
+        for (uint32_t b = 0; b < 2; ++b) {
+            mbar_init(scores_full + 8 * b, 1), mbar_init(scores_empty + 8 * b, 4);
+            mbar_init(weights_full + 8 * b, 4), mbar_init(weights_empty + 8 * b, 1);
+            mbar_init(query_full + 8 * b, 2), mbar_init(query_empty + 8 * b, 1);
+        }
+        mbar_init(group_bar, 4);
+        for (uint32_t i = 0; i < 1 + kThreads / 32; ++i) st->abort[i] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&st->tmem)), "r"(S::kTmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // Everything above runs while the launch before this one drains; from here on its results are read.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    {   // units of every sequence, and their running sum: four neighbouring sequences a thread
+        static_assert(kMaxSequences == 4 * kThreads, "four sequences a thread");
+        uint32_t count[4], sum = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t b = 4 * threadIdx.x + i;
+            count[i] = 0;
+            if (b < p.sequences) {
+                const int32_t from = p.token_starts[b], to = p.token_starts[b + 1];
+                int32_t length = p.lengths[b];
+                const int32_t room = static_cast<int32_t>(p.table_pages << p.page_shift);
+                const bool rows_fit = from >= 0 && to <= static_cast<int32_t>(p.rows) && to >= from && to - from <= static_cast<int32_t>(p.max_new);
+                if (!rows_fit && blockIdx.x == 0) atomicCAS(status, 0u, kStatusRows);
+                if (length > room) {
+                    length = room;
+                    if (blockIdx.x == 0) atomicCAS(status, 0u, kStatusPage);
+                }
+                if (length < 0) length = 0;
+                const uint32_t tokens = rows_fit ? static_cast<uint32_t>(to - from) : 0;
+                st->length[b] = static_cast<uint32_t>(length) | tokens << (kMaxTokensLog2 + 1);
+                if (tokens) count[i] = length ? (static_cast<uint32_t>(length) + kUnit - 1) / kUnit : 1;   // a row that sees nothing is written too
+            }
+            sum += count[i];
+        }
+        uint32_t before = sum;
+#pragma unroll
+        for (uint32_t step = 1; step < 32; step *= 2) {
+            const uint32_t other = __shfl_up_sync(0xffffffffu, before, step);
+            if (lane >= step) before += other;
+        }
+        if (lane == 31) st->scan[warp] = before;
+        before -= sum;
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+#pragma unroll
+        for (uint32_t w = 0; w < kThreads / 32; ++w) before += w < warp ? st->scan[w] : 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t b = 4 * threadIdx.x + i;
+            if (b < p.sequences) st->units[b] = before;
+            before += count[i];
+            if (b + 1 == p.sequences) st->units[p.sequences] = before;
+        }
+        __syncthreads();
+    }
+    const uint64_t total = static_cast<uint64_t>(st->units[p.sequences]) * p.kv_heads;
+    const uint32_t spans = total < p.spans ? static_cast<uint32_t>(total) : p.spans;
+    const uint64_t from = blockIdx.x < spans ? total * blockIdx.x / spans : 0, to = blockIdx.x < spans ? total * (blockIdx.x + 1) / spans : 0;
+    const uint32_t tmem = st->tmem, tmem_out = tmem + 2 * kN;
+    const uint32_t group = p.query_heads / p.kv_heads;
+
+    if (warp == 0) {
+        // ---------------- pages: K of a tile, then V of the tile before it ----------------
+        const uint32_t box_shift = p.page_shift < 6 ? p.page_shift : 6, boxes = kTile >> box_shift, box_bytes = 128u << box_shift;
+        Tiles tiles;
+        tiles.open(st, p, from, to);
+        uint32_t slot = 0, phase = 1, count = 0, row_before = 0, mask_before = 0;
+        bool alive = true;
+        // the row of the cache where this lane's box of the tile starts, and which lanes have one
+        auto look = [&](const Tiles& t, uint32_t* row, uint32_t* mask) {
+            const uint32_t key = t.key + (lane << box_shift);
+            bool there = false;
+            *row = 0;
+            if (lane < boxes && t.valid && key < t.walk.key_end) {
+                const int32_t page = __ldg(p.page_table + static_cast<uint64_t>(t.walk.sequence) * p.table_pages + (key >> p.page_shift));
+                there = page >= 0 && static_cast<uint32_t>(page) < p.pages;
+                if (there) *row = (((static_cast<uint32_t>(page) * p.kv_heads) + t.walk.head) << p.page_shift) + (key & ((1u << p.page_shift) - 1));
+                else atomicCAS(status, 0u, kStatusPage);
+            }
+            *mask = __ballot_sync(0xffffffffu, there);
+        };
+        auto load = [&](const CUtensorMap* map, uint32_t row, uint32_t mask) {
+            for (uint32_t c = 0; alive && c < S::kChunks; ++c) {
+                if (!warp_look_wait(empty + 8 * slot, phase, abort_flag, status, kStatusLoad)) {
+                    alive = false;
+                    break;
+                }
+                if (lane == 0) {
+                    if (mask) mbar_expect_tx(full + 8 * slot, __popc(mask) * box_bytes);
+                    else mbar_arrive(full + 8 * slot);
+                }
+                __syncwarp();
+                if (mask >> lane & 1) tma_load_2d(smem_u32(smem + slot * kSlotBytes) + lane * box_bytes, map, c * 128, row, full + 8 * slot);
+                __syncwarp();
+                if (++slot == S::kSlots) slot = 0, phase ^= 1;
+            }
+        };
+        uint32_t row, mask;
+        look(tiles, &row, &mask);
+        while (alive && (tiles.valid || count)) {
+            const bool has_keys = tiles.valid;
+            uint32_t row_next = 0, mask_next = 0;
+            if (has_keys) {
+                tiles.advance(st, p);
+                look(tiles, &row_next, &mask_next);   // ahead of its use by a tile
+                if (lane == 0) st->info[count % kInfos] = mask | (tiles.valid ? 0 : 0x80000000u);
+                load(&map_keys, row, mask);
+            }
+            if (count) load(&map_values, row_before, mask_before);
+            if (!has_keys) break;
+            row_before = row, mask_before = mask;
+            row = row_next, mask = mask_next;
+            ++count;
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer: S of a tile, then O of the tile before it ----------------
+        constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kN >> 3) << 17) | ((kTile >> 4) << 24);   // F32 += BF16 x BF16
+        constexpr uint32_t idesc_values = idesc | (1u << 15);                                                        // V is MN-major
+        const uint64_t slots = operand_desc(smem_u32(smem)), slots_values = value_desc(smem_u32(smem));
+        const uint64_t queries = operand_desc(smem_u32(query_smem)), weights = operand_desc(smem_u32(weight_smem));
+        Tiles ahead, now;
+        ahead.open(st, p, from, to);
+        now = ahead;
+        uint32_t slot = 0, phase = 0, scores = 0, products = 0, pair = 0;
+        bool alive = true;
+        auto scores_of_tile = [&]() {
+            const uint32_t buffer = scores & 1, query = S::kQueryBuffers == 2 ? pair & 1 : 0;
+            if (ahead.first() && !warp_look_wait(query_full + 8 * query, (S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1, abort_flag, status, kStatusMma)) return false;
+            if (!warp_look_wait(scores_empty + 8 * buffer, (scores >> 1 & 1) ^ 1, abort_flag, status, kStatusMma)) return false;
+            for (uint32_t c = 0; c < S::kChunks; ++c) {
+                if (!warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusMma)) return false;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t a = slots + slot * (kSlotBytes >> 4), b = queries + ((query * S::kQueryBytes + c * kN * 128) >> 4);
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) mma_bf16(tmem + buffer * kN, a + 2 * k, b + 2 * k, idesc, c | k);
+                    tc_commit(empty + 8 * slot);
+                }
+                __syncwarp();
+                if (++slot == S::kSlots) slot = 0, phase ^= 1;
+            }
+            if (elect_one()) {
+                tc_commit(scores_full + 8 * buffer);
+                if (ahead.last()) tc_commit(query_empty + 8 * query);
+            }
+            __syncwarp();
+            if (ahead.last()) ++pair;
+            ++scores;
+            ahead.advance(st, p);
+            return true;
+        };
+        if (ahead.valid) alive = scores_of_tile();
+        while (alive && now.valid) {
+            if (ahead.valid && !scores_of_tile()) break;
+            const uint32_t buffer = products & 1, steps = (now.keys() + 15) / 16;
+            if (!warp_look_wait(weights_full + 8 * buffer, products >> 1 & 1, abort_flag, status, kStatusProduct)) break;
+            for (uint32_t h = 0; alive && h < S::kHalves; ++h) {
+                for (uint32_t c = 0; c < 2; ++c) alive = alive && warp_look_wait(full + 8 * (slot + c), phase, abort_flag, status, kStatusProduct);
+                if (!alive) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t a = slots_values + slot * (kSlotBytes >> 4), b = weights + ((buffer * S::kWeightBytes) >> 4);
+                    for (uint32_t k = 0; k < steps; ++k) {   // 16 keys: 16 rows of V, 32 bytes of a row of P
+                        mma_bf16(tmem_out + h * kN, a + k * (16 * 128 >> 4), b + (k >> 2) * (kN * 128 >> 4) + (k & 3) * 2, idesc_values, !now.first() || k);
+                    }
+                    tc_commit(empty + 8 * slot);
+                    tc_commit(empty + 8 * (slot + 1));
+                }
+                __syncwarp();
+                slot += 2;
+                if (slot == S::kSlots) slot = 0, phase ^= 1;
+            }
+            if (!alive) break;
+            if (elect_one()) tc_commit(weights_empty + 8 * buffer);
+            __syncwarp();
+            ++products;
+            now.advance(st, p);
+        }
+    } else if (warp < 4) {
+        // ---------------- queries of a pair, in the 128-byte swizzle of the operand; rows past the last are zero ----------------
+        const uint32_t thread = threadIdx.x - 64;
+        Walk walk;
+        walk.open(st, p, from, to);
+        uint32_t pair = 0;
+        while (walk.next(st, p)) {
+            if (walk.key >= walk.key_end) continue;
+            const uint32_t buffer = S::kQueryBuffers == 2 ? pair & 1 : 0;
+            const uint32_t first_row = static_cast<uint32_t>(__ldg(p.token_starts + walk.sequence)), queries = walk.tokens * group;
+            if (!warp_look_wait(query_empty + 8 * buffer, ((S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1) ^ 1, abort_flag, status, kStatusQuery)) break;
+            constexpr uint32_t kPieces = kHeadDim / 8;
+            for (uint32_t i = thread; i < kN * kPieces; i += 64) {
+                const uint32_t row = i / kPieces, piece = i % kPieces;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (row < queries) {
+                    const uint32_t token = row / group;
+                    const uint64_t at = (static_cast<uint64_t>(first_row + token) * p.query_heads + walk.head * group + (row - token * group)) * kHeadDim;
+                    v = __ldg(reinterpret_cast<const uint4*>(p.query + at) + piece);
+                }
+                *reinterpret_cast<uint4*>(query_smem + buffer * S::kQueryBytes + (piece >> 3) * (kN * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = v;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(query_full + 8 * buffer);
+            ++pair;
+        }
+    } else {
+        // ---------------- softmax: thread = key of a tile, then dim of the output ----------------
+        const uint32_t thread = threadIdx.x - 128, quadrant = warp & 3, lanes = (quadrant * 32) << 16;
+        const uint32_t box_shift = p.page_shift < 6 ? p.page_shift : 6, boxes = kTile >> box_shift, all_boxes = (1u << boxes) - 1;
+        uint32_t tile = 0, meetings = 0;
+        JoinRecord record{};
+        // The four warps meet (a bounded wait, where a named barrier would hang on a warp that gave up).
+        auto meet = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(group_bar);
+            return warp_look_wait(group_bar, meetings++ & 1, abort_flag, status, kStatusGroup);
+        };
+        Walk walk;
+        walk.open(st, p, from, to);
+        bool alive = true;
+        while (alive && walk.next(st, p)) {
+            const uint32_t queries = walk.tokens * group;
+            const int32_t first_row = __ldg(p.token_starts + walk.sequence);
+            if (thread < kN) {
+                st->reference[thread] = -INFINITY;
+                st->limit[thread] = thread < queries ? static_cast<int32_t>(walk.length) - static_cast<int32_t>(walk.tokens) + static_cast<int32_t>(thread / group) + 1 : 0;
+            }
+            if (!meet()) break;
+            float sum[kN];
+#pragma unroll
+            for (uint32_t c = 0; c < kN; ++c) sum[c] = 0.0f;
+            const int32_t seen_by_all = static_cast<int32_t>(walk.length) - static_cast<int32_t>(walk.tokens) + 1;
+            for (uint32_t key = walk.key; key < walk.key_end; key += kTile, ++tile) {
+                const uint32_t buffer = tile & 1;
+                if (!warp_look_wait(scores_full + 8 * buffer, tile >> 1 & 1, abort_flag, status, kStatusScores)) {
+                    alive = false;
+                    break;
+                }
+                tc_fence_after();
+                float s[kN];
+#pragma unroll
+                for (uint32_t c = 0; c < kN; c += 16) load_columns16(tmem + lanes + buffer * kN + c, reinterpret_cast<uint32_t*>(s) + c);
+                tc_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(scores_empty + 8 * buffer);
+                const uint32_t info = st->info[tile % kInfos], there = info & 0x7fffffffu;
+                const uint32_t count = walk.key_end - key < kTile ? walk.key_end - key : kTile;
+                const bool whole = count == kTile && there == all_boxes;
+                const bool my_key = thread < count && (there >> (thread >> box_shift) & 1);
+#pragma unroll
+                for (uint32_t c = 0; c < kN; ++c) s[c] *= p.scale_log2;
+                if (!whole || static_cast<int32_t>(key + kTile) > seen_by_all) {
+#pragma unroll
+                    for (uint32_t c = 0; c < kN; ++c) s[c] = my_key && static_cast<int32_t>(key + thread) < st->limit[c] ? s[c] : -INFINITY;
+                }
+                bool above = false;
+#pragma unroll
+                for (uint32_t c = 0; c < kN; ++c) above |= s[c] > st->reference[c] + kSlack;
+                above = __any_sync(0xffffffffu, above);
+                if (lane == 0) reinterpret_cast<uint8_t*>(&st->needs[buffer])[quadrant] = above;
+                if (!meet()) {
+                    alive = false;
+                    break;
+                }
+                if (*const_cast<volatile uint32_t*>(&st->needs[buffer])) {
+                    // A reference moves up to the largest score so far, for all queries.
+#pragma unroll
+                    for (uint32_t c = 0; c < kN; ++c) {
+                        const float most = warp_max(s[c]);
+                        if (lane == (c & 31)) st->wide[quadrant][c] = most;
+                    }
+                    if (!meet()) {
+                        alive = false;
+                        break;
+                    }
+                    if (thread < kN) {
+                        const float old = st->reference[thread];
+                        const float most = fmaxf(fmaxf(fmaxf(st->wide[0][thread], st->wide[1][thread]), fmaxf(st->wide[2][thread], st->wide[3][thread])), old);
+                        st->factor[thread] = most == old ? 1.0f : exp2_fast(old - most);
+                        st->reference[thread] = most;
+                    }
+                    if (!meet()) {
+                        alive = false;
+                        break;
+                    }
+#pragma unroll
+                    for (uint32_t c = 0; c < kN; ++c) sum[c] *= st->factor[c];
+                    if (key != walk.key) {
+                        if (!warp_look_wait(weights_empty + 8 * (buffer ^ 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) {
+                            alive = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        for (uint32_t c = 0; c < S::kHalves * kN; c += 16) {
+                            uint32_t v[16];
+                            load_columns16(tmem_out + lanes + c, v);
+                            tc_wait_ld();
+#pragma unroll
+                            for (uint32_t i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * st->factor[(c + i) % kN]);
+                            store_columns16(tmem_out + lanes + c, v);
+                        }
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        tc_fence_before();
+                    }
+                }
+                if (!warp_look_wait(weights_empty + 8 * buffer, (tile >> 1 & 1) ^ 1, abort_flag, status, kStatusProduct)) {
+                    alive = false;
+                    break;
+                }
+                uint8_t* const to_weights = weight_smem + buffer * S::kWeightBytes + (thread >> 6) * (kN * 128) + (thread & 7) * 2;
+                const uint32_t unit = (thread & 63) >> 3;
+#pragma unroll
+                for (uint32_t c = 0; c < kN; ++c) {
+                    const float reference = st->reference[c];
+                    const __nv_bfloat16 weight = __float2bfloat16_rn(exp2_fast(s[c] - (reference == -INFINITY ? 0.0f : reference)));
+                    sum[c] += __bfloat162float(weight);
+                    *reinterpret_cast<__nv_bfloat16*>(to_weights + c * 128 + ((unit ^ (c & 7)) << 4)) = weight;
+                }
+                if (!whole) {
+                    // Rows of V that are no token's are multiplied with weights of zero: whatever lies there, they must be numbers.
+                    const uint32_t at = 2 * S::kChunks * (tile + 1) - (info >> 31 ? S::kChunks : 0);   // the tile's V among all slots that were loaded
+                    uint32_t slot = at % S::kSlots, phase = at / S::kSlots & 1;
+                    for (uint32_t c = 0; alive && c < S::kChunks; ++c) {
+                        if (!warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusValues)) {
+                            alive = false;
+                            break;
+                        }
+                        if (!my_key && thread < (count + 15) / 16 * 16) {
+                            uint4* row = reinterpret_cast<uint4*>(smem + slot * kSlotBytes + thread * 128);
+#pragma unroll
+                            for (uint32_t i = 0; i < 8; ++i) row[i] = make_uint4(0, 0, 0, 0);
+                        }
+                        if (++slot == S::kSlots) slot = 0, phase ^= 1;
+                    }
+                    if (!alive) break;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(weights_full + 8 * buffer);
+            }
+            if (!alive) break;
+            // ---- the pair's output, or its part ----
+            const bool any = walk.key < walk.key_end;
+#pragma unroll
+            for (uint32_t c = 0; c < kN; ++c) {
+#pragma unroll
+                for (uint32_t step = 16; step; step /= 2) sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], step);
+                if (lane == (c & 31)) st->wide[quadrant][c] = sum[c];
+            }
+            if (!meet()) break;
+            if (any) {
+                if (!warp_look_wait(weights_empty + 8 * ((tile - 1) & 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) break;
+                tc_fence_after();
+            }
+            const bool alone = walk.starts && walk.ends;
+            const uint32_t part = 2 * blockIdx.x + (walk.starts ? 1 : 0);
+            float* const part_out = p.parts + static_cast<uint64_t>(part) * kN * kHeadDim;
+            for (uint32_t h = 0; h < S::kHalves; ++h) {
+                for (uint32_t c0 = 0; c0 < kN && c0 < queries; c0 += 16) {
+                    uint32_t v[16];
+                    if (any) {
+                        load_columns16(tmem_out + lanes + h * kN + c0, v);
+                        tc_wait_ld();
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) {
+                        const uint32_t c = c0 + i;
+                        if (c < queries) {
+                            if (alone) {
+                                const uint32_t token = c / group;
+                                const float all = (st->wide[0][c] + st->wide[1][c]) + (st->wide[2][c] + st->wide[3][c]);
+                                const float value = !any || all == 0.0f ? 0.0f : __uint_as_float(v[i]) / all;
+                                p.output[(static_cast<uint64_t>(first_row + token) * p.query_heads + walk.head * group + (c - token * group)) * kHeadDim + h * 128 + thread] =
+                                    __float2bfloat16_rn(value);
+                            } else {
+                                part_out[static_cast<uint64_t>(c) * kHeadDim + h * 128 + thread] = __uint_as_float(v[i]);
+                            }
+                        }
+                    }
+                }
+            }
+            if (any) tc_fence_before();
+            if (!alone) {
+                if (thread < queries) {
+                    float* const stats = p.parts + static_cast<uint64_t>(2 * p.spans) * kN * kHeadDim + (static_cast<uint64_t>(part) * kN + thread) * 2;
+                    stats[0] = st->reference[thread];
+                    stats[1] = (st->wide[0][thread] + st->wide[1][thread]) + (st->wide[2][thread] + st->wide[3][thread]);
+                }
+                if (walk.starts) {
+                    const uint64_t units = st->units[walk.sequence + 1] - st->units[walk.sequence];
+                    const uint64_t last = static_cast<uint64_t>(st->units[walk.sequence]) * p.kv_heads + (walk.head + 1) * units;   // one past its last unit
+                    record.row = static_cast<uint32_t>(first_row), record.tokens = walk.tokens, record.head = walk.head;
+                    record.last = static_cast<uint32_t>((last * spans - 1) / total);
+                }
+            }
+            if (!meet()) break;   // before the next pair's state overwrites what the others still read
+        }
+        if (thread == 0) p.records[blockIdx.x] = record;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmem) : "memory");
+    }
+}
+
+// Joins the parts of one pair, in the order of their spans: four outputs a thread, blockIdx.y = which of the pair's queries.
+constexpr uint32_t kJoinThreads = 256;
+template <uint32_t kHeadDim, uint32_t kN>
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttentionParams p) {
+    constexpr uint32_t kLanes = kHeadDim / 4, kQueries = kJoinThreads / kLanes;
+    __shared__ float weight[kQueries][kMaxCtas];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    __syncthreads();
-    for (uint32_t b = threadIdx.x; b < p.sequences; b += 256) {
-        const int32_t from = p.token_starts[b], to = p.token_starts[b + 1];
-        if (from < 0 || to > static_cast<int32_t>(p.rows) || to - from > static_cast<int32_t>(p.max_new)) atomicCAS(p.status_word, 0u, kStatusRows);
-        else if (static_cast<int32_t>(row) >= from && static_cast<int32_t>(row) < to) sequence_at = static_cast<int32_t>(b);
-    }
-    __syncthreads();
-    if (sequence_at < 0) return;
-    const uint32_t b = static_cast<uint32_t>(sequence_at), kv_head = head / (p.query_heads / p.kv_heads);
-    const int64_t length = p.lengths[b], room = static_cast<int64_t>(p.table_pages) << p.page_shift;
-    if (length > room) atomicCAS(p.status_word, 0u, kStatusPage);
-    int64_t keys = length - p.token_starts[b + 1] + row + 1;
-    if (keys > room) keys = room;
-    float q[kPer], sum[kPer], top = -INFINITY, total = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < kPer; ++i) {
-        q[i] = __bfloat162float(p.query[(static_cast<uint64_t>(row) * p.query_heads + head) * kHeadDim + i * 32 + lane]);
-        sum[i] = 0.0f;
-    }
-    for (int64_t j = warp; j < keys; j += kWarps) {
-        const int32_t page = p.page_table[static_cast<uint64_t>(b) * p.table_pages + (j >> p.page_shift)];
-        if (page < 0 || static_cast<uint32_t>(page) >= p.pages) {
-            if (lane == 0) atomicCAS(p.status_word, 0u, kStatusPage);
-            continue;
+    const JoinRecord record = p.records[blockIdx.x];
+    const uint32_t group = p.query_heads / p.kv_heads, which = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, query = blockIdx.y * kQueries + which;
+    if (blockIdx.y * kQueries >= record.tokens * group) return;
+    const uint32_t parts = record.last - blockIdx.x + 1;
+    const bool live = query < record.tokens * group;
+    const float2* stats = reinterpret_cast<const float2*>(p.parts + static_cast<uint64_t>(2 * p.spans) * kN * kHeadDim) + query;
+    auto part = [&](uint32_t i) { return 2 * (blockIdx.x + i) + (i == 0 ? 1 : 0); };
+    float most = -INFINITY, all = 0.0f;
+    if (live) {
+        for (uint32_t i = 0; i < parts; ++i) most = fmaxf(most, stats[static_cast<uint64_t>(part(i)) * kN].x);
+        for (uint32_t i = 0; i < parts; ++i) {
+            const float2 s = stats[static_cast<uint64_t>(part(i)) * kN];
+            const float w = s.x == -INFINITY ? 0.0f : exp2_fast(s.x - most);
+            all += w * s.y;
+            if (lane == 0) weight[which][i] = w;
         }
-        const uint64_t at = (((static_cast<uint64_t>(page) * p.kv_heads + kv_head) << p.page_shift) + (j & ((1 << p.page_shift) - 1))) * kHeadDim + lane;
-        float dot = 0.0f;
-#pragma unroll
-        for (uint32_t i = 0; i < kPer; ++i) dot = fmaf(q[i], __bfloat162float(p.keys[at + i * 32]), dot);
-#pragma unroll
-        for (uint32_t step = 16; step; step /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, step);
-        const float score = dot * p.scale_log2, above = fmaxf(top, score);
-        if (above == -INFINITY) continue;
-        const float keep = exp2f(top - above), weight = exp2f(score - above);
-        top = above;
-        total = total * keep + weight;
-#pragma unroll
-        for (uint32_t i = 0; i < kPer; ++i) sum[i] = sum[i] * keep + weight * __bfloat162float(p.values[at + i * 32]);
     }
-#pragma unroll
-    for (uint32_t i = 0; i < kPer; ++i) part[warp][i * 32 + lane] = sum[i];
-    if (lane == 0) tops[warp] = top, sums[warp] = total;
     __syncthreads();
-    float above = -INFINITY, all = 0.0f;
-    for (uint32_t w = 0; w < kWarps; ++w) above = fmaxf(above, tops[w]);
-    for (uint32_t w = 0; w < kWarps; ++w) all += tops[w] == -INFINITY ? 0.0f : sums[w] * exp2f(tops[w] - above);
-    for (uint32_t d = threadIdx.x; d < kHeadDim; d += 256) {
-        float value = 0.0f;
-        for (uint32_t w = 0; w < kWarps; ++w) value += tops[w] == -INFINITY ? 0.0f : part[w][d] * exp2f(tops[w] - above);
-        p.output[(static_cast<uint64_t>(row) * p.query_heads + head) * kHeadDim + d] = __float2bfloat16_rn(above == -INFINITY ? 0.0f : value / all);
+    if (!live) return;
+    float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+    for (uint32_t i = 0; i < parts; ++i) {
+        const float4 v = reinterpret_cast<const float4*>(p.parts + (static_cast<uint64_t>(part(i)) * kN + query) * kHeadDim)[lane];
+        const float w = weight[which][i];
+        if (w != 0.0f) sum.x = fmaf(w, v.x, sum.x), sum.y = fmaf(w, v.y, sum.y), sum.z = fmaf(w, v.z, sum.z), sum.w = fmaf(w, v.w, sum.w);
     }
+    const float scale = all == 0.0f ? 0.0f : 1.0f / all;
+    const __nv_bfloat162 a = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum.x * scale, all == 0.0f ? 0.0f : sum.y * scale);
+    const __nv_bfloat162 b = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum.z * scale, all == 0.0f ? 0.0f : sum.w * scale);
+    const uint32_t token = query / group;
+    const uint64_t at = (static_cast<uint64_t>(record.row + token) * p.query_heads + record.head * group + (query - token * group)) * kHeadDim + 4 * lane;
+    *reinterpret_cast<uint2*>(p.output + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+uint32_t query_columns(uint32_t query_heads, uint32_t kv_heads, uint32_t max_new) { return (query_heads / kv_heads * max_new + 15) / 16 * 16; }
+uint32_t launch_spans(uint32_t sm_count) { return sm_count < kMaxCtas ? sm_count : kMaxCtas; }
+
+template <uint32_t kHeadDim, uint32_t kN>
+void launch_attention(cudaStream_t stream, const CUtensorMap& keys, const CUtensorMap& values, const AttentionParams& p) {
+    using S = Shape<kHeadDim, kN>;
+    launch_dependent(stream, paged_attention_kernel<kHeadDim, kN>, p.spans, kThreads, S::kSmem, keys, values, p);
+    constexpr uint32_t kQueries = kJoinThreads / (kHeadDim / 4);
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.stream = stream, config.attrs = &attribute, config.numAttrs = 1;
+    config.gridDim = dim3(p.spans, (p.query_heads / p.kv_heads * p.max_new + kQueries - 1) / kQueries), config.blockDim = dim3(kJoinThreads);
+    cudaLaunchKernelEx(&config, attention_join_kernel<kHeadDim, kN>, p);
+    count_launch(2);
+}
+
+template <uint32_t kHeadDim>
+cudaError_t configure() {
+    constexpr cudaFuncAttribute kSmem = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 16>, kSmem, Shape<kHeadDim, 16>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 32>, kSmem, Shape<kHeadDim, 32>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 48>, kSmem, Shape<kHeadDim, 48>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 64>, kSmem, Shape<kHeadDim, 64>::kSmem);
+    return e;
 }
 
 bool shape_ok(uint32_t query_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_new) {
@@ -94,6 +691,7 @@ bool check_attention(int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm
         return false;
     }
     if (!plan_ok(plan, d, s) || !kv_layer_ok(a->layer) || !kv_batch_ok(a->batch) || a->reserved != 0) return false;
+    if (static_cast<uint64_t>(a->batch.table_pages) * a->layer.page_tokens > (1u << kMaxTokensLog2)) return false;
     if (!shape_ok(a->query_heads, a->layer.kv_heads, a->layer.head_dim, a->max_new_tokens) || !std::isfinite(a->scale)) return false;
     const uint64_t bytes = static_cast<uint64_t>(a->batch.rows) * a->query_heads * a->layer.head_dim * 2;
     if (a->query_len_bytes != bytes || a->output_len_bytes != bytes) return false;
@@ -108,6 +706,12 @@ bool check_attention(int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm
 }
 
 }  // namespace
+
+cudaError_t attention_configure_device() {
+    const cudaError_t e = configure<128>();
+    return e == cudaSuccess ? configure<256>() : e;
+}
+
 }  // namespace augur_sm100
 
 using namespace augur_sm100;
@@ -115,7 +719,9 @@ using namespace augur_sm100;
 extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_paged_attention_scratch_extent_host_v1(
     uint32_t query_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_new_tokens, uint32_t sm_count, uint64_t* out_bytes) {
     if (!out_bytes || !shape_ok(query_heads, kv_heads, head_dim, max_new_tokens) || !sm_count || sm_count > 4096) return invalid();
-    *out_bytes = kCounterBytes;
+    // the counter regions of the plan's scratch stay as they are; behind them the records and the parts
+    const uint64_t spans = launch_spans(sm_count), columns = query_columns(query_heads, kv_heads, max_new_tokens);
+    *out_bytes = kCounterBytes + spans * sizeof(JoinRecord) + 2 * spans * columns * (head_dim + 2) * sizeof(float);
     return ok();
 }
 
@@ -134,8 +740,6 @@ extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_paged_att
     if (e != cudaSuccess) return make_result(AUGUR_CUDA_STATUS_RUNTIME_FAILURE, e);
     AttentionParams p{};
     p.query = reinterpret_cast<const __nv_bfloat16*>(a->query);
-    p.keys = reinterpret_cast<const __nv_bfloat16*>(a->layer.keys);
-    p.values = reinterpret_cast<const __nv_bfloat16*>(a->layer.values);
     p.output = reinterpret_cast<__nv_bfloat16*>(a->output);
     p.page_table = reinterpret_cast<const int32_t*>(a->batch.page_table);
     p.lengths = reinterpret_cast<const int32_t*>(a->batch.lengths);
@@ -143,13 +747,19 @@ extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_paged_att
     p.status_word = plan->status_word;
     p.rows = a->batch.rows, p.sequences = a->batch.sequences, p.table_pages = a->batch.table_pages, p.pages = a->layer.pages;
     p.query_heads = a->query_heads, p.kv_heads = a->layer.kv_heads, p.page_shift = static_cast<uint32_t>(__builtin_ctz(a->layer.page_tokens));
-    p.max_new = a->max_new_tokens;
+    p.max_new = a->max_new_tokens, p.spans = launch_spans(plan->sm_count);
     p.scale_log2 = a->scale * 1.4426950408889634f;
-    if (a->layer.head_dim == 256) {
-        launch_dependent(s->stream, attention_simple_kernel<256>, p.rows * p.query_heads, 256, 0, p);
-    } else {
-        launch_dependent(s->stream, attention_simple_kernel<128>, p.rows * p.query_heads, 256, 0, p);
+    p.records = reinterpret_cast<JoinRecord*>(plan->scratch + kCounterBytes);
+    p.parts = reinterpret_cast<float*>(p.records + p.spans);
+    const uint32_t head_dim = a->layer.head_dim, box = a->layer.page_tokens < kUnit ? a->layer.page_tokens : kUnit;
+    const uint64_t cache_rows = static_cast<uint64_t>(a->layer.pages) * a->layer.kv_heads * a->layer.page_tokens;
+    CUtensorMap keys, values;   // rows of head_dim * 2 bytes, as a map of packed codes with four times the columns
+    if (!make_code_map(&keys, a->layer.keys, cache_rows, head_dim * 4, box) || !make_code_map(&values, a->layer.values, cache_rows, head_dim * 4, box)) {
+        return make_result(AUGUR_CUDA_STATUS_RUNTIME_FAILURE);
     }
-    count_launch();
+    const uint32_t columns = query_columns(a->query_heads, a->layer.kv_heads, a->max_new_tokens);
+    auto launch = head_dim == 256 ? (columns == 16 ? launch_attention<256, 16> : columns == 32 ? launch_attention<256, 32> : columns == 48 ? launch_attention<256, 48> : launch_attention<256, 64>)
+                                  : (columns == 16 ? launch_attention<128, 16> : columns == 32 ? launch_attention<128, 32> : columns == 48 ? launch_attention<128, 48> : launch_attention<128, 64>);
+    launch(s->stream, keys, values, p);
     return submitted();
 }
