@@ -155,6 +155,7 @@ cudaError_t gemv_tc_configure_device();
 cudaError_t gemm_narrow_configure_device();
 cudaError_t gemv_split_configure_device();
 cudaError_t attention_configure_device();
+cudaError_t logprobs_configure_device();
 // Clusters of `parts` CTAs of 384 threads and 112 KB of shared memory (two per SM) that a launch may count on to run at once.
 uint32_t two_cta_clusters(int32_t ordinal, uint32_t parts);
 // CTAs per 128-row tile of a small-token linear on tensor memory (a cluster) where `clusters[parts]` clusters of `parts` run at once.
