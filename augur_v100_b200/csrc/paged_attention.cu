@@ -27,16 +27,17 @@ using namespace tc;
 static_assert(sizeof(augur_cuda_nvfp4_sm100_paged_attention_args_v1) == 160, "attention ABI");
 
 constexpr uint32_t kMaxQueries = 64;   // new tokens x query heads of a key-value head
-constexpr uint32_t kMaxCtas = 256;     // spans that a launch deals out
+constexpr uint32_t kMaxCtas = 256;     // spans that a launch deals out (the join has a thread for each)
 constexpr uint32_t kUnit = 64;         // tokens of a unit of work
 constexpr uint32_t kTile = 128;        // tokens of an MMA tile
 constexpr uint32_t kSlotBytes = kTile * 128;   // 64 dims of a tile
 constexpr uint32_t kMaxSequences = AUGUR_NVFP4_SM100_MAX_SEQUENCES;
+constexpr uint32_t kOnesBytes = kTile * 32;    // 16 k of ones, as the 128-row operand
 constexpr uint32_t kMaxTokensLog2 = 24;   // of a sequence
 constexpr float kSlack = 8.0f;            // how far, in powers of two, a score may pass the reference maximum
 constexpr uint32_t kStatusPage = 0x401, kStatusRows = 0x402;
 constexpr uint32_t kStatusLoad = 0x411, kStatusMma = 0x412, kStatusScores = 0x413, kStatusValues = 0x414, kStatusQuery = 0x415, kStatusGroup = 0x416, kStatusProduct = 0x417;
-constexpr uint32_t kThreads = 256;        // warp 0 loads, 1 MMA, 2 and 3 queries, 4..7 softmax
+constexpr uint32_t kThreads = 256;        // warp 0 loads keys, 1 MMA, 2 queries, 3 values, 4..7 softmax
 constexpr uint32_t kSmemLimit = 227 * 1024;
 constexpr uint32_t kInfos = 8;            // tiles that the loader is ahead of the softmax at most, rounded up
 
@@ -60,13 +61,13 @@ struct JoinRecord {
 // Small state of a CTA, behind the ring, the queries and the weights.
 struct State {
     uint64_t full[16], empty[16];
-    uint64_t scores_full[2], scores_empty[2], weights_full[2], weights_empty[2], query_full[2], query_empty[2], group;
+    uint64_t scores_full[2], scores_empty[2], weights_full[2], weights_empty[2], query_full[2], query_empty[2], group, keys_first;
     uint32_t tmem, abort[1 + kThreads / 32];
     uint32_t needs[2];                 // a byte per softmax warp: a reference has to move
     uint32_t info[kInfos];             // of a tile: pages that are there, a bit per box; bit 31: the last tile
     uint32_t scan[kThreads / 32];
     float reference[kMaxQueries], factor[kMaxQueries];
-    float wide[4][kMaxQueries];        // a value per softmax warp and query
+    float4 wide[kMaxQueries];          // the largest score per query and softmax warp
     int32_t limit[kMaxQueries];        // keys that a query sees
     uint32_t units[kMaxSequences + 1]; // before sequence b, of one head
     uint32_t length[kMaxSequences];    // | new tokens << 25
@@ -77,37 +78,38 @@ struct Shape {
     static constexpr uint32_t kChunks = kHeadDim / 64, kHalves = kHeadDim / 128;
     static constexpr uint32_t kQueryBytes = kN * kHeadDim * 2, kQueryBuffers = kQueryBytes > 24 * 1024 ? 1 : 2;
     static constexpr uint32_t kWeightBytes = kN * kTile * 2;
-    static constexpr uint32_t kRoom = kSmemLimit - 1024 - sizeof(State) - kQueryBuffers * kQueryBytes - 2 * kWeightBytes;
+    static constexpr uint32_t kFixed = 1024 + kOnesBytes + sizeof(State) + kQueryBuffers * kQueryBytes + 2 * kWeightBytes;
+    static constexpr uint32_t kRoom = kSmemLimit - kFixed;
     static constexpr uint32_t kSlots = kRoom / kSlotBytes / 2 * 2 > 16 ? 16 : kRoom / kSlotBytes / 2 * 2;
-    static constexpr uint32_t kSmem = 1024 + kSlots * kSlotBytes + kQueryBuffers * kQueryBytes + 2 * kWeightBytes + sizeof(State);
-    static constexpr uint32_t kColumns = (2 + kHalves) * kN, kTmem = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : 256;
-    static_assert(kSlots >= 2 * kChunks && kSmem <= kSmemLimit && kColumns <= 256, "a CTA's memory");
+    static constexpr uint32_t kSmem = kFixed + kSlots * kSlotBytes;
+    // tensor memory: two of S^T, O^T in halves of 128 dims, the denominators
+    static constexpr uint32_t kColumns = (3 + kHalves) * kN, kTmem = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
+    static_assert(kSlots >= 2 * kChunks && kSmem <= kSmemLimit && kColumns <= 512, "a CTA's memory");
 };
 
 // A CTA's way through its span: one (sequence, head) after the other, in each the keys [key, key_end).
 struct Walk {
-    uint64_t unit, end;
-    uint32_t sequence, head, key, key_end, length, tokens;
+    uint32_t unit, end, sequence, head, key, key_end, length, tokens;
     bool starts, ends;   // the pair's first and last key are in the span
 
-    __device__ void open(const State* st, const AttentionParams& p, uint64_t from, uint64_t to) {
+    __device__ void open(const State* st, const AttentionParams& p, uint32_t from, uint32_t to) {
         unit = from, end = to;
         uint32_t low = 0, high = p.sequences;   // the last sequence whose units start at or before `from`
         while (high - low > 1) {
             const uint32_t middle = (low + high) / 2;
-            if (static_cast<uint64_t>(st->units[middle]) * p.kv_heads <= from) low = middle;
+            if (st->units[middle] * p.kv_heads <= from) low = middle;
             else high = middle;
         }
         sequence = low;
     }
     __device__ bool next(const State* st, const AttentionParams& p) {
         if (unit >= end) return false;
-        while (unit >= static_cast<uint64_t>(st->units[sequence + 1]) * p.kv_heads) ++sequence;
+        while (unit >= st->units[sequence + 1] * p.kv_heads) ++sequence;
         const uint32_t count = st->units[sequence + 1] - st->units[sequence];
-        const uint32_t at = static_cast<uint32_t>(unit - static_cast<uint64_t>(st->units[sequence]) * p.kv_heads);
+        const uint32_t at = unit - st->units[sequence] * p.kv_heads;
         head = at / count;
         const uint32_t first = at - head * count;
-        const uint32_t take = static_cast<uint32_t>(end - unit < count - first ? end - unit : count - first);
+        const uint32_t take = end - unit < count - first ? end - unit : count - first;
         length = st->length[sequence] & ((1u << (kMaxTokensLog2 + 1)) - 1), tokens = st->length[sequence] >> (kMaxTokensLog2 + 1);
         starts = first == 0, ends = first + take == count;
         key = first * kUnit;
@@ -122,7 +124,7 @@ struct Tiles {
     Walk walk;
     uint32_t key;
     bool valid;
-    __device__ void open(const State* st, const AttentionParams& p, uint64_t from, uint64_t to) {
+    __device__ void open(const State* st, const AttentionParams& p, uint32_t from, uint32_t to) {
         walk.open(st, p, from, to);
         seek(st, p);
     }
@@ -145,6 +147,10 @@ __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uin
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
                  : "memory");
+}
+// The ones as the 128-row operand, without swizzle: 8 rows x 16 bytes are 128 bytes, the next 8 k 128 bytes further, the next 8 rows 256.
+__device__ __forceinline__ uint64_t ones_desc(uint32_t smem_addr) {
+    return static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4) | (uint64_t(128 >> 4) << 16) | (uint64_t(256 >> 4) << 32) | (uint64_t(1) << 46);
 }
 // V as the 128-row operand: 128-byte rows of 64 dims, one per key, so the rows are the k dimension; 8 keys are 1024 bytes, the next 64 dims
 // lie one ring slot further.
@@ -184,7 +190,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* const query_smem = smem + S::kSlots * kSlotBytes;
     uint8_t* const weight_smem = query_smem + S::kQueryBuffers * S::kQueryBytes;
-    State* const st = reinterpret_cast<State*>(weight_smem + 2 * S::kWeightBytes);
+    uint8_t* const ones_smem = weight_smem + 2 * S::kWeightBytes;
+    State* const st = reinterpret_cast<State*>(ones_smem + kOnesBytes);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full = smem_u32(st->full), empty = smem_u32(st->empty), scores_full = smem_u32(st->scores_full), scores_empty = smem_u32(st->scores_empty);
     const uint32_t weights_full = smem_u32(st->weights_full), weights_empty = smem_u32(st->weights_empty);
@@ -197,9 +204,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
         for (uint32_t b = 0; b < 2; ++b) {
             mbar_init(scores_full + 8 * b, 1), mbar_init(scores_empty + 8 * b, 4);
             mbar_init(weights_full + 8 * b, 4), mbar_init(weights_empty + 8 * b, 1);
-            mbar_init(query_full + 8 * b, 2), mbar_init(query_empty + 8 * b, 1);
+            mbar_init(query_full + 8 * b, 1), mbar_init(query_empty + 8 * b, 1);
         }
-        mbar_init(group_bar, 4);
+        mbar_init(group_bar, 4), mbar_init(smem_u32(&st->keys_first), 1);
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_keys) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_values) : "memory");
         for (uint32_t i = 0; i < 1 + kThreads / 32; ++i) st->abort[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -207,6 +216,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&st->tmem)), "r"(S::kTmem) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    for (uint32_t i = threadIdx.x; i < kOnesBytes / 16; i += kThreads) reinterpret_cast<uint4*>(ones_smem)[i] = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     // Everything above runs while the launch before this one drains; from here on its results are read.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     {   // units of every sequence, and their running sum: four neighbouring sequences a thread
@@ -255,71 +266,67 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
         }
         __syncthreads();
     }
-    const uint64_t total = static_cast<uint64_t>(st->units[p.sequences]) * p.kv_heads;
-    const uint32_t spans = total < p.spans ? static_cast<uint32_t>(total) : p.spans;
-    const uint64_t from = blockIdx.x < spans ? total * blockIdx.x / spans : 0, to = blockIdx.x < spans ? total * (blockIdx.x + 1) / spans : 0;
-    const uint32_t tmem = st->tmem, tmem_out = tmem + 2 * kN;
+    const uint32_t total = st->units[p.sequences] * p.kv_heads, spans = total < p.spans ? total : p.spans;
+    const uint32_t base = spans ? total / spans : 0, extra = total - base * spans;   // spans of `base` units, the first `extra` of one more
+    const uint32_t from = blockIdx.x * base + (blockIdx.x < extra ? blockIdx.x : extra), to = blockIdx.x < spans ? from + base + (blockIdx.x < extra ? 1 : 0) : from;
+    const uint32_t tmem = st->tmem, tmem_out = tmem + 2 * kN, tmem_sum = tmem_out + S::kHalves * kN;   // (one behind the other: scaled together)
     const uint32_t group = p.query_heads / p.kv_heads;
 
-    if (warp == 0) {
-        // ---------------- pages: K of a tile, then V of the tile before it ----------------
+    if (warp == 0 || warp == 3) {
+        // ---------------- pages: warp 0 the keys, warp 3 the values ----------------
+        // The ring's slots go round in the order of their use: K of tile 0, then K of tile t and V of tile t - 1, and V of the last.
         const uint32_t box_shift = p.page_shift < 6 ? p.page_shift : 6, boxes = kTile >> box_shift, box_bytes = 128u << box_shift;
+        const CUtensorMap* const map = warp == 0 ? &map_keys : &map_values;
         Tiles tiles;
         tiles.open(st, p, from, to);
-        uint32_t slot = 0, phase = 1, count = 0, row_before = 0, mask_before = 0;
         bool alive = true;
-        // the row of the cache where this lane's box of the tile starts, and which lanes have one
-        auto look = [&](const Tiles& t, uint32_t* row, uint32_t* mask) {
-            const uint32_t key = t.key + (lane << box_shift);
+        // The first tile's keys go before its values: the scores can be worked on while the values come.
+        const uint32_t keys_first = smem_u32(&st->keys_first);
+        if (warp == 3 && tiles.valid) alive = warp_look_wait(keys_first, 0, abort_flag, status, kStatusLoad);
+        for (uint32_t tile = 0; alive && tiles.valid; ++tile) {
+            // the row of the cache where this lane's box of the tile starts, and which lanes have one
+            const uint32_t key = tiles.key + (lane << box_shift);
+            uint32_t row = 0;
             bool there = false;
-            *row = 0;
-            if (lane < boxes && t.valid && key < t.walk.key_end) {
-                const int32_t page = __ldg(p.page_table + static_cast<uint64_t>(t.walk.sequence) * p.table_pages + (key >> p.page_shift));
+            if (lane < boxes && key < tiles.walk.key_end) {
+                const int32_t page = __ldg(p.page_table + static_cast<uint64_t>(tiles.walk.sequence) * p.table_pages + (key >> p.page_shift));
                 there = page >= 0 && static_cast<uint32_t>(page) < p.pages;
-                if (there) *row = (((static_cast<uint32_t>(page) * p.kv_heads) + t.walk.head) << p.page_shift) + (key & ((1u << p.page_shift) - 1));
+                if (there) row = ((static_cast<uint32_t>(page) * p.kv_heads + tiles.walk.head) << p.page_shift) + (key & ((1u << p.page_shift) - 1));
                 else atomicCAS(status, 0u, kStatusPage);
             }
-            *mask = __ballot_sync(0xffffffffu, there);
-        };
-        auto load = [&](const CUtensorMap* map, uint32_t row, uint32_t mask) {
-            for (uint32_t c = 0; alive && c < S::kChunks; ++c) {
+            const uint32_t mask = __ballot_sync(0xffffffffu, there);
+            tiles.advance(st, p);
+            uint32_t at = 2 * S::kChunks * tile;   // among all slots that are loaded
+            if (warp == 0) {
+                if (tile) at -= S::kChunks;
+                if (lane == 0) st->info[tile % kInfos] = mask | (tiles.valid ? 0 : 0x80000000u);
+            } else {
+                at += tiles.valid ? 2 * S::kChunks : S::kChunks;
+            }
+            uint32_t slot = at % S::kSlots, phase = at / S::kSlots & 1 ^ 1;
+            for (uint32_t c = 0; c < S::kChunks; ++c) {
                 if (!warp_look_wait(empty + 8 * slot, phase, abort_flag, status, kStatusLoad)) {
                     alive = false;
                     break;
                 }
+                const uint32_t bar = full + 8 * slot;
                 if (lane == 0) {
-                    if (mask) mbar_expect_tx(full + 8 * slot, __popc(mask) * box_bytes);
-                    else mbar_arrive(full + 8 * slot);
+                    if (mask) mbar_expect_tx(bar, __popc(mask) * box_bytes);
+                    else mbar_arrive(bar);
                 }
                 __syncwarp();
-                if (mask >> lane & 1) tma_load_2d(smem_u32(smem + slot * kSlotBytes) + lane * box_bytes, map, c * 128, row, full + 8 * slot);
+                if (there) tma_load_2d(smem_u32(smem) + slot * kSlotBytes + lane * box_bytes, map, c * 128, row, bar);
                 __syncwarp();
                 if (++slot == S::kSlots) slot = 0, phase ^= 1;
             }
-        };
-        uint32_t row, mask;
-        look(tiles, &row, &mask);
-        while (alive && (tiles.valid || count)) {
-            const bool has_keys = tiles.valid;
-            uint32_t row_next = 0, mask_next = 0;
-            if (has_keys) {
-                tiles.advance(st, p);
-                look(tiles, &row_next, &mask_next);   // ahead of its use by a tile
-                if (lane == 0) st->info[count % kInfos] = mask | (tiles.valid ? 0 : 0x80000000u);
-                load(&map_keys, row, mask);
-            }
-            if (count) load(&map_values, row_before, mask_before);
-            if (!has_keys) break;
-            row_before = row, mask_before = mask;
-            row = row_next, mask = mask_next;
-            ++count;
+            if (warp == 0 && tile == 0 && lane == 0) mbar_arrive(keys_first);
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer: S of a tile, then O of the tile before it ----------------
         constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kN >> 3) << 17) | ((kTile >> 4) << 24);   // F32 += BF16 x BF16
         constexpr uint32_t idesc_values = idesc | (1u << 15);                                                        // V is MN-major
         const uint64_t slots = operand_desc(smem_u32(smem)), slots_values = value_desc(smem_u32(smem));
-        const uint64_t queries = operand_desc(smem_u32(query_smem)), weights = operand_desc(smem_u32(weight_smem));
+        const uint64_t queries = operand_desc(smem_u32(query_smem)), weights = operand_desc(smem_u32(weight_smem)), ones = ones_desc(smem_u32(ones_smem));
         Tiles ahead, now;
         ahead.open(st, p, from, to);
         now = ahead;
@@ -356,6 +363,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             if (ahead.valid && !scores_of_tile()) break;
             const uint32_t buffer = products & 1, steps = (now.keys() + 15) / 16;
             if (!warp_look_wait(weights_full + 8 * buffer, products >> 1 & 1, abort_flag, status, kStatusProduct)) break;
+            tc_fence_after();
+            if (elect_one()) {   // denominators: the sum over the keys as one more product, into every lane
+                const uint64_t b = weights + ((buffer * S::kWeightBytes) >> 4);
+                for (uint32_t k = 0; k < steps; ++k) mma_bf16(tmem_sum, ones, b + (k >> 2) * (kN * 128 >> 4) + (k & 3) * 2, idesc, !now.first() || k);
+            }
+            __syncwarp();
             for (uint32_t h = 0; alive && h < S::kHalves; ++h) {
                 for (uint32_t c = 0; c < 2; ++c) alive = alive && warp_look_wait(full + 8 * (slot + c), phase, abort_flag, status, kStatusProduct);
                 if (!alive) break;
@@ -378,9 +391,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             ++products;
             now.advance(st, p);
         }
-    } else if (warp < 4) {
+    } else if (warp == 2) {
         // ---------------- queries of a pair, in the 128-byte swizzle of the operand; rows past the last are zero ----------------
-        const uint32_t thread = threadIdx.x - 64;
         Walk walk;
         walk.open(st, p, from, to);
         uint32_t pair = 0;
@@ -389,17 +401,19 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             const uint32_t buffer = S::kQueryBuffers == 2 ? pair & 1 : 0;
             const uint32_t first_row = static_cast<uint32_t>(__ldg(p.token_starts + walk.sequence)), queries = walk.tokens * group;
             if (!warp_look_wait(query_empty + 8 * buffer, ((S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1) ^ 1, abort_flag, status, kStatusQuery)) break;
-            constexpr uint32_t kPieces = kHeadDim / 8;
-            for (uint32_t i = thread; i < kN * kPieces; i += 64) {
-                const uint32_t row = i / kPieces, piece = i % kPieces;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (row < queries) {
-                    const uint32_t token = row / group;
-                    const uint64_t at = (static_cast<uint64_t>(first_row + token) * p.query_heads + walk.head * group + (row - token * group)) * kHeadDim;
-                    v = __ldg(reinterpret_cast<const uint4*>(p.query + at) + piece);
-                }
-                *reinterpret_cast<uint4*>(query_smem + buffer * S::kQueryBytes + (piece >> 3) * (kN * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = v;
+            // 16 bytes a copy, all of them under way together (as loads and stores they waited for one another: 1000 cycles a row)
+            constexpr uint32_t kPieces = kHeadDim / 8, kRows = 32 / kPieces;
+            const uint32_t piece = lane % kPieces, to = smem_u32(query_smem) + buffer * S::kQueryBytes + (piece >> 3) * (kN * 128);
+            const __nv_bfloat16* const from_here = p.query + (static_cast<uint64_t>(first_row) * p.query_heads + walk.head * group) * kHeadDim + piece * 8;
+            uint32_t token = 0, head = lane / kPieces;
+            for (uint32_t row = lane / kPieces; row < kN; row += kRows, head += kRows) {
+                while (head >= group) head -= group, ++token;
+                const bool live = row < queries;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + row * 128 + (((piece & 7) ^ (row & 7)) << 4)),
+                             "l"(live ? from_here + (static_cast<uint64_t>(token) * p.query_heads + head) * kHeadDim : p.query), "r"(live ? 16 : 0)
+                             : "memory");
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(query_full + 8 * buffer);
@@ -428,9 +442,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                 st->limit[thread] = thread < queries ? static_cast<int32_t>(walk.length) - static_cast<int32_t>(walk.tokens) + static_cast<int32_t>(thread / group) + 1 : 0;
             }
             if (!meet()) break;
-            float sum[kN];
-#pragma unroll
-            for (uint32_t c = 0; c < kN; ++c) sum[c] = 0.0f;
             const int32_t seen_by_all = static_cast<int32_t>(walk.length) - static_cast<int32_t>(walk.tokens) + 1;
             for (uint32_t key = walk.key; key < walk.key_end; key += kTile, ++tile) {
                 const uint32_t buffer = tile & 1;
@@ -439,38 +450,55 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                     break;
                 }
                 tc_fence_after();
-                float s[kN];
-#pragma unroll
-                for (uint32_t c = 0; c < kN; c += 16) load_columns16(tmem + lanes + buffer * kN + c, reinterpret_cast<uint32_t*>(s) + c);
-                tc_wait_ld();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(scores_empty + 8 * buffer);
                 const uint32_t info = st->info[tile % kInfos], there = info & 0x7fffffffu;
                 const uint32_t count = walk.key_end - key < kTile ? walk.key_end - key : kTile;
-                const bool whole = count == kTile && there == all_boxes;
+                const bool whole = count == kTile && there == all_boxes, masked = !whole || static_cast<int32_t>(key + kTile) > seen_by_all;
                 const bool my_key = thread < count && (there >> (thread >> box_shift) & 1);
+                // 16 queries' scores of this thread's key. Every step below goes through them again from tensor memory in a rolled loop: with all of 48
+                // queries in registers and the loops unrolled, a tile cost 4200 cycles more, for want of instructions from their cache.
+                float s[16];
+                auto scores = [&](uint32_t c0) {
+                    if (kN == 16 && c0 != 0) return;   // (there already)
+                    load_columns16(tmem + lanes + buffer * kN + c0 % kN, reinterpret_cast<uint32_t*>(s));
+                    tc_wait_ld();
 #pragma unroll
-                for (uint32_t c = 0; c < kN; ++c) s[c] *= p.scale_log2;
-                if (!whole || static_cast<int32_t>(key + kTile) > seen_by_all) {
+                    for (uint32_t i = 0; i < 16; ++i) s[i] *= p.scale_log2;
+                    if (masked) {
 #pragma unroll
-                    for (uint32_t c = 0; c < kN; ++c) s[c] = my_key && static_cast<int32_t>(key + thread) < st->limit[c] ? s[c] : -INFINITY;
+                        for (uint32_t i = 0; i < 16; ++i) s[i] = my_key && static_cast<int32_t>(key + thread) < st->limit[c0 % kN + i] ? s[i] : -INFINITY;
+                    }
+                };
+                constexpr uint32_t kAgain = kN == 16 ? kN : 0;   // for 16 queries they stay in registers
+                bool above = key == walk.key;   // a pair's first tile sets the references
+                if (!above) {
+#pragma unroll 1
+                    for (uint32_t c = 0; c < kN; c += 16) {
+                        scores(c);
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) above |= s[i] > st->reference[c + i] + kSlack;
+                    }
+                    above = __any_sync(0xffffffffu, above);
+                    if (lane == 0) reinterpret_cast<uint8_t*>(&st->needs[buffer])[quadrant] = above;
+                    if (!meet()) {
+                        alive = false;
+                        break;
+                    }
+                    above = *const_cast<volatile uint32_t*>(&st->needs[buffer]) != 0;
+                } else {
+                    scores(0);
                 }
-                bool above = false;
+                if (above) {
+                    // The references move up to the largest scores so far.
+#pragma unroll 1
+                    for (uint32_t c = 0; c < kN; c += 16) {
+                        scores(c + kAgain);
+                        float most = -INFINITY;
 #pragma unroll
-                for (uint32_t c = 0; c < kN; ++c) above |= s[c] > st->reference[c] + kSlack;
-                above = __any_sync(0xffffffffu, above);
-                if (lane == 0) reinterpret_cast<uint8_t*>(&st->needs[buffer])[quadrant] = above;
-                if (!meet()) {
-                    alive = false;
-                    break;
-                }
-                if (*const_cast<volatile uint32_t*>(&st->needs[buffer])) {
-                    // A reference moves up to the largest score so far, for all queries.
-#pragma unroll
-                    for (uint32_t c = 0; c < kN; ++c) {
-                        const float most = warp_max(s[c]);
-                        if (lane == (c & 31)) st->wide[quadrant][c] = most;
+                        for (uint32_t i = 0; i < 16; ++i) {
+                            const float x = warp_max(s[i]);
+                            if (lane == i) most = x;
+                        }
+                        if (lane < 16) reinterpret_cast<float*>(&st->wide[c + lane])[quadrant] = most;
                     }
                     if (!meet()) {
                         alive = false;
@@ -478,28 +506,28 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                     }
                     if (thread < kN) {
                         const float old = st->reference[thread];
-                        const float most = fmaxf(fmaxf(fmaxf(st->wide[0][thread], st->wide[1][thread]), fmaxf(st->wide[2][thread], st->wide[3][thread])), old);
-                        st->factor[thread] = most == old ? 1.0f : exp2_fast(old - most);
-                        st->reference[thread] = most;
+                        const float4 w = st->wide[thread];
+                        const float now = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), old);
+                        st->factor[thread] = now == old ? 1.0f : exp2_fast(old - now);
+                        st->reference[thread] = now;
                     }
                     if (!meet()) {
                         alive = false;
                         break;
                     }
-#pragma unroll
-                    for (uint32_t c = 0; c < kN; ++c) sum[c] *= st->factor[c];
                     if (key != walk.key) {
                         if (!warp_look_wait(weights_empty + 8 * (buffer ^ 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) {
                             alive = false;
                             break;
                         }
                         tc_fence_after();
-                        for (uint32_t c = 0; c < S::kHalves * kN; c += 16) {
+#pragma unroll 1
+                        for (uint32_t c = 0; c < (S::kHalves + 1) * kN; c += 16) {
                             uint32_t v[16];
                             load_columns16(tmem_out + lanes + c, v);
                             tc_wait_ld();
 #pragma unroll
-                            for (uint32_t i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * st->factor[(c + i) % kN]);
+                            for (uint32_t i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * st->factor[c % kN + i]);
                             store_columns16(tmem_out + lanes + c, v);
                         }
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -512,13 +540,22 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                 }
                 uint8_t* const to_weights = weight_smem + buffer * S::kWeightBytes + (thread >> 6) * (kN * 128) + (thread & 7) * 2;
                 const uint32_t unit = (thread & 63) >> 3;
+#pragma unroll 1
+                for (uint32_t c = 0; c < kN; c += 16) {
+                    scores(c + kAgain);
+                    float power[16];   // all references before the first store, which the compiler would not move them across
 #pragma unroll
-                for (uint32_t c = 0; c < kN; ++c) {
-                    const float reference = st->reference[c];
-                    const __nv_bfloat16 weight = __float2bfloat16_rn(exp2_fast(s[c] - (reference == -INFINITY ? 0.0f : reference)));
-                    sum[c] += __bfloat162float(weight);
-                    *reinterpret_cast<__nv_bfloat16*>(to_weights + c * 128 + ((unit ^ (c & 7)) << 4)) = weight;
+                    for (uint32_t i = 0; i < 16; ++i) power[i] = st->reference[c + i];
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) power[i] = exp2_fast(s[i] - (power[i] == -INFINITY ? 0.0f : power[i]));
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) {
+                        *reinterpret_cast<__nv_bfloat16*>(to_weights + (c + i) * 128 + ((unit ^ (i & 7)) << 4)) = __float2bfloat16_rn(power[i]);
+                    }
                 }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(scores_empty + 8 * buffer);
                 if (!whole) {
                     // Rows of V that are no token's are multiplied with weights of zero: whatever lies there, they must be numbers.
                     const uint32_t at = 2 * S::kChunks * (tile + 1) - (info >> 31 ? S::kChunks : 0);   // the tile's V among all slots that were loaded
@@ -544,59 +581,55 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             if (!alive) break;
             // ---- the pair's output, or its part ----
             const bool any = walk.key < walk.key_end;
-#pragma unroll
-            for (uint32_t c = 0; c < kN; ++c) {
-#pragma unroll
-                for (uint32_t step = 16; step; step /= 2) sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], step);
-                if (lane == (c & 31)) st->wide[quadrant][c] = sum[c];
-            }
-            if (!meet()) break;
             if (any) {
                 if (!warp_look_wait(weights_empty + 8 * ((tile - 1) & 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) break;
                 tc_fence_after();
             }
             const bool alone = walk.starts && walk.ends;
             const uint32_t part = 2 * blockIdx.x + (walk.starts ? 1 : 0);
-            float* const part_out = p.parts + static_cast<uint64_t>(part) * kN * kHeadDim;
-            for (uint32_t h = 0; h < S::kHalves; ++h) {
-                for (uint32_t c0 = 0; c0 < kN && c0 < queries; c0 += 16) {
-                    uint32_t v[16];
-                    if (any) {
-                        load_columns16(tmem_out + lanes + h * kN + c0, v);
-                        tc_wait_ld();
-                    }
+            float* const part_out = p.parts + static_cast<uint64_t>(part) * kN * kHeadDim + thread;
+            __nv_bfloat16* const out = p.output + (static_cast<uint64_t>(first_row) * p.query_heads + walk.head * group) * kHeadDim + thread;
+            const uint32_t next_token = (p.query_heads - group) * kHeadDim;   // from behind a token's queries to the next token's
+            float2* const stats = reinterpret_cast<float2*>(p.parts + static_cast<uint64_t>(2 * p.spans) * kN * kHeadDim) + part * kN;
+            uint32_t token_end = group;
+            uint64_t skipped = 0;
+#pragma unroll 1
+            for (uint32_t c0 = 0; c0 < queries; c0 += 16) {
+                uint32_t v[S::kHalves][16], sums[16];
+                if (any) {
+                    load_columns16(tmem_sum + lanes + c0, sums);
 #pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) {
-                        const uint32_t c = c0 + i;
-                        if (c < queries) {
-                            if (alone) {
-                                const uint32_t token = c / group;
-                                const float all = (st->wide[0][c] + st->wide[1][c]) + (st->wide[2][c] + st->wide[3][c]);
-                                const float value = !any || all == 0.0f ? 0.0f : __uint_as_float(v[i]) / all;
-                                p.output[(static_cast<uint64_t>(first_row + token) * p.query_heads + walk.head * group + (c - token * group)) * kHeadDim + h * 128 + thread] =
-                                    __float2bfloat16_rn(value);
-                            } else {
-                                part_out[static_cast<uint64_t>(c) * kHeadDim + h * 128 + thread] = __uint_as_float(v[i]);
-                            }
+                    for (uint32_t h = 0; h < S::kHalves; ++h) load_columns16(tmem_out + lanes + h * kN + c0, v[h]);
+                    tc_wait_ld();
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 16; ++i) {
+                    const uint32_t c = c0 + i;
+                    if (c >= queries) break;
+                    const float all = any ? __uint_as_float(sums[i]) : 0.0f;
+                    if (alone) {
+                        if (c == token_end) token_end += group, skipped += next_token;
+                        const float scale = 1.0f / all;
+#pragma unroll
+                        for (uint32_t h = 0; h < S::kHalves; ++h) {
+                            out[skipped + c * kHeadDim + h * 128] = __float2bfloat16_rn(all == 0.0f ? 0.0f : __uint_as_float(v[h][i]) * scale);
                         }
+                    } else {
+#pragma unroll
+                        for (uint32_t h = 0; h < S::kHalves; ++h) part_out[c * kHeadDim + h * 128] = __uint_as_float(v[h][i]);
+                        if (thread == c) stats[c] = make_float2(st->reference[c], all);
                     }
                 }
             }
             if (any) tc_fence_before();
             if (!alone) {
-                if (thread < queries) {
-                    float* const stats = p.parts + static_cast<uint64_t>(2 * p.spans) * kN * kHeadDim + (static_cast<uint64_t>(part) * kN + thread) * 2;
-                    stats[0] = st->reference[thread];
-                    stats[1] = (st->wide[0][thread] + st->wide[1][thread]) + (st->wide[2][thread] + st->wide[3][thread]);
-                }
                 if (walk.starts) {
-                    const uint64_t units = st->units[walk.sequence + 1] - st->units[walk.sequence];
-                    const uint64_t last = static_cast<uint64_t>(st->units[walk.sequence]) * p.kv_heads + (walk.head + 1) * units;   // one past its last unit
+                    const uint32_t units = st->units[walk.sequence + 1] - st->units[walk.sequence], longer = extra * (base + 1);
+                    const uint32_t last = st->units[walk.sequence] * p.kv_heads + (walk.head + 1) * units - 1;   // the pair's last unit
                     record.row = static_cast<uint32_t>(first_row), record.tokens = walk.tokens, record.head = walk.head;
-                    record.last = static_cast<uint32_t>((last * spans - 1) / total);
+                    record.last = last < longer ? last / (base + 1) : extra + (last - longer) / base;
                 }
             }
-            if (!meet()) break;   // before the next pair's state overwrites what the others still read
         }
         if (thread == 0) p.records[blockIdx.x] = record;
     }
@@ -608,46 +641,79 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
     }
 }
 
-// Joins the parts of one pair, in the order of their spans: four outputs a thread, blockIdx.y = which of the pair's queries.
-constexpr uint32_t kJoinThreads = 256;
+// Joins the parts of one pair, in the order of their spans. A CTA takes queries blockIdx.y, blockIdx.y + gridDim.y, ...; four outputs a
+// thread, and the threads of a query's outputs as many times over as there are, each with every so many-th part.
+constexpr uint32_t kJoinThreads = 256, kJoinRows = 8;
 template <uint32_t kHeadDim, uint32_t kN>
-__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttentionParams p) {
-    constexpr uint32_t kLanes = kHeadDim / 4, kQueries = kJoinThreads / kLanes;
-    __shared__ float weight[kQueries][kMaxCtas];
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttentionParams p) {
+    constexpr uint32_t kLanes = kHeadDim / 4, kShares = kJoinThreads / kLanes;
+    __shared__ float weight[kMaxCtas];
+    __shared__ float4 sums[kShares][kLanes];
+    __shared__ float wide[2][kJoinThreads / 32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const JoinRecord record = p.records[blockIdx.x];
-    const uint32_t group = p.query_heads / p.kv_heads, which = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, query = blockIdx.y * kQueries + which;
-    if (blockIdx.y * kQueries >= record.tokens * group) return;
+    const uint32_t group = p.query_heads / p.kv_heads, share = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, warp = threadIdx.x / 32;
     const uint32_t parts = record.last - blockIdx.x + 1;
-    const bool live = query < record.tokens * group;
-    const float2* stats = reinterpret_cast<const float2*>(p.parts + static_cast<uint64_t>(2 * p.spans) * kN * kHeadDim) + query;
     auto part = [&](uint32_t i) { return 2 * (blockIdx.x + i) + (i == 0 ? 1 : 0); };
-    float most = -INFINITY, all = 0.0f;
-    if (live) {
-        for (uint32_t i = 0; i < parts; ++i) most = fmaxf(most, stats[static_cast<uint64_t>(part(i)) * kN].x);
-        for (uint32_t i = 0; i < parts; ++i) {
-            const float2 s = stats[static_cast<uint64_t>(part(i)) * kN];
-            const float w = s.x == -INFINITY ? 0.0f : exp2_fast(s.x - most);
-            all += w * s.y;
-            if (lane == 0) weight[which][i] = w;
+    for (uint32_t query = blockIdx.y; query < record.tokens * group; query += gridDim.y) {
+        // a part a thread: its weight 2^(reference - largest reference)
+        float2 mine = make_float2(-INFINITY, 0.0f);
+        if (threadIdx.x < parts) mine = reinterpret_cast<const float2*>(p.parts + static_cast<uint64_t>(2 * p.spans) * kN * kHeadDim)[part(threadIdx.x) * kN + query];
+        // the first of this thread's part of the outputs, on their way meanwhile
+        const float4* const from = reinterpret_cast<const float4*>(p.parts + static_cast<uint64_t>(query) * kHeadDim) + lane;
+        constexpr uint32_t kAhead = 4;
+        float4 v[kAhead];
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            if (share + i * kShares < parts) v[i] = from[part(share + i * kShares) * (kN * kLanes)];
         }
+        float most = mine.x;
+#pragma unroll
+        for (uint32_t step = 16; step; step /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, step));
+        if (threadIdx.x % 32 == 0) wide[0][warp] = most;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t w = 0; w < kJoinThreads / 32; ++w) most = fmaxf(most, wide[0][w]);
+        const float w = mine.x == -INFINITY ? 0.0f : exp2_fast(mine.x - most);
+        weight[threadIdx.x] = w;
+        float all = w * mine.y;
+        if (w == 0.0f) all = 0.0f;
+#pragma unroll
+        for (uint32_t step = 16; step; step /= 2) all += __shfl_xor_sync(0xffffffffu, all, step);
+        if (threadIdx.x % 32 == 0) wide[1][warp] = all;
+        __syncthreads();
+        float4 sum = make_float4(0, 0, 0, 0);
+        auto add = [&](const float4& x, uint32_t i) {
+            const float f = weight[i];
+            if (f != 0.0f) sum.x = fmaf(f, x.x, sum.x), sum.y = fmaf(f, x.y, sum.y), sum.z = fmaf(f, x.z, sum.z), sum.w = fmaf(f, x.w, sum.w);
+        };
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            if (share + i * kShares < parts) add(v[i], share + i * kShares);
+        }
+#pragma unroll 4
+        for (uint32_t i = share + kAhead * kShares; i < parts; i += kShares) add(from[part(i) * (kN * kLanes)], i);
+        sums[share][lane] = sum;
+        __syncthreads();
+        if (share == 0) {
+#pragma unroll
+            for (uint32_t i = 1; i < kShares; ++i) {
+                const float4 x = sums[i][lane];
+                sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+            }
+            all = wide[1][0];
+#pragma unroll
+            for (uint32_t i = 1; i < kJoinThreads / 32; ++i) all += wide[1][i];
+            const float scale = 1.0f / all;
+            const __nv_bfloat162 a = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum.x * scale, all == 0.0f ? 0.0f : sum.y * scale);
+            const __nv_bfloat162 b = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum.z * scale, all == 0.0f ? 0.0f : sum.w * scale);
+            const uint32_t token = query / group;
+            const uint64_t at = (static_cast<uint64_t>(record.row + token) * p.query_heads + record.head * group + (query - token * group)) * kHeadDim + 4 * lane;
+            *reinterpret_cast<uint2*>(p.output + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        }
+        __syncthreads();   // the next query's values go to the same places
     }
-    __syncthreads();
-    if (!live) return;
-    float4 sum = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-    for (uint32_t i = 0; i < parts; ++i) {
-        const float4 v = reinterpret_cast<const float4*>(p.parts + (static_cast<uint64_t>(part(i)) * kN + query) * kHeadDim)[lane];
-        const float w = weight[which][i];
-        if (w != 0.0f) sum.x = fmaf(w, v.x, sum.x), sum.y = fmaf(w, v.y, sum.y), sum.z = fmaf(w, v.z, sum.z), sum.w = fmaf(w, v.w, sum.w);
-    }
-    const float scale = all == 0.0f ? 0.0f : 1.0f / all;
-    const __nv_bfloat162 a = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum.x * scale, all == 0.0f ? 0.0f : sum.y * scale);
-    const __nv_bfloat162 b = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum.z * scale, all == 0.0f ? 0.0f : sum.w * scale);
-    const uint32_t token = query / group;
-    const uint64_t at = (static_cast<uint64_t>(record.row + token) * p.query_heads + record.head * group + (query - token * group)) * kHeadDim + 4 * lane;
-    *reinterpret_cast<uint2*>(p.output + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
 uint32_t query_columns(uint32_t query_heads, uint32_t kv_heads, uint32_t max_new) { return (query_heads / kv_heads * max_new + 15) / 16 * 16; }
@@ -657,13 +723,13 @@ template <uint32_t kHeadDim, uint32_t kN>
 void launch_attention(cudaStream_t stream, const CUtensorMap& keys, const CUtensorMap& values, const AttentionParams& p) {
     using S = Shape<kHeadDim, kN>;
     launch_dependent(stream, paged_attention_kernel<kHeadDim, kN>, p.spans, kThreads, S::kSmem, keys, values, p);
-    constexpr uint32_t kQueries = kJoinThreads / (kHeadDim / 4);
+    const uint32_t queries = p.query_heads / p.kv_heads * p.max_new;
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
     config.stream = stream, config.attrs = &attribute, config.numAttrs = 1;
-    config.gridDim = dim3(p.spans, (p.query_heads / p.kv_heads * p.max_new + kQueries - 1) / kQueries), config.blockDim = dim3(kJoinThreads);
+    config.gridDim = dim3(p.spans, queries < kJoinRows ? queries : kJoinRows), config.blockDim = dim3(kJoinThreads);
     cudaLaunchKernelEx(&config, attention_join_kernel<kHeadDim, kN>, p);
     count_launch(2);
 }
@@ -692,6 +758,7 @@ bool check_attention(int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm
     }
     if (!plan_ok(plan, d, s) || !kv_layer_ok(a->layer) || !kv_batch_ok(a->batch) || a->reserved != 0) return false;
     if (static_cast<uint64_t>(a->batch.table_pages) * a->layer.page_tokens > (1u << kMaxTokensLog2)) return false;
+    if (static_cast<uint64_t>(a->batch.sequences) * ((a->batch.table_pages * a->layer.page_tokens + kUnit - 1) / kUnit) * a->layer.kv_heads > INT32_MAX) return false;
     if (!shape_ok(a->query_heads, a->layer.kv_heads, a->layer.head_dim, a->max_new_tokens) || !std::isfinite(a->scale)) return false;
     const uint64_t bytes = static_cast<uint64_t>(a->batch.rows) * a->query_heads * a->layer.head_dim * 2;
     if (a->query_len_bytes != bytes || a->output_len_bytes != bytes) return false;
