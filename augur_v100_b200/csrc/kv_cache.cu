@@ -22,38 +22,49 @@ struct AppendParams {
     uint32_t half;                       // rotary pairs
     uint32_t sections[3], interleaved;
     float epsilon;
-    uint32_t parts;                      // CTAs that share a row's heads
 };
 
-constexpr uint32_t kAppendThreads = 256;
+constexpr uint32_t kAppendThreads = 256, kAppendCtas = 1184;   // eight an SM
 
 // A CTA turns some of the heads of one row, head_dim / 8 neighbouring lanes to a head with eight elements (one 16-byte access) each. The
 // sines and cosines of the row are formed once per CTA. What the rotation pairs lies rotary_dim / 16 lanes away: a shuffle.
+// A decoding step's few rows are a matter of latency: heads are dealt out so that a lane has one, whose load is under way before the row's sequence
+// and angles are known. (One CTA a row, loads behind them: 8 rows of 24 + 2 x 4 heads of 256 5.9 us; now 5.0, most of it the launch.)
 template <uint32_t kHeadDim>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
     constexpr uint32_t kLanes = kHeadDim / 8, kGroups = kAppendThreads / kLanes;
-    __shared__ float cosine[kHeadDim / 2], sine[kHeadDim / 2];
+    __shared__ __align__(16) float cosine[kHeadDim / 2], sine[kHeadDim / 2];
     __shared__ int32_t sequence_at, slot_page, slot_offset;
-    const uint32_t row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+    const uint32_t row = blockIdx.x, heads = p.query_heads + 2 * p.kv_heads;
     const uint32_t group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
     if (threadIdx.x == 0) sequence_at = -1;
+    __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    __syncthreads();
+    auto load = [&](uint32_t h) {
+        const __nv_bfloat16* from;
+        if (h < p.query_heads) from = p.query + row * p.query_row_stride + h * p.query_head_stride;
+        else if (h < p.query_heads + p.kv_heads) from = p.key + row * p.key_row_stride + (h - p.query_heads) * p.key_head_stride;
+        else from = p.value + row * p.value_row_stride + (h - p.query_heads - p.kv_heads) * p.value_head_stride;
+        return __ldg(reinterpret_cast<const uint4*>(from) + lane);
+    };
+    uint32_t h = blockIdx.y * kGroups + group;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (h < heads) raw = load(h);
     for (uint32_t b = threadIdx.x; b < p.sequences; b += kAppendThreads) {
-        const int32_t from = p.token_starts[b], to = p.token_starts[b + 1];
+        const int32_t from = __ldg(p.token_starts + b), to = __ldg(p.token_starts + b + 1), length = __ldg(p.lengths + b);
         if (static_cast<int32_t>(row) >= from && static_cast<int32_t>(row) < to) {
-            const int64_t position = static_cast<int64_t>(p.lengths[b]) - to + row;   // in the cache
+            const int64_t position = static_cast<int64_t>(length) - to + row;   // in the cache
             const int64_t page = position >> p.page_shift;
             int32_t at = -1;
-            if (position >= 0 && page < p.table_pages) at = p.page_table[static_cast<uint64_t>(b) * p.table_pages + page];
+            if (position >= 0 && page < p.table_pages) at = __ldg(p.page_table + static_cast<uint64_t>(b) * p.table_pages + page);
             sequence_at = static_cast<int32_t>(b);
             slot_page = at >= 0 && static_cast<uint32_t>(at) < p.pages ? at : -1;
             slot_offset = static_cast<int32_t>(position & ((int64_t(1) << p.page_shift) - 1));
         }
     }
-    if (threadIdx.x < p.half) {
-        const uint32_t i = threadIdx.x;
+    const uint32_t i = kAppendThreads - 1 - threadIdx.x;   // the last threads: the first ones are busy with few sequences
+    if (i < p.half) {
         uint32_t axis;
         if (p.interleaved) {
             axis = i % 3;
@@ -62,70 +73,73 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
             axis = (i >= p.sections[0] ? 1u : 0u) + (i >= p.sections[0] + p.sections[1] ? 1u : 0u);
         }
         // In turns, in 64 bits: a position of 2^20 leaves 2^-33 of a turn, where the F32 product would have lost 2^-7.
-        const double turns = static_cast<double>(p.positions[static_cast<uint64_t>(axis) * p.rows + row]) * static_cast<double>(p.inv_freq[i]) * 0.15915494309189535;
+        const double turns = static_cast<double>(__ldg(p.positions + static_cast<uint64_t>(axis) * p.rows + row)) * static_cast<double>(__ldg(p.inv_freq + i)) * 0.15915494309189535;
         const float part_turn = static_cast<float>(turns - rint(turns));
         sincospif(2.0f * part_turn, &sine[i], &cosine[i]);
     }
     __syncthreads();
     if (sequence_at < 0) return;
     const int32_t page = slot_page;
-    const uint32_t heads = p.query_heads + 2 * p.kv_heads, half_lanes = p.half / 8;
-    for (uint32_t h = part * kGroups + group; h < heads; h += p.parts * kGroups) {   // the lanes of a head stay together
-        const __nv_bfloat16* from;
+    const uint32_t half_lanes = p.half / 8;
+    const bool turns = lane < 2 * half_lanes, upper = lane >= half_lanes;
+    const uint32_t partner = !turns ? lane : upper ? lane - half_lanes : lane + half_lanes;
+    const uint32_t pair = turns ? 8 * (upper ? lane - half_lanes : lane) : 0;
+    const unsigned mask = kLanes == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);   // the lanes of a head stay together
+    for (; h < heads; h += gridDim.y * kGroups) {
+        const uint4 now = raw;
+        if (h + gridDim.y * kGroups < heads) raw = load(h + gridDim.y * kGroups);
+        const bool is_query = h < p.query_heads, is_value = h >= p.query_heads + p.kv_heads;
+        if (!is_query && page < 0) continue;
         __nv_bfloat16* to;
-        const float* norm = nullptr;
-        bool turn = true;
-        if (h < p.query_heads) {
-            from = p.query + row * p.query_row_stride + h * p.query_head_stride;
+        if (is_query) {
             to = p.query_out + (static_cast<uint64_t>(row) * p.query_heads + h) * kHeadDim;
-            norm = p.query_norm;
         } else {
-            const bool is_key = h < p.query_heads + p.kv_heads;
-            const uint32_t head = h - p.query_heads - (is_key ? 0 : p.kv_heads);
-            if (page < 0) continue;
-            const uint64_t slot = ((static_cast<uint64_t>(page) * p.kv_heads + head) << p.page_shift) + slot_offset;
-            from = is_key ? p.key + row * p.key_row_stride + head * p.key_head_stride : p.value + row * p.value_row_stride + head * p.value_head_stride;
-            to = (is_key ? p.keys : p.values) + slot * kHeadDim;
-            norm = is_key ? p.key_norm : nullptr;
-            turn = is_key;
+            const uint32_t head = h - p.query_heads - (is_value ? p.kv_heads : 0);
+            to = (is_value ? p.values : p.keys) + (((static_cast<uint64_t>(page) * p.kv_heads + head) << p.page_shift) + slot_offset) * kHeadDim;
         }
-        uint4 raw = *reinterpret_cast<const uint4*>(from + 8 * lane);
-        if (turn) {
-            const unsigned mask = kLanes == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
+        uint4 result = now;
+        if (!is_value) {
+            const float* const norm = is_query ? p.query_norm : p.key_norm;
             float x[8];
-            const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+            const uint32_t word[4] = {now.x, now.y, now.z, now.w};
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                x[2 * i] = __uint_as_float(word[i] << 16);
-                x[2 * i + 1] = __uint_as_float(word[i] & 0xffff0000u);
+            for (uint32_t e = 0; e < 4; ++e) {
+                x[2 * e] = __uint_as_float(word[e] << 16);
+                x[2 * e + 1] = __uint_as_float(word[e] & 0xffff0000u);
             }
             if (norm) {
-                float sum = 0.0f;
+                float weight[8], sum = 0.0f;   // (weights are aligned to an element only)
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+                for (uint32_t e = 0; e < 8; ++e) weight[e] = __ldg(norm + 8 * lane + e);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
 #pragma unroll
                 for (uint32_t step = kLanes / 2; step; step /= 2) sum += __shfl_xor_sync(mask, sum, step);
                 const float scale = __frsqrt_rn(sum * (1.0f / kHeadDim) + p.epsilon);
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) x[i] = x[i] * scale * norm[8 * lane + i];
+                for (uint32_t e = 0; e < 8; ++e) x[e] = x[e] * scale * weight[e];
             }
-            const bool upper = lane >= half_lanes;
-            const uint32_t partner = lane >= 2 * half_lanes ? lane : upper ? lane - half_lanes : lane + half_lanes;
-            const uint32_t pair = 8 * (upper ? lane - half_lanes : lane);
+            float c[8], n[8];
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const float other = __shfl_sync(mask, x[i], partner, kLanes);
-                if (lane < 2 * half_lanes) x[i] = fmaf(x[i], cosine[pair + i], (upper ? other : -other) * sine[pair + i]);
+            for (uint32_t e = 0; e < 8; e += 4) {
+                const float4 a = *reinterpret_cast<const float4*>(cosine + pair + e), b = *reinterpret_cast<const float4*>(sine + pair + e);
+                c[e] = a.x, c[e + 1] = a.y, c[e + 2] = a.z, c[e + 3] = a.w;
+                n[e] = b.x, n[e + 1] = b.y, n[e + 2] = b.z, n[e + 3] = b.w;
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                const float other = __shfl_sync(mask, x[e], partner, kLanes);
+                if (turns) x[e] = fmaf(x[e], c[e], (upper ? other : -other) * n[e]);
             }
             uint32_t packed[4];
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const __nv_bfloat162 two = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-                packed[i] = *reinterpret_cast<const uint32_t*>(&two);
+            for (uint32_t e = 0; e < 4; ++e) {
+                const __nv_bfloat162 two = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+                packed[e] = *reinterpret_cast<const uint32_t*>(&two);
             }
-            raw = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+            result = make_uint4(packed[0], packed[1], packed[2], packed[3]);
         }
-        *reinterpret_cast<uint4*>(to + 8 * lane) = raw;
+        *(reinterpret_cast<uint4*>(to) + lane) = result;
     }
 }
 
@@ -171,13 +185,17 @@ bool check_append(int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm100
 
 // ---- page copies ---------------------------------------------------------------------------------
 
-constexpr uint32_t kPairsPerLaunch = 1000;   // the page numbers travel as launch parameters: nothing to copy ahead, nothing to keep
+// The page numbers travel as launch parameters: nothing to copy ahead, nothing to keep. Few pairs (a fork) in a short list: a launch with 8 KB of
+// parameters costs the host 2 us more than one with 64 bytes.
+constexpr uint32_t kPairsPerLaunch = 1000, kFewPairs = 8;
 constexpr uint32_t kCopyThreads = 256, kCopyPiece = kCopyThreads * 16 * 4;
+template <uint32_t kPairs>
 struct PagePairs {
-    uint32_t source[kPairsPerLaunch], destination[kPairsPerLaunch];
+    uint32_t source[kPairs], destination[kPairs];
 };
 
-__global__ void __launch_bounds__(kCopyThreads) kv_page_copy_kernel(const __grid_constant__ PagePairs pairs, uint8_t* keys, uint8_t* values, uint64_t page_bytes,
+template <uint32_t kPairs>
+__global__ void __launch_bounds__(kCopyThreads) kv_page_copy_kernel(const __grid_constant__ PagePairs<kPairs> pairs, uint8_t* keys, uint8_t* values, uint64_t page_bytes,
                                                                     uint32_t pages, uint32_t layers, uint32_t pieces) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     uint32_t at = blockIdx.x;
@@ -216,6 +234,16 @@ bool check_page_copy(int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm
     const Range r[2] = {{a->keys, a->len_bytes, 16}, {a->values, a->len_bytes, 16}};
     if (!all_disjoint(r, 2)) return false;
     return !full || inspect_device_ranges(d, r, 2, failure);
+}
+
+template <uint32_t kPairs>
+void launch_copies(cudaStream_t stream, uint32_t grid, const uint32_t* sources, const uint32_t* destinations, uint32_t count,
+                   const augur_cuda_nvfp4_sm100_kv_page_copy_args_v1* a, uint32_t pieces) {
+    PagePairs<kPairs> pairs{};
+    for (uint32_t i = 0; i < count; ++i) pairs.source[i] = sources[i], pairs.destination[i] = destinations[i];
+    launch_dependent(stream, kv_page_copy_kernel<kPairs>, grid, kCopyThreads, 0, pairs, reinterpret_cast<uint8_t*>(a->keys), reinterpret_cast<uint8_t*>(a->values),
+                     a->page_bytes, a->pages, a->layers, pieces);
+    count_launch();
 }
 
 // Destinations distinct, none of them a source, all inside the cache.
@@ -282,12 +310,17 @@ extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append
     p.half = a->rotary_dim / 2;
     for (uint32_t i = 0; i < 3; ++i) p.sections[i] = a->sections[i];
     p.interleaved = a->interleaved, p.epsilon = a->epsilon;
-    p.parts = 1;
-    if (a->layer.head_dim == 256) {
-        launch_dependent(s->stream, kv_append_kernel<256>, p.rows * p.parts, kAppendThreads, 0, p);
-    } else {
-        launch_dependent(s->stream, kv_append_kernel<128>, p.rows * p.parts, kAppendThreads, 0, p);
-    }
+    // A head per group of lanes while that many CTAs run at once; more rows hide their loads behind one another, and share the angles.
+    const uint32_t groups = kAppendThreads / (a->layer.head_dim / 8), heads = a->query_heads + 2 * a->layer.kv_heads;
+    const uint32_t each = (heads + groups - 1) / groups, fits = kAppendCtas / p.rows;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.stream = s->stream, config.attrs = &attribute, config.numAttrs = 1;
+    config.gridDim = dim3(p.rows, each < fits ? each : fits > 1 ? fits : 1), config.blockDim = dim3(kAppendThreads);
+    if (a->layer.head_dim == 256) cudaLaunchKernelEx(&config, kv_append_kernel<256>, p);
+    else cudaLaunchKernelEx(&config, kv_append_kernel<128>, p);
     count_launch();
     return submitted();
 }
@@ -312,14 +345,13 @@ extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_c
     const uint32_t pieces = static_cast<uint32_t>((a->page_bytes + kCopyPiece - 1) / kCopyPiece);
     const uint64_t per_pair = static_cast<uint64_t>(pieces) * 2 * a->layers;        // below 2^28
     const uint32_t most = static_cast<uint32_t>(per_pair * kPairsPerLaunch < INT32_MAX ? kPairsPerLaunch : INT32_MAX / per_pair);
-    PagePairs pairs;
     for (uint32_t at = 0; at < count;) {
-        const uint32_t take = count - at < most ? count - at : most;
-        for (uint32_t i = 0; i < take; ++i) pairs.source[i] = sources[at + i], pairs.destination[i] = destinations[at + i];
-        for (uint32_t i = take; i < kPairsPerLaunch; ++i) pairs.source[i] = pairs.destination[i] = 0;
-        launch_dependent(s->stream, kv_page_copy_kernel, static_cast<uint32_t>(per_pair * take), kCopyThreads, 0, pairs, reinterpret_cast<uint8_t*>(a->keys),
-                         reinterpret_cast<uint8_t*>(a->values), a->page_bytes, a->pages, a->layers, pieces);
-        count_launch();
+        const uint32_t take = count - at < most ? count - at : most, grid = static_cast<uint32_t>(per_pair * take);
+        if (take <= kFewPairs) {
+            launch_copies<kFewPairs>(s->stream, grid, sources + at, destinations + at, take, a, pieces);
+        } else {
+            launch_copies<kPairsPerLaunch>(s->stream, grid, sources + at, destinations + at, take, a, pieces);
+        }
         at += take;
     }
     return submitted();

@@ -46,16 +46,17 @@ struct AttentionParams {
     __nv_bfloat16* output;
     const int32_t *page_table, *lengths, *token_starts;
     uint32_t* status_word;
-    struct JoinRecord* records;   // [spans]
+    struct JoinRecord* records;   // [joins]
     float* parts;                 // [spans][2][kN][head_dim], then [spans][2][kN] (reference maximum, denominator)
-    uint32_t rows, sequences, table_pages, pages, query_heads, kv_heads, page_shift, max_new, spans;
+    uint32_t rows, sequences, table_pages, pages, query_heads, kv_heads, page_shift, max_new, spans, joins;
     float scale_log2;             // scale * log2(e)
 };
 
-// What the join has to know of the pair whose first part span `c` holds (tokens 0: none).
+// What the join has to know of a pair that several spans share (tokens 0: of none). Records are by pair or, where there are more pairs than spans, by the
+// span that holds the pair's first part.
 struct JoinRecord {
-    uint32_t row, tokens, head, last;   // first token row, new tokens, key-value head, last span
-    uint32_t reserved[4];
+    uint32_t row, tokens, head, first, last;   // first token row, new tokens, key-value head, first and last span
+    uint32_t reserved[3];
 };
 
 // Small state of a CTA, behind the ring, the queries and the weights.
@@ -71,6 +72,7 @@ struct State {
     int32_t limit[kMaxQueries];        // keys that a query sees
     uint32_t units[kMaxSequences + 1]; // before sequence b, of one head
     uint32_t length[kMaxSequences];    // | new tokens << 25
+    uint32_t row[kMaxSequences];       // the first token row
 };
 
 template <uint32_t kHeadDim, uint32_t kN>
@@ -143,20 +145,33 @@ struct Tiles {
     __device__ uint32_t keys() const { return walk.key_end - key < kTile ? walk.key_end - key : kTile; }
 };
 
-__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-                 : "memory");
+// Operand descriptors, low and high word: address and leading offset, stride offset, version and swizzle.
+// K and the narrow operands (K-major, 128-byte swizzle: 8 rows are 1024 bytes). V (MN-major): 128-byte rows of 64 dims, one per key, so the rows
+// are the k dimension; 8 keys are 1024 bytes, the next 64 dims lie one ring slot further. The ones (K-major, no swizzle): 8 rows x 16 bytes are
+// 128 bytes, the next 8 k 128 bytes further, the next 8 rows 256.
+constexpr uint32_t kHighSwizzled = (1024 >> 4) | (1u << 14) | (2u << 29), kHighPlain = (256 >> 4) | (1u << 14);
+__device__ __forceinline__ uint32_t low_word(uint32_t smem_addr, uint32_t leading) { return ((smem_addr & 0x3ffffu) >> 4) | ((leading >> 4) << 16); }
+// Up to four MMAs of 16 k of a converged warp, the 128-row operand kStep (of 16 bytes) further and the narrow one 32 bytes further each time, as
+// predicated instructions whose operands are uniform (behind a branch, one by one, an MMA took 65 cycles to issue; the pipe needs 32).
+template <uint32_t kHigh, uint32_t kStep>
+__device__ __forceinline__ void mma_block(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate, uint32_t steps) {
+    asm volatile(
+        "{\n.reg .pred e, p, q, e1, e2, e3;\n.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n.reg .b32 l1, l2, l3, m1, m2, m3;\n"
+        "elect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\nsetp.eq.u32 q, 0, 0;\n"
+        "setp.gt.and.u32 e1, %5, 1, e;\nsetp.gt.and.u32 e2, %5, 2, e;\nsetp.gt.and.u32 e3, %5, 3, e;\n"
+        "add.s32 l1, %1, %8;\nadd.s32 l2, l1, %8;\nadd.s32 l3, l2, %8;\nadd.s32 m1, %2, 2;\nadd.s32 m2, %2, 4;\nadd.s32 m3, %2, 6;\n"
+        "mov.b64 a0, {%1, %6};\nmov.b64 a1, {l1, %6};\nmov.b64 a2, {l2, %6};\nmov.b64 a3, {l3, %6};\n"
+        "mov.b64 b0, {%2, %7};\nmov.b64 b1, {m1, %7};\nmov.b64 b2, {m2, %7};\nmov.b64 b3, {m3, %7};\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a0, b0, %3, p;\n"
+        "@e1 tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, q;\n"
+        "@e2 tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, q;\n"
+        "@e3 tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, q;\n}"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(steps), "r"(kHigh), "r"(kHighSwizzled), "n"(kStep)
+        : "memory");
 }
-// The ones as the 128-row operand, without swizzle: 8 rows x 16 bytes are 128 bytes, the next 8 k 128 bytes further, the next 8 rows 256.
-__device__ __forceinline__ uint64_t ones_desc(uint32_t smem_addr) {
-    return static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4) | (uint64_t(128 >> 4) << 16) | (uint64_t(256 >> 4) << 32) | (uint64_t(1) << 46);
-}
-// V as the 128-row operand: 128-byte rows of 64 dims, one per key, so the rows are the k dimension; 8 keys are 1024 bytes, the next 64 dims
-// lie one ring slot further.
-__device__ __forceinline__ uint64_t value_desc(uint32_t smem_addr) {
-    return static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4) | (static_cast<uint64_t>(kSlotBytes >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
-           (uint64_t(1) << 46) | (uint64_t(2) << 61);
+// The elected lane's commit (elect.sync always names the same lane of a whole warp: the one that issued the MMAs).
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void load_columns16(uint32_t taddr, uint32_t* v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -239,7 +254,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                 }
                 if (length < 0) length = 0;
                 const uint32_t tokens = rows_fit ? static_cast<uint32_t>(to - from) : 0;
+                st->row[b] = static_cast<uint32_t>(from);
                 st->length[b] = static_cast<uint32_t>(length) | tokens << (kMaxTokensLog2 + 1);
+                if (!tokens && p.joins < p.spans && blockIdx.x == b % p.spans) {
+                    for (uint32_t h = 0; h < p.kv_heads; ++h) p.records[b * p.kv_heads + h] = JoinRecord{};   // an idle slot's
+                }
                 if (tokens) count[i] = length ? (static_cast<uint32_t>(length) + kUnit - 1) / kUnit : 1;   // a row that sees nothing is written too
             }
             sum += count[i];
@@ -325,8 +344,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
         // ---------------- MMA issuer: S of a tile, then O of the tile before it ----------------
         constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kN >> 3) << 17) | ((kTile >> 4) << 24);   // F32 += BF16 x BF16
         constexpr uint32_t idesc_values = idesc | (1u << 15);                                                        // V is MN-major
-        const uint64_t slots = operand_desc(smem_u32(smem)), slots_values = value_desc(smem_u32(smem));
-        const uint64_t queries = operand_desc(smem_u32(query_smem)), weights = operand_desc(smem_u32(weight_smem)), ones = ones_desc(smem_u32(ones_smem));
+        const uint32_t slots = low_word(smem_u32(smem), 16), slots_values = low_word(smem_u32(smem), kSlotBytes);
+        const uint32_t queries = low_word(smem_u32(query_smem), 16), weights = low_word(smem_u32(weight_smem), 16), ones = low_word(smem_u32(ones_smem), 128);
         Tiles ahead, now;
         ahead.open(st, p, from, to);
         now = ahead;
@@ -339,21 +358,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             for (uint32_t c = 0; c < S::kChunks; ++c) {
                 if (!warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusMma)) return false;
                 tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t a = slots + slot * (kSlotBytes >> 4), b = queries + ((query * S::kQueryBytes + c * kN * 128) >> 4);
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) mma_bf16(tmem + buffer * kN, a + 2 * k, b + 2 * k, idesc, c | k);
-                    tc_commit(empty + 8 * slot);
-                }
-                __syncwarp();
+                mma_block<kHighSwizzled, 2>(tmem + buffer * kN, slots + slot * (kSlotBytes >> 4), queries + ((query * S::kQueryBytes + c * kN * 128) >> 4), idesc, c, 4);
+                commit(empty + 8 * slot);
                 if (++slot == S::kSlots) slot = 0, phase ^= 1;
             }
-            if (elect_one()) {
-                tc_commit(scores_full + 8 * buffer);
-                if (ahead.last()) tc_commit(query_empty + 8 * query);
+            commit(scores_full + 8 * buffer);
+            if (ahead.last()) {
+                commit(query_empty + 8 * query);
+                ++pair;
             }
-            __syncwarp();
-            if (ahead.last()) ++pair;
             ++scores;
             ahead.advance(st, p);
             return true;
@@ -364,30 +377,25 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             const uint32_t buffer = products & 1, steps = (now.keys() + 15) / 16;
             if (!warp_look_wait(weights_full + 8 * buffer, products >> 1 & 1, abort_flag, status, kStatusProduct)) break;
             tc_fence_after();
-            if (elect_one()) {   // denominators: the sum over the keys as one more product, into every lane
-                const uint64_t b = weights + ((buffer * S::kWeightBytes) >> 4);
-                for (uint32_t k = 0; k < steps; ++k) mma_bf16(tmem_sum, ones, b + (k >> 2) * (kN * 128 >> 4) + (k & 3) * 2, idesc, !now.first() || k);
-            }
-            __syncwarp();
+            const uint32_t follows = !now.first(), weights_now = weights + ((buffer * S::kWeightBytes) >> 4);
+            // denominators: the sum over the keys as one more product, into every lane
+            mma_block<kHighPlain, 0>(tmem_sum, ones, weights_now, idesc, follows, steps);
+            if (steps > 4) mma_block<kHighPlain, 0>(tmem_sum, ones, weights_now + (kN * 128 >> 4), idesc, 1, steps - 4);
             for (uint32_t h = 0; alive && h < S::kHalves; ++h) {
                 for (uint32_t c = 0; c < 2; ++c) alive = alive && warp_look_wait(full + 8 * (slot + c), phase, abort_flag, status, kStatusProduct);
                 if (!alive) break;
                 tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t a = slots_values + slot * (kSlotBytes >> 4), b = weights + ((buffer * S::kWeightBytes) >> 4);
-                    for (uint32_t k = 0; k < steps; ++k) {   // 16 keys: 16 rows of V, 32 bytes of a row of P
-                        mma_bf16(tmem_out + h * kN, a + k * (16 * 128 >> 4), b + (k >> 2) * (kN * 128 >> 4) + (k & 3) * 2, idesc_values, !now.first() || k);
-                    }
-                    tc_commit(empty + 8 * slot);
-                    tc_commit(empty + 8 * (slot + 1));
-                }
-                __syncwarp();
+                // 16 keys: 16 rows of V, 32 bytes of a row of P
+                const uint32_t a = slots_values + slot * (kSlotBytes >> 4), d = tmem_out + h * kN;
+                mma_block<kHighSwizzled, (16 * 128 >> 4)>(d, a, weights_now, idesc_values, follows, steps);
+                if (steps > 4) mma_block<kHighSwizzled, (16 * 128 >> 4)>(d, a + 4 * (16 * 128 >> 4), weights_now + (kN * 128 >> 4), idesc_values, 1, steps - 4);
+                commit(empty + 8 * slot);
+                commit(empty + 8 * (slot + 1));
                 slot += 2;
                 if (slot == S::kSlots) slot = 0, phase ^= 1;
             }
             if (!alive) break;
-            if (elect_one()) tc_commit(weights_empty + 8 * buffer);
-            __syncwarp();
+            commit(weights_empty + 8 * buffer);
             ++products;
             now.advance(st, p);
         }
@@ -399,7 +407,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
         while (walk.next(st, p)) {
             if (walk.key >= walk.key_end) continue;
             const uint32_t buffer = S::kQueryBuffers == 2 ? pair & 1 : 0;
-            const uint32_t first_row = static_cast<uint32_t>(__ldg(p.token_starts + walk.sequence)), queries = walk.tokens * group;
+            const uint32_t first_row = st->row[walk.sequence], queries = walk.tokens * group;
             if (!warp_look_wait(query_empty + 8 * buffer, ((S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1) ^ 1, abort_flag, status, kStatusQuery)) break;
             // 16 bytes a copy, all of them under way together (as loads and stores they waited for one another: 1000 cycles a row)
             constexpr uint32_t kPieces = kHeadDim / 8, kRows = 32 / kPieces;
@@ -436,7 +444,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
         bool alive = true;
         while (alive && walk.next(st, p)) {
             const uint32_t queries = walk.tokens * group;
-            const int32_t first_row = __ldg(p.token_starts + walk.sequence);
+            const uint32_t first_row = st->row[walk.sequence];
             if (thread < kN) {
                 st->reference[thread] = -INFINITY;
                 st->limit[thread] = thread < queries ? static_cast<int32_t>(walk.length) - static_cast<int32_t>(walk.tokens) + static_cast<int32_t>(thread / group) + 1 : 0;
@@ -626,12 +634,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                 if (walk.starts) {
                     const uint32_t units = st->units[walk.sequence + 1] - st->units[walk.sequence], longer = extra * (base + 1);
                     const uint32_t last = st->units[walk.sequence] * p.kv_heads + (walk.head + 1) * units - 1;   // the pair's last unit
-                    record.row = static_cast<uint32_t>(first_row), record.tokens = walk.tokens, record.head = walk.head;
+                    record.row = first_row, record.tokens = walk.tokens, record.head = walk.head, record.first = blockIdx.x;
                     record.last = last < longer ? last / (base + 1) : extra + (last - longer) / base;
                 }
             }
+            if (p.joins < p.spans && walk.starts && thread == 0) p.records[walk.sequence * p.kv_heads + walk.head] = alone ? JoinRecord{} : record;
         }
-        if (thread == 0) p.records[blockIdx.x] = record;
+        if (p.joins == p.spans && thread == 0) p.records[blockIdx.x] = record;
     }
     tc_fence_before();
     __syncthreads();
@@ -643,7 +652,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
 
 // Joins the parts of one pair, in the order of their spans. A CTA takes queries blockIdx.y, blockIdx.y + gridDim.y, ...; four outputs a
 // thread, and the threads of a query's outputs as many times over as there are, each with every so many-th part.
-constexpr uint32_t kJoinThreads = 256, kJoinRows = 8;
+constexpr uint32_t kJoinThreads = 256, kJoinCtas = 1184;   // about as many as run at once
 template <uint32_t kHeadDim, uint32_t kN>
 __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttentionParams p) {
     constexpr uint32_t kLanes = kHeadDim / 4, kShares = kJoinThreads / kLanes;
@@ -654,8 +663,10 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const JoinRecord record = p.records[blockIdx.x];
     const uint32_t group = p.query_heads / p.kv_heads, share = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, warp = threadIdx.x / 32;
-    const uint32_t parts = record.last - blockIdx.x + 1;
-    auto part = [&](uint32_t i) { return 2 * (blockIdx.x + i) + (i == 0 ? 1 : 0); };
+    // (a launch that gave up may have left a record of an earlier one)
+    if (record.tokens * group > kN || record.row + record.tokens > p.rows || record.head >= p.kv_heads || record.last >= p.spans || record.first > record.last) return;
+    const uint32_t parts = record.last - record.first + 1;
+    auto part = [&](uint32_t i) { return 2 * (record.first + i) + (i == 0 ? 1 : 0); };
     for (uint32_t query = blockIdx.y; query < record.tokens * group; query += gridDim.y) {
         // a part a thread: its weight 2^(reference - largest reference)
         float2 mine = make_float2(-INFINITY, 0.0f);
@@ -729,7 +740,8 @@ void launch_attention(cudaStream_t stream, const CUtensorMap& keys, const CUtens
     attribute.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
     config.stream = stream, config.attrs = &attribute, config.numAttrs = 1;
-    config.gridDim = dim3(p.spans, queries < kJoinRows ? queries : kJoinRows), config.blockDim = dim3(kJoinThreads);
+    const uint32_t rows = (kJoinCtas + p.joins - 1) / p.joins;
+    config.gridDim = dim3(p.joins, queries < rows ? queries : rows), config.blockDim = dim3(kJoinThreads);
     cudaLaunchKernelEx(&config, attention_join_kernel<kHeadDim, kN>, p);
     count_launch(2);
 }
@@ -815,6 +827,7 @@ extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_paged_att
     p.rows = a->batch.rows, p.sequences = a->batch.sequences, p.table_pages = a->batch.table_pages, p.pages = a->layer.pages;
     p.query_heads = a->query_heads, p.kv_heads = a->layer.kv_heads, p.page_shift = static_cast<uint32_t>(__builtin_ctz(a->layer.page_tokens));
     p.max_new = a->max_new_tokens, p.spans = launch_spans(plan->sm_count);
+    p.joins = static_cast<uint64_t>(p.sequences) * p.kv_heads < p.spans ? p.sequences * p.kv_heads : p.spans;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.records = reinterpret_cast<JoinRecord*>(plan->scratch + kCounterBytes);
     p.parts = reinterpret_cast<float*>(p.records + p.spans);

@@ -742,6 +742,8 @@ class TokenLogprobs:
         a.rows, a.vocabulary, a.alternatives = rows, vocabulary, alternatives
         a.logits_type = abi.LOGITS_F32 if logits.dtype == torch.float32 else abi.LOGITS_BF16
         self.args = a
+        self._enqueue = functools.partial(abi.lib().augur_cuda_nvfp4_sm100_token_logprobs_prevalidated_submit_v1, plan.stream.ordinal, plan.stream.handle,
+                                          plan.handle, byref(a))
 
     @classmethod
     def bind(cls, plan: Plan, logits: torch.Tensor, targets: torch.Tensor, alternatives: int = 0):
@@ -752,9 +754,7 @@ class TokenLogprobs:
         return self
 
     def submit_for_plan(self) -> None:
-        s = self.plan.stream
-        _check("token_logprobs_submit", abi.lib().augur_cuda_nvfp4_sm100_token_logprobs_prevalidated_submit_v1(
-            s.ordinal, s.handle, self.plan.handle, byref(self.args)))
+        _check("token_logprobs_submit", self._enqueue())
 
 
 SHAPE_SMALL_BATCH = "small-batch"

@@ -10,7 +10,7 @@ enqueues on the stream it was bound to, and the binding keeps its tensors alive.
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 import heapq
 from ctypes import byref, c_uint32, c_uint64
 from typing import NamedTuple
@@ -110,6 +110,7 @@ class KvAppend:
         for i, section in enumerate(sections):
             a.sections[i] = section
         self.args = a
+        self._enqueue = functools.partial(abi.lib().augur_cuda_nvfp4_sm100_kv_append_prevalidated_submit_v1, stream.ordinal, stream.handle, byref(a))
 
     @classmethod
     def bind(cls, stream: Stream, cache: KvCache, layer: int, q, k, v, positions, frequencies, sections, table, lengths, starts,
@@ -123,8 +124,7 @@ class KvAppend:
         return self
 
     def submit(self) -> None:
-        _check("kv_append_submit", abi.lib().augur_cuda_nvfp4_sm100_kv_append_prevalidated_submit_v1(
-            self.stream.ordinal, self.stream.handle, byref(self.args)))
+        _check("kv_append_submit", self._enqueue())
 
 
 def paged_attention_scratch_bytes(query_heads: int, kv_heads: int, head_dim: int, tokens: int = abi.MAX_SMALL_TOKENS, sms: int = 0) -> int:
@@ -153,6 +153,8 @@ class PagedAttention:
         a.output, a.output_len_bytes = _ptr(out), _nbytes(out)
         a.query_heads, a.max_new_tokens, a.scale = query_heads, tokens, scale
         self.args = a
+        self._enqueue = functools.partial(abi.lib().augur_cuda_nvfp4_sm100_paged_attention_prevalidated_submit_v1, plan.stream.ordinal, plan.stream.handle,
+                                          plan.handle, byref(a))
 
     @classmethod
     def bind(cls, plan: Plan, cache: KvCache, layer: int, q, table, lengths, starts, tokens: int = 1, out: torch.Tensor | None = None,
@@ -166,9 +168,7 @@ class PagedAttention:
         return self
 
     def submit_for_plan(self) -> None:
-        s = self.plan.stream
-        _check("paged_attention_submit", abi.lib().augur_cuda_nvfp4_sm100_paged_attention_prevalidated_submit_v1(
-            s.ordinal, s.handle, self.plan.handle, byref(self.args)))
+        _check("paged_attention_submit", self._enqueue())
 
 
 class KvPageCopy:
@@ -182,6 +182,7 @@ class KvPageCopy:
         a.page_bytes = cache.kv_heads * cache.page_tokens * cache.head_dim * 2
         a.layers, a.pages = cache.layers, cache.pages
         self.args = a
+        self._enqueue = functools.partial(abi.lib().augur_cuda_nvfp4_sm100_kv_page_copy_prevalidated_submit_v1, stream.ordinal, stream.handle, byref(a))
 
     @classmethod
     def bind(cls, stream: Stream, cache: KvCache):
@@ -193,12 +194,10 @@ class KvPageCopy:
         count = len(sources)
         if len(destinations) != count:
             raise ValueError("one destination for every source")
-        if any(not 0 <= page < self.cache.pages for page in (*sources, *destinations)):
+        if count and (min(min(sources), min(destinations)) < 0 or max(max(sources), max(destinations)) >= self.cache.pages):
             raise ValueError("a page outside the cache")       # ctypes would wrap a negative number round
         array = c_uint32 * count
-        _check("kv_page_copy_submit", abi.lib().augur_cuda_nvfp4_sm100_kv_page_copy_prevalidated_submit_v1(
-            self.stream.ordinal, self.stream.handle, byref(self.args), ctypes.cast(array(*sources), abi._U32P),
-            ctypes.cast(array(*destinations), abi._U32P), count))
+        _check("kv_page_copy_submit", self._enqueue(array(*sources), array(*destinations), count))
 
 
 class PageCopies(NamedTuple):
