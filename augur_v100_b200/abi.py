@@ -230,7 +230,6 @@ class TokenLogprobsArgs(Structure):
 
 # Every symbol the header declares: name -> (restype, argtypes).
 _U8P = POINTER(c_uint8)
-_U32P = POINTER(c_uint32)
 EXPORTS = {
     "augur_cuda_nvfp4_sm100_abi_version": (c_uint32, []),
     "augur_cuda_nvfp4_sm100_build_capability_v1": (c_uint32, []),
@@ -292,7 +291,7 @@ EXPORTS = {
     "augur_cuda_nvfp4_sm100_paged_attention_preflight_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(PagedAttentionArgs)]),
     "augur_cuda_nvfp4_sm100_paged_attention_prevalidated_submit_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(PagedAttentionArgs)]),
     "augur_cuda_nvfp4_sm100_kv_page_copy_preflight_v1": (Result, [c_int32, c_void_p, POINTER(KvPageCopyArgs)]),
-    "augur_cuda_nvfp4_sm100_kv_page_copy_prevalidated_submit_v1": (Result, [c_int32, c_void_p, POINTER(KvPageCopyArgs), _U32P, _U32P, c_uint32]),
+    "augur_cuda_nvfp4_sm100_kv_page_copy_prevalidated_submit_v1": (Result, [c_int32, c_void_p, POINTER(KvPageCopyArgs), c_void_p, c_void_p, c_uint32]),
     "augur_cuda_nvfp4_sm100_token_logprobs_scratch_extent_host_v1": (Result, [c_uint32, c_uint32, c_uint32, POINTER(c_uint64)]),
     "augur_cuda_nvfp4_sm100_token_logprobs_preflight_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(TokenLogprobsArgs)]),
     "augur_cuda_nvfp4_sm100_token_logprobs_prevalidated_submit_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(TokenLogprobsArgs)]),

@@ -233,34 +233,49 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
     }
     for (uint32_t i = threadIdx.x; i < kOnesBytes / 16; i += kThreads) reinterpret_cast<uint4*>(ones_smem)[i] = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
     // Everything above runs while the launch before this one drains; from here on its results are read.
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    {   // units of every sequence, and their running sum: four neighbouring sequences a thread
+    // Units of every sequence, and their running sum.
+    auto units_of = [&](uint32_t b) {
+        const int32_t from = p.token_starts[b], to = p.token_starts[b + 1];
+        int32_t length = p.lengths[b];
+        const int32_t room = static_cast<int32_t>(p.table_pages << p.page_shift);
+        const bool rows_fit = from >= 0 && to <= static_cast<int32_t>(p.rows) && to >= from && to - from <= static_cast<int32_t>(p.max_new);
+        if (!rows_fit && blockIdx.x == 0) atomicCAS(status, 0u, kStatusRows);
+        if (length > room) {
+            length = room;
+            if (blockIdx.x == 0) atomicCAS(status, 0u, kStatusPage);
+        }
+        if (length < 0) length = 0;
+        const uint32_t tokens = rows_fit ? static_cast<uint32_t>(to - from) : 0;
+        st->row[b] = static_cast<uint32_t>(from);
+        st->length[b] = static_cast<uint32_t>(length) | tokens << (kMaxTokensLog2 + 1);
+        if (!tokens && p.joins < p.spans && blockIdx.x == b % p.spans) {
+            for (uint32_t h = 0; h < p.kv_heads; ++h) p.records[b * p.kv_heads + h] = JoinRecord{};   // an idle slot's
+        }
+        return !tokens ? 0 : length ? (static_cast<uint32_t>(length) + kUnit - 1) / kUnit : 1;   // a row that sees nothing is written too
+    };
+    if (p.sequences <= 32) {   // every warp for itself, all with the same result
+        const uint32_t count = lane < p.sequences ? units_of(lane) : 0;
+        uint32_t before = count;
+#pragma unroll
+        for (uint32_t step = 1; step < 32; step *= 2) {
+            const uint32_t other = __shfl_up_sync(0xffffffffu, before, step);
+            if (lane >= step) before += other;
+        }
+        if (lane < p.sequences) st->units[lane + 1] = before;
+        if (lane == 0) st->units[0] = 0;
+        __syncwarp();
+    } else {   // four neighbouring sequences a thread
         static_assert(kMaxSequences == 4 * kThreads, "four sequences a thread");
         uint32_t count[4], sum = 0;
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
             const uint32_t b = 4 * threadIdx.x + i;
-            count[i] = 0;
-            if (b < p.sequences) {
-                const int32_t from = p.token_starts[b], to = p.token_starts[b + 1];
-                int32_t length = p.lengths[b];
-                const int32_t room = static_cast<int32_t>(p.table_pages << p.page_shift);
-                const bool rows_fit = from >= 0 && to <= static_cast<int32_t>(p.rows) && to >= from && to - from <= static_cast<int32_t>(p.max_new);
-                if (!rows_fit && blockIdx.x == 0) atomicCAS(status, 0u, kStatusRows);
-                if (length > room) {
-                    length = room;
-                    if (blockIdx.x == 0) atomicCAS(status, 0u, kStatusPage);
-                }
-                if (length < 0) length = 0;
-                const uint32_t tokens = rows_fit ? static_cast<uint32_t>(to - from) : 0;
-                st->row[b] = static_cast<uint32_t>(from);
-                st->length[b] = static_cast<uint32_t>(length) | tokens << (kMaxTokensLog2 + 1);
-                if (!tokens && p.joins < p.spans && blockIdx.x == b % p.spans) {
-                    for (uint32_t h = 0; h < p.kv_heads; ++h) p.records[b * p.kv_heads + h] = JoinRecord{};   // an idle slot's
-                }
-                if (tokens) count[i] = length ? (static_cast<uint32_t>(length) + kUnit - 1) / kUnit : 1;   // a row that sees nothing is written too
-            }
+            count[i] = b < p.sequences ? units_of(b) : 0;
             sum += count[i];
         }
         uint32_t before = sum;
@@ -271,9 +286,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
         }
         if (lane == 31) st->scan[warp] = before;
         before -= sum;
-        tc_fence_before();
         __syncthreads();
-        tc_fence_after();
 #pragma unroll
         for (uint32_t w = 0; w < kThreads / 32; ++w) before += w < warp ? st->scan[w] : 0;
 #pragma unroll
@@ -671,14 +684,18 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
         // a part a thread: its weight 2^(reference - largest reference)
         float2 mine = make_float2(-INFINITY, 0.0f);
         if (threadIdx.x < parts) mine = reinterpret_cast<const float2*>(p.parts + static_cast<uint64_t>(2 * p.spans) * kN * kHeadDim)[part(threadIdx.x) * kN + query];
-        // the first of this thread's part of the outputs, on their way meanwhile
+        // this thread's part of the outputs of the first parts, on their way meanwhile
         const float4* const from = reinterpret_cast<const float4*>(p.parts + static_cast<uint64_t>(query) * kHeadDim) + lane;
-        constexpr uint32_t kAhead = 4;
+        constexpr uint32_t kAhead = 10;
         float4 v[kAhead];
+        auto load = [&](uint32_t first) {
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            if (share + i * kShares < parts) v[i] = from[part(share + i * kShares) * (kN * kLanes)];
-        }
+            for (uint32_t i = 0; i < kAhead; ++i) {
+                v[i] = make_float4(0, 0, 0, 0);
+                if (first + i * kShares < parts) v[i] = from[part(first + i * kShares) * (kN * kLanes)];
+            }
+        };
+        load(share);
         float most = mine.x;
 #pragma unroll
         for (uint32_t step = 16; step; step /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, step));
@@ -695,16 +712,14 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
         if (threadIdx.x % 32 == 0) wide[1][warp] = all;
         __syncthreads();
         float4 sum = make_float4(0, 0, 0, 0);
-        auto add = [&](const float4& x, uint32_t i) {
-            const float f = weight[i];
-            if (f != 0.0f) sum.x = fmaf(f, x.x, sum.x), sum.y = fmaf(f, x.y, sum.y), sum.z = fmaf(f, x.z, sum.z), sum.w = fmaf(f, x.w, sum.w);
-        };
+        for (uint32_t first = share; first < parts; first += kAhead * kShares) {
+            if (first != share) load(first);
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            if (share + i * kShares < parts) add(v[i], share + i * kShares);
+            for (uint32_t i = 0; i < kAhead; ++i) {
+                const float f = first + i * kShares < parts ? weight[first + i * kShares] : 0.0f;
+                if (f != 0.0f) sum.x = fmaf(f, v[i].x, sum.x), sum.y = fmaf(f, v[i].y, sum.y), sum.z = fmaf(f, v[i].z, sum.z), sum.w = fmaf(f, v[i].w, sum.w);
+            }
         }
-#pragma unroll 4
-        for (uint32_t i = share + kAhead * kShares; i < parts; i += kShares) add(from[part(i) * (kN * kLanes)], i);
         sums[share][lane] = sum;
         __syncthreads();
         if (share == 0) {
