@@ -41,8 +41,7 @@ constexpr uint32_t kMaxAlternatives = AUGUR_NVFP4_SM100_MAX_ALTERNATIVES;
 constexpr uint32_t kFew = 64;                       // collected before the floor moves up
 constexpr uint32_t kBlock = 8;                      // units between two meetings of the threads
 constexpr uint32_t kGroups = kThreads / 2;          // maxima that a floor is found from
-// Collected at most, above an exact floor: the elements of k groups in a unit, or k candidates of each of the two parts of k groups at a join,
-// on top of the few that are there.
+// Collected at most, above an exact floor of a unit: the elements of k groups, on top of the few that are there. (A join wants less, and a key for each part.)
 constexpr uint32_t kRoom = kMaxAlternatives * 2 * kMaxAlternatives;
 constexpr uint32_t kBuffer = kFew + kRoom;
 static_assert(kMaxAlternatives * 2 * kPer <= kRoom && kMaxAlternatives <= kFew && kMaxAlternatives <= kGroups, "room for what is collected");
@@ -254,7 +253,7 @@ __device__ void prune(Shared& sh, uint32_t k) {
         rank_into_best(sh, sh.few, sh.few_count, k);
     }
     if (threadIdx.x < k) sh.buffer[threadIdx.x] = sh.best[threadIdx.x];
-    if (threadIdx.x == 0) sh.count = count < k ? count : k;   // (of a join: k, zeros among them)
+    if (threadIdx.x == 0) sh.count = count < k ? count : k;
     __syncthreads();
 }
 
@@ -512,23 +511,54 @@ __global__ void __launch_bounds__(kThreads, kSelect ? 3 : 4) token_logprobs_kern
             float4 f = make_float4(0, 0, 0, 0);
             if (mine) f = __ldcg(reinterpret_cast<const float4*>(part_of(from + threadIdx.x)));
             if constexpr (kSelect) {
-                // All candidates of as many parts as there is room for at once, four lanes a part: their loads are under way together. (Following each part's
-                // list down to a floor found from the lists' heads took up to k loads one after the other: 8 rows 21.4 us, 64 rows 44.8.)
-                const uint32_t even = (k + 1) / 2 * 2, at_once = kRoom / even;
-                for (uint32_t c0 = from; c0 <= to; c0 += at_once) {
-                    const uint32_t parts = to - c0 + 1 < at_once ? to - c0 + 1 : at_once, before = c0 == from ? 0 : even;
-                    if (c0 != from && threadIdx.x == 0 && even > k) sh.buffer[k] = 0;
-                    for (uint32_t c = threadIdx.x / 4; c < parts; c += kThreads / 4) {
-                        const Part* const one = part_of(c0 + c);
-                        for (uint32_t i = 2 * (threadIdx.x % 4); i < k; i += 8) {
-                            ulonglong2 two = __ldcg(reinterpret_cast<const ulonglong2*>(&one->best[i]));
-                            if (i + 1 == k) two.y = 0;
-                            *reinterpret_cast<ulonglong2*>(&sh.buffer[before + c * even + i]) = two;
-                        }
+                // A floor from one candidate of each of the P parts, its depth-th: the j-th largest of those, j depth >= k, is reached by k candidates, and by at
+                // most j k + (P - j) (depth - 1) < 1024. All loads are under way together. (Ranking all candidates of 61 parts took 6100 cycles;
+                // following each part's list down to a floor, up to k loads one after the other, 8 rows 21.4 us.)
+                const uint32_t parts = to - from + 1, depth = (k + parts - 1) / parts, wanted = (k + depth - 1) / depth;
+                static_assert(kRoom / 2 + kMaxSpans <= kBuffer && kMaxAlternatives * kMaxAlternatives <= kRoom / 2, "candidates, and a key for each part behind them");
+                Key* const heads = sh.buffer + kRoom / 2;
+                for (uint32_t c = threadIdx.x; c < parts; c += kThreads) heads[c] = __ldcg(&part_of(from + c)->best[depth - 1]);
+                constexpr uint32_t kHeld = kMaxAlternatives / 8;   // pairs of candidates that one of the four lanes of a part has
+                ulonglong2 held[kHeld];
+                auto load = [&](uint32_t c) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kHeld; ++i) {
+                        const uint32_t at = 2 * (threadIdx.x % 4) + 8 * i;
+                        held[i] = make_ulonglong2(0, 0);
+                        if (c < parts && at < k) held[i] = __ldcg(reinterpret_cast<const ulonglong2*>(&part_of(from + c)->best[at]));
+                        if (at + 1 >= k) held[i].y = 0;
                     }
-                    if (threadIdx.x == 0) sh.count = before + parts * even;
-                    prune(sh, k);
+                };
+                load(threadIdx.x / 4);
+                if (threadIdx.x == 0) sh.count = 0, sh.floor = 0;
+                __syncthreads();
+                for (uint32_t c = threadIdx.x / 4; c < (parts + 7) / 8 * 8; c += kThreads / 4) {   // (whole warps)
+                    const Key value = c < parts ? heads[c] : 0;
+                    uint32_t rank = 0;
+                    for (uint32_t i = threadIdx.x % 4; i < parts; i += 4) rank += heads[i] > value ? 1u : 0u;
+                    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+                    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+                    if (value && rank == wanted - 1) sh.floor = value;
                 }
+                __syncthreads();
+                const Key least = sh.floor;    // 0: fewer than k candidates in all
+                for (uint32_t c = threadIdx.x / 4; c < (parts + 7) / 8 * 8; c += kThreads / 4) {
+                    if (c != threadIdx.x / 4) load(c);
+                    uint32_t passed = 0, after;
+#pragma unroll
+                    for (uint32_t i = 0; i < kHeld; ++i) {
+                        passed += held[i].x && held[i].x >= least ? 1 : 0;
+                        passed += held[i].y && held[i].y >= least ? 1 : 0;
+                    }
+                    uint32_t at = reserve(&sh.count, passed, &after);
+#pragma unroll
+                    for (uint32_t i = 0; i < kHeld; ++i) {
+                        if (held[i].x && held[i].x >= least) sh.buffer[at++] = held[i].x;
+                        if (held[i].y && held[i].y >= least) sh.buffer[at++] = held[i].y;
+                    }
+                }
+                __syncthreads();
+                rank_into_best(sh, sh.buffer, sh.count, k);
             }
             s = Statistics{mine ? f.x : -INFINITY, f.y, f.z};
             for (uint32_t c = from + threadIdx.x + kThreads; c <= to; c += kThreads) {
