@@ -13,7 +13,7 @@
 // values equal, or rising) take the slow way: the k-th largest of 128 maxima of distinct numbers is a floor that only k groups of elements
 // reach, so what is collected is bounded whatever the row looks like.
 //
-// Work: rows in units of 4096 elements, dealt out evenly as one span of units per CTA (three CTAs an SM), so a row may begin
+// Work: rows in units of 16 KB, dealt out evenly as one span of units per CTA (three CTAs an SM), so a row may begin
 // in one CTA and end in another. Such a row's parts (statistics and k candidates) meet in the plan's scratch; the CTA that comes last
 // joins them in the order of the spans.
 //
@@ -33,8 +33,8 @@ namespace {
 static_assert(sizeof(augur_cuda_nvfp4_sm100_token_logprobs_args_v1) == 128, "log probabilities ABI");
 
 constexpr uint32_t kThreads = 256, kWarps = kThreads / 32;
-constexpr uint32_t kPer = 16;                       // elements of a thread and unit
-constexpr uint32_t kUnit = kThreads * kPer;
+constexpr uint32_t kVectors = 4;                    // of 16 bytes that a thread has in a unit: 4096 F32 elements, 8192 BF16
+constexpr uint32_t kUnitBytes = kThreads * kVectors * 16, kMostPer = kVectors * 8;
 constexpr uint32_t kMaxSpans = 1024;                // of a launch
 constexpr uint32_t kRingBytes = 48 * 1024;          // what a CTA has copied ahead
 constexpr uint32_t kMaxAlternatives = AUGUR_NVFP4_SM100_MAX_ALTERNATIVES;
@@ -44,7 +44,7 @@ constexpr uint32_t kGroups = kThreads / 2;          // maxima that a floor is fo
 // Collected at most, above an exact floor of a unit: the elements of k groups, on top of the few that are there. (A join wants less, and a key for each part.)
 constexpr uint32_t kRoom = kMaxAlternatives * 2 * kMaxAlternatives;
 constexpr uint32_t kBuffer = kFew + kRoom;
-static_assert(kMaxAlternatives * 2 * kPer <= kRoom && kMaxAlternatives <= kFew && kMaxAlternatives <= kGroups, "room for what is collected");
+static_assert(kMaxAlternatives * 2 * kMostPer <= kRoom && kMaxAlternatives <= kFew && kMaxAlternatives <= kGroups, "room for what is collected");
 constexpr uint32_t kSome = kMaxAlternatives * 2 * (kBuffer / kThreads + 1);   // of the buffer, above an exact floor under its strided maxima
 constexpr float kLowest = -200.0f;                  // e^-200 is 0 in F32: differences below it need not be told apart, infinities among them
 
@@ -110,14 +110,40 @@ struct Statistics {
 
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-// 16 bytes of logits.
-__device__ __forceinline__ void widen(const uint4& f, float* v, float) {
-    v[0] = __uint_as_float(f.x), v[1] = __uint_as_float(f.y), v[2] = __uint_as_float(f.z), v[3] = __uint_as_float(f.w);
+// 16 bytes of logits as they lie in memory: elements 2 i and 2 i + 1; the largest of four times 16 bytes; -infinity in the place of element i.
+__device__ __forceinline__ uint32_t word_of(const uint4& f, uint32_t i) { return i == 0 ? f.x : i == 1 ? f.y : i == 2 ? f.z : f.w; }
+__device__ __forceinline__ float2 two_of(const uint4& f, uint32_t i, float) { return make_float2(__uint_as_float(word_of(f, 2 * i)), __uint_as_float(word_of(f, 2 * i + 1))); }
+__device__ __forceinline__ float2 two_of(const uint4& f, uint32_t i, __nv_bfloat16) {
+    const uint32_t word = word_of(f, i);
+    return make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u));
 }
-__device__ __forceinline__ void widen(const uint4& f, float* v, __nv_bfloat16) {
-    const uint32_t word[4] = {f.x, f.y, f.z, f.w};
+__device__ __forceinline__ float largest(const uint4 (&f)[kVectors], float) {
+    float most = __uint_as_float(f[0].x);
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(word[i] << 16), v[2 * i + 1] = __uint_as_float(word[i] & 0xffff0000u);
+    for (uint32_t j = 0; j < kVectors; ++j) {
+        most = max_nan(most, __uint_as_float(f[j].x), __uint_as_float(f[j].y));
+        most = max_nan(most, __uint_as_float(f[j].z), __uint_as_float(f[j].w));
+    }
+    return most;
+}
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    uint32_t c;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    return c;
+}
+__device__ __forceinline__ float largest(const uint4 (&f)[kVectors], __nv_bfloat16) {
+    uint32_t most = f[0].x;
+#pragma unroll
+    for (uint32_t j = 0; j < kVectors; ++j) most = max2_nan(max2_nan(most, max2_nan(f[j].x, f[j].y)), max2_nan(f[j].z, f[j].w));
+    return max_nan(__uint_as_float(most << 16), __uint_as_float(most & 0xffff0000u));
+}
+__device__ __forceinline__ void set_lowest(uint4& f, uint32_t i, bool where, float) {
+    uint32_t& word = i == 0 ? f.x : i == 1 ? f.y : i == 2 ? f.z : f.w;
+    word = where ? 0xff800000u : word;
+}
+__device__ __forceinline__ void set_lowest(uint4& f, uint32_t i, bool where, __nv_bfloat16) {
+    uint32_t& word = i / 2 == 0 ? f.x : i / 2 == 1 ? f.y : i / 2 == 2 ? f.z : f.w;
+    word = !where ? word : i % 2 ? (word & 0xffffu) | 0xff800000u : (word & 0xffff0000u) | 0xff80u;
 }
 
 struct Meeting {
@@ -296,7 +322,7 @@ template <class T, bool kSelect>
 __global__ void __launch_bounds__(kThreads, kSelect ? 3 : 4) token_logprobs_kernel(const __grid_constant__ LogprobsParams p) {
     __shared__ std::conditional_t<kSelect, Shared, Meeting> sh;
     extern __shared__ uint4 ring[];                                             // [stages][vectors of a thread][threads]
-    constexpr uint32_t kVector = 16 / sizeof(T), kVectors = kPer / kVector, kStages = kRingBytes / (kUnit * sizeof(T));
+    constexpr uint32_t kVector = 16 / sizeof(T), kPer = kVectors * kVector, kUnit = kThreads * kPer, kStages = kRingBytes / kUnitBytes;
     const uint32_t k = kSelect ? p.alternatives : 0;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -389,6 +415,7 @@ __global__ void __launch_bounds__(kThreads, kSelect ? 3 : 4) token_logprobs_kern
             if (threadIdx.x == 0) sh.count = sh.few_count;
             for (uint32_t u = block; u < until; ++u) {
                 Key key[kPer], mine = 0;
+#pragma unroll 1
                 for (uint32_t j = 0; j < kPer; ++j) {
                     const uint32_t i = u * kUnit + (j / kVector * kThreads + threadIdx.x) * kVector + j % kVector - shift;
                     key[j] = i < p.vocabulary ? make_key(as_float(x[i]), i) : 0;
@@ -405,20 +432,18 @@ __global__ void __launch_bounds__(kThreads, kSelect ? 3 : 4) token_logprobs_kern
         for (uint32_t u = first; u < stop; ++u) {
             fetch();
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-            float v[kPer];
+            uint4 raw[kVectors];
 #pragma unroll
-            for (uint32_t j = 0; j < kVectors; ++j) widen(ring[(stage * kVectors + j) * kThreads + threadIdx.x], v + j * kVector, T{});
+            for (uint32_t j = 0; j < kVectors; ++j) raw[j] = ring[(stage * kVectors + j) * kThreads + threadIdx.x];
             [[maybe_unused]] const uint32_t stage_now = stage;
             if (++stage == kStages) stage = 0;
             auto index_of = [&](uint32_t j) { return u * kUnit + (j / kVector * kThreads + threadIdx.x) * kVector + j % kVector - shift; };   // below the row: huge
             const bool inside = (u || shift == 0) && (u + 1) * kUnit - shift <= p.vocabulary;
             if (!inside) {
 #pragma unroll
-                for (uint32_t j = 0; j < kPer; ++j) v[j] = index_of(j) < p.vocabulary ? v[j] : -INFINITY;
+                for (uint32_t j = 0; j < kPer; ++j) set_lowest(raw[j / kVector], j % kVector, index_of(j) >= p.vocabulary, T{});
             }
-            float most = max_nan(v[0], v[1]);
-#pragma unroll
-            for (uint32_t j = 2; j < kPer; j += 2) most = max_nan(most, v[j], v[j + 1]);
+            const float most = largest(raw, T{});
             // One reference for the warp: a new maximum in one of 32 lanes is frequent, in a unit of the whole warp soon rare.
             float warp_most;
             asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(warp_most) : "f"(most));
@@ -428,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, kSelect ? 3 : 4) token_logprobs_kern
             float2 sum[2] = {make_float2(s.sum, 0.0f), make_float2(0.0f, 0.0f)}, moment[2] = {make_float2(s.moment, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
             for (uint32_t j = 0; j < kPer; j += 2) {
-                float2 below = __fadd2_rn(make_float2(v[j], v[j + 1]), minus_base);
+                float2 below = __fadd2_rn(two_of(raw[j / kVector], j % kVector / 2, T{}), minus_base);
                 below.x = max_nan(below.x, kLowest), below.y = max_nan(below.y, kLowest);
                 const float2 power = __fmul2_rn(below, log2e), weight = make_float2(exp2_fast(power.x), exp2_fast(power.y));
                 sum[j / 2 % 2] = __fadd2_rn(sum[j / 2 % 2], weight);
@@ -440,7 +465,10 @@ __global__ void __launch_bounds__(kThreads, kSelect ? 3 : 4) token_logprobs_kern
                 auto collect = [&](auto passes) {
                     uint32_t mask = 0, after;
 #pragma unroll
-                    for (uint32_t j = 0; j < kPer; ++j) mask |= passes(v[j]) ? 1u << j : 0;
+                    for (uint32_t j = 0; j < kPer; j += 2) {
+                        const float2 two = two_of(raw[j / kVector], j % kVector / 2, T{});
+                        mask |= (passes(two.x) ? 1u << j : 0) | (passes(two.y) ? 2u << j : 0);
+                    }
                     if (!inside) {
 #pragma unroll
                         for (uint32_t j = 0; j < kPer; ++j) mask &= index_of(j) < p.vocabulary ? ~0u : ~(1u << j);
@@ -665,7 +693,7 @@ void launch_logprobs(cudaStream_t stream, const LogprobsParams& p) {
 uint32_t units_of(const augur_cuda_nvfp4_sm100_token_logprobs_args_v1* a) {
     const uint32_t size = a->logits_type == AUGUR_NVFP4_SM100_LOGITS_F32 ? 4 : 2;
     const bool aligned = a->logits % 16 == 0 && (a->rows == 1 || a->row_stride * size % 16 == 0);
-    return (a->vocabulary + (aligned ? 0 : 16 / size - 1) + kUnit - 1) / kUnit;
+    return (a->vocabulary + (aligned ? 0 : 16 / size - 1) + kUnitBytes / size - 1) / (kUnitBytes / size);
 }
 uint32_t most_spans(uint32_t sm_count, uint32_t alternatives) {
     const uint32_t ctas = (alternatives ? 3 : 4) * sm_count;
