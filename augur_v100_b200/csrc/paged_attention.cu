@@ -9,10 +9,11 @@
 //   S^T[key][query]   = K Q^T          K as it lies in the pages (rows of head_dim: K-major), 128 keys a tile
 //   O^T[dim][query]  += V^T P^T        V as it lies in the pages (the key is the k dimension: MN-major)
 //
-// A thread of the four softmax warps holds one key and all queries of S^T. The running maximum is a reference that only
+// A thread of the four softmax warps holds one key and, up to 16 at a time, the queries of S^T. The running maximum is a reference that only
 // moves when a score passes it by more than 2^8: then O^T is scaled down in tensor memory; otherwise a tile costs a thread one comparison, one
-// exponential and one 2-byte store per query. p is rounded to BF16 for the second product (its relative error of 2^-9 averages
-// out over the keys and stays below the output's own rounding) and counted in the denominator as rounded.
+// exponential and two 2-byte stores per query. p enters the second product as two BF16 terms, good to 2^-16 of it: with one its rounding was as
+// large an error as the output's own. The terms lie side by side on the narrow operand, where they cost next to nothing (as products one
+// behind the other a pass over V took the pipe twice: 64 ragged sequences 167 us against 155). The denominators are the same terms times ones.
 //
 // Work: the cached tokens of all (sequence, key-value head) pairs in units of 64, dealt out evenly as one span of units per SM. A pair
 // that lies in several spans leaves an unnormalised part per span in the plan's scratch, and a second launch joins those, in
@@ -78,15 +79,17 @@ struct State {
 template <uint32_t kHeadDim, uint32_t kN>
 struct Shape {
     static constexpr uint32_t kChunks = kHeadDim / 64, kHalves = kHeadDim / 128;
-    static constexpr uint32_t kQueryBytes = kN * kHeadDim * 2, kQueryBuffers = kQueryBytes > 24 * 1024 ? 1 : 2;
-    static constexpr uint32_t kWeightBytes = kN * kTile * 2;
+    // Columns of S^T (the MMA wants 16 at least), and of P^T and O^T: two BF16 terms of P side by side. kBlock of them are worked on at a time.
+    static constexpr uint32_t kScores = kN < 16 ? 16 : kN, kTerms = 2 * kN, kBlock = kN < 16 ? kN : 16;
+    static constexpr uint32_t kQueryBytes = kScores * kHeadDim * 2, kQueryBuffers = kQueryBytes > 24 * 1024 ? 1 : 2;
+    static constexpr uint32_t kWeightBytes = kTerms * kTile * 2;
     static constexpr uint32_t kFixed = 1024 + kOnesBytes + sizeof(State) + kQueryBuffers * kQueryBytes + 2 * kWeightBytes;
     static constexpr uint32_t kRoom = kSmemLimit - kFixed;
     static constexpr uint32_t kSlots = kRoom / kSlotBytes / 2 * 2 > 16 ? 16 : kRoom / kSlotBytes / 2 * 2;
     static constexpr uint32_t kSmem = kFixed + kSlots * kSlotBytes;
     // tensor memory: two of S^T, O^T in halves of 128 dims, the denominators
-    static constexpr uint32_t kColumns = (3 + kHalves) * kN, kTmem = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
-    static_assert(kSlots >= 2 * kChunks && kSmem <= kSmemLimit && kColumns <= 512, "a CTA's memory");
+    static constexpr uint32_t kColumns = 2 * kScores + (kHalves + 1) * kTerms, kTmem = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
+    static_assert(kSlots >= kChunks + 2 /* K of a tile and half of the V before it */ && kSmem <= kSmemLimit && kColumns <= 512, "a CTA's memory");
 };
 
 // A CTA's way through its span: one (sequence, head) after the other, in each the keys [key, key_end).
@@ -173,12 +176,21 @@ __device__ __forceinline__ void mma_block(uint32_t d, uint32_t a, uint32_t b, ui
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void load_columns16(uint32_t taddr, uint32_t* v) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
-                   "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                 : "r"(taddr)
-                 : "memory");
+template <uint32_t kCount>
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t* v) {
+    static_assert(kCount == 8 || kCount == 16, "columns at a time");
+    if constexpr (kCount == 8) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                     : "r"(taddr)
+                     : "memory");
+    } else {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                       "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                     : "r"(taddr)
+                     : "memory");
+    }
 }
 __device__ __forceinline__ void store_columns16(uint32_t taddr, const uint32_t* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
@@ -301,7 +313,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
     const uint32_t total = st->units[p.sequences] * p.kv_heads, spans = total < p.spans ? total : p.spans;
     const uint32_t base = spans ? total / spans : 0, extra = total - base * spans;   // spans of `base` units, the first `extra` of one more
     const uint32_t from = blockIdx.x * base + (blockIdx.x < extra ? blockIdx.x : extra), to = blockIdx.x < spans ? from + base + (blockIdx.x < extra ? 1 : 0) : from;
-    const uint32_t tmem = st->tmem, tmem_out = tmem + 2 * kN, tmem_sum = tmem_out + S::kHalves * kN;   // (one behind the other: scaled together)
+    const uint32_t tmem = st->tmem, tmem_out = tmem + 2 * S::kScores, tmem_sum = tmem_out + S::kHalves * S::kTerms;   // (one behind the other: scaled together)
     const uint32_t group = p.query_heads / p.kv_heads;
 
     if (warp == 0 || warp == 3) {
@@ -355,8 +367,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer: S of a tile, then O of the tile before it ----------------
-        constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kN >> 3) << 17) | ((kTile >> 4) << 24);   // F32 += BF16 x BF16
-        constexpr uint32_t idesc_values = idesc | (1u << 15);                                                        // V is MN-major
+        constexpr uint32_t idesc_any = (1u << 4) | (1u << 7) | (1u << 10) | ((kTile >> 4) << 24);   // F32 += BF16 x BF16
+        constexpr uint32_t idesc = idesc_any | ((S::kScores >> 3) << 17), idesc_sum = idesc_any | ((S::kTerms >> 3) << 17), idesc_values = idesc_sum | (1u << 15);                                                        // V is MN-major
         const uint32_t slots = low_word(smem_u32(smem), 16), slots_values = low_word(smem_u32(smem), kSlotBytes);
         const uint32_t queries = low_word(smem_u32(query_smem), 16), weights = low_word(smem_u32(weight_smem), 16), ones = low_word(smem_u32(ones_smem), 128);
         Tiles ahead, now;
@@ -371,7 +383,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             for (uint32_t c = 0; c < S::kChunks; ++c) {
                 if (!warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusMma)) return false;
                 tc_fence_after();
-                mma_block<kHighSwizzled, 2>(tmem + buffer * kN, slots + slot * (kSlotBytes >> 4), queries + ((query * S::kQueryBytes + c * kN * 128) >> 4), idesc, c, 4);
+                mma_block<kHighSwizzled, 2>(tmem + buffer * S::kScores, slots + slot * (kSlotBytes >> 4), queries + ((query * S::kQueryBytes + c * S::kScores * 128) >> 4), idesc, c, 4);
                 commit(empty + 8 * slot);
                 if (++slot == S::kSlots) slot = 0, phase ^= 1;
             }
@@ -392,16 +404,16 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             tc_fence_after();
             const uint32_t follows = !now.first(), weights_now = weights + ((buffer * S::kWeightBytes) >> 4);
             // denominators: the sum over the keys as one more product, into every lane
-            mma_block<kHighPlain, 0>(tmem_sum, ones, weights_now, idesc, follows, steps);
-            if (steps > 4) mma_block<kHighPlain, 0>(tmem_sum, ones, weights_now + (kN * 128 >> 4), idesc, 1, steps - 4);
+            mma_block<kHighPlain, 0>(tmem_sum, ones, weights_now, idesc_sum, follows, steps);
+            if (steps > 4) mma_block<kHighPlain, 0>(tmem_sum, ones, weights_now + (S::kTerms * 128 >> 4), idesc_sum, 1, steps - 4);
             for (uint32_t h = 0; alive && h < S::kHalves; ++h) {
                 for (uint32_t c = 0; c < 2; ++c) alive = alive && warp_look_wait(full + 8 * (slot + c), phase, abort_flag, status, kStatusProduct);
                 if (!alive) break;
                 tc_fence_after();
                 // 16 keys: 16 rows of V, 32 bytes of a row of P
-                const uint32_t a = slots_values + slot * (kSlotBytes >> 4), d = tmem_out + h * kN;
+                const uint32_t a = slots_values + slot * (kSlotBytes >> 4), d = tmem_out + h * S::kTerms;
                 mma_block<kHighSwizzled, (16 * 128 >> 4)>(d, a, weights_now, idesc_values, follows, steps);
-                if (steps > 4) mma_block<kHighSwizzled, (16 * 128 >> 4)>(d, a + 4 * (16 * 128 >> 4), weights_now + (kN * 128 >> 4), idesc_values, 1, steps - 4);
+                if (steps > 4) mma_block<kHighSwizzled, (16 * 128 >> 4)>(d, a + 4 * (16 * 128 >> 4), weights_now + (S::kTerms * 128 >> 4), idesc_values, 1, steps - 4);
                 commit(empty + 8 * slot);
                 commit(empty + 8 * (slot + 1));
                 slot += 2;
@@ -424,10 +436,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             if (!warp_look_wait(query_empty + 8 * buffer, ((S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1) ^ 1, abort_flag, status, kStatusQuery)) break;
             // 16 bytes a copy, all of them under way together (as loads and stores they waited for one another: 1000 cycles a row)
             constexpr uint32_t kPieces = kHeadDim / 8, kRows = 32 / kPieces;
-            const uint32_t piece = lane % kPieces, to = smem_u32(query_smem) + buffer * S::kQueryBytes + (piece >> 3) * (kN * 128);
+            const uint32_t piece = lane % kPieces, to = smem_u32(query_smem) + buffer * S::kQueryBytes + (piece >> 3) * (S::kScores * 128);
             const __nv_bfloat16* const from_here = p.query + (static_cast<uint64_t>(first_row) * p.query_heads + walk.head * group) * kHeadDim + piece * 8;
             uint32_t token = 0, head = lane / kPieces;
-            for (uint32_t row = lane / kPieces; row < kN; row += kRows, head += kRows) {
+            for (uint32_t row = lane / kPieces; row < S::kScores; row += kRows, head += kRows) {
                 while (head >= group) head -= group, ++token;
                 const bool live = row < queries;
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + row * 128 + (((piece & 7) ^ (row & 7)) << 4)),
@@ -444,6 +456,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
         // ---------------- softmax: thread = key of a tile, then dim of the output ----------------
         const uint32_t thread = threadIdx.x - 128, quadrant = warp & 3, lanes = (quadrant * 32) << 16;
         const uint32_t box_shift = p.page_shift < 6 ? p.page_shift : 6, boxes = kTile >> box_shift, all_boxes = (1u << boxes) - 1;
+        constexpr uint32_t kBlock = S::kBlock;
         uint32_t tile = 0, meetings = 0;
         JoinRecord record{};
         // The four warps meet (a bounded wait, where a named barrier would hang on a warp that gave up).
@@ -477,26 +490,26 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                 const bool my_key = thread < count && (there >> (thread >> box_shift) & 1);
                 // 16 queries' scores of this thread's key. Every step below goes through them again from tensor memory in a rolled loop: with all of 48
                 // queries in registers and the loops unrolled, a tile cost 4200 cycles more, for want of instructions from their cache.
-                float s[16];
+                float s[kBlock];
                 auto scores = [&](uint32_t c0) {
-                    if (kN == 16 && c0 != 0) return;   // (there already)
-                    load_columns16(tmem + lanes + buffer * kN + c0 % kN, reinterpret_cast<uint32_t*>(s));
+                    if (kN == kBlock && c0 != 0) return;   // (there already)
+                    load_columns<kBlock>(tmem + lanes + buffer * S::kScores + c0 % kN, reinterpret_cast<uint32_t*>(s));
                     tc_wait_ld();
 #pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) s[i] *= p.scale_log2;
+                    for (uint32_t i = 0; i < kBlock; ++i) s[i] *= p.scale_log2;
                     if (masked) {
 #pragma unroll
-                        for (uint32_t i = 0; i < 16; ++i) s[i] = my_key && static_cast<int32_t>(key + thread) < st->limit[c0 % kN + i] ? s[i] : -INFINITY;
+                        for (uint32_t i = 0; i < kBlock; ++i) s[i] = my_key && static_cast<int32_t>(key + thread) < st->limit[c0 % kN + i] ? s[i] : -INFINITY;
                     }
                 };
-                constexpr uint32_t kAgain = kN == 16 ? kN : 0;   // for 16 queries they stay in registers
+                constexpr uint32_t kAgain = kN == kBlock ? kN : 0;   // up to 16 queries' stay in registers
                 bool above = key == walk.key;   // a pair's first tile sets the references
                 if (!above) {
 #pragma unroll 1
-                    for (uint32_t c = 0; c < kN; c += 16) {
+                    for (uint32_t c = 0; c < kN; c += kBlock) {
                         scores(c);
 #pragma unroll
-                        for (uint32_t i = 0; i < 16; ++i) above |= s[i] > st->reference[c + i] + kSlack;
+                        for (uint32_t i = 0; i < kBlock; ++i) above |= s[i] > st->reference[c + i] + kSlack;
                     }
                     above = __any_sync(0xffffffffu, above);
                     if (lane == 0) reinterpret_cast<uint8_t*>(&st->needs[buffer])[quadrant] = above;
@@ -511,15 +524,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                 if (above) {
                     // The references move up to the largest scores so far.
 #pragma unroll 1
-                    for (uint32_t c = 0; c < kN; c += 16) {
+                    for (uint32_t c = 0; c < kN; c += kBlock) {
                         scores(c + kAgain);
                         float most = -INFINITY;
 #pragma unroll
-                        for (uint32_t i = 0; i < 16; ++i) {
+                        for (uint32_t i = 0; i < kBlock; ++i) {
                             const float x = warp_max(s[i]);
                             if (lane == i) most = x;
                         }
-                        if (lane < 16) reinterpret_cast<float*>(&st->wide[c + lane])[quadrant] = most;
+                        if (lane < kBlock) reinterpret_cast<float*>(&st->wide[c + lane])[quadrant] = most;
                     }
                     if (!meet()) {
                         alive = false;
@@ -543,12 +556,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                         }
                         tc_fence_after();
 #pragma unroll 1
-                        for (uint32_t c = 0; c < (S::kHalves + 1) * kN; c += 16) {
+                        for (uint32_t c = 0; c < (S::kHalves + 1) * S::kTerms; c += 16) {
                             uint32_t v[16];
-                            load_columns16(tmem_out + lanes + c, v);
+                            load_columns<16>(tmem_out + lanes + c, v);
                             tc_wait_ld();
 #pragma unroll
-                            for (uint32_t i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * st->factor[c % kN + i]);
+                            for (uint32_t i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * st->factor[kN < 16 ? i % kN : c % kN + i]);
                             store_columns16(tmem_out + lanes + c, v);
                         }
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -559,19 +572,22 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                     alive = false;
                     break;
                 }
-                uint8_t* const to_weights = weight_smem + buffer * S::kWeightBytes + (thread >> 6) * (kN * 128) + (thread & 7) * 2;
+                uint8_t* const to_weights = weight_smem + buffer * S::kWeightBytes + (thread >> 6) * (S::kTerms * 128) + (thread & 7) * 2;
                 const uint32_t unit = (thread & 63) >> 3;
 #pragma unroll 1
-                for (uint32_t c = 0; c < kN; c += 16) {
+                for (uint32_t c = 0; c < kN; c += kBlock) {
                     scores(c + kAgain);
-                    float power[16];   // all references before the first store, which the compiler would not move them across
+                    float power[kBlock];   // all references before the first store, which the compiler would not move them across
 #pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) power[i] = st->reference[c + i];
+                    for (uint32_t i = 0; i < kBlock; ++i) power[i] = st->reference[c + i];
 #pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) power[i] = exp2_fast(s[i] - (power[i] == -INFINITY ? 0.0f : power[i]));
+                    for (uint32_t i = 0; i < kBlock; ++i) power[i] = exp2_fast(s[i] - (power[i] == -INFINITY ? 0.0f : power[i]));
 #pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) {
-                        *reinterpret_cast<__nv_bfloat16*>(to_weights + (c + i) * 128 + ((unit ^ (i & 7)) << 4)) = __float2bfloat16_rn(power[i]);
+                    for (uint32_t i = 0; i < kBlock; ++i) {
+                        uint8_t* const to = to_weights + (c + i) * 128 + ((unit ^ (i & 7)) << 4);
+                        const __nv_bfloat16 high = __float2bfloat16_rn(power[i]);
+                        *reinterpret_cast<__nv_bfloat16*>(to) = high;
+                        *reinterpret_cast<__nv_bfloat16*>(to + kN * 128) = __float2bfloat16_rn(power[i] - __bfloat162float(high));
                     }
                 }
                 tc_fence_before();
@@ -615,19 +631,26 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             uint32_t token_end = group;
             uint64_t skipped = 0;
 #pragma unroll 1
-            for (uint32_t c0 = 0; c0 < queries; c0 += 16) {
-                uint32_t v[S::kHalves][16], sums[16];
+            for (uint32_t c0 = 0; c0 < queries; c0 += kBlock) {
+                uint32_t v[S::kHalves + 1][kBlock], low[S::kHalves + 1][kBlock];   // both terms' sums; the last are the denominators
                 if (any) {
-                    load_columns16(tmem_sum + lanes + c0, sums);
 #pragma unroll
-                    for (uint32_t h = 0; h < S::kHalves; ++h) load_columns16(tmem_out + lanes + h * kN + c0, v[h]);
+                    for (uint32_t h = 0; h <= S::kHalves; ++h) {
+                        load_columns<kBlock>(tmem_out + lanes + h * S::kTerms + c0, v[h]);
+                        load_columns<kBlock>(tmem_out + lanes + h * S::kTerms + kN + c0, low[h]);
+                    }
                     tc_wait_ld();
+#pragma unroll
+                    for (uint32_t h = 0; h <= S::kHalves; ++h) {
+#pragma unroll
+                        for (uint32_t i = 0; i < kBlock; ++i) v[h][i] = __float_as_uint(__uint_as_float(v[h][i]) + __uint_as_float(low[h][i]));
+                    }
                 }
 #pragma unroll
-                for (uint32_t i = 0; i < 16; ++i) {
+                for (uint32_t i = 0; i < kBlock; ++i) {
                     const uint32_t c = c0 + i;
                     if (c >= queries) break;
-                    const float all = any ? __uint_as_float(sums[i]) : 0.0f;
+                    const float all = any ? __uint_as_float(v[S::kHalves][i]) : 0.0f;
                     if (alone) {
                         if (c == token_end) token_end += group, skipped += next_token;
                         const float scale = 1.0f / all;
@@ -742,7 +765,10 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
     }
 }
 
-uint32_t query_columns(uint32_t query_heads, uint32_t kv_heads, uint32_t max_new) { return (query_heads / kv_heads * max_new + 15) / 16 * 16; }
+uint32_t query_columns(uint32_t query_heads, uint32_t kv_heads, uint32_t max_new) {
+    const uint32_t queries = query_heads / kv_heads * max_new;
+    return queries <= 8 ? 8 : (queries + 15) / 16 * 16;
+}
 uint32_t launch_spans(uint32_t sm_count) { return sm_count < kMaxCtas ? sm_count : kMaxCtas; }
 
 template <uint32_t kHeadDim, uint32_t kN>
@@ -761,10 +787,23 @@ void launch_attention(cudaStream_t stream, const CUtensorMap& keys, const CUtens
     count_launch(2);
 }
 
+using Launch = void (*)(cudaStream_t, const CUtensorMap&, const CUtensorMap&, const AttentionParams&);
+template <uint32_t kHeadDim>
+Launch launch_of(uint32_t columns) {
+    switch (columns) {
+        case 8: return launch_attention<kHeadDim, 8>;
+        case 16: return launch_attention<kHeadDim, 16>;
+        case 32: return launch_attention<kHeadDim, 32>;
+        case 48: return launch_attention<kHeadDim, 48>;
+        default: return launch_attention<kHeadDim, 64>;
+    }
+}
+
 template <uint32_t kHeadDim>
 cudaError_t configure() {
     constexpr cudaFuncAttribute kSmem = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 16>, kSmem, Shape<kHeadDim, 16>::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 8>, kSmem, Shape<kHeadDim, 8>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 16>, kSmem, Shape<kHeadDim, 16>::kSmem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 32>, kSmem, Shape<kHeadDim, 32>::kSmem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 48>, kSmem, Shape<kHeadDim, 48>::kSmem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 64>, kSmem, Shape<kHeadDim, 64>::kSmem);
@@ -853,8 +892,7 @@ extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_paged_att
         return make_result(AUGUR_CUDA_STATUS_RUNTIME_FAILURE);
     }
     const uint32_t columns = query_columns(a->query_heads, a->layer.kv_heads, a->max_new_tokens);
-    auto launch = head_dim == 256 ? (columns == 16 ? launch_attention<256, 16> : columns == 32 ? launch_attention<256, 32> : columns == 48 ? launch_attention<256, 48> : launch_attention<256, 64>)
-                                  : (columns == 16 ? launch_attention<128, 16> : columns == 32 ? launch_attention<128, 32> : columns == 48 ? launch_attention<128, 48> : launch_attention<128, 64>);
+    auto launch = head_dim == 256 ? launch_of<256>(columns) : launch_of<128>(columns);
     launch(s->stream, keys, values, p);
     return submitted();
 }

@@ -50,8 +50,8 @@ class Batch:
 def attention_reference(batch, scale, layer=0, q=None):
     """(output, bound of the error) of every row in 64 bits, NaN where a row belongs to no sequence.
 
-    The bound, for outputs o = sum w_j v_j: the result is rounded to BF16 once (2^-8 |o|). Every weight is rounded to BF16 before the
-    product and counted in the denominator as rounded: w_j is off by 2^-8 from either, and sum w_j |v_j| takes both. A score's F32 sum of
+    The bound, for outputs o = sum w_j v_j: the result is rounded to BF16 once (2^-8 |o|). Every weight is the sum of two BF16 terms, off by 2^-8 of
+    the first one's rounding error, 2^-8 of it again, in the product and in the denominator: sum w_j |v_j| takes 2^-16 from either. A score's F32 sum of
     head_dim exact products, added in any order and with truncation, is off by head_dim 2^-23 sum |q_i k_ji| at most; scaled to
     a power of two and taken to it, with another 2^-22 for the exponential, that is a relative error of w_j, in numerator and denominator.
     Sums of the weights and of the products in F32, with truncation: the number of tokens times 2^-23."""
@@ -73,7 +73,7 @@ def attention_reference(batch, scale, layer=0, q=None):
         score_error = (w * size).amax(-1) * 0 + size.masked_fill(hidden[:, None, None], 0).amax(-1) * batch.head_dim * 2.0 ** -23 + 2.0 ** -22
         value = torch.einsum("nhgj,hjd->nhgd", w, v)
         spread = torch.einsum("nhgj,hjd->nhgd", w, v.abs())
-        relative = 2 * BF16_HALF_ULP + 2 * score_error[..., None] + 2 * length * 2.0 ** -23
+        relative = 2 * BF16_HALF_ULP ** 2 + 2 * score_error[..., None] + 2 * length * 2.0 ** -23
         out[rows] = value.reshape(new, batch.query_heads, -1)
         bound[rows] = (BF16_HALF_ULP * value.abs() + relative * spread * (1 + BF16_HALF_ULP)).reshape(new, batch.query_heads, -1)
     return out, bound
