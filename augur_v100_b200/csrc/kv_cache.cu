@@ -24,47 +24,65 @@ struct AppendParams {
     float epsilon;
 };
 
-constexpr uint32_t kAppendThreads = 256, kAppendCtas = 1184;   // eight an SM
+constexpr uint32_t kAppendThreads = 256, kAppendCtas = 2368;   // two rounds of eight an SM
 
-// A CTA turns some of the heads of one row, head_dim / 8 neighbouring lanes to a head with eight elements (one 16-byte access) each. The
-// sines and cosines of the row are formed once per CTA. What the rotation pairs lies rotary_dim / 16 lanes away: a shuffle.
-// A decoding step's few rows are a matter of latency: heads are dealt out so that a lane has one, whose load is under way before the row's sequence
-// and angles are known. (One CTA a row, loads behind them: 8 rows of 24 + 2 x 4 heads of 256 5.9 us; now 5.0, most of it the launch.)
-template <uint32_t kHeadDim>
+// head_dim / 8 neighbouring lanes turn one head, eight elements (one 16-byte access) each, for kRows rows one after the other; blockIdx.y deals out the
+// heads. The sines and cosines of a row are formed once per CTA. What the rotation pairs lies rotary_dim / 16 lanes away: a shuffle.
+// A step of few rows is a matter of latency: a row a CTA, every load under way before the row's sequence and angles are known (one CTA for all
+// heads of a row, loads behind them: 8 rows of 24 + 2 x 4 heads of 256 5.9 us, now 3.5, which is the host's submit). With many rows the chain of lookups
+// counts as often as there are rounds of CTAs: four rows at once (1024 rows of those heads with head norms 17.5 -> 11.3 us, 640 rows 11.1 -> 8.3; 480 rows of 32 + 2 x 8
+// heads of 128, which are 1440 CTAs, 5.4 one by one and 6.2 by fours).
+template <uint32_t kHeadDim, uint32_t kRows>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
     constexpr uint32_t kLanes = kHeadDim / 8, kGroups = kAppendThreads / kLanes;
-    __shared__ __align__(16) float cosine[kHeadDim / 2], sine[kHeadDim / 2];
-    __shared__ int32_t sequence_at, slot_page, slot_offset;
-    const uint32_t row = blockIdx.x, heads = p.query_heads + 2 * p.kv_heads;
-    const uint32_t group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
-    if (threadIdx.x == 0) sequence_at = -1;
+    __shared__ __align__(16) float cosine[kRows][kHeadDim / 2], sine[kRows][kHeadDim / 2];
+    __shared__ int32_t sequence_at[kRows], slot_page[kRows], slot_offset[kRows];
+    const uint32_t row0 = blockIdx.x * kRows, heads = p.query_heads + 2 * p.kv_heads;
+    const uint32_t h = blockIdx.y * kGroups + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+    if (threadIdx.x < kRows) sequence_at[threadIdx.x] = -1;
     __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    auto load = [&](uint32_t h) {
-        const __nv_bfloat16* from;
-        if (h < p.query_heads) from = p.query + row * p.query_row_stride + h * p.query_head_stride;
-        else if (h < p.query_heads + p.kv_heads) from = p.key + row * p.key_row_stride + (h - p.query_heads) * p.key_head_stride;
-        else from = p.value + row * p.value_row_stride + (h - p.query_heads - p.kv_heads) * p.value_head_stride;
-        return __ldg(reinterpret_cast<const uint4*>(from) + lane);
-    };
-    uint32_t h = blockIdx.y * kGroups + group;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (h < heads) raw = load(h);
+    const bool is_query = h < p.query_heads, is_value = h >= p.query_heads + p.kv_heads, live = h < heads;
+    const uint32_t head = is_query ? h : is_value ? h - p.query_heads - p.kv_heads : h - p.query_heads;
+    const __nv_bfloat16* const from = is_query ? p.query + head * p.query_head_stride : is_value ? p.value + head * p.value_head_stride : p.key + head * p.key_head_stride;
+    const uint64_t row_stride = is_query ? p.query_row_stride : is_value ? p.value_row_stride : p.key_row_stride;
+    const float* const norm = is_query ? p.query_norm : is_value ? nullptr : p.key_norm;
+    uint4 raw[kRows];
+#pragma unroll
+    for (uint32_t r = 0; r < kRows; ++r) {
+        raw[r] = make_uint4(0, 0, 0, 0);
+        if (live && row0 + r < p.rows) raw[r] = __ldg(reinterpret_cast<const uint4*>(from + (row0 + r) * row_stride) + lane);
+    }
+    float weight[8];
+    if (live && norm) {
+        if (reinterpret_cast<uint64_t>(norm) % 16 == 0) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(norm) + 2 * lane), b = __ldg(reinterpret_cast<const float4*>(norm) + 2 * lane + 1);
+            weight[0] = a.x, weight[1] = a.y, weight[2] = a.z, weight[3] = a.w, weight[4] = b.x, weight[5] = b.y, weight[6] = b.z, weight[7] = b.w;
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) weight[e] = __ldg(norm + 8 * lane + e);
+        }
+    }
     for (uint32_t b = threadIdx.x; b < p.sequences; b += kAppendThreads) {
-        const int32_t from = __ldg(p.token_starts + b), to = __ldg(p.token_starts + b + 1), length = __ldg(p.lengths + b);
-        if (static_cast<int32_t>(row) >= from && static_cast<int32_t>(row) < to) {
-            const int64_t position = static_cast<int64_t>(length) - to + row;   // in the cache
+        const int32_t first = __ldg(p.token_starts + b), end = __ldg(p.token_starts + b + 1), length = __ldg(p.lengths + b);
+#pragma unroll
+        for (uint32_t r = 0; r < kRows; ++r) {
+            const int32_t row = static_cast<int32_t>(row0 + r);
+            if (row < first || row >= end || row0 + r >= p.rows) continue;
+            const int64_t position = static_cast<int64_t>(length) - end + row;   // in the cache
             const int64_t page = position >> p.page_shift;
             int32_t at = -1;
             if (position >= 0 && page < p.table_pages) at = __ldg(p.page_table + static_cast<uint64_t>(b) * p.table_pages + page);
-            sequence_at = static_cast<int32_t>(b);
-            slot_page = at >= 0 && static_cast<uint32_t>(at) < p.pages ? at : -1;
-            slot_offset = static_cast<int32_t>(position & ((int64_t(1) << p.page_shift) - 1));
+            sequence_at[r] = static_cast<int32_t>(b);
+            slot_page[r] = at >= 0 && static_cast<uint32_t>(at) < p.pages ? at : -1;
+            slot_offset[r] = static_cast<int32_t>(position & ((int64_t(1) << p.page_shift) - 1));
         }
     }
-    const uint32_t i = kAppendThreads - 1 - threadIdx.x;   // the last threads: the first ones are busy with few sequences
-    if (i < p.half) {
+    // (from the last threads on: the first ones are busy with few sequences)
+    for (uint32_t j = kAppendThreads - 1 - threadIdx.x; j < kRows * p.half; j += kAppendThreads) {
+        const uint32_t r = j / p.half, i = j - r * p.half;
+        if (row0 + r >= p.rows) break;
         uint32_t axis;
         if (p.interleaved) {
             axis = i % 3;
@@ -73,44 +91,35 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
             axis = (i >= p.sections[0] ? 1u : 0u) + (i >= p.sections[0] + p.sections[1] ? 1u : 0u);
         }
         // In turns, in 64 bits: a position of 2^20 leaves 2^-33 of a turn, where the F32 product would have lost 2^-7.
-        const double turns = static_cast<double>(__ldg(p.positions + static_cast<uint64_t>(axis) * p.rows + row)) * static_cast<double>(__ldg(p.inv_freq + i)) * 0.15915494309189535;
+        const double turns =
+            static_cast<double>(__ldg(p.positions + static_cast<uint64_t>(axis) * p.rows + row0 + r)) * static_cast<double>(__ldg(p.inv_freq + i)) * 0.15915494309189535;
         const float part_turn = static_cast<float>(turns - rint(turns));
-        sincospif(2.0f * part_turn, &sine[i], &cosine[i]);
+        sincospif(2.0f * part_turn, &sine[r][i], &cosine[r][i]);
     }
     __syncthreads();
-    if (sequence_at < 0) return;
-    const int32_t page = slot_page;
+    if (!live) return;   // (whole groups; nothing is waited for below)
     const uint32_t half_lanes = p.half / 8;
     const bool turns = lane < 2 * half_lanes, upper = lane >= half_lanes;
     const uint32_t partner = !turns ? lane : upper ? lane - half_lanes : lane + half_lanes;
     const uint32_t pair = turns ? 8 * (upper ? lane - half_lanes : lane) : 0;
     const unsigned mask = kLanes == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);   // the lanes of a head stay together
-    for (; h < heads; h += gridDim.y * kGroups) {
-        const uint4 now = raw;
-        if (h + gridDim.y * kGroups < heads) raw = load(h + gridDim.y * kGroups);
-        const bool is_query = h < p.query_heads, is_value = h >= p.query_heads + p.kv_heads;
-        if (!is_query && page < 0) continue;
+#pragma unroll
+    for (uint32_t r = 0; r < kRows; ++r) {
+        if (row0 + r >= p.rows || sequence_at[r] < 0 || (!is_query && slot_page[r] < 0)) continue;
         __nv_bfloat16* to;
-        if (is_query) {
-            to = p.query_out + (static_cast<uint64_t>(row) * p.query_heads + h) * kHeadDim;
-        } else {
-            const uint32_t head = h - p.query_heads - (is_value ? p.kv_heads : 0);
-            to = (is_value ? p.values : p.keys) + (((static_cast<uint64_t>(page) * p.kv_heads + head) << p.page_shift) + slot_offset) * kHeadDim;
-        }
-        uint4 result = now;
+        if (is_query) to = p.query_out + (static_cast<uint64_t>(row0 + r) * p.query_heads + head) * kHeadDim;
+        else to = (is_value ? p.values : p.keys) + (((static_cast<uint64_t>(slot_page[r]) * p.kv_heads + head) << p.page_shift) + slot_offset[r]) * kHeadDim;
+        uint4 result = raw[r];
         if (!is_value) {
-            const float* const norm = is_query ? p.query_norm : p.key_norm;
             float x[8];
-            const uint32_t word[4] = {now.x, now.y, now.z, now.w};
+            const uint32_t word[4] = {raw[r].x, raw[r].y, raw[r].z, raw[r].w};
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e) {
                 x[2 * e] = __uint_as_float(word[e] << 16);
                 x[2 * e + 1] = __uint_as_float(word[e] & 0xffff0000u);
             }
             if (norm) {
-                float weight[8], sum = 0.0f;   // (weights are aligned to an element only)
-#pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) weight[e] = __ldg(norm + 8 * lane + e);
+                float sum = 0.0f;
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
 #pragma unroll
@@ -119,17 +128,15 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) x[e] = x[e] * scale * weight[e];
             }
-            float c[8], n[8];
 #pragma unroll
             for (uint32_t e = 0; e < 8; e += 4) {
-                const float4 a = *reinterpret_cast<const float4*>(cosine + pair + e), b = *reinterpret_cast<const float4*>(sine + pair + e);
-                c[e] = a.x, c[e + 1] = a.y, c[e + 2] = a.z, c[e + 3] = a.w;
-                n[e] = b.x, n[e + 1] = b.y, n[e + 2] = b.z, n[e + 3] = b.w;
-            }
+                const float4 c = *reinterpret_cast<const float4*>(cosine[r] + pair + e), n = *reinterpret_cast<const float4*>(sine[r] + pair + e);
+                const float cosines[4] = {c.x, c.y, c.z, c.w}, sines[4] = {n.x, n.y, n.z, n.w};
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) {
-                const float other = __shfl_sync(mask, x[e], partner, kLanes);
-                if (turns) x[e] = fmaf(x[e], c[e], (upper ? other : -other) * n[e]);
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const float other = __shfl_sync(mask, x[e + i], partner, kLanes);
+                    if (turns) x[e + i] = fmaf(x[e + i], cosines[i], (upper ? other : -other) * sines[i]);
+                }
             }
             uint32_t packed[4];
 #pragma unroll
@@ -310,17 +317,16 @@ extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append
     p.half = a->rotary_dim / 2;
     for (uint32_t i = 0; i < 3; ++i) p.sections[i] = a->sections[i];
     p.interleaved = a->interleaved, p.epsilon = a->epsilon;
-    // A head per group of lanes while that many CTAs run at once; more rows hide their loads behind one another, and share the angles.
-    const uint32_t groups = kAppendThreads / (a->layer.head_dim / 8), heads = a->query_heads + 2 * a->layer.kv_heads;
-    const uint32_t each = (heads + groups - 1) / groups, fits = kAppendCtas / p.rows;
+    const uint32_t groups = kAppendThreads / (a->layer.head_dim / 8), heads = a->query_heads + 2 * a->layer.kv_heads, slices = (heads + groups - 1) / groups;
+    const bool many = static_cast<uint64_t>(p.rows) * slices > kAppendCtas;
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
     config.stream = s->stream, config.attrs = &attribute, config.numAttrs = 1;
-    config.gridDim = dim3(p.rows, each < fits ? each : fits > 1 ? fits : 1), config.blockDim = dim3(kAppendThreads);
-    if (a->layer.head_dim == 256) cudaLaunchKernelEx(&config, kv_append_kernel<256>, p);
-    else cudaLaunchKernelEx(&config, kv_append_kernel<128>, p);
+    config.gridDim = dim3(many ? (p.rows + 3) / 4 : p.rows, slices), config.blockDim = dim3(kAppendThreads);
+    if (a->layer.head_dim == 256) cudaLaunchKernelEx(&config, many ? kv_append_kernel<256, 4> : kv_append_kernel<256, 1>, p);
+    else cudaLaunchKernelEx(&config, many ? kv_append_kernel<128, 4> : kv_append_kernel<128, 1>, p);
     count_launch();
     return submitted();
 }

@@ -527,9 +527,9 @@ __global__ void __launch_bounds__(kThreads, kSelect ? 3 : 4) token_logprobs_kern
             if (threadIdx.x == 0) part->most = s.most, part->sum = s.sum, part->moment = s.moment;
             __syncthreads();
             if (threadIdx.x == 0) {   // releases what all threads wrote, and acquires what the others did
-                __threadfence();
-                sh.last = atomicAdd(p.arrivals + from, 1u) == to - from;
-                __threadfence();
+                uint32_t before;
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrivals + from) : "memory");
+                sh.last = before == to - from;
             }
             __syncthreads();
             if (!sh.last) continue;
