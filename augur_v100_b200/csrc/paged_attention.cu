@@ -630,9 +630,27 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             float2* const stats = reinterpret_cast<float2*>(p.parts + static_cast<uint64_t>(2 * p.spans) * kN * kHeadDim) + part * kN;
             uint32_t token_end = group;
             uint64_t skipped = 0;
+            float2 mine = make_float2(0.0f, 0.0f);   // statistics of query `thread`
+            // (No branch by query where 16 are there or a part is written, which has room for all columns: with one, 48 queries took 7000 cycles.)
+            auto write = [&](const uint32_t (&v)[S::kHalves + 1][kBlock], uint32_t c0, uint32_t i) {
+                const uint32_t c = c0 + i;
+                if (c == token_end) token_end += group, skipped += next_token;
+                const float all = __uint_as_float(v[S::kHalves][i]);
+                float scale;
+                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(scale) : "f"(all));   // good to 2^-23
+#pragma unroll
+                for (uint32_t h = 0; h < S::kHalves; ++h) {
+                    out[skipped + c * kHeadDim + h * 128] = __float2bfloat16_rn(all == 0.0f ? 0.0f : __uint_as_float(v[h][i]) * scale);
+                }
+            };
 #pragma unroll 1
             for (uint32_t c0 = 0; c0 < queries; c0 += kBlock) {
                 uint32_t v[S::kHalves + 1][kBlock], low[S::kHalves + 1][kBlock];   // both terms' sums; the last are the denominators
+#pragma unroll
+                for (uint32_t h = 0; h <= S::kHalves; ++h) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kBlock; ++i) v[h][i] = 0;
+                }
                 if (any) {
 #pragma unroll
                     for (uint32_t h = 0; h <= S::kHalves; ++h) {
@@ -646,24 +664,27 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                         for (uint32_t i = 0; i < kBlock; ++i) v[h][i] = __float_as_uint(__uint_as_float(v[h][i]) + __uint_as_float(low[h][i]));
                     }
                 }
+                if (!alone) {
+                    float* const to = part_out + c0 * kHeadDim;
 #pragma unroll
-                for (uint32_t i = 0; i < kBlock; ++i) {
-                    const uint32_t c = c0 + i;
-                    if (c >= queries) break;
-                    const float all = any ? __uint_as_float(v[S::kHalves][i]) : 0.0f;
-                    if (alone) {
-                        if (c == token_end) token_end += group, skipped += next_token;
-                        const float scale = 1.0f / all;
+                    for (uint32_t i = 0; i < kBlock; ++i) {
 #pragma unroll
-                        for (uint32_t h = 0; h < S::kHalves; ++h) {
-                            out[skipped + c * kHeadDim + h * 128] = __float2bfloat16_rn(all == 0.0f ? 0.0f : __uint_as_float(v[h][i]) * scale);
-                        }
-                    } else {
+                        for (uint32_t h = 0; h < S::kHalves; ++h) to[i * kHeadDim + h * 128] = __uint_as_float(v[h][i]);
+                        if (thread == c0 + i) mine.y = __uint_as_float(v[S::kHalves][i]);
+                    }
+                } else if (c0 + kBlock <= queries) {
 #pragma unroll
-                        for (uint32_t h = 0; h < S::kHalves; ++h) part_out[c * kHeadDim + h * 128] = __uint_as_float(v[h][i]);
-                        if (thread == c) stats[c] = make_float2(st->reference[c], all);
+                    for (uint32_t i = 0; i < kBlock; ++i) write(v, c0, i);
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < kBlock; ++i) {
+                        if (c0 + i < queries) write(v, c0, i);
                     }
                 }
+            }
+            if (!alone && thread < queries) {
+                mine.x = st->reference[thread];
+                stats[thread] = mine;
             }
             if (any) tc_fence_before();
             if (!alone) {
@@ -689,9 +710,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
 // Joins the parts of one pair, in the order of their spans. A CTA takes queries blockIdx.y, blockIdx.y + gridDim.y, ...; four outputs a
 // thread, and the threads of a query's outputs as many times over as there are, each with every so many-th part.
 constexpr uint32_t kJoinThreads = 256, kJoinCtas = 1184;   // about as many as run at once
+// Few queries have few CTAs, and as many loads under way as the parts of one sequence want; many queries more CTAs at once.
 template <uint32_t kHeadDim, uint32_t kN>
-__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttentionParams p) {
-    constexpr uint32_t kLanes = kHeadDim / 4, kShares = kJoinThreads / kLanes;
+__global__ void __launch_bounds__(kJoinThreads, kN <= 16 ? 1 : 6) attention_join_kernel(const __grid_constant__ AttentionParams p) {
+    constexpr uint32_t kLanes = kHeadDim / 4, kShares = kJoinThreads / kLanes, kAhead = kN <= 16 ? 10 : 6;
     __shared__ float weight[kMaxCtas];
     __shared__ float4 sums[kShares][kLanes];
     __shared__ float wide[2][kJoinThreads / 32];
@@ -709,7 +731,6 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
         if (threadIdx.x < parts) mine = reinterpret_cast<const float2*>(p.parts + static_cast<uint64_t>(2 * p.spans) * kN * kHeadDim)[part(threadIdx.x) * kN + query];
         // this thread's part of the outputs of the first parts, on their way meanwhile
         const float4* const from = reinterpret_cast<const float4*>(p.parts + static_cast<uint64_t>(query) * kHeadDim) + lane;
-        constexpr uint32_t kAhead = 10;
         float4 v[kAhead];
         auto load = [&](uint32_t first) {
 #pragma unroll
