@@ -66,7 +66,7 @@ struct State {
     uint64_t scores_full[2], scores_empty[2], weights_full[2], weights_empty[2], query_full[2], query_empty[2], group, keys_first;
     uint32_t tmem, abort[1 + kThreads / 32];
     uint32_t needs[2];                 // a byte per softmax warp: a reference has to move
-    uint32_t info[kInfos];             // of a tile: pages that are there, a bit per box; bit 31: the last tile
+    uint32_t info[kInfos];             // of a tile: pages that are there, a bit per box
     uint32_t scan[kThreads / 32];
     float reference[kMaxQueries], factor[kMaxQueries];
     float4 wide[kMaxQueries];          // the largest score per query and softmax warp
@@ -85,11 +85,14 @@ struct Shape {
     static constexpr uint32_t kWeightBytes = kTerms * kTile * 2;
     static constexpr uint32_t kFixed = 1024 + kOnesBytes + sizeof(State) + kQueryBuffers * kQueryBytes + 2 * kWeightBytes;
     static constexpr uint32_t kRoom = kSmemLimit - kFixed;
+    // A ring each for the keys and the values: a slot's uses then all belong to one of the two warps that load, which waits for them in turn. (With
+    // slots that go from one warp to the other, a warp could take the end of the use before last for the end of the last one.)
     static constexpr uint32_t kSlots = kRoom / kSlotBytes / 2 * 2 > 16 ? 16 : kRoom / kSlotBytes / 2 * 2;
+    static constexpr uint32_t kValueSlots = (kSlots / 2 + 1) / 2 * 2, kKeySlots = kSlots - kValueSlots;   // (pairs of value slots are one operand)
     static constexpr uint32_t kSmem = kFixed + kSlots * kSlotBytes;
     // tensor memory: two of S^T, O^T in halves of 128 dims, the denominators
     static constexpr uint32_t kColumns = 2 * kScores + (kHalves + 1) * kTerms, kTmem = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
-    static_assert(kSlots >= kChunks + 2 /* K of a tile and half of the V before it */ && kSmem <= kSmemLimit && kColumns <= 512, "a CTA's memory");
+    static_assert(kKeySlots >= 2 && kValueSlots >= kChunks /* a tile's values are looked at before any is used */ && kSmem <= kSmemLimit && kColumns <= 512, "a CTA's memory");
 };
 
 // A CTA's way through its span: one (sequence, head) after the other, in each the keys [key, key_end).
@@ -318,7 +321,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
 
     if (warp == 0 || warp == 3) {
         // ---------------- pages: warp 0 the keys, warp 3 the values ----------------
-        // The ring's slots go round in the order of their use: K of tile 0, then K of tile t and V of tile t - 1, and V of the last.
         const uint32_t box_shift = p.page_shift < 6 ? p.page_shift : 6, boxes = kTile >> box_shift, box_bytes = 128u << box_shift;
         const CUtensorMap* const map = warp == 0 ? &map_keys : &map_values;
         Tiles tiles;
@@ -340,14 +342,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             }
             const uint32_t mask = __ballot_sync(0xffffffffu, there);
             tiles.advance(st, p);
-            uint32_t at = 2 * S::kChunks * tile;   // among all slots that are loaded
-            if (warp == 0) {
-                if (tile) at -= S::kChunks;
-                if (lane == 0) st->info[tile % kInfos] = mask | (tiles.valid ? 0 : 0x80000000u);
-            } else {
-                at += tiles.valid ? 2 * S::kChunks : S::kChunks;
-            }
-            uint32_t slot = at % S::kSlots, phase = at / S::kSlots & 1 ^ 1;
+            if (warp == 0 && lane == 0) st->info[tile % kInfos] = mask;
+            const uint32_t first_slot = warp == 0 ? 0 : S::kKeySlots, slots = warp == 0 ? S::kKeySlots : S::kValueSlots, use = S::kChunks * tile;
+            uint32_t slot = first_slot + use % slots, phase = use / slots & 1 ^ 1;
             for (uint32_t c = 0; c < S::kChunks; ++c) {
                 if (!warp_look_wait(empty + 8 * slot, phase, abort_flag, status, kStatusLoad)) {
                     alive = false;
@@ -361,7 +358,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                 __syncwarp();
                 if (there) tma_load_2d(smem_u32(smem) + slot * kSlotBytes + lane * box_bytes, map, c * 128, row, bar);
                 __syncwarp();
-                if (++slot == S::kSlots) slot = 0, phase ^= 1;
+                if (++slot == first_slot + slots) slot = first_slot, phase ^= 1;
             }
             if (warp == 0 && tile == 0 && lane == 0) mbar_arrive(keys_first);
         }
@@ -374,18 +371,18 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
         Tiles ahead, now;
         ahead.open(st, p, from, to);
         now = ahead;
-        uint32_t slot = 0, phase = 0, scores = 0, products = 0, pair = 0;
+        uint32_t key_slot = 0, key_phase = 0, slot = S::kKeySlots, phase = 0, scores = 0, products = 0, pair = 0;
         bool alive = true;
         auto scores_of_tile = [&]() {
             const uint32_t buffer = scores & 1, query = S::kQueryBuffers == 2 ? pair & 1 : 0;
             if (ahead.first() && !warp_look_wait(query_full + 8 * query, (S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1, abort_flag, status, kStatusMma)) return false;
             if (!warp_look_wait(scores_empty + 8 * buffer, (scores >> 1 & 1) ^ 1, abort_flag, status, kStatusMma)) return false;
             for (uint32_t c = 0; c < S::kChunks; ++c) {
-                if (!warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusMma)) return false;
+                if (!warp_look_wait(full + 8 * key_slot, key_phase, abort_flag, status, kStatusMma)) return false;
                 tc_fence_after();
-                mma_block<kHighSwizzled, 2>(tmem + buffer * S::kScores, slots + slot * (kSlotBytes >> 4), queries + ((query * S::kQueryBytes + c * S::kScores * 128) >> 4), idesc, c, 4);
-                commit(empty + 8 * slot);
-                if (++slot == S::kSlots) slot = 0, phase ^= 1;
+                mma_block<kHighSwizzled, 2>(tmem + buffer * S::kScores, slots + key_slot * (kSlotBytes >> 4), queries + ((query * S::kQueryBytes + c * S::kScores * 128) >> 4), idesc, c, 4);
+                commit(empty + 8 * key_slot);
+                if (++key_slot == S::kKeySlots) key_slot = 0, key_phase ^= 1;
             }
             commit(scores_full + 8 * buffer);
             if (ahead.last()) {
@@ -417,7 +414,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                 commit(empty + 8 * slot);
                 commit(empty + 8 * (slot + 1));
                 slot += 2;
-                if (slot == S::kSlots) slot = 0, phase ^= 1;
+                if (slot == S::kSlots) slot = S::kKeySlots, phase ^= 1;
             }
             if (!alive) break;
             commit(weights_empty + 8 * buffer);
@@ -484,7 +481,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                     break;
                 }
                 tc_fence_after();
-                const uint32_t info = st->info[tile % kInfos], there = info & 0x7fffffffu;
+                const uint32_t there = st->info[tile % kInfos];
                 const uint32_t count = walk.key_end - key < kTile ? walk.key_end - key : kTile;
                 const bool whole = count == kTile && there == all_boxes, masked = !whole || static_cast<int32_t>(key + kTile) > seen_by_all;
                 const bool my_key = thread < count && (there >> (thread >> box_shift) & 1);
@@ -595,8 +592,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                 if (lane == 0) mbar_arrive(scores_empty + 8 * buffer);
                 if (!whole) {
                     // Rows of V that are no token's are multiplied with weights of zero: whatever lies there, they must be numbers.
-                    const uint32_t at = 2 * S::kChunks * (tile + 1) - (info >> 31 ? S::kChunks : 0);   // the tile's V among all slots that were loaded
-                    uint32_t slot = at % S::kSlots, phase = at / S::kSlots & 1;
+                    // These warps do not wait for every use of a slot, so they must not be more than one ahead: the tile before has to be through. (They
+                    // took the end of the use before last for that of this one, and wrote their zeros into the values of the tile before.)
+                    if (tile && !warp_look_wait(weights_empty + 8 * (buffer ^ 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) {
+                        alive = false;
+                        break;
+                    }
+                    const uint32_t use = S::kChunks * tile;
+                    uint32_t slot = S::kKeySlots + use % S::kValueSlots, phase = use / S::kValueSlots & 1;
                     for (uint32_t c = 0; alive && c < S::kChunks; ++c) {
                         if (!warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusValues)) {
                             alive = false;
@@ -607,7 +610,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
 #pragma unroll
                             for (uint32_t i = 0; i < 8; ++i) row[i] = make_uint4(0, 0, 0, 0);
                         }
-                        if (++slot == S::kSlots) slot = 0, phase ^= 1;
+                        if (++slot == S::kSlots) slot = S::kKeySlots, phase ^= 1;
                     }
                     if (!alive) break;
                 }

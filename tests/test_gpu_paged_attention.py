@@ -199,3 +199,22 @@ def test_layers_of_one_cache_and_allocations(stream):
     for bad in (dict(q=batch.q.float()), dict(q=batch.q[:, :, ::2]), dict(out=torch.zeros(1, device="cuda:0"))):
         with pytest.raises(ValueError):
             _bind(stream, batch, 1, plan=plan, **bad)
+
+
+@pytest.mark.parametrize("heads,tokens", [(LAYER, 1), (LAYER, 3), (LAYER, 8), ((16, 2, 256), 5), ((32, 8, 128), 4), ((64, 8, 128), 8)])
+def test_many_tiles_in_every_ring(stream, heads, tokens):
+    # spans of dozens of tiles and several pairs each, again and again: every slot of the rings goes round many times while the warps that load run ahead
+    shape = [(3400 - 31 * b, tokens) for b in range(36)] + [(5100 + 17 * b, 1) for b in range(6)]
+    batch = Batch(shape, *heads, 32, seed=tokens)
+    a = _bind(stream, batch, tokens)
+    first = None
+    for _ in range(12):
+        a.out.fill_(77.0)
+        torch.cuda.synchronize()
+        a.submit_for_plan()
+        stream.synchronize()
+        if first is None:
+            first = a.out.clone()
+            _close(first, batch, heads[2] ** -0.5)
+        assert torch.equal(a.out, first)
+    assert a.plan.device_status() == 0
