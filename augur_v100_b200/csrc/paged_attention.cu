@@ -81,13 +81,15 @@ struct Shape {
     static constexpr uint32_t kChunks = kHeadDim / 64, kHalves = kHeadDim / 128;
     // Columns of S^T (the MMA wants 16 at least), and of P^T and O^T: two BF16 terms of P side by side. kBlock of them are worked on at a time.
     static constexpr uint32_t kScores = kN < 16 ? 16 : kN, kTerms = 2 * kN, kBlock = kN < 16 ? kN : 16;
-    static constexpr uint32_t kQueryBytes = kScores * kHeadDim * 2, kQueryBuffers = kQueryBytes > 24 * 1024 ? 1 : 2;
+    static constexpr uint32_t kQueryBytes = kScores * kHeadDim * 2, kQueryBuffers = kQueryBytes >= 12 * 1024 ? 1 : 2;
     static constexpr uint32_t kWeightBytes = kTerms * kTile * 2;
     static constexpr uint32_t kFixed = 1024 + kOnesBytes + sizeof(State) + kQueryBuffers * kQueryBytes + 2 * kWeightBytes;
     static constexpr uint32_t kRoom = kSmemLimit - kFixed;
     // A ring each for the keys and the values: a slot's uses then all belong to one of the two warps that load, which waits for them in turn. (With
     // slots that go from one warp to the other, a warp could take the end of the use before last for the end of the last one.)
-    static constexpr uint32_t kSlots = kRoom / kSlotBytes / 2 * 2 > 16 ? 16 : kRoom / kSlotBytes / 2 * 2;
+    // Where there are few slots, an odd one goes to the keys, and the queries are held once to gain it (8 tokens of 6 heads each, 4 x 16385 tokens: 59 us
+    // with 5 + 4 slots, 67 with 4 + 4); ten and more are kept even (one token, 2 x 131071: 163 us with 4 + 6, 168 with 5 + 6).
+    static constexpr uint32_t kFit = kRoom / kSlotBytes > 16 ? 16 : kRoom / kSlotBytes, kSlots = kFit < 10 ? kFit : kFit / 2 * 2;
     static constexpr uint32_t kValueSlots = (kSlots / 2 + 1) / 2 * 2, kKeySlots = kSlots - kValueSlots;   // (pairs of value slots are one operand)
     static constexpr uint32_t kSmem = kFixed + kSlots * kSlotBytes;
     // tensor memory: two of S^T, O^T in halves of 128 dims, the denominators
