@@ -4,7 +4,7 @@
 //
 // The cache is read once (4 kv_heads head_dim bytes a token) and that is the bound: for up to 64 queries per key-value head (new tokens x query
 // heads that share it) the products are small change for the tensor cores. So no thread touches a key or a value: TMA brings pages
-// into a ring in shared memory, and tcgen05.mma reads them there as the 128-row operand, the queries as the narrow one:
+// into two rings in shared memory, and tcgen05.mma reads them there as the 128-row operand, the queries as the narrow one:
 //
 //   S^T[key][query]   = K Q^T          K as it lies in the pages (rows of head_dim: K-major), 128 keys a tile
 //   O^T[dim][query]  += V^T P^T        V as it lies in the pages (the key is the k dimension: MN-major)
@@ -60,7 +60,7 @@ struct JoinRecord {
     uint32_t reserved[3];
 };
 
-// Small state of a CTA, behind the ring, the queries and the weights.
+// Small state of a CTA, behind the rings, the queries and the weights.
 struct State {
     uint64_t full[16], empty[16];
     uint64_t scores_full[2], scores_empty[2], weights_full[2], weights_empty[2], query_full[2], query_empty[2], group, keys_first;
