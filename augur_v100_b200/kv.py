@@ -215,7 +215,8 @@ class KvPagePool:
 
     A sequence is a number that `create` or `fork` hands out. Full pages are shared between a sequence and its forks and are
     never written again, a partly filled one is copied at the fork. Where a call answers with `PageCopies`, those are to
-    be enqueued (`KvPageCopy.submit`) on the stream of the steps before the next step uses the pages."""
+    be enqueued (`KvPageCopy.submit`) on the stream of the steps before the next step uses the pages: the answer of each call by
+    itself and in the order of the calls, since a later call may give away a page that an earlier one copies from."""
 
     def __init__(self, pages: int, page_tokens: int):
         if pages < 1 or page_tokens < 1:

@@ -661,7 +661,8 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_interleave_gate_up_h
 /* The reference keeps one contiguous cache per session (its attention and cache kernels are sm_70 code outside the
  * quantised linear); the entries below have no counterpart of the same form there. One layer of the cache is two BF16
  * tensors [pages][kv_heads][page_tokens][head_dim]; a sequence's tokens fill the pages of its page-table row in order.
- * page_tokens: a power of two, 16..1024. head_dim: 128 or 256. pages * kv_heads * page_tokens below 2^31. */
+ * page_tokens: a power of two, 16..1024. head_dim: 128 or 256. pages * kv_heads * page_tokens below 2^31, query and
+ * key-value heads up to 1024 each, a step's rows up to 2^20. */
 typedef struct augur_cuda_nvfp4_sm100_kv_layer_v1 {
     augur_cuda_device_ptr_t keys;
     augur_cuda_device_ptr_t values;
@@ -740,7 +741,7 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append_prevalidat
 /* Attention of up to max_new_tokens (1..8) new tokens per sequence over its cache, their own keys and values included:
  *   output[row][h] = sum_j p_j values[j],  p = softmax over j of scale * query[row][h] . keys[j]
  * for all cached j up to the row's own token. query_heads is a multiple of kv_heads; query_heads / kv_heads * max_new_tokens
- * is at most 64. Products of BF16 are exact, sums, maxima and exponentials F32; the weights p enter the product with the values as two
+ * is at most 64, table_pages * page_tokens at most 2^24. Products of BF16 are exact, sums, maxima and exponentials F32; the weights p enter the product with the values as two
  * BF16 terms (good to 2^-16 of p), and the denominator as the same. A row that sees no token gets zeros. What the pages hold
  * behind a sequence's length is never used, infinities and NaN included; a value that is not finite among the sequence's own
  * new tokens may reach all of that sequence's rows. A page outside the cache counts as not there and sets the plan's status word to
@@ -802,7 +803,7 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_copy_prevali
  * The reference selects on the host or with its own top-k kernels behind the same head; there is no counterpart of this
  * form. F32 logits (bf16_head) or BF16 ones (a linear's output); sums and statistics F32. A row of -infinities has entropy 0 and
  * log probabilities -infinity; a NaN or +infinity in a row gives what the formulas give (NaN), NaN ordered above all
- * numbers. row_stride in elements, at least `vocabulary`, vocabulary up to 2^24, alternatives 0..32 (and at most
+ * numbers. row_stride in elements, at least `vocabulary`, vocabulary up to 2^24, rows up to 2^20, alternatives 0..32 (and at most
  * vocabulary; 0: ids and alternative_logprobs are 0, with 0 bytes). */
 #define AUGUR_NVFP4_SM100_MAX_ALTERNATIVES 32
 #define AUGUR_NVFP4_SM100_LOGITS_F32 UINT32_C(0)
