@@ -36,6 +36,7 @@ constexpr uint32_t kMaxSequences = AUGUR_NVFP4_SM100_MAX_SEQUENCES;
 constexpr uint32_t kOnesBytes = kTile * 32;    // 16 k of ones, as the 128-row operand
 constexpr uint32_t kMaxTokensLog2 = 24;   // of a sequence
 constexpr float kSlack = 8.0f;            // how far, in powers of two, a score may pass the reference maximum
+constexpr float kNoNumber = -3.0e38f;     // a part's reference where a query sees keys but no score above -infinity (-infinity: sees none)
 constexpr uint32_t kStatusPage = 0x401, kStatusRows = 0x402;
 constexpr uint32_t kStatusLoad = 0x411, kStatusMma = 0x412, kStatusScores = 0x413, kStatusValues = 0x414, kStatusQuery = 0x415, kStatusGroup = 0x416, kStatusProduct = 0x417;
 constexpr uint32_t kThreads = 256;        // warp 0 loads keys, 1 MMA, 2 queries, 3 values, 4..7 softmax
@@ -688,7 +689,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                 }
             }
             if (!alone && thread < queries) {
+                // A part all of whose scores are NaN or -infinity has the reference -infinity too, but counts: its sums may be NaN.
                 mine.x = st->reference[thread];
+                if (mine.x == -INFINITY && st->limit[thread] > static_cast<int32_t>(walk.key)) mine.x = kNoNumber;
                 stats[thread] = mine;
             }
             if (any) tc_fence_before();
@@ -752,10 +755,12 @@ __global__ void __launch_bounds__(kJoinThreads, kN <= 16 ? 1 : 6) attention_join
         __syncthreads();
 #pragma unroll
         for (uint32_t w = 0; w < kJoinThreads / 32; ++w) most = fmaxf(most, wide[0][w]);
-        const float w = mine.x == -INFINITY ? 0.0f : exp2_fast(mine.x - most);
-        weight[threadIdx.x] = w;
-        float all = w * mine.y;
-        if (w == 0.0f) all = 0.0f;
+        // Parts of which the query sees nothing are passed over, whatever other queries' keys left in them. All others count, with a weight of zero too:
+        // zero times a NaN is one, as in a pair that lies in one span.
+        const bool sees = mine.x != -INFINITY;
+        const float w = sees ? exp2_fast(mine.x - most) : 0.0f;
+        weight[threadIdx.x] = sees ? w : -1.0f;
+        float all = sees ? w * mine.y : 0.0f;
 #pragma unroll
         for (uint32_t step = 16; step; step /= 2) all += __shfl_xor_sync(0xffffffffu, all, step);
         if (threadIdx.x % 32 == 0) wide[1][warp] = all;
@@ -765,8 +770,8 @@ __global__ void __launch_bounds__(kJoinThreads, kN <= 16 ? 1 : 6) attention_join
             if (first != share) load(first);
 #pragma unroll
             for (uint32_t i = 0; i < kAhead; ++i) {
-                const float f = first + i * kShares < parts ? weight[first + i * kShares] : 0.0f;
-                if (f != 0.0f) sum.x = fmaf(f, v[i].x, sum.x), sum.y = fmaf(f, v[i].y, sum.y), sum.z = fmaf(f, v[i].z, sum.z), sum.w = fmaf(f, v[i].w, sum.w);
+                const float f = first + i * kShares < parts ? weight[first + i * kShares] : -1.0f;
+                if (!(f < 0.0f)) sum.x = fmaf(f, v[i].x, sum.x), sum.y = fmaf(f, v[i].y, sum.y), sum.z = fmaf(f, v[i].z, sum.z), sum.w = fmaf(f, v[i].w, sum.w);
             }
         }
         sums[share][lane] = sum;

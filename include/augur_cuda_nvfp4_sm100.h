@@ -742,7 +742,9 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append_prevalidat
  *   output[row][h] = sum_j p_j values[j],  p = softmax over j of scale * query[row][h] . keys[j]
  * for all cached j up to the row's own token. query_heads is a multiple of kv_heads; query_heads / kv_heads * max_new_tokens
  * is at most 64, table_pages * page_tokens at most 2^24. Products of BF16 are exact, sums, maxima and exponentials F32; the weights p enter the product with the values as two
- * BF16 terms (good to 2^-16 of p), and the denominator as the same. A row that sees no token gets zeros. What the pages hold
+ * BF16 terms (good to 2^-16 of p), and the denominator as the same. A row that sees no token gets zeros, and so does one all of whose
+ * scores are -infinity (where the formula has no value). A NaN in a row's query, or in a key or value that it sees, gives NaN as in the
+ * formula, as does a score of +infinity; an infinite value that it sees gives an infinity or NaN in that element. What the pages hold
  * behind a sequence's length is never used, infinities and NaN included; a value that is not finite among the sequence's own
  * new tokens may reach all of that sequence's rows. A page outside the cache counts as not there and sets the plan's status word to
  * 0x401, as does a length beyond the table; rows outside the tensors or more than max_new_tokens rows set 0x402, and such a
