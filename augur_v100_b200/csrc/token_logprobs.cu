@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, kSelect ? 3 : 4) token_logprobs_kern
             // One reference for the warp: a new maximum in one of 32 lanes is frequent, in a unit of the whole warp soon rare.
             float warp_most;
             asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(warp_most) : "f"(most));
-            if (!(warp_most <= s.most)) s.move_to(warp_most);
+            if (!(warp_most <= s.most)) s.move_to(max_nan(s.most, warp_most));   // (a NaN stays the maximum)
             const float base = s.most == -INFINITY ? 0.0f : s.most;
             const float2 minus_base = make_float2(-base, -base), log2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
             float2 sum[2] = {make_float2(s.sum, 0.0f), make_float2(0.0f, 0.0f)}, moment[2] = {make_float2(s.moment, 0.0f), make_float2(0.0f, 0.0f)};
