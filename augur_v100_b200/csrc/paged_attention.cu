@@ -19,6 +19,7 @@
 // that lies in several spans leaves an unnormalised part per span in the plan's scratch, and a second launch joins those, in
 // the order of the spans. The spans follow from the lengths alone (read on the device, so that a captured call can be replayed).
 #include "kv_cache.cuh"
+#include "kv_join_record.h"
 #include "nvfp4_gemm.cuh"
 
 namespace augur_sm100 {
@@ -48,17 +49,10 @@ struct AttentionParams {
     __nv_bfloat16* output;
     const int32_t *page_table, *lengths, *token_starts;
     uint32_t* status_word;
-    struct JoinRecord* records;   // [joins]
+    JoinRecord* records;          // [joins]
     float* parts;                 // [spans][2][kN][head_dim], then [spans][2][kN] (reference maximum, denominator)
     uint32_t rows, sequences, table_pages, pages, query_heads, kv_heads, page_shift, max_new, spans, joins;
     float scale_log2;             // scale * log2(e)
-};
-
-// What the join has to know of a pair that several spans share (tokens 0: of none). Records are by pair or, where there are more pairs than spans, by the
-// span that holds the pair's first part.
-struct JoinRecord {
-    uint32_t row, tokens, head, first, last;   // first token row, new tokens, key-value head, first and last span
-    uint32_t reserved[3];
 };
 
 // Small state of a CTA, behind the rings, the queries and the weights.
@@ -729,8 +723,7 @@ __global__ void __launch_bounds__(kJoinThreads, kN <= 16 ? 1 : 6) attention_join
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const JoinRecord record = p.records[blockIdx.x];
     const uint32_t group = p.query_heads / p.kv_heads, share = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, warp = threadIdx.x / 32;
-    // (a launch that gave up may have left a record of an earlier one)
-    if (record.tokens * group > kN || record.row + record.tokens > p.rows || record.head >= p.kv_heads || record.last >= p.spans || record.first > record.last) return;
+    if (!join_record_ok(record, group, kN, p.rows, p.kv_heads, p.spans)) return;   // (a launch that gave up may have left anything)
     const uint32_t parts = record.last - record.first + 1;
     auto part = [&](uint32_t i) { return 2 * (record.first + i) + (i == 0 ? 1 : 0); };
     for (uint32_t query = blockIdx.y; query < record.tokens * group; query += gridDim.y) {
