@@ -727,9 +727,10 @@ class TokenLogprobs:
             raise ValueError(f"0 to {abi.MAX_ALTERNATIVES} alternatives")
         self.plan, self.logits, self.targets = plan, logits, targets
         empty = functools.partial(torch.empty, device=logits.device)
-        self.logprobs, self.entropy = empty(rows, dtype=torch.float32), empty(rows, dtype=torch.float32)
-        self.ids = empty((rows, alternatives), dtype=torch.int32)
-        self.alternative_logprobs = empty((rows, alternatives), dtype=torch.float32)
+        with torch.cuda.stream(plan.stream.torch_stream):   # memory of that stream's: nothing enqueued elsewhere still uses it
+            self.logprobs, self.entropy = empty(rows, dtype=torch.float32), empty(rows, dtype=torch.float32)
+            self.ids = empty((rows, alternatives), dtype=torch.int32)
+            self.alternative_logprobs = empty((rows, alternatives), dtype=torch.float32)
         a = abi.header(abi.TokenLogprobsArgs)
         a.row_stride = logits.stride(0) if rows > 1 else vocabulary
         a.logits, a.logits_len_bytes = _ptr(logits), ((rows - 1) * a.row_stride + vocabulary) * logits.element_size()

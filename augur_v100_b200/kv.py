@@ -43,7 +43,8 @@ class KvCache:
     @classmethod
     def allocate(cls, stream: Stream, layers: int, pages: int, kv_heads: int, page_tokens: int, head_dim: int):
         shape, device = (layers, pages, kv_heads, page_tokens, head_dim), torch.device("cuda", stream.ordinal)
-        return cls(torch.empty(shape, dtype=torch.bfloat16, device=device), torch.empty(shape, dtype=torch.bfloat16, device=device))
+        with torch.cuda.stream(stream.torch_stream):
+            return cls(torch.empty(shape, dtype=torch.bfloat16, device=device), torch.empty(shape, dtype=torch.bfloat16, device=device))
 
     def layer_args(self, layer: int) -> abi.KvLayer:
         if not 0 <= layer < self.layers:
@@ -117,7 +118,8 @@ class KvAppend:
              interleaved: bool = False, q_out: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
              k_norm: torch.Tensor | None = None, epsilon: float = 1e-6):
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+            with torch.cuda.stream(stream.torch_stream):   # memory of that stream's: nothing enqueued elsewhere still uses it
+                q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
         self = cls(stream, cache, layer, q, k, v, positions, frequencies, sections, table, lengths, starts, interleaved, q_out, q_norm, k_norm,
                    epsilon)
         _check("kv_append_preflight", abi.lib().augur_cuda_nvfp4_sm100_kv_append_preflight_v1(stream.ordinal, stream.handle, byref(self.args)))
@@ -160,7 +162,8 @@ class PagedAttention:
     def bind(cls, plan: Plan, cache: KvCache, layer: int, q, table, lengths, starts, tokens: int = 1, out: torch.Tensor | None = None,
              scale: float | None = None):
         if out is None:
-            out = torch.zeros_like(q)
+            with torch.cuda.stream(plan.stream.torch_stream):   # the zeros go ahead of the submits
+                out = torch.zeros_like(q)
         self = cls(plan, cache, layer, q, table, lengths, starts, tokens, out, cache.head_dim ** -0.5 if scale is None else scale)
         s = plan.stream
         _check("paged_attention_preflight", abi.lib().augur_cuda_nvfp4_sm100_paged_attention_preflight_v1(
