@@ -105,8 +105,9 @@ def gemv_scratch_bytes(rows: int, cols: int, tokens: int = 8) -> int:
     return int(out.value)
 
 
-def sm_count() -> int:
-    return torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
+def sm_count(ordinal: int | None = None) -> int:
+    """SMs of a device (None: the current one)."""
+    return torch.cuda.get_device_properties(torch.cuda.current_device() if ordinal is None else ordinal).multi_processor_count
 
 
 def gemm_plan_scratch_bytes(sm_count: int = 0) -> int:
@@ -704,7 +705,8 @@ class Bf16Head:
 
 
 def logprobs_scratch_bytes(rows: int, alternatives: int, sms: int = 0) -> int:
-    """Plan scratch of a `TokenLogprobs` (`sms` 0: of this device), whatever the vocabulary."""
+    """Plan scratch of a `TokenLogprobs`, whatever the vocabulary. `sms`: `sm_count(stream.ordinal)` of the plan's device (0: of the current device; a plan on
+    one with more SMs wants more, and binding to it is refused)."""
     out = c_uint64()
     _check("token_logprobs_scratch_extent", abi.lib().augur_cuda_nvfp4_sm100_token_logprobs_scratch_extent_host_v1(
         rows, alternatives, sms or sm_count(), byref(out)))

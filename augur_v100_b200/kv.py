@@ -130,7 +130,8 @@ class KvAppend:
 
 
 def paged_attention_scratch_bytes(query_heads: int, kv_heads: int, head_dim: int, tokens: int = abi.MAX_SMALL_TOKENS, sms: int = 0) -> int:
-    """Plan scratch of a `PagedAttention` of up to `tokens` new tokens per sequence (`sms` 0: of this device)."""
+    """Plan scratch of a `PagedAttention` of up to `tokens` new tokens per sequence. `sms`: `host.sm_count(stream.ordinal)` of the plan's device (0: of the
+    current device; a plan on one with more SMs wants more, and binding to it is refused)."""
     out = c_uint64()
     _check("paged_attention_scratch_extent", abi.lib().augur_cuda_nvfp4_sm100_paged_attention_scratch_extent_host_v1(
         query_heads, kv_heads, head_dim, tokens, sms or sm_count(), byref(out)))
