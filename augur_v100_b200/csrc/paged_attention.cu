@@ -76,21 +76,29 @@ struct Shape {
     static constexpr uint32_t kChunks = kHeadDim / 64, kHalves = kHeadDim / 128;
     // Columns of S^T (the MMA wants 16 at least), and of P^T and O^T: two BF16 terms of P side by side. kBlock of them are worked on at a time.
     static constexpr uint32_t kScores = kN < 16 ? 16 : kN, kTerms = 2 * kN, kBlock = kN < 16 ? kN : 16;
-    static constexpr uint32_t kQueryBytes = kScores * kHeadDim * 2, kQueryBuffers = kQueryBytes >= 12 * 1024 ? 1 : 2;
-    static constexpr uint32_t kWeightBytes = kTerms * kTile * 2;
-    static constexpr uint32_t kFixed = 1024 + kOnesBytes + sizeof(State) + kQueryBuffers * kQueryBytes + 2 * kWeightBytes;
-    static constexpr uint32_t kRoom = kSmemLimit - kFixed;
+    static constexpr uint32_t kQueryBytes = kScores * kHeadDim * 2, kWeightBytes = kTerms * kTile * 2;
+    static constexpr uint32_t fixed(uint32_t buffers) { return 1024 + kOnesBytes + sizeof(State) + buffers * kQueryBytes + 2 * kWeightBytes; }
+    static constexpr uint32_t slots(uint32_t buffers) {
+        const uint32_t fit = (kSmemLimit - fixed(buffers)) / kSlotBytes / 2 * 2;
+        return fit < 16 ? fit : 16;
+    }
     // A ring each for the keys and the values: a slot's uses then all belong to one of the two warps that load, which waits for them in turn. (With
     // slots that go from one warp to the other, a warp could take the end of the use before last for the end of the last one.)
-    // Where there are few slots, an odd one goes to the keys, and the queries are held once to gain it (8 tokens of 6 heads each, 4 x 16385 tokens: 59 us
-    // with 5 + 4 slots, 67 with 4 + 4); ten and more are kept even (one token, 2 x 131071: 163 us with 4 + 6, 168 with 5 + 6).
-    static constexpr uint32_t kFit = kRoom / kSlotBytes > 16 ? 16 : kRoom / kSlotBytes, kSlots = kFit < 10 ? kFit : kFit / 2 * 2;
+    // The queries of a pair are held twice, so that the next pair's are there in time, but once where that gains slots: 48 and 64 columns of head size 256
+    // (8 tokens of 6 heads each, 4 x 16385 tokens: 61.1 us with 4 + 4 slots, 69.3 with 2 + 4). The slots are even in number: an odd one, which went to the keys,
+    // was worth nothing (5 + 4 against 4 + 4: 5 tokens of 6 heads each 57.3 and 56.5 us; 3 + 4 against 2 + 4: 8 tokens of 8 heads of 128 95.6 and 94.1; one token,
+    // 2 x 131071: 5 + 6 against 4 + 6 168 and 163).
+    static constexpr uint32_t kQueryBuffers = slots(1) > slots(2) ? 1 : 2, kSlots = slots(kQueryBuffers), kFixed = fixed(kQueryBuffers);
     static constexpr uint32_t kValueSlots = (kSlots / 2 + 1) / 2 * 2, kKeySlots = kSlots - kValueSlots;   // (pairs of value slots are one operand)
     static constexpr uint32_t kSmem = kFixed + kSlots * kSlotBytes;
     // tensor memory: two of S^T, O^T in halves of 128 dims, the denominators
     static constexpr uint32_t kColumns = 2 * kScores + (kHalves + 1) * kTerms, kTmem = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
-    static_assert(kKeySlots >= 2 && kValueSlots >= kChunks /* a tile's values are looked at before any is used */ && kSmem <= kSmemLimit && kColumns <= 512, "a CTA's memory");
+    static_assert(kKeySlots >= 2 && kSlots % 2 == 0 && kValueSlots >= kChunks /* a tile's values are looked at before any is used */ && kSmem <= kSmemLimit && kColumns <= 512, "a CTA's memory");
 };
+
+static_assert(Shape<256, 8>::kKeySlots == 4 && Shape<256, 8>::kValueSlots == 6 && Shape<256, 48>::kKeySlots == 4 && Shape<256, 48>::kValueSlots == 4 &&
+                  Shape<256, 48>::kQueryBuffers == 1 && Shape<256, 32>::kSlots == 8 && Shape<256, 32>::kQueryBuffers == 2 && Shape<128, 64>::kSlots == 6,
+              "the slots that the figures above belong to");
 
 // A CTA's way through its span: one (sequence, head) after the other, in each the keys [key, key_end).
 struct Walk {
