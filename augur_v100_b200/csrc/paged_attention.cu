@@ -84,11 +84,12 @@ struct Shape {
     }
     // A ring each for the keys and the values: a slot's uses then all belong to one of the two warps that load, which waits for them in turn. (With
     // slots that go from one warp to the other, a warp could take the end of the use before last for the end of the last one.)
-    // The queries of a pair are held twice, so that the next pair's are there in time, but once where that gains slots: 48 and 64 columns of head size 256
-    // (8 tokens of 6 heads each, 4 x 16385 tokens: 61.1 us with 4 + 4 slots, 69.3 with 2 + 4). The slots are even in number: an odd one, which went to the keys,
-    // was worth nothing (5 + 4 against 4 + 4: 5 tokens of 6 heads each 57.3 and 56.5 us; 3 + 4 against 2 + 4: 8 tokens of 8 heads of 128 95.6 and 94.1; one token,
-    // 2 x 131071: 5 + 6 against 4 + 6 168 and 163).
-    static constexpr uint32_t kQueryBuffers = slots(1) > slots(2) ? 1 : 2, kSlots = slots(kQueryBuffers), kFixed = fixed(kQueryBuffers);
+    // The queries of a pair are held twice, so that the next pair's are there in time, but once where a tile of keys and one of values would not fit beside them: 48
+    // and 64 columns of head size 256 (8 tokens of 6 heads each, 4 x 16385 tokens: 61.1 us with 4 + 4 slots, 69.3 with 2 + 4). Elsewhere the slots gained are
+    // worth less than the second copy (one token of 4 heads of 128 each, 2 x 131071 tokens: 161.8 us with 4 + 6 slots, 171.6 with 6 + 6 and one copy; 8 tokens of
+    // them, 4 x 16385: 61.9 with 4 + 4, 62.3 with 4 + 6 and one copy). The slots are even in number: an odd one, which went to the keys, was worth nothing (5 + 4
+    // against 4 + 4: 5 tokens of 6 heads of 256 each 57.3 and 56.5 us; 3 + 4 against 2 + 4: 8 tokens of 8 heads of 128 95.6 and 94.1).
+    static constexpr uint32_t kQueryBuffers = slots(2) < 2 * kChunks ? 1 : 2, kSlots = slots(kQueryBuffers), kFixed = fixed(kQueryBuffers);
     static constexpr uint32_t kValueSlots = (kSlots / 2 + 1) / 2 * 2, kKeySlots = kSlots - kValueSlots;   // (pairs of value slots are one operand)
     static constexpr uint32_t kSmem = kFixed + kSlots * kSlotBytes;
     // tensor memory: two of S^T, O^T in halves of 128 dims, the denominators
@@ -96,8 +97,10 @@ struct Shape {
     static_assert(kKeySlots >= 2 && kSlots % 2 == 0 && kValueSlots >= kChunks /* a tile's values are looked at before any is used */ && kSmem <= kSmemLimit && kColumns <= 512, "a CTA's memory");
 };
 
-static_assert(Shape<256, 8>::kKeySlots == 4 && Shape<256, 8>::kValueSlots == 6 && Shape<256, 48>::kKeySlots == 4 && Shape<256, 48>::kValueSlots == 4 &&
-                  Shape<256, 48>::kQueryBuffers == 1 && Shape<256, 32>::kSlots == 8 && Shape<256, 32>::kQueryBuffers == 2 && Shape<128, 64>::kSlots == 6,
+template <uint32_t kHeadDim, uint32_t kN>
+constexpr uint32_t kLayout = 100 * Shape<kHeadDim, kN>::kKeySlots + 10 * Shape<kHeadDim, kN>::kValueSlots + Shape<kHeadDim, kN>::kQueryBuffers;
+static_assert(kLayout<128, 8> == 462 && kLayout<128, 16> == 462 && kLayout<128, 32> == 442 && kLayout<128, 48> == 442 && kLayout<128, 64> == 242 && kLayout<256, 8> == 462 &&
+                  kLayout<256, 16> == 462 && kLayout<256, 32> == 442 && kLayout<256, 48> == 441 && kLayout<256, 64> == 241,
               "the slots that the figures above belong to");
 
 // A CTA's way through its span: one (sequence, head) after the other, in each the keys [key, key_end).
