@@ -676,7 +676,7 @@ typedef struct augur_cuda_nvfp4_sm100_kv_layer_v1 {
 /* The sequences of one step, all in device memory, so that a captured program can be replayed with new contents:
  * sequence b owns the token rows [token_starts[b], token_starts[b + 1]) of the step, which are the last tokens of the
  * lengths[b] that its cache holds with them. Sequences without new tokens are allowed (idle slots); rows outside every
- * sequence are neither read nor written. Contents that do not fit (a page outside the cache, a length beyond the table,
+ * sequence are not written, and what they hold is not used (the cache write may read it). Contents that do not fit (a page outside the cache, a length beyond the table,
  * row numbers outside `rows`) never lead to an access out of bounds; each entry says what it does with them. */
 #define AUGUR_NVFP4_SM100_MAX_SEQUENCES 1024
 typedef struct augur_cuda_nvfp4_sm100_kv_batch_v1 {
@@ -698,10 +698,10 @@ typedef struct augur_cuda_nvfp4_sm100_kv_batch_v1 {
  * the first rotary_dim elements by positions[axis(i)][row] * inv_freq[i]. axis(i): sections one behind the other (time,
  * height, width; they add up to rotary_dim / 2) or, `interleaved`, i mod 3 while i < 3 * sections[i mod 3], else 0. With text
  * all three axes hold the same positions. The angle is formed in 64 bits and reduced to one turn there, so that positions of
- * millions lose nothing; the rest is F32, rounded once. Inputs are BF16 with strides (in elements, multiples of 8;
+ * millions lose nothing; the rest is F32, rounded once, the sum of a head's squares included (so a head norm wants elements below 2^60). Inputs are BF16 with strides (in elements, multiples of 8;
  * a head's elements are contiguous), so that q may be the query half of a query|gate projection: query_len_bytes and its
- * like are the bytes from the first to the last element. A row whose page is not in the table or outside the cache is rotated
- * into query_out, and its key and value are not written. Any number of rows per sequence (a chunk of a prompt too). */
+ * like are the bytes from the first to the last element. A row whose page is not in the table or outside the cache, or
+ * that lies before the cache's first token (fewer cached tokens than rows), is rotated into query_out, and its key and value are not written. Any number of rows per sequence (a chunk of a prompt too). */
 typedef struct augur_cuda_nvfp4_sm100_kv_append_args_v1 {
     uint32_t abi_version;
     uint32_t struct_size;
@@ -741,13 +741,13 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append_prevalidat
 /* Attention of up to max_new_tokens (1..8) new tokens per sequence over its cache, their own keys and values included:
  *   output[row][h] = sum_j p_j values[j],  p = softmax over j of scale * query[row][h] . keys[j]
  * for all cached j up to the row's own token. query_heads is a multiple of kv_heads; query_heads / kv_heads * max_new_tokens
- * is at most 64, table_pages * page_tokens at most 2^24. Products of BF16 are exact, sums, maxima and exponentials F32; the weights p enter the product with the values as two
+ * is at most 64, table_pages * page_tokens at most 2^24, sequences * kv_heads * (that / 64, rounded up) below 2^31. Products of BF16 are exact, sums, maxima and exponentials F32; the weights p enter the product with the values as two
  * BF16 terms (good to 2^-16 of p), and the denominator as the same. A row that sees no token gets zeros, and so does one all of whose
  * scores are -infinity (where the formula has no value). A NaN in a row's query, or in a key or value that it sees, gives NaN as in the
  * formula, as does a score of +infinity; an infinite value that it sees gives an infinity or NaN in that element. What the pages hold
  * behind a sequence's length is never used, infinities and NaN included; a value that is not finite among the sequence's own
  * new tokens may reach all of that sequence's rows. A page outside the cache counts as not there and sets the plan's status word to
- * 0x401, as does a length beyond the table; rows outside the tensors or more than max_new_tokens rows set 0x402, and such a
+ * 0x401, as does a length beyond the table, which counts as the table's; a negative length counts as 0; rows outside the tensors or more than max_new_tokens rows set 0x402, and such a
  * sequence is left out. A wait that runs out sets 0x411..0x417. The results of a call depend on its inputs
  * and on the device's SM count alone, not on the order in which CTAs finish. */
 typedef struct augur_cuda_nvfp4_sm100_paged_attention_args_v1 {
@@ -805,8 +805,8 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_copy_prevali
  * The reference selects on the host or with its own top-k kernels behind the same head; there is no counterpart of this
  * form. F32 logits (bf16_head) or BF16 ones (a linear's output); sums and statistics F32. A row of -infinities has entropy 0 and
  * log probabilities -infinity; a NaN or +infinity in a row gives what the formulas give (NaN), NaN ordered above all
- * numbers. row_stride in elements, at least `vocabulary`, vocabulary up to 2^24, rows up to 2^20, alternatives 0..32 (and at most
- * vocabulary; 0: ids and alternative_logprobs are 0, with 0 bytes). */
+ * numbers. row_stride in elements, at least `vocabulary` and at most 2^32, vocabulary up to 2^24, rows up to 2^20 (and units of 16 KB, a row's
+ * rounded up, below 2^31 in all), alternatives 0..32 (and at most vocabulary; 0: ids and alternative_logprobs are 0, with 0 bytes). */
 #define AUGUR_NVFP4_SM100_MAX_ALTERNATIVES 32
 #define AUGUR_NVFP4_SM100_LOGITS_F32 UINT32_C(0)
 #define AUGUR_NVFP4_SM100_LOGITS_BF16 UINT32_C(1)
