@@ -18,6 +18,8 @@
 // Work: the cached tokens of all (sequence, key-value head) pairs in units of 64, dealt out evenly as one span of units per SM. A pair
 // that lies in several spans leaves an unnormalised part per span in the plan's scratch, and a second launch joins those, in
 // the order of the spans. The spans follow from the lengths alone (read on the device, so that a captured call can be replayed).
+#include <cfloat>
+
 #include "kv_cache.cuh"
 #include "kv_join_record.h"
 #include "nvfp4_gemm.cuh"
@@ -37,7 +39,7 @@ constexpr uint32_t kMaxSequences = AUGUR_NVFP4_SM100_MAX_SEQUENCES;
 constexpr uint32_t kOnesBytes = kTile * 32;    // 16 k of ones, as the 128-row operand
 constexpr uint32_t kMaxTokensLog2 = 24;   // of a sequence
 constexpr float kSlack = 8.0f;            // how far, in powers of two, a score may pass the reference maximum
-constexpr float kNoNumber = -3.0e38f;     // a part's reference where a query sees keys but no score above -infinity (-infinity: sees none)
+constexpr float kNoNumber = -FLT_MAX;     // a part's reference where a query sees keys but no score above -infinity (-infinity: sees none)
 constexpr uint32_t kStatusPage = 0x401, kStatusRows = 0x402;
 constexpr uint32_t kStatusLoad = 0x411, kStatusMma = 0x412, kStatusScores = 0x413, kStatusValues = 0x414, kStatusQuery = 0x415, kStatusGroup = 0x416, kStatusProduct = 0x417;
 constexpr uint32_t kThreads = 256;        // warp 0 loads keys, 1 MMA, 2 queries, 3 values, 4..7 softmax

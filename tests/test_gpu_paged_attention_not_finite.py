@@ -162,6 +162,26 @@ def test_a_row_whose_scores_are_all_minus_infinity(stream, length):
     assert bool(out[0, 20].isnan().all())
 
 
+@pytest.mark.parametrize("length", LENGTHS[1:])
+def test_lowest_scores_beside_minus_infinity(stream, length):
+    # The first half's scores are all -1.3 2^127, in powers of two -1.87 2^127, among the lowest that F32 holds; the second half's are -infinity. The first half weighs
+    # the same, and the row gets its mean: as good as sums of fewer than 2^15 terms, each rounded by 2^-23 of what is summed, and the output's rounding.
+    batch = Batch([(length, 1)], *LAYER, 64, seed=length + 4)
+    batch.k.zero_()
+    batch.q.zero_()
+    batch.q[0, :, 7] = 1.296875 * 2.0 ** 63
+    half = (length + 1) // 2
+    position = torch.arange(length, device="cuda:0")
+    batch.k[0, batch.table[0, position // 64].long(), :, position % 64, 7] = torch.where(position < half, -2.0 ** 64, -math.inf).to(torch.bfloat16)[:, None]
+    plan = host.Plan(stream, kv.paged_attention_scratch_bytes(*LAYER, 1))
+    call = kv.PagedAttention.bind(plan, kv.KvCache(batch.k, batch.v), 0, batch.q, batch.table, batch.lengths, batch.starts, 1, scale=1.0)
+    call.submit_for_plan()
+    stream.synchronize()
+    _, v = batch.cached(0)
+    want, spread = v[:, :half].mean(1), v[:, :half].abs().mean(1)
+    _within(call.out[0].reshape(4, 6, 256), want[:, None], (BF16_HALF_ULP * want.abs() + half * 2.0 ** -22 * spread)[:, None])
+
+
 @pytest.mark.parametrize("length", LENGTHS)
 def test_infinity_and_nan_in_a_value(stream, length):
     # Documented: an infinity that a row sees gives an infinity or NaN, in its own element of the head only.
