@@ -67,6 +67,19 @@ class Stream:
             pass
 
 
+def allocated(stream: Stream, make, *args, **kwargs) -> torch.Tensor:
+    """What `make` makes, on the stream's own memory: nothing enqueued elsewhere still uses it, and what `make` enqueues goes ahead of the submits. It goes back to
+    the stream once the stream that is current now, where results are read, is done with it too."""
+    reader = torch.cuda.current_stream(stream.ordinal)
+    if reader == stream.torch_stream:
+        return make(*args, **kwargs)
+    with torch.cuda.stream(stream.torch_stream):
+        made = make(*args, **kwargs)
+    if made.is_cuda:
+        made.record_stream(reader)
+    return made
+
+
 class Plan:
     """Stream-owned scratch (split-K partials, arrival counters, activation staging)."""
 
@@ -728,11 +741,10 @@ class TokenLogprobs:
         if not 0 <= alternatives <= abi.MAX_ALTERNATIVES:
             raise ValueError(f"0 to {abi.MAX_ALTERNATIVES} alternatives")
         self.plan, self.logits, self.targets = plan, logits, targets
-        empty = functools.partial(torch.empty, device=logits.device)
-        with torch.cuda.stream(plan.stream.torch_stream):   # memory of that stream's: nothing enqueued elsewhere still uses it
-            self.logprobs, self.entropy = empty(rows, dtype=torch.float32), empty(rows, dtype=torch.float32)
-            self.ids = empty((rows, alternatives), dtype=torch.int32)
-            self.alternative_logprobs = empty((rows, alternatives), dtype=torch.float32)
+        empty = functools.partial(allocated, plan.stream, torch.empty, device=logits.device)
+        self.logprobs, self.entropy = empty(rows, dtype=torch.float32), empty(rows, dtype=torch.float32)
+        self.ids = empty((rows, alternatives), dtype=torch.int32)
+        self.alternative_logprobs = empty((rows, alternatives), dtype=torch.float32)
         a = abi.header(abi.TokenLogprobsArgs)
         a.row_stride = logits.stride(0) if rows > 1 else vocabulary
         a.logits, a.logits_len_bytes = _ptr(logits), ((rows - 1) * a.row_stride + vocabulary) * logits.element_size()

@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from . import abi
-from .host import Plan, Stream, _check, _nbytes, _ptr, sm_count
+from .host import Plan, Stream, _check, _nbytes, _ptr, allocated, sm_count
 
 
 def _require(tensor: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device | None = None) -> torch.Tensor:
@@ -43,8 +43,7 @@ class KvCache:
     @classmethod
     def allocate(cls, stream: Stream, layers: int, pages: int, kv_heads: int, page_tokens: int, head_dim: int):
         shape, device = (layers, pages, kv_heads, page_tokens, head_dim), torch.device("cuda", stream.ordinal)
-        with torch.cuda.stream(stream.torch_stream):
-            return cls(torch.empty(shape, dtype=torch.bfloat16, device=device), torch.empty(shape, dtype=torch.bfloat16, device=device))
+        return cls(*(allocated(stream, torch.empty, shape, dtype=torch.bfloat16, device=device) for _ in range(2)))
 
     def layer_args(self, layer: int) -> abi.KvLayer:
         if not 0 <= layer < self.layers:
@@ -118,8 +117,7 @@ class KvAppend:
              interleaved: bool = False, q_out: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
              k_norm: torch.Tensor | None = None, epsilon: float = 1e-6):
         if q_out is None:
-            with torch.cuda.stream(stream.torch_stream):   # memory of that stream's: nothing enqueued elsewhere still uses it
-                q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+            q_out = allocated(stream, torch.empty, q.shape, dtype=torch.bfloat16, device=q.device)
         self = cls(stream, cache, layer, q, k, v, positions, frequencies, sections, table, lengths, starts, interleaved, q_out, q_norm, k_norm,
                    epsilon)
         _check("kv_append_preflight", abi.lib().augur_cuda_nvfp4_sm100_kv_append_preflight_v1(stream.ordinal, stream.handle, byref(self.args)))
@@ -163,8 +161,7 @@ class PagedAttention:
     def bind(cls, plan: Plan, cache: KvCache, layer: int, q, table, lengths, starts, tokens: int = 1, out: torch.Tensor | None = None,
              scale: float | None = None):
         if out is None:
-            with torch.cuda.stream(plan.stream.torch_stream):   # the zeros go ahead of the submits
-                out = torch.zeros_like(q)
+            out = allocated(plan.stream, torch.zeros_like, q)
         self = cls(plan, cache, layer, q, table, lengths, starts, tokens, out, cache.head_dim ** -0.5 if scale is None else scale)
         s = plan.stream
         _check("paged_attention_preflight", abi.lib().augur_cuda_nvfp4_sm100_paged_attention_preflight_v1(

@@ -92,3 +92,24 @@ def test_cache(side):
         cache.values.fill_(4)
     torch.cuda.synchronize()
     assert bool((cache.keys == 3).all()) and bool((cache.values == 4).all())
+
+
+def test_an_output_that_the_current_stream_still_reads(side):
+    # the current stream lags, then copies an output whose owner is gone: the next owner's output lies elsewhere
+    batch = Batch([(300, 1), (40, 1)], 24, 4, 256, 64, seed=5)
+    plan = host.Plan(side, kv.paged_attention_scratch_bytes(24, 4, 256, 1))
+    bind = lambda q: kv.PagedAttention.bind(plan, kv.KvCache(batch.k, batch.v), 0, q, batch.table, batch.lengths, batch.starts)  # noqa: E731
+    other = -batch.q
+    torch.cuda.synchronize()
+    call = bind(batch.q)
+    call.submit_for_plan()
+    side.synchronize()
+    want = call.out.clone()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(CYCLES)
+    got = call.out.clone()
+    del call
+    second = bind(other)
+    second.submit_for_plan()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and not torch.equal(second.out, want)
