@@ -375,7 +375,7 @@ def exact(case, seed):
                  for b in range(len(lengths)) for row in range(starts[b], starts[b + 1])]
         at, offset = (torch.tensor(x, device=DEVICE) for x in zip(*slots))
         for held, x, which in ((k, rotated(state["k"], state["k_norm"]), 0), (v, state["v"].double(), 1)):
-            power = torch.exp2(torch.ceil(torch.log2(x.abs().amax(-1, keepdim=True) / 448)).clamp(-60, 60))
+            power = torch.exp2(torch.ceil(torch.log2(x.abs().amax(-1, keepdim=True) / 448) - 1e-9).clamp(-60, 60))   # (log2 of a power of two may be an ulp off)
             held[0, at, :, offset] = _nearest_e4m3(x / power)
             scales[0, at, :, offset, which] = power[..., 0]
         return {"q": rotated(state["q"], state["q_norm"]), "k": k, "v": v, "scales": scales}
