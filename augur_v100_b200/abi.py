@@ -216,6 +216,35 @@ class KvPageCopyArgs(Structure):
                 ("layers", c_uint32), ("pages", c_uint32)]
 
 
+class KvE4m3Layer(Structure):
+    _fields_ = [("keys", c_uint64), ("values", c_uint64), ("scales", c_uint64), ("len_bytes", c_uint64), ("scales_len_bytes", c_uint64),
+                ("pages", c_uint32), ("kv_heads", c_uint32), ("page_tokens", c_uint32), ("head_dim", c_uint32)]
+
+
+class KvAppendE4m3Args(Structure):
+    _fields_ = [(name, KvE4m3Layer if name == "layer" else kind) for name, kind in KvAppendArgs._fields_]
+
+
+class PagedAttentionE4m3Args(Structure):
+    _fields_ = [(name, KvE4m3Layer if name == "layer" else kind) for name, kind in PagedAttentionArgs._fields_]
+
+
+class KvPageCopyE4m3Args(Structure):
+    _fields_ = [("abi_version", c_uint32), ("struct_size", c_uint32),
+                ("keys", c_uint64), ("values", c_uint64), ("scales", c_uint64), ("len_bytes", c_uint64), ("scales_len_bytes", c_uint64),
+                ("page_bytes", c_uint64), ("scale_page_bytes", c_uint64), ("layers", c_uint32), ("pages", c_uint32)]
+
+
+class SharedPrefixAttentionArgs(Structure):
+    _fields_ = [("abi_version", c_uint32), ("struct_size", c_uint32),
+                ("layer", KvLayer), ("batch", KvBatch),
+                ("prefix_pages", c_uint64), ("prefix_pages_len_bytes", c_uint64),
+                ("prefix_tokens", c_uint64), ("prefix_tokens_len_bytes", c_uint64),
+                ("query", c_uint64), ("query_len_bytes", c_uint64),
+                ("output", c_uint64), ("output_len_bytes", c_uint64),
+                ("query_heads", c_uint32), ("max_new_tokens", c_uint32), ("scale", c_float), ("reserved", c_uint32)]
+
+
 class TokenLogprobsArgs(Structure):
     _fields_ = [("abi_version", c_uint32), ("struct_size", c_uint32),
                 ("logits", c_uint64), ("logits_len_bytes", c_uint64),
@@ -292,6 +321,15 @@ EXPORTS = {
     "augur_cuda_nvfp4_sm100_paged_attention_prevalidated_submit_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(PagedAttentionArgs)]),
     "augur_cuda_nvfp4_sm100_kv_page_copy_preflight_v1": (Result, [c_int32, c_void_p, POINTER(KvPageCopyArgs)]),
     "augur_cuda_nvfp4_sm100_kv_page_copy_prevalidated_submit_v1": (Result, [c_int32, c_void_p, POINTER(KvPageCopyArgs), c_void_p, c_void_p, c_uint32]),
+    "augur_cuda_nvfp4_sm100_kv_append_e4m3_preflight_v1": (Result, [c_int32, c_void_p, POINTER(KvAppendE4m3Args)]),
+    "augur_cuda_nvfp4_sm100_kv_append_e4m3_prevalidated_submit_v1": (Result, [c_int32, c_void_p, POINTER(KvAppendE4m3Args)]),
+    "augur_cuda_nvfp4_sm100_paged_attention_e4m3_preflight_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(PagedAttentionE4m3Args)]),
+    "augur_cuda_nvfp4_sm100_paged_attention_e4m3_prevalidated_submit_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(PagedAttentionE4m3Args)]),
+    "augur_cuda_nvfp4_sm100_kv_page_copy_e4m3_preflight_v1": (Result, [c_int32, c_void_p, POINTER(KvPageCopyE4m3Args)]),
+    "augur_cuda_nvfp4_sm100_kv_page_copy_e4m3_prevalidated_submit_v1": (Result, [c_int32, c_void_p, POINTER(KvPageCopyE4m3Args), c_void_p, c_void_p, c_uint32]),
+    "augur_cuda_nvfp4_sm100_shared_prefix_attention_scratch_extent_host_v1": (Result, [c_uint32, c_uint32, c_uint32, c_uint32, c_uint32, c_uint32, POINTER(c_uint64)]),
+    "augur_cuda_nvfp4_sm100_shared_prefix_attention_preflight_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(SharedPrefixAttentionArgs)]),
+    "augur_cuda_nvfp4_sm100_shared_prefix_attention_prevalidated_submit_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(SharedPrefixAttentionArgs)]),
     "augur_cuda_nvfp4_sm100_token_logprobs_scratch_extent_host_v1": (Result, [c_uint32, c_uint32, c_uint32, POINTER(c_uint64)]),
     "augur_cuda_nvfp4_sm100_token_logprobs_preflight_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(TokenLogprobsArgs)]),
     "augur_cuda_nvfp4_sm100_token_logprobs_prevalidated_submit_v1": (Result, [c_int32, c_void_p, c_void_p, POINTER(TokenLogprobsArgs)]),

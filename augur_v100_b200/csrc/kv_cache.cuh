@@ -23,6 +23,26 @@ inline bool kv_layer_ok(const augur_cuda_nvfp4_sm100_kv_layer_v1& l) {
     return rows < (UINT64_C(1) << 31) && l.len_bytes == rows * l.head_dim * 2;
 }
 
+inline bool kv_layer_ok(const augur_cuda_nvfp4_sm100_kv_e4m3_layer_v1& l) {
+    const uint64_t rows = static_cast<uint64_t>(l.pages) * l.kv_heads * l.page_tokens;
+    return kv_layer_ok(augur_cuda_nvfp4_sm100_kv_layer_v1{l.keys, l.values, 2 * l.len_bytes, l.pages, l.kv_heads, l.page_tokens, l.head_dim}) &&
+           l.len_bytes <= UINT64_MAX / 2 && l.scales_len_bytes == rows * 2;
+}
+
+// The tensors of a layer, for the checks of ranges: at most kKvRanges.
+constexpr size_t kKvRanges = 3;
+inline size_t kv_ranges(const augur_cuda_nvfp4_sm100_kv_layer_v1& l, Range* to) {
+    to[0] = {l.keys, l.len_bytes, 16}, to[1] = {l.values, l.len_bytes, 16};
+    return 2;
+}
+inline size_t kv_ranges(const augur_cuda_nvfp4_sm100_kv_e4m3_layer_v1& l, Range* to) {
+    to[0] = {l.keys, l.len_bytes, 16}, to[1] = {l.values, l.len_bytes, 16}, to[2] = {l.scales, l.scales_len_bytes, 16};
+    return 3;
+}
+
+// Scale bytes of the E4M3 cache: 2^(byte - 127).
+constexpr uint32_t kE4m3LeastScale = 127 - 60, kE4m3LargestScale = 127 + 60;
+
 inline bool kv_batch_ok(const augur_cuda_nvfp4_sm100_kv_batch_v1& b) {
     return b.sequences >= 1 && b.sequences <= AUGUR_NVFP4_SM100_MAX_SEQUENCES && b.table_pages >= 1 && b.table_pages <= (1u << 24) && b.rows >= 1 &&
            b.rows <= (1u << 20) && b.reserved == 0 && b.page_table_len_bytes == static_cast<uint64_t>(b.sequences) * b.table_pages * 4 &&

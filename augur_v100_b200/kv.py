@@ -52,6 +52,45 @@ class KvCache:
         return abi.KvLayer(_ptr(keys), _ptr(values), _nbytes(keys), self.pages, self.kv_heads, self.page_tokens, self.head_dim)
 
 
+class KvCacheE4m3:
+    """Keys and values of all layers in 8 bits: two tensors of E4M3 codes [layers, pages, kv_heads, page_tokens, head_dim] and
+    the scales of every token's heads, E8M0 [layers, pages, kv_heads, page_tokens, 2] (keys, values); an element is code times scale.
+
+    `KvAppend`, `PagedAttention` and `KvPageCopy` take it in a `KvCache`'s place. It holds half the bytes, and attention over it reads half;
+    an element keeps four significant bits (2^-4 relative at most, near a head's largest element as far below it)."""
+
+    def __init__(self, keys: torch.Tensor, values: torch.Tensor, scales: torch.Tensor):
+        if keys.dim() != 5:
+            raise ValueError("keys: [layers, pages, kv_heads, page_tokens, head_dim]")
+        _require(keys, "keys", torch.float8_e4m3fn, keys.shape)
+        _require(values, "values", torch.float8_e4m3fn, keys.shape, keys.device)
+        _require(scales, "scales", torch.float8_e8m0fnu, (*keys.shape[:4], 2), keys.device)
+        self.keys, self.values, self.scales = keys, values, scales
+        self.layers, self.pages, self.kv_heads, self.page_tokens, self.head_dim = keys.shape
+
+    @classmethod
+    def allocate(cls, stream: Stream, layers: int, pages: int, kv_heads: int, page_tokens: int, head_dim: int):
+        shape, device = (layers, pages, kv_heads, page_tokens, head_dim), torch.device("cuda", stream.ordinal)
+        codes = [allocated(stream, torch.empty, shape, dtype=torch.float8_e4m3fn, device=device) for _ in range(2)]
+        return cls(*codes, allocated(stream, torch.empty, (*shape[:4], 2), dtype=torch.float8_e8m0fnu, device=device))
+
+    def layer_args(self, layer: int) -> abi.KvE4m3Layer:
+        if not 0 <= layer < self.layers:
+            raise ValueError("no such layer")
+        keys, values, scales = self.keys[layer], self.values[layer], self.scales[layer]
+        return abi.KvE4m3Layer(_ptr(keys), _ptr(values), _ptr(scales), _nbytes(keys), _nbytes(scales), self.pages, self.kv_heads, self.page_tokens, self.head_dim)
+
+
+def _entries(cache, name: str, arguments: str):
+    """The descriptor and the two entries of an operator for the kind of cache."""
+    if isinstance(cache, KvCacheE4m3):
+        name, arguments = name + "_e4m3", arguments.replace("Args", "E4m3Args")
+    elif not isinstance(cache, KvCache):
+        raise ValueError("cache: a KvCache or a KvCacheE4m3")
+    lib, prefix = abi.lib(), "augur_cuda_nvfp4_sm100_" + name
+    return abi.header(getattr(abi, arguments)), getattr(lib, prefix + "_preflight_v1"), getattr(lib, prefix + "_prevalidated_submit_v1")
+
+
 def _batch_args(table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, rows: int, device: torch.device) -> abi.KvBatch:
     if table.dim() != 2:
         raise ValueError("page table: [sequences, pages]")
@@ -82,13 +121,13 @@ class KvAppend:
     every head first. Rows of sequence b are [starts[b], starts[b + 1]), the last of the lengths[b] tokens that its pages hold
     with them, any number of them."""
 
-    def __init__(self, stream: Stream, cache: KvCache, layer: int, q, k, v, positions, frequencies, sections, table, lengths, starts,
+    def __init__(self, stream: Stream, cache: KvCache | KvCacheE4m3, layer: int, q, k, v, positions, frequencies, sections, table, lengths, starts,
                  interleaved: bool, q_out, q_norm, k_norm, epsilon: float):
         rows, query_heads, head_dim = q.shape
         device = cache.keys.device
         self.stream, self.cache, self.q_out = stream, cache, q_out
         self._keep = (q, k, v, positions, frequencies, table, lengths, starts, q_norm, k_norm)
-        a = abi.header(abi.KvAppendArgs)
+        a, self._preflight, enqueue = _entries(cache, "kv_append", "KvAppendArgs")
         a.layer, a.batch = cache.layer_args(layer), _batch_args(table, lengths, starts, rows, device)
         a.query, a.query_len_bytes, a.query_row_stride, a.query_head_stride = _strided(q, "q", rows, query_heads, cache.head_dim, device)
         a.key, a.key_len_bytes, a.key_row_stride, a.key_head_stride = _strided(k, "k", rows, cache.kv_heads, cache.head_dim, device)
@@ -110,17 +149,17 @@ class KvAppend:
         for i, section in enumerate(sections):
             a.sections[i] = section
         self.args = a
-        self._enqueue = functools.partial(abi.lib().augur_cuda_nvfp4_sm100_kv_append_prevalidated_submit_v1, stream.ordinal, stream.handle, byref(a))
+        self._enqueue = functools.partial(enqueue, stream.ordinal, stream.handle, byref(a))
 
     @classmethod
-    def bind(cls, stream: Stream, cache: KvCache, layer: int, q, k, v, positions, frequencies, sections, table, lengths, starts,
+    def bind(cls, stream: Stream, cache: KvCache | KvCacheE4m3, layer: int, q, k, v, positions, frequencies, sections, table, lengths, starts,
              interleaved: bool = False, q_out: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
              k_norm: torch.Tensor | None = None, epsilon: float = 1e-6):
         if q_out is None:
             q_out = allocated(stream, torch.empty, q.shape, dtype=torch.bfloat16, device=q.device)
         self = cls(stream, cache, layer, q, k, v, positions, frequencies, sections, table, lengths, starts, interleaved, q_out, q_norm, k_norm,
                    epsilon)
-        _check("kv_append_preflight", abi.lib().augur_cuda_nvfp4_sm100_kv_append_preflight_v1(stream.ordinal, stream.handle, byref(self.args)))
+        _check("kv_append_preflight", self._preflight(stream.ordinal, stream.handle, byref(self.args)))
         return self
 
     def submit(self) -> None:
@@ -141,54 +180,106 @@ class PagedAttention:
     `q` [rows, query_heads, head_dim] BF16 (what `KvAppend` leaves in `q_out`) -> `out`, the same shape. Rows outside every
     sequence keep what `out` holds. query_heads / kv_heads * tokens is at most 64."""
 
-    def __init__(self, plan: Plan, cache: KvCache, layer: int, q, table, lengths, starts, tokens: int, out, scale: float):
+    def __init__(self, plan: Plan, cache: KvCache | KvCacheE4m3, layer: int, q, table, lengths, starts, tokens: int, out, scale: float):
         rows, query_heads, head_dim = q.shape
         device = cache.keys.device
         _require(q, "q", torch.bfloat16, (rows, query_heads, cache.head_dim), device)
         _require(out, "out", torch.bfloat16, q.shape, device)
         self.plan, self.cache, self.q, self.out = plan, cache, q, out
         self._keep = (table, lengths, starts)
-        a = abi.header(abi.PagedAttentionArgs)
+        a, self._preflight, enqueue = _entries(cache, "paged_attention", "PagedAttentionArgs")
         a.layer, a.batch = cache.layer_args(layer), _batch_args(table, lengths, starts, rows, device)
         a.query, a.query_len_bytes = _ptr(q), _nbytes(q)
         a.output, a.output_len_bytes = _ptr(out), _nbytes(out)
         a.query_heads, a.max_new_tokens, a.scale = query_heads, tokens, scale
         self.args = a
-        self._enqueue = functools.partial(abi.lib().augur_cuda_nvfp4_sm100_paged_attention_prevalidated_submit_v1, plan.stream.ordinal, plan.stream.handle,
-                                          plan.handle, byref(a))
+        self._enqueue = functools.partial(enqueue, plan.stream.ordinal, plan.stream.handle, plan.handle, byref(a))
 
     @classmethod
-    def bind(cls, plan: Plan, cache: KvCache, layer: int, q, table, lengths, starts, tokens: int = 1, out: torch.Tensor | None = None,
+    def bind(cls, plan: Plan, cache: KvCache | KvCacheE4m3, layer: int, q, table, lengths, starts, tokens: int = 1, out: torch.Tensor | None = None,
              scale: float | None = None):
         if out is None:
             out = allocated(plan.stream, torch.zeros_like, q)
         self = cls(plan, cache, layer, q, table, lengths, starts, tokens, out, cache.head_dim ** -0.5 if scale is None else scale)
         s = plan.stream
-        _check("paged_attention_preflight", abi.lib().augur_cuda_nvfp4_sm100_paged_attention_preflight_v1(
-            s.ordinal, s.handle, plan.handle, byref(self.args)))
+        _check("paged_attention_preflight", self._preflight(s.ordinal, s.handle, plan.handle, byref(self.args)))
         return self
 
     def submit_for_plan(self) -> None:
         _check("paged_attention_submit", self._enqueue())
 
 
-class KvPageCopy:
-    """Copies pages of a cache, keys and values of all layers: `submit(sources, destinations)` with two lists of page numbers.
-    Destinations are distinct and none is a source; anything else is refused with nothing enqueued."""
+def shared_prefix_attention_scratch_bytes(query_heads: int, kv_heads: int, head_dim: int, rows: int, tokens: int = abi.MAX_SMALL_TOKENS, sms: int = 0) -> int:
+    """Plan scratch of a `SharedPrefixAttention` of `rows` token rows and up to `tokens` new tokens per sequence (`sms` as for `paged_attention_scratch_bytes`)."""
+    out = c_uint64()
+    _check("shared_prefix_attention_scratch_extent", abi.lib().augur_cuda_nvfp4_sm100_shared_prefix_attention_scratch_extent_host_v1(
+        query_heads, kv_heads, head_dim, rows, tokens, sms or sm_count(), byref(out)))
+    return int(out.value)
 
-    def __init__(self, stream: Stream, cache: KvCache):
-        self.stream, self.cache = stream, cache
-        a = abi.header(abi.KvPageCopyArgs)
-        a.keys, a.values, a.len_bytes = _ptr(cache.keys), _ptr(cache.values), _nbytes(cache.keys)
-        a.page_bytes = cache.kv_heads * cache.page_tokens * cache.head_dim * 2
-        a.layers, a.pages = cache.layers, cache.pages
+
+class SharedPrefixAttention:
+    """`PagedAttention` over a BF16 cache for sequences that begin with the same tokens (a system prompt, the forks of one conversation), whose keys and
+    values are read once for all of them. `prefix_pages` int32 [n]: the pages of those tokens (`KvPagePool.shared_prefix` has them);
+    `prefix_tokens` int32 [1]: how many they are, counted in whole pages; both device memory. `lengths` count the shared tokens too, and the
+    page table has its columns for them, whatever it says there. Behind the prefix everything is as for `PagedAttention`."""
+
+    def __init__(self, plan: Plan, cache: KvCache, layer: int, q, table, lengths, starts, prefix_pages, prefix_tokens, tokens: int, out, scale: float):
+        if not isinstance(cache, KvCache):
+            raise ValueError("cache: a KvCache")
+        rows, query_heads, _ = q.shape
+        device = cache.keys.device
+        _require(q, "q", torch.bfloat16, (rows, query_heads, cache.head_dim), device)
+        _require(out, "out", torch.bfloat16, q.shape, device)
+        if prefix_pages.dim() != 1 or prefix_pages.shape[0] < 1:
+            raise ValueError("prefix pages: [n], at least one")
+        _require(prefix_pages, "prefix pages", torch.int32, prefix_pages.shape, device)
+        _require(prefix_tokens, "prefix tokens", torch.int32, (1,), device)
+        self.plan, self.cache, self.q, self.out = plan, cache, q, out
+        self._keep = (table, lengths, starts, prefix_pages, prefix_tokens)
+        a, self._preflight, enqueue = _entries(cache, "shared_prefix_attention", "SharedPrefixAttentionArgs")
+        a.layer, a.batch = cache.layer_args(layer), _batch_args(table, lengths, starts, rows, device)
+        a.prefix_pages, a.prefix_pages_len_bytes = _ptr(prefix_pages), _nbytes(prefix_pages)
+        a.prefix_tokens, a.prefix_tokens_len_bytes = _ptr(prefix_tokens), _nbytes(prefix_tokens)
+        a.query, a.query_len_bytes = _ptr(q), _nbytes(q)
+        a.output, a.output_len_bytes = _ptr(out), _nbytes(out)
+        a.query_heads, a.max_new_tokens, a.scale = query_heads, tokens, scale
         self.args = a
-        self._enqueue = functools.partial(abi.lib().augur_cuda_nvfp4_sm100_kv_page_copy_prevalidated_submit_v1, stream.ordinal, stream.handle, byref(a))
+        self._enqueue = functools.partial(enqueue, plan.stream.ordinal, plan.stream.handle, plan.handle, byref(a))
 
     @classmethod
-    def bind(cls, stream: Stream, cache: KvCache):
+    def bind(cls, plan: Plan, cache: KvCache, layer: int, q, table, lengths, starts, prefix_pages, prefix_tokens, tokens: int = 1,
+             out: torch.Tensor | None = None, scale: float | None = None):
+        if out is None:
+            out = allocated(plan.stream, torch.zeros_like, q)
+        self = cls(plan, cache, layer, q, table, lengths, starts, prefix_pages, prefix_tokens, tokens, out,
+                   cache.head_dim ** -0.5 if scale is None else scale)
+        s = plan.stream
+        _check("shared_prefix_attention_preflight", self._preflight(s.ordinal, s.handle, plan.handle, byref(self.args)))
+        return self
+
+    def submit_for_plan(self) -> None:
+        _check("shared_prefix_attention_submit", self._enqueue())
+
+
+class KvPageCopy:
+    """Copies pages of a cache, keys and values (and scales) of all layers: `submit(sources, destinations)` with two lists of page numbers.
+    Destinations are distinct and none is a source; anything else is refused with nothing enqueued."""
+
+    def __init__(self, stream: Stream, cache: KvCache | KvCacheE4m3):
+        self.stream, self.cache = stream, cache
+        a, self._preflight, enqueue = _entries(cache, "kv_page_copy", "KvPageCopyArgs")
+        a.keys, a.values, a.len_bytes = _ptr(cache.keys), _ptr(cache.values), _nbytes(cache.keys)
+        a.page_bytes = cache.kv_heads * cache.page_tokens * cache.head_dim * cache.keys.element_size()
+        if isinstance(cache, KvCacheE4m3):
+            a.scales, a.scales_len_bytes, a.scale_page_bytes = _ptr(cache.scales), _nbytes(cache.scales), cache.kv_heads * cache.page_tokens * 2
+        a.layers, a.pages = cache.layers, cache.pages
+        self.args = a
+        self._enqueue = functools.partial(enqueue, stream.ordinal, stream.handle, byref(a))
+
+    @classmethod
+    def bind(cls, stream: Stream, cache: KvCache | KvCacheE4m3):
         self = cls(stream, cache)
-        _check("kv_page_copy_preflight", abi.lib().augur_cuda_nvfp4_sm100_kv_page_copy_preflight_v1(stream.ordinal, stream.handle, byref(self.args)))
+        _check("kv_page_copy_preflight", self._preflight(stream.ordinal, stream.handle, byref(self.args)))
         return self
 
     def submit(self, sources, destinations) -> None:
@@ -309,6 +400,18 @@ class KvPagePool:
         for page in self._pages.pop(sequence):
             self._drop(page)
         del self._length[sequence]
+
+    def shared_prefix(self, sequences) -> list[int]:
+        """The pages that all of the sequences (None is an idle slot) begin with, in order; all of them are full. For `SharedPrefixAttention`."""
+        held = [(self._pages[s], self._length[s]) for s in sequences if s is not None]
+        if not held:
+            return []
+        full = min(length // self.page_tokens for _, length in held)
+        first = held[0][0]
+        for i in range(full):
+            if any(pages[i] != first[i] for pages, _ in held):
+                return first[:i]
+        return first[:full]
 
     def compact(self) -> PageCopies:
         """Moves the pages in use to the front of the cache: the highest ones into the lowest free ones. The tables change at once."""

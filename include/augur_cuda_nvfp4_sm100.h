@@ -796,6 +796,148 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_copy_prevali
     int32_t ordinal, augur_cuda_stream_t stream, const augur_cuda_nvfp4_sm100_kv_page_copy_args_v1* args,
     const uint32_t* sources, const uint32_t* destinations, uint32_t count);
 
+/* ---- the cache in 8 bits ------------------------------------------------------------------------- */
+/* One layer of it is two tensors of E4M3 codes [pages][kv_heads][page_tokens][head_dim] and one of scale bytes
+ * [pages][kv_heads][page_tokens][2] (keys, values): an element is code * 2^(byte - 127), one scale for a token's head. Half of what the BF16
+ * cache takes, and half of what a decoding step reads. Limits as for the BF16 cache. Scale bytes are 67..187 (2^-60..2^60); smaller ones
+ * count as 67, larger ones as 187, and 255 as NaN. The reference's 8-bit cache holds whole numbers with a scale for 32 of them; here the matrix
+ * units multiply the codes as they lie in the pages, which a scale within a token's head would not allow. */
+typedef struct augur_cuda_nvfp4_sm100_kv_e4m3_layer_v1 {
+    augur_cuda_device_ptr_t keys;
+    augur_cuda_device_ptr_t values;
+    augur_cuda_device_ptr_t scales;
+    uint64_t len_bytes;                     /* of keys and of values */
+    uint64_t scales_len_bytes;
+    uint32_t pages;
+    uint32_t kv_heads;
+    uint32_t page_tokens;
+    uint32_t head_dim;
+} augur_cuda_nvfp4_sm100_kv_e4m3_layer_v1;
+
+/* kv_append into such a cache. Everything is as there, query_out too; a token's key (behind norm and rotation, F32) and its value are
+ * quantised: with a the largest magnitude among the elements that are numbers, the scale is the smallest 2^e (e >= -60) for which
+ * a <= 448 * 2^e, and the codes are the elements * 2^-e to the nearest, ties to the even code. NaN stays NaN; an infinity, or
+ * a magnitude above 448 * 2^60, becomes NaN too (the type has no infinity). */
+typedef struct augur_cuda_nvfp4_sm100_kv_append_e4m3_args_v1 {
+    uint32_t abi_version;
+    uint32_t struct_size;
+    augur_cuda_nvfp4_sm100_kv_e4m3_layer_v1 layer;
+    augur_cuda_nvfp4_sm100_kv_batch_v1 batch;
+    augur_cuda_device_ptr_t query;
+    uint64_t query_len_bytes;
+    augur_cuda_device_ptr_t key;
+    uint64_t key_len_bytes;
+    augur_cuda_device_ptr_t value;
+    uint64_t value_len_bytes;
+    uint64_t query_row_stride, query_head_stride;
+    uint64_t key_row_stride, key_head_stride;
+    uint64_t value_row_stride, value_head_stride;
+    augur_cuda_device_ptr_t positions;
+    uint64_t positions_len_bytes;
+    augur_cuda_device_ptr_t inv_freq_f32;
+    uint64_t inv_freq_len_bytes;
+    augur_cuda_device_ptr_t query_norm_f32;
+    augur_cuda_device_ptr_t key_norm_f32;
+    uint64_t norm_len_bytes;
+    augur_cuda_device_ptr_t query_out;
+    uint64_t query_out_len_bytes;
+    uint32_t query_heads;
+    uint32_t rotary_dim;
+    uint32_t sections[3];
+    uint32_t interleaved;
+    float epsilon;
+    uint32_t reserved;
+} augur_cuda_nvfp4_sm100_kv_append_e4m3_args_v1;
+
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append_e4m3_preflight_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, const augur_cuda_nvfp4_sm100_kv_append_e4m3_args_v1* args);
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append_e4m3_prevalidated_submit_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, const augur_cuda_nvfp4_sm100_kv_append_e4m3_args_v1* args);
+
+/* paged_attention over such a cache: the same formula on the values that codes and scales stand for, the same limits, scratch
+ * (paged_attention_scratch_extent_host_v1) and status words. */
+typedef struct augur_cuda_nvfp4_sm100_paged_attention_e4m3_args_v1 {
+    uint32_t abi_version;
+    uint32_t struct_size;
+    augur_cuda_nvfp4_sm100_kv_e4m3_layer_v1 layer;
+    augur_cuda_nvfp4_sm100_kv_batch_v1 batch;
+    augur_cuda_device_ptr_t query;          /* [rows][query_heads][head_dim] BF16 */
+    uint64_t query_len_bytes;
+    augur_cuda_device_ptr_t output;         /* [rows][query_heads][head_dim] BF16 */
+    uint64_t output_len_bytes;
+    uint32_t query_heads;
+    uint32_t max_new_tokens;
+    float scale;
+    uint32_t reserved;
+} augur_cuda_nvfp4_sm100_paged_attention_e4m3_args_v1;
+
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_paged_attention_e4m3_preflight_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, augur_cuda_nvfp4_sm100_plan_v1* plan,
+    const augur_cuda_nvfp4_sm100_paged_attention_e4m3_args_v1* args);
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_paged_attention_e4m3_prevalidated_submit_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, augur_cuda_nvfp4_sm100_plan_v1* plan,
+    const augur_cuda_nvfp4_sm100_paged_attention_e4m3_args_v1* args);
+
+/* kv_page_copy for such a cache, scales included. */
+typedef struct augur_cuda_nvfp4_sm100_kv_page_copy_e4m3_args_v1 {
+    uint32_t abi_version;
+    uint32_t struct_size;
+    augur_cuda_device_ptr_t keys;           /* [layers][pages][page_bytes] */
+    augur_cuda_device_ptr_t values;
+    augur_cuda_device_ptr_t scales;         /* [layers][pages][scale_page_bytes] */
+    uint64_t len_bytes;                     /* of keys and of values */
+    uint64_t scales_len_bytes;
+    uint64_t page_bytes;                    /* multiples of 16 */
+    uint64_t scale_page_bytes;
+    uint32_t layers;
+    uint32_t pages;
+} augur_cuda_nvfp4_sm100_kv_page_copy_e4m3_args_v1;
+
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_copy_e4m3_preflight_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, const augur_cuda_nvfp4_sm100_kv_page_copy_e4m3_args_v1* args);
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_copy_e4m3_prevalidated_submit_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, const augur_cuda_nvfp4_sm100_kv_page_copy_e4m3_args_v1* args,
+    const uint32_t* sources, const uint32_t* destinations, uint32_t count);
+
+/* ---- attention of a batch whose sequences share a prefix ------------------------------------------ */
+/* paged_attention (BF16 cache) of sequences that all begin with the same P tokens, whose keys and values are read once for the batch.
+ * P = prefix_tokens[0] (device memory, as the batch's), in whole pages: what is over is read from each sequence's own pages.
+ * The pages of the first P tokens are those of prefix_pages, whatever a sequence's page-table row says there; lengths[b] counts them too, and a
+ * row of a sequence that is shorter than P sees its own length of them. P <= 0 is a batch without a prefix. P beyond prefix_pages counts as
+ * those and sets the status word to 0x401, as does a page outside the cache, which counts as not there. All else is as for
+ * paged_attention: limits on heads, tokens and table, rows that are not written, rows that see nothing, status words (the waits
+ * of the prefix set 0x421..0x427). A value of the prefix that is not finite may reach every row of the batch, those too short to see it included.
+ * The weights of the prefix enter their product with the values as one BF16 term (good to 2^-8 of each, and the denominator sums the
+ * same terms): for a batch, these products are the bound. */
+typedef struct augur_cuda_nvfp4_sm100_shared_prefix_attention_args_v1 {
+    uint32_t abi_version;
+    uint32_t struct_size;
+    augur_cuda_nvfp4_sm100_kv_layer_v1 layer;
+    augur_cuda_nvfp4_sm100_kv_batch_v1 batch;
+    augur_cuda_device_ptr_t prefix_pages;   /* int32, prefix_pages_len_bytes / 4 of them, at least one */
+    uint64_t prefix_pages_len_bytes;
+    augur_cuda_device_ptr_t prefix_tokens;  /* [1] int32 */
+    uint64_t prefix_tokens_len_bytes;       /* 4 */
+    augur_cuda_device_ptr_t query;          /* [rows][query_heads][head_dim] BF16 */
+    uint64_t query_len_bytes;
+    augur_cuda_device_ptr_t output;         /* [rows][query_heads][head_dim] BF16 */
+    uint64_t output_len_bytes;
+    uint32_t query_heads;
+    uint32_t max_new_tokens;
+    float scale;
+    uint32_t reserved;
+} augur_cuda_nvfp4_sm100_shared_prefix_attention_args_v1;
+
+/* Bytes of plan scratch: the parts of every row from the prefix and from its own tokens. */
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_shared_prefix_attention_scratch_extent_host_v1(
+    uint32_t query_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t rows, uint32_t max_new_tokens, uint32_t sm_count, uint64_t* out_bytes);
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_shared_prefix_attention_preflight_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, augur_cuda_nvfp4_sm100_plan_v1* plan,
+    const augur_cuda_nvfp4_sm100_shared_prefix_attention_args_v1* args);
+augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_shared_prefix_attention_prevalidated_submit_v1(
+    int32_t ordinal, augur_cuda_stream_t stream, augur_cuda_nvfp4_sm100_plan_v1* plan,
+    const augur_cuda_nvfp4_sm100_shared_prefix_attention_args_v1* args);
+
 /* ---- log probabilities behind the vocabulary head -------------------------------------------------- */
 /* For every row x of logits, with m = max x, L = sum e^(x - m):
  *   logprobs[row] = x[targets[row]] - m - ln L       (NaN where targets[row] is outside the vocabulary)
