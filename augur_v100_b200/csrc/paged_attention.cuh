@@ -3,6 +3,8 @@
 
 #include <cfloat>
 
+#include <cuda_fp16.h>
+
 #include "kv_cache.cuh"
 #include "kv_join_record.h"
 #include "nvfp4_gemm.cuh"
