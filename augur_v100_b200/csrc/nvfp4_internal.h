@@ -156,6 +156,7 @@ cudaError_t gemm_narrow_configure_device();
 cudaError_t gemv_split_configure_device();
 cudaError_t attention_configure_device();
 cudaError_t attention_e4m3_configure_device();
+cudaError_t shared_prefix_configure_device();
 cudaError_t logprobs_configure_device();
 // Clusters of `parts` CTAs of 384 threads and 112 KB of shared memory (two per SM) that a launch may count on to run at once.
 uint32_t two_cta_clusters(int32_t ordinal, uint32_t parts);

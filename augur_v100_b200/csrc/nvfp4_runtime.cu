@@ -199,6 +199,7 @@ extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_plan_crea
     if (e == cudaSuccess) e = gemm_narrow_configure_device();
     if (e == cudaSuccess) e = attention_configure_device();
     if (e == cudaSuccess) e = attention_e4m3_configure_device();
+    if (e == cudaSuccess) e = shared_prefix_configure_device();
     if (e == cudaSuccess) e = logprobs_configure_device();
     if (e != cudaSuccess) return make_result(AUGUR_CUDA_STATUS_RUNTIME_FAILURE, e);
     const uint64_t rounded = (scratch_len_bytes + 255) / 256 * 256;

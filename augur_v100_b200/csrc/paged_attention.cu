@@ -72,28 +72,6 @@ static_assert(kLayout<128, 8> == 462 && kLayout<128, 16> == 462 && kLayout<128, 
                   kLayout<256, 16> == 462 && kLayout<256, 32> == 442 && kLayout<256, 48> == 441 && kLayout<256, 64> == 241,
               "the slots that the figures above belong to");
 
-// Operand descriptors, low and high word: address and leading offset, stride offset, version and swizzle.
-// K and the narrow operands (K-major, 128-byte swizzle: 8 rows are 1024 bytes). V (MN-major): 128-byte rows of 64 dims, one per key, so the rows
-// are the k dimension; 8 keys are 1024 bytes, the next 64 dims lie one ring slot further. The ones (K-major, no swizzle): 8 rows x 16 bytes are
-// 128 bytes, the next 8 k 128 bytes further, the next 8 rows 256.
-// Up to four MMAs of 16 k of a converged warp, the 128-row operand kStep (of 16 bytes) further and the narrow one 32 bytes further each time, as
-// predicated instructions whose operands are uniform (behind a branch, one by one, an MMA took 65 cycles to issue; the pipe needs 32).
-template <uint32_t kHigh, uint32_t kStep>
-__device__ __forceinline__ void mma_block(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate, uint32_t steps) {
-    asm volatile(
-        "{\n.reg .pred e, p, q, e1, e2, e3;\n.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n.reg .b32 l1, l2, l3, m1, m2, m3;\n"
-        "elect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\nsetp.eq.u32 q, 0, 0;\n"
-        "setp.gt.and.u32 e1, %5, 1, e;\nsetp.gt.and.u32 e2, %5, 2, e;\nsetp.gt.and.u32 e3, %5, 3, e;\n"
-        "add.s32 l1, %1, %8;\nadd.s32 l2, l1, %8;\nadd.s32 l3, l2, %8;\nadd.s32 m1, %2, 2;\nadd.s32 m2, %2, 4;\nadd.s32 m3, %2, 6;\n"
-        "mov.b64 a0, {%1, %6};\nmov.b64 a1, {l1, %6};\nmov.b64 a2, {l2, %6};\nmov.b64 a3, {l3, %6};\n"
-        "mov.b64 b0, {%2, %7};\nmov.b64 b1, {m1, %7};\nmov.b64 b2, {m2, %7};\nmov.b64 b3, {m3, %7};\n"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a0, b0, %3, p;\n"
-        "@e1 tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, q;\n"
-        "@e2 tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, q;\n"
-        "@e3 tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, q;\n}"
-        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(steps), "r"(kHigh), "r"(kHighSwizzled), "n"(kStep)
-        : "memory");
-}
 template <uint32_t kHeadDim, uint32_t kN, bool kPrefix>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __grid_constant__ CUtensorMap map_values, const __grid_constant__ AttentionParams p) {
@@ -581,6 +559,10 @@ cudaError_t attention_configure_device() {
     if (e == cudaSuccess) e = configure<256, false>();
     if (e == cudaSuccess) e = configure<128, true>();
     return e == cudaSuccess ? configure<256, true>() : e;
+}
+
+void launch_own_attention(cudaStream_t stream, uint32_t head_dim, uint32_t columns, const CUtensorMap& keys, const CUtensorMap& values, const AttentionParams& p) {
+    (head_dim == 256 ? launch_of<256, true>(columns) : launch_of<128, true>(columns))(stream, keys, values, p);
 }
 
 }  // namespace augur_sm100

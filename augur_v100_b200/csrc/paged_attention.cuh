@@ -27,6 +27,8 @@ constexpr uint32_t kStatusLoad = 0x411, kStatusMma = 0x412, kStatusScores = 0x41
 constexpr uint32_t kThreads = 256;        // warp 0 loads keys, 1 MMA, 2 queries, 3 values, 4..7 softmax
 constexpr uint32_t kSmemLimit = 227 * 1024;
 
+}  // namespace
+
 struct AttentionParams {
     const __nv_bfloat16* query;
     __nv_bfloat16* output;
@@ -44,6 +46,11 @@ struct AttentionParams {
     float* own_sums;
     float2* own_stats;
 };
+
+// The paged attention's launches behind a shared prefix (paged_attention.cu): sums for `own_sums` and `own_stats`.
+void launch_own_attention(cudaStream_t stream, uint32_t head_dim, uint32_t columns, const CUtensorMap& keys, const CUtensorMap& values, const AttentionParams& p);
+
+namespace {
 
 // The shared tokens that are read from the prefix's pages: whole pages, as many as there are.
 __device__ __forceinline__ uint32_t shared_tokens(const int32_t* prefix_tokens, uint32_t prefix_pages, uint32_t page_shift) {
@@ -182,8 +189,30 @@ struct Tiles {
     __device__ uint32_t keys() const { return walk.key_end - key < kTile ? walk.key_end - key : kTile; }
 };
 
+// Operand descriptors, low and high word: address and leading offset, stride offset, version and swizzle.
+// K and the narrow operands (K-major, 128-byte swizzle: 8 rows are 1024 bytes). V (MN-major): 128-byte rows of 64 dims, one per key, so the rows
+// are the k dimension; 8 keys are 1024 bytes, the next 64 dims lie one ring slot further. The ones (K-major, no swizzle): 8 rows x 16 bytes are
+// 128 bytes, the next 8 k 128 bytes further, the next 8 rows 256.
 constexpr uint32_t kHighSwizzled = (1024 >> 4) | (1u << 14) | (2u << 29), kHighPlain = (256 >> 4) | (1u << 14);
 __device__ __forceinline__ uint32_t low_word(uint32_t smem_addr, uint32_t leading) { return ((smem_addr & 0x3ffffu) >> 4) | ((leading >> 4) << 16); }
+// Up to four MMAs of 16 k of a converged warp, the 128-row operand kStep (of 16 bytes) further and the narrow one 32 bytes further each time, as
+// predicated instructions whose operands are uniform (behind a branch, one by one, an MMA took 65 cycles to issue; the pipe needs 32).
+template <uint32_t kHigh, uint32_t kStep>
+__device__ __forceinline__ void mma_block(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate, uint32_t steps) {
+    asm volatile(
+        "{\n.reg .pred e, p, q, e1, e2, e3;\n.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n.reg .b32 l1, l2, l3, m1, m2, m3;\n"
+        "elect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\nsetp.eq.u32 q, 0, 0;\n"
+        "setp.gt.and.u32 e1, %5, 1, e;\nsetp.gt.and.u32 e2, %5, 2, e;\nsetp.gt.and.u32 e3, %5, 3, e;\n"
+        "add.s32 l1, %1, %8;\nadd.s32 l2, l1, %8;\nadd.s32 l3, l2, %8;\nadd.s32 m1, %2, 2;\nadd.s32 m2, %2, 4;\nadd.s32 m3, %2, 6;\n"
+        "mov.b64 a0, {%1, %6};\nmov.b64 a1, {l1, %6};\nmov.b64 a2, {l2, %6};\nmov.b64 a3, {l3, %6};\n"
+        "mov.b64 b0, {%2, %7};\nmov.b64 b1, {m1, %7};\nmov.b64 b2, {m2, %7};\nmov.b64 b3, {m3, %7};\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a0, b0, %3, p;\n"
+        "@e1 tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, q;\n"
+        "@e2 tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, q;\n"
+        "@e3 tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, q;\n}"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(steps), "r"(kHigh), "r"(kHighSwizzled), "n"(kStep)
+        : "memory");
+}
 // The elected lane's commit (elect.sync always names the same lane of a whole warp: the one that issued the MMAs).
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar) : "memory");

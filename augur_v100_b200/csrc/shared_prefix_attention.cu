@@ -1,10 +1,504 @@
-// Attention of a step's new tokens over a paged cache whose sequences share a prefix, on sm_100a.
-#include "attention_simple.cuh"
+// Attention of a step's new tokens over a paged BF16 cache whose sequences share a prefix, on sm_100a.
+//
+//   o = (sum over the prefix + sum over a row's own tokens) of 2^(s_j - m) v_j, over the same sum of 2^(s_j - m),  s_j = scale log2(e) q . k_j
+//
+// The prefix's keys and values are the same for every row, so its part is two dense products of all rows' queries: 4 head_dim operations
+// per query and token against 4 head_dim bytes per token, that is: bound by HBM up to some 250 queries of a key-value head, by the matrix units and what
+// feeds them above. The rows' own tokens are left to the paged attention's kernel, which leaves its sums instead of outputs; a last launch joins both.
+//
+// A CTA takes 128 queries of a key-value head (token rows x the heads that share it, packed) through a run of 128-token tiles of the prefix:
+//
+//   S[query][key]  = Q K^T           both from shared memory, two S in tensor memory in turn
+//   O[query][dim] += P V             P from tensor memory, where it takes the place of the S that it came from; V as it lies in the pages (MN-major)
+//
+// A softmax thread holds one query, so nothing of the softmax passes between threads. Its reference maximum moves when a score passes it by more than 2^8 (then
+// O is scaled in tensor memory). P is one BF16 term (2^-8 of each weight at most; the denominator sums the same terms): a second one would
+// cost half as much again of the product that bounds the kernel. With head_dim 128 two groups of softmax warps take the tiles in turn,
+// each with an O of its own: one group's exponentials take as long as a tile's products there.
+#include "paged_attention.cuh"
 
 namespace augur_sm100 {
+
 namespace {
 
 static_assert(sizeof(augur_cuda_nvfp4_sm100_shared_prefix_attention_args_v1) == 192, "attention ABI");
+
+constexpr uint32_t kRowsM = 128;               // queries of a CTA
+constexpr uint32_t kRounds = 3;                // a device's worth of CTAs, at most so many times, where the prefix is split for it
+constexpr uint32_t kInfoRing = 8;
+constexpr uint32_t kStatusPrefixLoad = 0x421, kStatusPrefixMma = 0x422, kStatusPrefixScores = 0x423, kStatusPrefixQuery = 0x424, kStatusPrefixProduct = 0x425, kStatusPrefixInfo = 0x426;
+
+struct PrefixParams {
+    AttentionParams a;
+    const int32_t* prefix_table;
+    float* parts;              // [items][streams][head_dim / 4][kRowsM][4], then [items][streams][kRowsM] (reference maximum, denominator)
+    uint64_t max_items;        // that there is room for
+    uint32_t tiles;            // of kRowsM queries
+};
+
+template <uint32_t kHeadDim>
+struct PrefixShape {
+    static constexpr uint32_t kChunks = kHeadDim / 64, kStreams = kHeadDim == 128 ? 2 : 1;
+    static constexpr uint32_t kThreads = 128 + 128 * kStreams;   // warp 0 loads, 1 MMA, 2 and 3 queries, then the softmax
+    static constexpr uint32_t kQueryBytes = kRowsM * kHeadDim * 2, kSlots = (224 * 1024 - kQueryBytes) / kSlotBytes;
+    static constexpr uint32_t kSmem = 1024 + kQueryBytes + kSlots * kSlotBytes + 1024;
+    static constexpr uint32_t kScoresAt = 0, kOutAt = 256;       // tensor memory: two of S, one O per stream
+    static_assert(kSmem <= kSmemLimit && kOutAt + kStreams * kHeadDim == 512, "a CTA's memory");
+};
+
+struct PrefixState {
+    uint64_t full[16], empty[16], scores_full[2], weights_full[2], products[2], query_full, query_empty, info_full[kInfoRing];
+    uint32_t tmem, abort[1 + 12], info[kInfoRing];
+};
+static_assert(sizeof(PrefixState) <= 1024, "the state's room");
+
+// An item is 128 queries of a key-value head over a `split`-th of the prefix's tiles. Items are dealt out round by round, those of the same keys next to one
+// another, so that the keys come from L2 for all but the first.
+struct Items {
+    uint32_t key_tiles, split, tokens;
+    uint64_t count;
+    __device__ __forceinline__ void locate(const PrefixParams& p, uint64_t item, uint32_t* head, uint32_t* tile, uint32_t* first, uint32_t* last) const {
+        const uint64_t rest = item / p.tiles;
+        *tile = static_cast<uint32_t>(item - rest * p.tiles);
+        *head = static_cast<uint32_t>(rest / split);
+        const uint32_t part = static_cast<uint32_t>(rest - static_cast<uint64_t>(*head) * split);
+        *first = static_cast<uint32_t>(static_cast<uint64_t>(part) * key_tiles / split), *last = static_cast<uint32_t>(static_cast<uint64_t>(part + 1) * key_tiles / split);
+    }
+};
+// The split that a simple model takes for quickest: rounds of items, each its tiles and four for beginning and end, and a 32nd of a tile for every part to
+// be joined. A warp together.
+__device__ __forceinline__ Items items_of(const PrefixParams& p, uint32_t ctas) {
+    Items x;
+    x.tokens = shared_tokens(p.a.prefix_tokens, p.a.prefix_pages, p.a.page_shift);
+    x.key_tiles = (x.tokens + kTile - 1) / kTile;
+    const uint64_t pairs = static_cast<uint64_t>(p.a.kv_heads) * p.tiles, room = p.max_items / pairs;
+    uint32_t most = x.key_tiles < room ? x.key_tiles : static_cast<uint32_t>(room);
+    uint64_t best = UINT64_MAX;
+    for (uint32_t split = 1 + threadIdx.x % 32; split <= most; split += 32) {
+        const uint64_t items = pairs * split, cost = (items + ctas - 1) / ctas * ((x.key_tiles + split - 1) / split + 4) * 32 + items, key = cost << 16 | (split < 65535 ? split : 65535);
+        if (key < best) best = key;
+    }
+#pragma unroll
+    for (uint32_t step = 16; step; step /= 2) {
+        const uint64_t other = __shfl_xor_sync(0xffffffffu, best, step);
+        if (other < best) best = other;
+    }
+    x.split = x.key_tiles ? static_cast<uint32_t>(best & 0xffff) : 1;
+    x.count = x.key_tiles ? pairs * x.split : 0;
+    return x;
+}
+
+// Up to four MMAs of 16 k, the 128-row operand from tensor memory (8 columns a step), the narrow one kStep (of 16 bytes) further each time.
+template <uint32_t kStep>
+__device__ __forceinline__ void mma_block_from_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred e, p, q;\n.reg .b64 b0, b1, b2, b3;\n.reg .b32 l1, l2, l3, m1, m2, m3;\n"
+        "elect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\nsetp.eq.u32 q, 0, 0;\n"
+        "add.s32 l1, %1, 8;\nadd.s32 l2, %1, 16;\nadd.s32 l3, %1, 24;\nadd.s32 m1, %2, %6;\nadd.s32 m2, m1, %6;\nadd.s32 m3, m2, %6;\n"
+        "mov.b64 b0, {%2, %5};\nmov.b64 b1, {m1, %5};\nmov.b64 b2, {m2, %5};\nmov.b64 b3, {m3, %5};\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b0, %3, p;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [l1], b1, %3, q;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [l2], b2, %3, q;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [l3], b3, %3, q;\n}"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kHighSwizzled), "n"(kStep)
+        : "memory");
+}
+
+template <uint32_t kHeadDim>
+__global__ void __launch_bounds__(PrefixShape<kHeadDim>::kThreads, 1)
+prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __grid_constant__ CUtensorMap map_values, const __grid_constant__ PrefixParams p) {
+    using S = PrefixShape<kHeadDim>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* const query_smem = smem + S::kSlots * kSlotBytes;
+    PrefixState* const st = reinterpret_cast<PrefixState*>(query_smem + S::kQueryBytes);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t full = smem_u32(st->full), empty = smem_u32(st->empty), scores_full = smem_u32(st->scores_full), weights_full = smem_u32(st->weights_full);
+    const uint32_t products = smem_u32(st->products), query_full = smem_u32(&st->query_full), query_empty = smem_u32(&st->query_empty), info_full = smem_u32(st->info_full);
+    volatile uint32_t* abort_flag = st->abort;
+    uint32_t* const status = p.a.status_word;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < S::kSlots; ++s) mbar_init(full + 8 * s, 1), mbar_init(empty + 8 * s, 1);
+        for (uint32_t b = 0; b < 2; ++b) mbar_init(scores_full + 8 * b, 1), mbar_init(weights_full + 8 * b, 4), mbar_init(products + 8 * b, 1);
+        for (uint32_t i = 0; i < kInfoRing; ++i) mbar_init(info_full + 8 * i, 1);
+        mbar_init(query_full, 2), mbar_init(query_empty, 1);
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_keys) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_values) : "memory");
+        for (uint32_t i = 0; i < 1 + 12; ++i) st->abort[i] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&st->tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    // Everything above runs while the launch before this one drains; from here on its results are read.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Items items = items_of(p, gridDim.x);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && *p.a.prefix_tokens > static_cast<int32_t>(p.a.prefix_pages << p.a.page_shift)) atomicCAS(status, 0u, kStatusPage);
+    // Does any row end within the prefix?
+    bool ends_within = false;
+    const int32_t room = static_cast<int32_t>(p.a.table_pages << p.a.page_shift);   // a length beyond the table counts as the table's
+    for (uint32_t b = threadIdx.x; b < p.a.sequences; b += S::kThreads) {
+        const int32_t from = p.a.token_starts[b], to = p.a.token_starts[b + 1];
+        ends_within |= to > from && static_cast<int64_t>(min(p.a.lengths[b], room)) - to + from + 1 < static_cast<int64_t>(items.tokens);
+    }
+    ends_within = __syncthreads_or(ends_within);
+    const uint32_t tmem = st->tmem, group = p.a.query_heads / p.a.kv_heads;
+    const uint32_t all_queries = p.a.rows * group;   // of a key-value head; below 2^26
+
+    if (warp == 0) {
+        // ---------------- pages: a tile's keys, then the values of the tile before it, as they are used ----------------
+        const uint32_t box_shift = p.a.page_shift < 6 ? p.a.page_shift : 6, boxes = kTile >> box_shift, box_bytes = 128u << box_shift;
+        const uint32_t beyond = (p.a.pages * p.a.kv_heads) << p.a.page_shift;   // a row behind the cache: TMA reads zeros there
+        uint32_t slot = 0, phase = 1, count = 0;
+        bool alive = true;
+        auto load = [&](const CUtensorMap* map, uint32_t row) {
+            for (uint32_t c = 0; c < S::kChunks; ++c) {
+                if (!warp_look_wait(empty + 8 * slot, phase, abort_flag, status, kStatusPrefixLoad)) return false;
+                if (lane == 0) mbar_expect_tx(full + 8 * slot, kSlotBytes);
+                __syncwarp();
+                if (lane < boxes) tma_load_2d(smem_u32(smem) + slot * kSlotBytes + lane * box_bytes, map, c * 128, row, full + 8 * slot);
+                __syncwarp();
+                if (++slot == S::kSlots) slot = 0, phase ^= 1;
+            }
+            return true;
+        };
+        for (uint64_t item = blockIdx.x; alive && item < items.count; item += gridDim.x) {
+            uint32_t head, tile, first, last, before = 0;
+            items.locate(p, item, &head, &tile, &first, &last);
+            auto page_of = [&](uint32_t t) {
+                const uint32_t key = t * kTile + (lane << box_shift);
+                return t < last && lane < boxes && key < items.tokens ? __ldg(p.prefix_table + (key >> p.a.page_shift)) : INT32_MIN;
+            };
+            int32_t page = page_of(first);
+            for (uint32_t t = first; alive && t < last; ++t, ++count) {
+                const uint32_t key = t * kTile + (lane << box_shift);
+                const bool there = page >= 0 && static_cast<uint32_t>(page) < p.a.pages;
+                if (!there && page != INT32_MIN) atomicCAS(status, 0u, kStatusPage);
+                const uint32_t row = there ? ((static_cast<uint32_t>(page) * p.a.kv_heads + head) << p.a.page_shift) + (key & ((1u << p.a.page_shift) - 1)) : beyond;
+                const uint32_t mask = __ballot_sync(0xffffffffu, there);
+                page = page_of(t + 1);
+                // (the ring is that long: a tile's keys are loaded behind the products of two tiles before, which wait for the softmax of those)
+                if (lane == 0) {
+                    st->info[count % kInfoRing] = mask;
+                    mbar_arrive(info_full + 8 * (count % kInfoRing));
+                }
+                __syncwarp();
+                alive = load(&map_keys, row) && (t == first || load(&map_values, before));
+                before = row;
+            }
+            alive = alive && load(&map_values, before);
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer: S of a tile, then O of the tile before it ----------------
+        constexpr uint32_t idesc_any = (1u << 4) | (1u << 7) | (1u << 10) | ((kRowsM >> 4) << 24);   // F32 += BF16 x BF16
+        constexpr uint32_t idesc = idesc_any | ((kTile >> 3) << 17), idesc_values = idesc_any | ((64 >> 3) << 17) | (1u << 16);   // V is MN-major
+        const uint32_t slots = low_word(smem_u32(smem), 16), queries = low_word(smem_u32(query_smem), 16);
+        uint32_t slot = 0, phase = 0, scores = 0, done = 0, round = 0;
+        bool alive = true;
+        auto next_slot = [&]() {
+            if (++slot == S::kSlots) slot = 0, phase ^= 1;
+        };
+        auto scores_of_tile = [&]() {
+            for (uint32_t c = 0; c < S::kChunks; ++c) {
+                if (!warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusPrefixMma)) return false;
+                tc_fence_after();
+                mma_block<kHighSwizzled, 2>(tmem + S::kScoresAt + (scores & 1) * kTile, queries + c * (kSlotBytes >> 4), slots + slot * (kSlotBytes >> 4), idesc, c, 4);
+                commit(empty + 8 * slot);
+                next_slot();
+            }
+            commit(scores_full + 8 * (scores & 1));
+            ++scores;
+            return true;
+        };
+        for (uint64_t item = blockIdx.x; alive && item < items.count; item += gridDim.x, ++round) {
+            uint32_t head, tile, first, last;
+            items.locate(p, item, &head, &tile, &first, &last);
+            if (!warp_look_wait(query_full, round & 1, abort_flag, status, kStatusPrefixMma)) break;
+            // (S of a tile goes where the weights of two tiles before were read by MMAs that were issued earlier; a new item's where the last one's were)
+            alive = scores_of_tile();
+            for (uint32_t t = first; alive && t < last; ++t) {
+                if (t + 1 < last) {
+                    if (!(alive = scores_of_tile())) break;
+                }
+                if (t + 1 >= last) commit(query_empty);
+                const uint32_t buffer = done & 1, d = tmem + S::kOutAt + (S::kStreams == 2 ? buffer * kHeadDim : 0);
+                const uint32_t follows = t >= first + S::kStreams;
+                if (!(alive = warp_look_wait(weights_full + 8 * buffer, done >> 1 & 1, abort_flag, status, kStatusPrefixProduct))) break;
+                for (uint32_t c = 0; c < S::kChunks; ++c) {
+                    if (!(alive = warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusPrefixProduct))) break;
+                    tc_fence_after();
+                    const uint32_t a = tmem + S::kScoresAt + buffer * kTile, b = slots + slot * (kSlotBytes >> 4);   // 16 keys: 8 columns of P, 16 rows of V
+                    mma_block_from_tmem<(16 * 128 >> 4)>(d + c * 64, a, b, idesc_values, follows);
+                    mma_block_from_tmem<(16 * 128 >> 4)>(d + c * 64, a + 32, b + 4 * (16 * 128 >> 4), idesc_values, 1);
+                    commit(empty + 8 * slot);
+                    next_slot();
+                }
+                if (!alive) break;
+                commit(products + 8 * buffer);
+                ++done;
+            }
+        }
+    } else if (warp < 4) {
+        // ---------------- queries of an item, in the 128-byte swizzle of the operand; past the last they are zero ----------------
+        constexpr uint32_t kPieces = kHeadDim / 8;   // of 16 bytes
+        uint32_t round = 0;
+        for (uint64_t item = blockIdx.x; item < items.count; item += gridDim.x, ++round) {
+            uint32_t head, tile, first, last;
+            items.locate(p, item, &head, &tile, &first, &last);
+            if (!warp_look_wait(query_empty, (round & 1) ^ 1, abort_flag, status, kStatusPrefixQuery)) break;
+            for (uint32_t i = (warp - 2) * 32 + lane; i < kRowsM * kPieces; i += 64) {
+                const uint32_t row = i / kPieces, piece = i % kPieces, query = tile * kRowsM + row, token = query / group;
+                const bool live = query < all_queries;
+                const __nv_bfloat16* const at = p.a.query + (static_cast<uint64_t>(live ? token : 0) * p.a.query_heads + head * group + (live ? query - token * group : 0)) * kHeadDim + piece * 8;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                             ::"r"(smem_u32(query_smem) + (piece >> 3) * kSlotBytes + row * 128 + (((piece & 7) ^ (row & 7)) << 4)), "l"(at), "r"(live ? 16 : 0)
+                             : "memory");
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(query_full);
+        }
+    } else {
+        // ---------------- softmax: a query a thread ----------------
+        const uint32_t stream = (warp - 4) / 4, thread = threadIdx.x & 127, lanes = ((warp & 3) * 32) << 16;
+        const uint32_t box_shift = p.a.page_shift < 6 ? p.a.page_shift : 6, all_boxes = (1u << (kTile >> box_shift)) - 1;
+        const uint32_t out = tmem + S::kOutAt + stream * (S::kStreams == 2 ? kHeadDim : 0) + lanes;
+        const float scale = p.a.scale_log2;
+        uint32_t count = 0;   // tiles of this CTA
+        bool alive = true;
+        for (uint64_t item = blockIdx.x; alive && item < items.count; item += gridDim.x) {
+            uint32_t head, tile, first, last;
+            items.locate(p, item, &head, &tile, &first, &last);
+            // How many tokens of the prefix this row sees.
+            uint32_t limit = items.tokens;
+            if (ends_within) {
+                const int32_t row = static_cast<int32_t>((tile * kRowsM + thread) / group);
+                uint32_t low = 0, high = p.a.sequences;   // the last sequence that starts at or before the row
+                while (high - low > 1) {
+                    const uint32_t middle = (low + high) / 2;
+                    if (p.a.token_starts[middle] <= row) low = middle;
+                    else high = middle;
+                }
+                const int64_t seen = static_cast<int64_t>(min(p.a.lengths[low], room)) - p.a.token_starts[low + 1] + row + 1;
+                limit = seen <= 0 ? 0 : seen < static_cast<int64_t>(limit) ? static_cast<uint32_t>(seen) : limit;
+            }
+            const uint32_t seen_by_all = __reduce_min_sync(0xffffffffu, limit);
+            float reference = -INFINITY, sum0 = 0.0f, sum1 = 0.0f;
+            bool started = false;
+            uint32_t first_key = 0;
+            for (uint32_t t = first; t < last; ++t, ++count) {
+                const uint32_t buffer = count & 1;
+                if (S::kStreams == 2 && buffer != stream) continue;
+                if (!warp_look_wait(info_full + 8 * (count % kInfoRing), count / kInfoRing & 1, abort_flag, status, kStatusPrefixInfo) ||
+                    !warp_look_wait(scores_full + 8 * buffer, count >> 1 & 1, abort_flag, status, kStatusPrefixScores)) {
+                    alive = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t there = st->info[count % kInfoRing], key = t * kTile, from = tmem + S::kScoresAt + buffer * kTile + lanes;
+                const bool masked = there != all_boxes || key + kTile > seen_by_all;
+                // Which of 32 keys from c on this row sees.
+                auto seen = [&](uint32_t c) {
+                    uint32_t bits = limit <= key + c ? 0 : limit - key - c >= 32 ? 0xffffffffu : (1u << (limit - key - c)) - 1;
+                    if (box_shift >= 5) bits = there >> (c >> box_shift) & 1 ? bits : 0;
+                    else bits &= (there >> (c >> 4) & 1 ? 0xffffu : 0) | (there >> ((c >> 4) + 1) & 1 ? 0xffff0000u : 0);
+                    return bits;
+                };
+                // The largest score: of scale * S, the product with the largest S or, with a scale below zero, the smallest.
+                float most = scale < 0.0f ? INFINITY : -INFINITY;
+#pragma unroll 1
+                for (uint32_t c = 0; c < kTile; c += 32) {
+                    uint32_t v[32];
+                    tc_load32(from + c, v);
+                    tc_wait_ld();
+                    const uint32_t bits = masked ? seen(c) : 0xffffffffu;
+                    if (masked) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; ++i) v[i] = bits >> i & 1 ? v[i] : __float_as_uint(scale < 0.0f ? INFINITY : -INFINITY);
+                    }
+                    if (scale < 0.0f) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; ++i) most = fminf(most, __uint_as_float(v[i]));
+                    } else {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; ++i) most = fmaxf(most, __uint_as_float(v[i]));
+                    }
+                }
+                const float top = fmaxf(reference, most * scale);
+                const bool above = top > reference + kSlack || (!started && top > reference);
+                if (__any_sync(0xffffffffu, above)) {
+                    const float now = above ? top : reference, factor = now == reference ? 1.0f : exp2_fast(reference - now);
+                    reference = now;
+                    sum0 *= factor, sum1 *= factor;
+                    if (started) {
+                        // the stream's tile before has to be through
+                        const uint32_t earlier = count - S::kStreams;
+                        if (!warp_look_wait(products + 8 * (earlier & 1), earlier >> 1 & 1, abort_flag, status, kStatusPrefixProduct)) {
+                            alive = false;
+                            break;
+                        }
+                        tc_fence_after();
+#pragma unroll 1
+                        for (uint32_t c = 0; c < kHeadDim; c += 16) {
+                            uint32_t v[16];
+                            load_columns<16>(out + c, v);
+                            tc_wait_ld();
+#pragma unroll
+                            for (uint32_t i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * factor);
+                            store_columns16(out + c, v);
+                        }
+                    }
+                }
+                if (!started) first_key = key;
+                started = true;
+                const float minus = reference == -INFINITY ? 0.0f : -reference;
+#pragma unroll 1
+                for (uint32_t c = 0; c < kTile; c += 32) {
+                    uint32_t v[32], packed[16];
+                    tc_load32(from + c, v);
+                    tc_wait_ld();
+                    const uint32_t bits = masked ? seen(c) : 0xffffffffu;
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; ++i) v[i] = __float_as_uint(exp2_fast(fmaf(__uint_as_float(v[i]), scale, minus)));
+                    if (masked) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; ++i) v[i] = bits >> i & 1 ? v[i] : 0;
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) {
+                        const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                        packed[i] = *reinterpret_cast<const uint32_t*>(&two);
+                        sum0 += __uint_as_float(packed[i] << 16), sum1 += __uint_as_float(packed[i] & 0xffff0000u);
+                    }
+                    store_columns16(from + c / 2, packed);
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(weights_full + 8 * buffer);
+            }
+            if (!alive) break;
+            // ---- the item's part ----
+            const uint64_t part = item * S::kStreams + stream;
+            if (started) {
+                const uint32_t final = count - 1 - (S::kStreams == 2 && ((count - 1) & 1) != stream ? 1 : 0);   // the stream's last tile
+                if (!warp_look_wait(products + 8 * (final & 1), final >> 1 & 1, abort_flag, status, kStatusPrefixProduct)) break;
+                tc_fence_after();
+                float4* const to = reinterpret_cast<float4*>(p.parts) + part * (kHeadDim / 4) * kRowsM + thread;
+#pragma unroll 1
+                for (uint32_t c = 0; c < kHeadDim; c += 32) {
+                    uint32_t v[32];
+                    tc_load32(out + c, v);
+                    tc_wait_ld();
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i += 4) {
+                        to[(c + i) / 4 * kRowsM] = make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+                    }
+                }
+                tc_fence_before();
+            }
+            // (a part all of whose scores are NaN or -infinity has the reference -infinity too, but counts: its sums may be NaN)
+            if (started && reference == -INFINITY && limit > first_key) reference = kNoNumber;
+            reinterpret_cast<float2*>(p.parts + p.max_items * S::kStreams * kRowsM * kHeadDim)[part * kRowsM + thread] = make_float2(reference, sum0 + sum1);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// Joins the parts of the prefix, in their order, and the sums over the row's own tokens. A CTA takes eight queries of an item's 128.
+constexpr uint32_t kMergeThreads = 256, kMergeQueries = 8;
+template <uint32_t kHeadDim>
+__global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const __grid_constant__ PrefixParams p, uint32_t ctas) {
+    using S = PrefixShape<kHeadDim>;
+    constexpr uint32_t kEach = kHeadDim / 4 / 32;   // float4 of a thread
+    __shared__ uint32_t live[kMergeQueries];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Items items = items_of(p, ctas);
+    const uint32_t group = p.a.query_heads / p.a.kv_heads, all_queries = p.a.rows * group;
+    constexpr uint32_t kSlices = kRowsM / kMergeQueries;
+    const uint32_t slice = blockIdx.x % kSlices, tile = blockIdx.x / kSlices % p.tiles, head = blockIdx.x / kSlices / p.tiles;
+    const uint32_t query0 = tile * kRowsM + slice * kMergeQueries;
+    if (query0 >= all_queries) return;
+    // The rows that belong to a sequence.
+    if (threadIdx.x < kMergeQueries) live[threadIdx.x] = 0;
+    __syncthreads();
+    for (uint32_t b = threadIdx.x; b < p.a.sequences; b += kMergeThreads) {
+        const int32_t from = p.a.token_starts[b], to = p.a.token_starts[b + 1];
+        if (from < 0 || to > static_cast<int32_t>(p.a.rows) || to < from || to - from > static_cast<int32_t>(p.a.max_new)) continue;
+        for (uint32_t i = 0; i < kMergeQueries; ++i) {
+            const int32_t row = static_cast<int32_t>((query0 + i) / group);
+            if (from <= row && row < to) live[i] = 1;
+        }
+    }
+    __syncthreads();
+    // lanes: eight queries, four neighbouring float4 of each
+    const uint32_t i = threadIdx.x % kMergeQueries, query = query0 + i, column = threadIdx.x / kMergeQueries;
+    if (!live[i] || query >= all_queries) return;
+    const uint32_t token = query / group;
+    const uint64_t place = static_cast<uint64_t>(token) * p.a.query_heads + head * group + (query - token * group);
+    const uint32_t row = slice * kMergeQueries + i, parts = items.key_tiles ? items.split * S::kStreams : 0;
+    auto part_of = [&](uint32_t n) { return ((static_cast<uint64_t>(head) * items.split + n / S::kStreams) * p.tiles + tile) * S::kStreams + n % S::kStreams; };
+    const float2* const stats = reinterpret_cast<const float2*>(p.parts + p.max_items * S::kStreams * kRowsM * kHeadDim);
+    const float2 own = p.a.own_stats[place];
+    float most = own.x;
+    for (uint32_t n = 0; n < parts; ++n) most = fmaxf(most, stats[part_of(n) * kRowsM + row].x);
+    float4 sum[kEach];
+    float all = 0.0f;
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; ++e) sum[e] = make_float4(0, 0, 0, 0);
+    auto add = [&](float2 stat, const float4* from, uint32_t stride) {
+        // Parts of which the query sees nothing are passed over. All others count, with a weight of zero too: zero times a NaN is one.
+        if (stat.x == -INFINITY) return;
+        const float w = exp2_fast(stat.x - most);
+        all = fmaf(w, stat.y, all);
+#pragma unroll
+        for (uint32_t e = 0; e < kEach; ++e) {
+            const float4 x = from[e * 32 * stride];
+            sum[e].x = fmaf(w, x.x, sum[e].x), sum[e].y = fmaf(w, x.y, sum[e].y), sum[e].z = fmaf(w, x.z, sum[e].z), sum[e].w = fmaf(w, x.w, sum[e].w);
+        }
+    };
+    for (uint32_t n = 0; n < parts; ++n) {
+        const uint64_t part = part_of(n);
+        add(stats[part * kRowsM + row], reinterpret_cast<const float4*>(p.parts) + (part * (kHeadDim / 4) + column) * kRowsM + row, kRowsM);
+    }
+    add(own, reinterpret_cast<const float4*>(p.a.own_sums + place * kHeadDim) + column, 1);
+    const float inverse = 1.0f / all;
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; ++e) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum[e].x * inverse, all == 0.0f ? 0.0f : sum[e].y * inverse);
+        const __nv_bfloat162 b = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum[e].z * inverse, all == 0.0f ? 0.0f : sum[e].w * inverse);
+        reinterpret_cast<uint2*>(p.a.output + place * kHeadDim)[column + e * 32] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+}
+
+// What the plan's scratch holds, in bytes from its start.
+struct Layout {
+    uint64_t own_sums, own_stats, parts, max_items, bytes;
+};
+Layout layout_of(uint32_t query_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t rows, uint32_t max_new, uint32_t sm_count) {
+    const uint64_t spans = launch_spans(sm_count), columns = query_columns(query_heads, kv_heads, max_new), outputs = static_cast<uint64_t>(rows) * query_heads;
+    const uint64_t pairs = kv_heads * ((static_cast<uint64_t>(rows) * (query_heads / kv_heads) + kRowsM - 1) / kRowsM), streams = head_dim == 128 ? 2 : 1;
+    Layout l;
+    auto aligned = [](uint64_t x) { return (x + 255) / 256 * 256; };
+    l.own_sums = aligned(kCounterBytes + spans * sizeof(JoinRecord) + 2 * spans * columns * (head_dim + 2) * sizeof(float));   // (behind the paged attention's)
+    l.own_stats = aligned(l.own_sums + outputs * head_dim * sizeof(float));
+    l.parts = aligned(l.own_stats + outputs * sizeof(float2));
+    l.max_items = pairs > kRounds * static_cast<uint64_t>(sm_count) ? pairs : kRounds * static_cast<uint64_t>(sm_count);
+    l.bytes = l.parts + l.max_items * streams * kRowsM * (head_dim + 2) * sizeof(float);
+    return l;
+}
 
 bool check_shared(int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm100_plan_v1* plan, const augur_cuda_nvfp4_sm100_shared_prefix_attention_args_v1* a,
                   bool full, augur_cuda_result_v1* failure) {
@@ -12,10 +506,9 @@ bool check_shared(int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm100
     size_t count;
     if (!attention_args_ok(d, s, plan, a, ranges, &count, failure)) return false;
     const uint64_t pages = a->prefix_pages_len_bytes / 4;
-    if (!pages || a->prefix_pages_len_bytes % 4 != 0 || pages * a->layer.page_tokens > (1u << kMaxTokensLog2) || pages > (1u << kMaxTokensLog2) || a->prefix_tokens_len_bytes != 4) return false;
-    ranges[count] = ranges[count - 1];   // the scratch stays the last
-    ranges[count - 1] = {a->prefix_pages, a->prefix_pages_len_bytes, 4};
-    ranges[count + 1] = ranges[count], ranges[count] = {a->prefix_tokens, 4, 4};
+    if (!pages || a->prefix_pages_len_bytes % 4 != 0 || pages > (1u << kMaxTokensLog2) || pages * a->layer.page_tokens > (1u << kMaxTokensLog2) || a->prefix_tokens_len_bytes != 4) return false;
+    ranges[count + 1] = ranges[count - 1];   // the scratch stays the last
+    ranges[count - 1] = {a->prefix_pages, a->prefix_pages_len_bytes, 4}, ranges[count] = {a->prefix_tokens, 4, 4};
     count += 2;
     if (!all_disjoint(ranges, count)) return false;
     uint64_t need = 0;
@@ -24,7 +517,23 @@ bool check_shared(int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm100
     return !full || inspect_device_ranges(d, ranges, count - 1, failure);
 }
 
+template <uint32_t kHeadDim>
+void launch_prefix(cudaStream_t stream, const CUtensorMap& keys, const CUtensorMap& values, const PrefixParams& p, uint32_t sm_count, uint32_t columns) {
+    using S = PrefixShape<kHeadDim>;
+    launch_dependent(stream, prefix_attention_kernel<kHeadDim>, sm_count, S::kThreads, S::kSmem, keys, values, p);
+    launch_own_attention(stream, kHeadDim, columns, keys, values, p.a);
+    launch_dependent(stream, prefix_merge_kernel<kHeadDim>, p.a.kv_heads * p.tiles * (kRowsM / kMergeQueries), kMergeThreads, 0, p, sm_count);
+    count_launch(2);
+}
+
 }  // namespace
+
+cudaError_t shared_prefix_configure_device() {
+    constexpr cudaFuncAttribute kSmem = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    const cudaError_t e = cudaFuncSetAttribute(prefix_attention_kernel<128>, kSmem, PrefixShape<128>::kSmem);
+    return e == cudaSuccess ? cudaFuncSetAttribute(prefix_attention_kernel<256>, kSmem, PrefixShape<256>::kSmem) : e;
+}
+
 }  // namespace augur_sm100
 
 using namespace augur_sm100;
@@ -32,7 +541,8 @@ using namespace augur_sm100;
 extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_shared_prefix_attention_scratch_extent_host_v1(
     uint32_t query_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t rows, uint32_t max_new_tokens, uint32_t sm_count, uint64_t* out_bytes) {
     if (!out_bytes || !shape_ok(query_heads, kv_heads, head_dim, max_new_tokens) || !sm_count || sm_count > 4096 || !rows || rows > (1u << 20)) return invalid();
-    return augur_cuda_nvfp4_sm100_paged_attention_scratch_extent_host_v1(query_heads, kv_heads, head_dim, max_new_tokens, sm_count, out_bytes);
+    *out_bytes = layout_of(query_heads, kv_heads, head_dim, rows, max_new_tokens, sm_count).bytes;
+    return ok();
 }
 
 extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_shared_prefix_attention_preflight_v1(
@@ -48,12 +558,25 @@ extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_shared_pr
     if (consume_injected_fault()) return make_result(AUGUR_CUDA_STATUS_DIAGNOSTIC_FAULT_INJECTED);
     const cudaError_t e = cudaSetDevice(d);
     if (e != cudaSuccess) return make_result(AUGUR_CUDA_STATUS_RUNTIME_FAILURE, e);
-    AttentionParams p = attention_params(plan, a);
-    p.prefix_tokens = reinterpret_cast<const int32_t*>(a->prefix_tokens);
-    p.prefix_pages = static_cast<uint32_t>(a->prefix_pages_len_bytes / 4);
-    auto kernel = a->layer.head_dim == 256 ? attention_simple_kernel<256, false> : attention_simple_kernel<128, false>;
-    kernel<<<dim3(p.rows, p.query_heads), 128, 0, s->stream>>>(reinterpret_cast<const void*>(a->layer.keys), reinterpret_cast<const void*>(a->layer.values),
-                                                             reinterpret_cast<const int32_t*>(a->prefix_pages), p);
-    count_launch();
+    const uint32_t head_dim = a->layer.head_dim, kv_heads = a->layer.kv_heads, box = a->layer.page_tokens < kUnit ? a->layer.page_tokens : kUnit;
+    const Layout l = layout_of(a->query_heads, kv_heads, head_dim, a->batch.rows, a->max_new_tokens, plan->sm_count);
+    PrefixParams p{};
+    p.a = attention_params(plan, a);
+    p.a.prefix_tokens = reinterpret_cast<const int32_t*>(a->prefix_tokens);
+    p.a.prefix_pages = static_cast<uint32_t>(a->prefix_pages_len_bytes / 4);
+    p.a.own_sums = reinterpret_cast<float*>(plan->scratch + l.own_sums);
+    p.a.own_stats = reinterpret_cast<float2*>(plan->scratch + l.own_stats);
+    p.prefix_table = reinterpret_cast<const int32_t*>(a->prefix_pages);
+    p.parts = reinterpret_cast<float*>(plan->scratch + l.parts);
+    p.max_items = l.max_items;
+    p.tiles = static_cast<uint32_t>((static_cast<uint64_t>(a->batch.rows) * (a->query_heads / kv_heads) + kRowsM - 1) / kRowsM);
+    const uint64_t cache_rows = static_cast<uint64_t>(a->layer.pages) * kv_heads * a->layer.page_tokens;
+    CUtensorMap keys, values;
+    if (!make_code_map(&keys, a->layer.keys, cache_rows, head_dim * 4, box) || !make_code_map(&values, a->layer.values, cache_rows, head_dim * 4, box)) {
+        return make_result(AUGUR_CUDA_STATUS_RUNTIME_FAILURE);
+    }
+    const uint32_t columns = query_columns(a->query_heads, kv_heads, a->max_new_tokens);
+    if (head_dim == 256) launch_prefix<256>(s->stream, keys, values, p, plan->sm_count, columns);
+    else launch_prefix<128>(s->stream, keys, values, p, plan->sm_count, columns);
     return submitted();
 }
