@@ -72,7 +72,7 @@ static_assert(kLayout<128, 8> == 462 && kLayout<128, 16> == 462 && kLayout<128, 
                   kLayout<256, 16> == 462 && kLayout<256, 32> == 442 && kLayout<256, 48> == 441 && kLayout<256, 64> == 241,
               "the slots that the figures above belong to");
 
-template <uint32_t kHeadDim, uint32_t kN, bool kPrefix>
+template <uint32_t kHeadDim, uint32_t kN>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __grid_constant__ CUtensorMap map_values, const __grid_constant__ AttentionParams p) {
     using S = Shape<kHeadDim, kN>;
@@ -113,7 +113,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
     tc_fence_after();
     // Everything above runs while the launch before this one drains; from here on its results are read.
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    scan_units<kPrefix>(st, p, warp, lane);
+    scan_units(st, p, warp, lane);
     const uint32_t total = st->units[p.sequences] * p.kv_heads, spans = total < p.spans ? total : p.spans;
     const uint32_t base = spans ? total / spans : 0, extra = total - base * spans;   // spans of `base` units, the first `extra` of one more
     const uint32_t from = blockIdx.x * base + (blockIdx.x < extra ? blockIdx.x : extra), to = blockIdx.x < spans ? from + base + (blockIdx.x < extra ? 1 : 0) : from;
@@ -124,7 +124,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
         // ---------------- pages: warp 0 the keys, warp 3 the values ----------------
         const uint32_t box_shift = p.page_shift < 6 ? p.page_shift : 6, boxes = kTile >> box_shift, box_bytes = 128u << box_shift;
         const CUtensorMap* const map = warp == 0 ? &map_keys : &map_values;
-        const uint32_t skipped_pages = kPrefix ? shared_tokens(p.prefix_tokens, p.prefix_pages, p.page_shift) >> p.page_shift : 0;
         Tiles tiles;
         tiles.open(st, p, from, to);
         bool alive = true;
@@ -137,7 +136,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             uint32_t row = 0;
             bool there = false;
             if (lane < boxes && key < tiles.walk.key_end) {
-                const int32_t page = __ldg(p.page_table + static_cast<uint64_t>(tiles.walk.sequence) * p.table_pages + skipped_pages + (key >> p.page_shift));
+                const int32_t page = __ldg(p.page_table + static_cast<uint64_t>(tiles.walk.sequence) * p.table_pages + (key >> p.page_shift));
                 there = page >= 0 && static_cast<uint32_t>(page) < p.pages;
                 if (there) row = ((static_cast<uint32_t>(page) * p.kv_heads + tiles.walk.head) << p.page_shift) + (key & ((1u << p.page_shift) - 1));
                 else atomicCAS(status, 0u, kStatusPage);
@@ -440,13 +439,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
             auto write = [&](const uint32_t (&v)[S::kHalves + 1][kBlock], uint32_t c0, uint32_t i) {
                 const uint32_t c = c0 + i;
                 if (c == token_end) token_end += group, skipped += next_token;
-                if constexpr (kPrefix) {
-                    float* const own = p.own_sums + (static_cast<uint64_t>(first_row) * p.query_heads + walk.head * group) * kHeadDim + thread;
-#pragma unroll
-                    for (uint32_t h = 0; h < S::kHalves; ++h) own[skipped + c * kHeadDim + h * 128] = __uint_as_float(v[h][i]);
-                    if (thread == c) mine.y = __uint_as_float(v[S::kHalves][i]);
-                    return;
-                }
                 const float all = __uint_as_float(v[S::kHalves][i]);
                 float scale;
                 asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(scale) : "f"(all));   // good to 2^-23
@@ -494,12 +486,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
                     }
                 }
             }
-            if ((kPrefix || !alone) && thread < queries) {
+            if (!alone && thread < queries) {
                 // A part all of whose scores are NaN or -infinity has the reference -infinity too, but counts: its sums may be NaN.
                 mine.x = st->reference[thread];
                 if (mine.x == -INFINITY && st->limit[thread] > static_cast<int32_t>(walk.key)) mine.x = kNoNumber;
-                if (kPrefix && alone) p.own_stats[(static_cast<uint64_t>(first_row) + thread / group) * p.query_heads + walk.head * group + thread % group] = mine;
-                else stats[thread] = mine;
+                stats[thread] = mine;
             }
             if (any) tc_fence_before();
             if (!alone) {
@@ -522,47 +513,41 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gri
     }
 }
 
-template <uint32_t kHeadDim, uint32_t kN, bool kPrefix>
+template <uint32_t kHeadDim, uint32_t kN>
 void launch_attention(cudaStream_t stream, const CUtensorMap& keys, const CUtensorMap& values, const AttentionParams& p) {
-    launch_dependent(stream, paged_attention_kernel<kHeadDim, kN, kPrefix>, p.spans, kThreads, Shape<kHeadDim, kN>::kSmem, keys, values, p);
-    launch_join<kHeadDim, kN, kPrefix>(stream, p);
+    launch_dependent(stream, paged_attention_kernel<kHeadDim, kN>, p.spans, kThreads, Shape<kHeadDim, kN>::kSmem, keys, values, p);
+    launch_join<kHeadDim, kN>(stream, p);
     count_launch(2);
 }
 
 using Launch = void (*)(cudaStream_t, const CUtensorMap&, const CUtensorMap&, const AttentionParams&);
-template <uint32_t kHeadDim, bool kPrefix>
+template <uint32_t kHeadDim>
 Launch launch_of(uint32_t columns) {
     switch (columns) {
-        case 8: return launch_attention<kHeadDim, 8, kPrefix>;
-        case 16: return launch_attention<kHeadDim, 16, kPrefix>;
-        case 32: return launch_attention<kHeadDim, 32, kPrefix>;
-        case 48: return launch_attention<kHeadDim, 48, kPrefix>;
-        default: return launch_attention<kHeadDim, 64, kPrefix>;
+        case 8: return launch_attention<kHeadDim, 8>;
+        case 16: return launch_attention<kHeadDim, 16>;
+        case 32: return launch_attention<kHeadDim, 32>;
+        case 48: return launch_attention<kHeadDim, 48>;
+        default: return launch_attention<kHeadDim, 64>;
     }
 }
 
-template <uint32_t kHeadDim, bool kPrefix>
+template <uint32_t kHeadDim>
 cudaError_t configure() {
     constexpr cudaFuncAttribute kSmem = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 8, kPrefix>, kSmem, Shape<kHeadDim, 8>::kSmem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 16, kPrefix>, kSmem, Shape<kHeadDim, 16>::kSmem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 32, kPrefix>, kSmem, Shape<kHeadDim, 32>::kSmem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 48, kPrefix>, kSmem, Shape<kHeadDim, 48>::kSmem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 64, kPrefix>, kSmem, Shape<kHeadDim, 64>::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 8>, kSmem, Shape<kHeadDim, 8>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 16>, kSmem, Shape<kHeadDim, 16>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 32>, kSmem, Shape<kHeadDim, 32>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 48>, kSmem, Shape<kHeadDim, 48>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<kHeadDim, 64>, kSmem, Shape<kHeadDim, 64>::kSmem);
     return e;
 }
 
 }  // namespace
 
 cudaError_t attention_configure_device() {
-    cudaError_t e = configure<128, false>();
-    if (e == cudaSuccess) e = configure<256, false>();
-    if (e == cudaSuccess) e = configure<128, true>();
-    return e == cudaSuccess ? configure<256, true>() : e;
-}
-
-void launch_own_attention(cudaStream_t stream, uint32_t head_dim, uint32_t columns, const CUtensorMap& keys, const CUtensorMap& values, const AttentionParams& p) {
-    (head_dim == 256 ? launch_of<256, true>(columns) : launch_of<128, true>(columns))(stream, keys, values, p);
+    const cudaError_t e = configure<128>();
+    return e == cudaSuccess ? configure<256>() : e;
 }
 
 }  // namespace augur_sm100
@@ -599,7 +584,7 @@ extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_paged_att
         return make_result(AUGUR_CUDA_STATUS_RUNTIME_FAILURE);
     }
     const uint32_t columns = query_columns(a->query_heads, a->layer.kv_heads, a->max_new_tokens);
-    auto launch = head_dim == 256 ? launch_of<256, false>(columns) : launch_of<128, false>(columns);
+    auto launch = head_dim == 256 ? launch_of<256>(columns) : launch_of<128>(columns);
     launch(s->stream, keys, values, p);
     return submitted();
 }

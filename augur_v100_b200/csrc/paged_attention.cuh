@@ -39,25 +39,9 @@ struct AttentionParams {
     uint32_t rows, sequences, table_pages, pages, query_heads, kv_heads, page_shift, max_new, spans, joins;
     float scale_log2;             // scale * log2(e)
     const uint8_t* scales;        // of an E4M3 cache
-    // Behind a shared prefix, whose pages and tokens are left to another launch: sums and (reference maximum, denominator) by row and query head
-    // in the output's place.
-    const int32_t* prefix_tokens;
-    uint32_t prefix_pages;
-    float* own_sums;
-    float2* own_stats;
 };
 
-// The paged attention's launches behind a shared prefix (paged_attention.cu): sums for `own_sums` and `own_stats`.
-void launch_own_attention(cudaStream_t stream, uint32_t head_dim, uint32_t columns, const CUtensorMap& keys, const CUtensorMap& values, const AttentionParams& p);
-
 namespace {
-
-// The shared tokens that are read from the prefix's pages: whole pages, as many as there are.
-__device__ __forceinline__ uint32_t shared_tokens(const int32_t* prefix_tokens, uint32_t prefix_pages, uint32_t page_shift) {
-    const int32_t tokens = *prefix_tokens;
-    const uint32_t whole = tokens > 0 ? static_cast<uint32_t>(tokens) >> page_shift : 0;
-    return (whole < prefix_pages ? whole : prefix_pages) << page_shift;
-}
 
 // What a launch knows of its sequences.
 struct BatchState {
@@ -68,9 +52,7 @@ struct BatchState {
 };
 
 // Units of every sequence, and their running sum. All threads of the CTA; ends with everything written visible to all of them.
-template <bool kPrefix>
 __device__ __forceinline__ void scan_units(BatchState* st, const AttentionParams& p, uint32_t warp, uint32_t lane) {
-    const uint32_t shared = kPrefix ? shared_tokens(p.prefix_tokens, p.prefix_pages, p.page_shift) : 0;
     auto units_of = [&](uint32_t b) {
         const int32_t from = p.token_starts[b], to = p.token_starts[b + 1];
         int32_t length = p.lengths[b];
@@ -81,7 +63,6 @@ __device__ __forceinline__ void scan_units(BatchState* st, const AttentionParams
             length = room;
             if (blockIdx.x == 0) atomicCAS(p.status_word, 0u, kStatusPage);
         }
-        if (kPrefix) length = length > static_cast<int32_t>(shared) ? length - static_cast<int32_t>(shared) : 0;
         if (length < 0) length = 0;
         const uint32_t tokens = rows_fit ? static_cast<uint32_t>(to - from) : 0;
         st->row[b] = static_cast<uint32_t>(from);
@@ -254,7 +235,7 @@ __device__ __forceinline__ float warp_max(float x) {
 // thread, and the threads of a query's outputs as many times over as there are, each with every so many-th part.
 constexpr uint32_t kJoinThreads = 256, kJoinCtas = 1184;   // about as many as run at once
 // Few queries have few CTAs, and as many loads under way as the parts of one sequence want; many queries more CTAs at once.
-template <uint32_t kHeadDim, uint32_t kN, bool kPrefix>
+template <uint32_t kHeadDim, uint32_t kN>
 __global__ void __launch_bounds__(kJoinThreads, kN <= 16 ? 1 : 6) attention_join_kernel(const __grid_constant__ AttentionParams p) {
     constexpr uint32_t kLanes = kHeadDim / 4, kShares = kJoinThreads / kLanes, kAhead = kN <= 16 ? 10 : 6;
     __shared__ float weight[kMaxCtas];
@@ -321,21 +302,16 @@ __global__ void __launch_bounds__(kJoinThreads, kN <= 16 ? 1 : 6) attention_join
             for (uint32_t i = 1; i < kJoinThreads / 32; ++i) all += wide[1][i];
             const uint32_t token = query / group;
             const uint64_t place = static_cast<uint64_t>(record.row + token) * p.query_heads + record.head * group + (query - token * group), at = place * kHeadDim + 4 * lane;
-            if constexpr (kPrefix) {
-                *reinterpret_cast<float4*>(p.own_sums + at) = sum;
-                if (lane == 0) p.own_stats[place] = make_float2(most, all);
-            } else {
             const float scale = 1.0f / all;
             const __nv_bfloat162 a = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum.x * scale, all == 0.0f ? 0.0f : sum.y * scale);
             const __nv_bfloat162 b = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum.z * scale, all == 0.0f ? 0.0f : sum.w * scale);
             *reinterpret_cast<uint2*>(p.output + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-            }
         }
         __syncthreads();   // the next query's values go to the same places
     }
 }
 
-template <uint32_t kHeadDim, uint32_t kN, bool kPrefix>
+template <uint32_t kHeadDim, uint32_t kN>
 void launch_join(cudaStream_t stream, const AttentionParams& p) {
     const uint32_t queries = p.query_heads / p.kv_heads * p.max_new;
     cudaLaunchAttribute attribute{};
@@ -345,7 +321,7 @@ void launch_join(cudaStream_t stream, const AttentionParams& p) {
     config.stream = stream, config.attrs = &attribute, config.numAttrs = 1;
     const uint32_t rows = (kJoinCtas + p.joins - 1) / p.joins;
     config.gridDim = dim3(p.joins, queries < rows ? queries : rows), config.blockDim = dim3(kJoinThreads);
-    cudaLaunchKernelEx(&config, attention_join_kernel<kHeadDim, kN, kPrefix>, p);
+    cudaLaunchKernelEx(&config, attention_join_kernel<kHeadDim, kN>, p);
 }
 
 uint32_t query_columns(uint32_t query_heads, uint32_t kv_heads, uint32_t max_new) {

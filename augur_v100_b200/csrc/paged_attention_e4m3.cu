@@ -152,7 +152,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
     tc_fence_after();
     // Everything above runs while the launch before this one drains; from here on its results are read.
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    scan_units<false>(st, p, warp, lane);
+    scan_units(st, p, warp, lane);
     const uint32_t total = st->units[p.sequences] * p.kv_heads, spans = total < p.spans ? total : p.spans;
     const uint32_t base = spans ? total / spans : 0, extra = total - base * spans;   // spans of `base` units, the first `extra` of one more
     const uint32_t from = blockIdx.x * base + (blockIdx.x < extra ? blockIdx.x : extra), to = blockIdx.x < spans ? from + base + (blockIdx.x < extra ? 1 : 0) : from;
@@ -685,7 +685,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
 template <uint32_t kHeadDim, uint32_t kN>
 void launch_attention(cudaStream_t stream, const CUtensorMap& keys, const CUtensorMap& values, const AttentionParams& p) {
     launch_dependent(stream, paged_attention_e4m3_kernel<kHeadDim, kN>, p.spans, kThreads, ShapeE4m3<kHeadDim, kN>::kSmem, keys, values, p);
-    launch_join<kHeadDim, kN, false>(stream, p);
+    launch_join<kHeadDim, kN>(stream, p);
     count_launch(2);
 }
 

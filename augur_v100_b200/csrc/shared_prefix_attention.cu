@@ -25,25 +25,40 @@ static_assert(sizeof(augur_cuda_nvfp4_sm100_shared_prefix_attention_args_v1) == 
 
 constexpr uint32_t kRowsM = 128;               // queries of a CTA
 constexpr uint32_t kRounds = 3;                // a device's worth of CTAs, at most so many times, where the prefix is split for it
+constexpr uint32_t kMaxSplit = 512;             // of the prefix, and of a sequence's own tokens
+constexpr uint32_t kMaxChunks = 32;
 constexpr uint32_t kInfoRing = 8;
 constexpr uint32_t kStatusPrefixLoad = 0x421, kStatusPrefixMma = 0x422, kStatusPrefixScores = 0x423, kStatusPrefixQuery = 0x424, kStatusPrefixProduct = 0x425, kStatusPrefixInfo = 0x426;
 
 struct PrefixParams {
     AttentionParams a;
-    const int32_t* prefix_table;
+    const int32_t *prefix_table, *prefix_tokens;
     float* parts;              // [items][streams][head_dim / 4][kRowsM][4], then [items][streams][kRowsM] (reference maximum, denominator)
-    uint64_t max_items;        // that there is room for
+    float* own_parts;          // [rows][query_heads][chunks][head_dim]
+    float2* own_stats;         // [rows][query_heads][chunks]
+    uint32_t prefix_pages;
+    uint32_t max_items;        // that there is room for
     uint32_t tiles;            // of kRowsM queries
+    uint32_t chunks;           // that the tokens of a sequence are cut into
 };
+
+// The shared tokens that are read from the prefix's pages: whole pages, as many as there are.
+__device__ __forceinline__ uint32_t shared_tokens(const PrefixParams& p) {
+    const int32_t tokens = *p.prefix_tokens;
+    const uint32_t whole = tokens > 0 ? static_cast<uint32_t>(tokens) >> p.a.page_shift : 0;
+    return (whole < p.prefix_pages ? whole : p.prefix_pages) << p.a.page_shift;
+}
 
 template <uint32_t kHeadDim>
 struct PrefixShape {
     static constexpr uint32_t kChunks = kHeadDim / 64, kStreams = kHeadDim == 128 ? 2 : 1;
-    static constexpr uint32_t kThreads = 128 + 128 * kStreams;   // warp 0 loads, 1 MMA, 2 and 3 queries, then the softmax
+    static constexpr uint32_t kThreads = 128 + 128 * kStreams;   // warp 0 loads keys, 1 MMA, 2 queries, 3 values, then the softmax
     static constexpr uint32_t kQueryBytes = kRowsM * kHeadDim * 2, kSlots = (224 * 1024 - kQueryBytes) / kSlotBytes;
+    // A ring each for the keys and the values, so that two warps deal out the copies: one alone took 80 cycles a copy, and pages of 16 tokens are eight copies a slot.
+    static constexpr uint32_t kValueSlots = (kSlots / 2 + 1) / 2 * 2, kKeySlots = kSlots - kValueSlots;   // (pairs of value slots are one operand)
     static constexpr uint32_t kSmem = 1024 + kQueryBytes + kSlots * kSlotBytes + 1024;
     static constexpr uint32_t kScoresAt = 0, kOutAt = 256;       // tensor memory: two of S, one O per stream
-    static_assert(kSmem <= kSmemLimit && kOutAt + kStreams * kHeadDim == 512, "a CTA's memory");
+    static_assert(kKeySlots >= kChunks && kValueSlots >= kChunks && kChunks % 2 == 0 && kSmem <= kSmemLimit && kOutAt + kStreams * kHeadDim == 512, "a CTA's memory");
 };
 
 struct PrefixState {
@@ -69,13 +84,14 @@ struct Items {
 // be joined. A warp together.
 __device__ __forceinline__ Items items_of(const PrefixParams& p, uint32_t ctas) {
     Items x;
-    x.tokens = shared_tokens(p.a.prefix_tokens, p.a.prefix_pages, p.a.page_shift);
+    x.tokens = shared_tokens(p);
     x.key_tiles = (x.tokens + kTile - 1) / kTile;
     const uint64_t pairs = static_cast<uint64_t>(p.a.kv_heads) * p.tiles, room = p.max_items / pairs;
     uint32_t most = x.key_tiles < room ? x.key_tiles : static_cast<uint32_t>(room);
+    most = most < kMaxSplit ? most : kMaxSplit;
     uint64_t best = UINT64_MAX;
     for (uint32_t split = 1 + threadIdx.x % 32; split <= most; split += 32) {
-        const uint64_t items = pairs * split, cost = (items + ctas - 1) / ctas * ((x.key_tiles + split - 1) / split + 4) * 32 + items, key = cost << 16 | (split < 65535 ? split : 65535);
+        const uint64_t items = pairs * split, cost = (items + ctas - 1) / ctas * ((x.key_tiles + split - 1) / split + 4) * 32 + items, key = cost << 16 | split;
         if (key < best) best = key;
     }
 #pragma unroll
@@ -104,6 +120,16 @@ __device__ __forceinline__ void mma_block_from_tmem(uint32_t d, uint32_t a, uint
         : "memory");
 }
 
+// Two F32 operations in one instruction: x * scale + shift, and sums.
+__device__ __forceinline__ void fma2(uint32_t& x0, uint32_t& x1, float scale, float shift) {
+    asm("{\n.reg .b64 x, a, b;\nmov.b64 x, {%0, %1};\nmov.b64 a, {%2, %2};\nmov.b64 b, {%3, %3};\nfma.rn.ftz.f32x2 x, x, a, b;\nmov.b64 {%0, %1}, x;\n}"
+        : "+r"(x0), "+r"(x1)
+        : "r"(__float_as_uint(scale)), "r"(__float_as_uint(shift)));
+}
+__device__ __forceinline__ void add2(float& x0, float& x1, uint32_t y0, uint32_t y1) {
+    asm("{\n.reg .b64 x, y;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nadd.rn.ftz.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}" : "+f"(x0), "+f"(x1) : "r"(y0), "r"(y1));
+}
+
 template <uint32_t kHeadDim>
 __global__ void __launch_bounds__(PrefixShape<kHeadDim>::kThreads, 1)
 prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __grid_constant__ CUtensorMap map_values, const __grid_constant__ PrefixParams p) {
@@ -122,7 +148,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
         for (uint32_t s = 0; s < S::kSlots; ++s) mbar_init(full + 8 * s, 1), mbar_init(empty + 8 * s, 1);
         for (uint32_t b = 0; b < 2; ++b) mbar_init(scores_full + 8 * b, 1), mbar_init(weights_full + 8 * b, 4), mbar_init(products + 8 * b, 1);
         for (uint32_t i = 0; i < kInfoRing; ++i) mbar_init(info_full + 8 * i, 1);
-        mbar_init(query_full, 2), mbar_init(query_empty, 1);
+        mbar_init(query_full, 1), mbar_init(query_empty, 1);
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_keys) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_values) : "memory");
         for (uint32_t i = 0; i < 1 + 12; ++i) st->abort[i] = 0;
@@ -138,7 +164,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
     // Everything above runs while the launch before this one drains; from here on its results are read.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Items items = items_of(p, gridDim.x);
-    if (blockIdx.x == 0 && threadIdx.x == 0 && *p.a.prefix_tokens > static_cast<int32_t>(p.a.prefix_pages << p.a.page_shift)) atomicCAS(status, 0u, kStatusPage);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && *p.prefix_tokens > static_cast<int32_t>(p.prefix_pages << p.a.page_shift)) atomicCAS(status, 0u, kStatusPage);
     // Does any row end within the prefix?
     bool ends_within = false;
     const int32_t room = static_cast<int32_t>(p.a.table_pages << p.a.page_shift);   // a length beyond the table counts as the table's
@@ -150,25 +176,16 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
     const uint32_t tmem = st->tmem, group = p.a.query_heads / p.a.kv_heads;
     const uint32_t all_queries = p.a.rows * group;   // of a key-value head; below 2^26
 
-    if (warp == 0) {
-        // ---------------- pages: a tile's keys, then the values of the tile before it, as they are used ----------------
+    if (warp == 0 || warp == 3) {
+        // ---------------- pages: warp 0 the keys, warp 3 the values ----------------
         const uint32_t box_shift = p.a.page_shift < 6 ? p.a.page_shift : 6, boxes = kTile >> box_shift, box_bytes = 128u << box_shift;
         const uint32_t beyond = (p.a.pages * p.a.kv_heads) << p.a.page_shift;   // a row behind the cache: TMA reads zeros there
-        uint32_t slot = 0, phase = 1, count = 0;
+        const CUtensorMap* const map = warp == 0 ? &map_keys : &map_values;
+        const uint32_t first_slot = warp == 0 ? 0 : S::kKeySlots, end_slot = warp == 0 ? S::kKeySlots : S::kSlots;
+        uint32_t slot = first_slot, phase = 1, count = 0;
         bool alive = true;
-        auto load = [&](const CUtensorMap* map, uint32_t row) {
-            for (uint32_t c = 0; c < S::kChunks; ++c) {
-                if (!warp_look_wait(empty + 8 * slot, phase, abort_flag, status, kStatusPrefixLoad)) return false;
-                if (lane == 0) mbar_expect_tx(full + 8 * slot, kSlotBytes);
-                __syncwarp();
-                if (lane < boxes) tma_load_2d(smem_u32(smem) + slot * kSlotBytes + lane * box_bytes, map, c * 128, row, full + 8 * slot);
-                __syncwarp();
-                if (++slot == S::kSlots) slot = 0, phase ^= 1;
-            }
-            return true;
-        };
         for (uint64_t item = blockIdx.x; alive && item < items.count; item += gridDim.x) {
-            uint32_t head, tile, first, last, before = 0;
+            uint32_t head, tile, first, last;
             items.locate(p, item, &head, &tile, &first, &last);
             auto page_of = [&](uint32_t t) {
                 const uint32_t key = t * kTile + (lane << box_shift);
@@ -182,34 +199,35 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
                 const uint32_t row = there ? ((static_cast<uint32_t>(page) * p.a.kv_heads + head) << p.a.page_shift) + (key & ((1u << p.a.page_shift) - 1)) : beyond;
                 const uint32_t mask = __ballot_sync(0xffffffffu, there);
                 page = page_of(t + 1);
-                // (the ring is that long: a tile's keys are loaded behind the products of two tiles before, which wait for the softmax of those)
-                if (lane == 0) {
+                if (warp == 0 && lane == 0) {   // (the ring is that long: keys are loaded three tiles ahead at most of those whose scores the softmax has)
                     st->info[count % kInfoRing] = mask;
                     mbar_arrive(info_full + 8 * (count % kInfoRing));
                 }
                 __syncwarp();
-                alive = load(&map_keys, row) && (t == first || load(&map_values, before));
-                before = row;
+                for (uint32_t c = 0; c < S::kChunks; ++c) {
+                    if (!(alive = warp_look_wait(empty + 8 * slot, phase, abort_flag, status, kStatusPrefixLoad))) break;
+                    if (lane == 0) mbar_expect_tx(full + 8 * slot, kSlotBytes);
+                    __syncwarp();
+                    if (lane < boxes) tma_load_2d(smem_u32(smem) + slot * kSlotBytes + lane * box_bytes, map, c * 128, row, full + 8 * slot);
+                    __syncwarp();
+                    if (++slot == end_slot) slot = first_slot, phase ^= 1;
+                }
             }
-            alive = alive && load(&map_values, before);
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer: S of a tile, then O of the tile before it ----------------
         constexpr uint32_t idesc_any = (1u << 4) | (1u << 7) | (1u << 10) | ((kRowsM >> 4) << 24);   // F32 += BF16 x BF16
-        constexpr uint32_t idesc = idesc_any | ((kTile >> 3) << 17), idesc_values = idesc_any | ((64 >> 3) << 17) | (1u << 16);   // V is MN-major
-        const uint32_t slots = low_word(smem_u32(smem), 16), queries = low_word(smem_u32(query_smem), 16);
-        uint32_t slot = 0, phase = 0, scores = 0, done = 0, round = 0;
+        constexpr uint32_t idesc = idesc_any | ((kTile >> 3) << 17), idesc_values = idesc_any | ((128 >> 3) << 17) | (1u << 16);   // V is MN-major
+        const uint32_t slots = low_word(smem_u32(smem), 16), slots_values = low_word(smem_u32(smem), kSlotBytes), queries = low_word(smem_u32(query_smem), 16);
+        uint32_t key_slot = 0, key_phase = 0, slot = S::kKeySlots, phase = 0, scores = 0, done = 0, round = 0;
         bool alive = true;
-        auto next_slot = [&]() {
-            if (++slot == S::kSlots) slot = 0, phase ^= 1;
-        };
         auto scores_of_tile = [&]() {
             for (uint32_t c = 0; c < S::kChunks; ++c) {
-                if (!warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusPrefixMma)) return false;
+                if (!warp_look_wait(full + 8 * key_slot, key_phase, abort_flag, status, kStatusPrefixMma)) return false;
                 tc_fence_after();
-                mma_block<kHighSwizzled, 2>(tmem + S::kScoresAt + (scores & 1) * kTile, queries + c * (kSlotBytes >> 4), slots + slot * (kSlotBytes >> 4), idesc, c, 4);
-                commit(empty + 8 * slot);
-                next_slot();
+                mma_block<kHighSwizzled, 2>(tmem + S::kScoresAt + (scores & 1) * kTile, queries + c * (kSlotBytes >> 4), slots + key_slot * (kSlotBytes >> 4), idesc, c, 4);
+                commit(empty + 8 * key_slot);
+                if (++key_slot == S::kKeySlots) key_slot = 0, key_phase ^= 1;
             }
             commit(scores_full + 8 * (scores & 1));
             ++scores;
@@ -229,21 +247,24 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
                 const uint32_t buffer = done & 1, d = tmem + S::kOutAt + (S::kStreams == 2 ? buffer * kHeadDim : 0);
                 const uint32_t follows = t >= first + S::kStreams;
                 if (!(alive = warp_look_wait(weights_full + 8 * buffer, done >> 1 & 1, abort_flag, status, kStatusPrefixProduct))) break;
-                for (uint32_t c = 0; c < S::kChunks; ++c) {
-                    if (!(alive = warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusPrefixProduct))) break;
+                for (uint32_t c = 0; c < S::kChunks; c += 2) {   // 128 dims: two slots, side by side
+                    alive = warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusPrefixProduct) && warp_look_wait(full + 8 * (slot + 1), phase, abort_flag, status, kStatusPrefixProduct);
+                    if (!alive) break;
                     tc_fence_after();
-                    const uint32_t a = tmem + S::kScoresAt + buffer * kTile, b = slots + slot * (kSlotBytes >> 4);   // 16 keys: 8 columns of P, 16 rows of V
+                    const uint32_t a = tmem + S::kScoresAt + buffer * kTile, b = slots_values + slot * (kSlotBytes >> 4);   // 16 keys: 8 columns of P, 16 rows of V
                     mma_block_from_tmem<(16 * 128 >> 4)>(d + c * 64, a, b, idesc_values, follows);
                     mma_block_from_tmem<(16 * 128 >> 4)>(d + c * 64, a + 32, b + 4 * (16 * 128 >> 4), idesc_values, 1);
                     commit(empty + 8 * slot);
-                    next_slot();
+                    commit(empty + 8 * (slot + 1));
+                    slot += 2;
+                    if (slot == S::kSlots) slot = S::kKeySlots, phase ^= 1;
                 }
                 if (!alive) break;
                 commit(products + 8 * buffer);
                 ++done;
             }
         }
-    } else if (warp < 4) {
+    } else if (warp == 2) {
         // ---------------- queries of an item, in the 128-byte swizzle of the operand; past the last they are zero ----------------
         constexpr uint32_t kPieces = kHeadDim / 8;   // of 16 bytes
         uint32_t round = 0;
@@ -251,7 +272,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
             uint32_t head, tile, first, last;
             items.locate(p, item, &head, &tile, &first, &last);
             if (!warp_look_wait(query_empty, (round & 1) ^ 1, abort_flag, status, kStatusPrefixQuery)) break;
-            for (uint32_t i = (warp - 2) * 32 + lane; i < kRowsM * kPieces; i += 64) {
+            for (uint32_t i = lane; i < kRowsM * kPieces; i += 32) {
                 const uint32_t row = i / kPieces, piece = i % kPieces, query = tile * kRowsM + row, token = query / group;
                 const bool live = query < all_queries;
                 const __nv_bfloat16* const at = p.a.query + (static_cast<uint64_t>(live ? token : 0) * p.a.query_heads + head * group + (live ? query - token * group : 0)) * kHeadDim + piece * 8;
@@ -289,7 +310,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
                 limit = seen <= 0 ? 0 : seen < static_cast<int64_t>(limit) ? static_cast<uint32_t>(seen) : limit;
             }
             const uint32_t seen_by_all = __reduce_min_sync(0xffffffffu, limit);
-            float reference = -INFINITY, sum0 = 0.0f, sum1 = 0.0f;
+            float reference = -INFINITY, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             bool started = false;
             uint32_t first_key = 0;
             for (uint32_t t = first; t < last; ++t, ++count) {
@@ -310,32 +331,37 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
                     else bits &= (there >> (c >> 4) & 1 ? 0xffffu : 0) | (there >> ((c >> 4) + 1) & 1 ? 0xffff0000u : 0);
                     return bits;
                 };
+                uint32_t v[kTile];
+#pragma unroll
+                for (uint32_t c = 0; c < kTile; c += 32) tc_load32(from + c, reinterpret_cast<uint32_t(&)[32]>(v[c]));
+                tc_wait_ld();
+                if (masked) {
+#pragma unroll
+                    for (uint32_t c = 0; c < kTile; c += 32) {
+                        const uint32_t bits = seen(c);
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; ++i) v[c + i] = bits >> i & 1 ? v[c + i] : __float_as_uint(scale < 0.0f ? INFINITY : -INFINITY);
+                    }
+                }
                 // The largest score: of scale * S, the product with the largest S or, with a scale below zero, the smallest.
-                float most = scale < 0.0f ? INFINITY : -INFINITY;
-#pragma unroll 1
-                for (uint32_t c = 0; c < kTile; c += 32) {
-                    uint32_t v[32];
-                    tc_load32(from + c, v);
-                    tc_wait_ld();
-                    const uint32_t bits = masked ? seen(c) : 0xffffffffu;
-                    if (masked) {
+                float most;
+                if (scale < 0.0f) {
+                    float m[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
 #pragma unroll
-                        for (uint32_t i = 0; i < 32; ++i) v[i] = bits >> i & 1 ? v[i] : __float_as_uint(scale < 0.0f ? INFINITY : -INFINITY);
-                    }
-                    if (scale < 0.0f) {
+                    for (uint32_t i = 0; i < kTile; i += 2) m[i / 2 % 4] = fminf(fminf(m[i / 2 % 4], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
+                    most = fminf(fminf(m[0], m[1]), fminf(m[2], m[3]));
+                } else {
+                    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (uint32_t i = 0; i < 32; ++i) most = fminf(most, __uint_as_float(v[i]));
-                    } else {
-#pragma unroll
-                        for (uint32_t i = 0; i < 32; ++i) most = fmaxf(most, __uint_as_float(v[i]));
-                    }
+                    for (uint32_t i = 0; i < kTile; i += 2) m[i / 2 % 4] = fmaxf(fmaxf(m[i / 2 % 4], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
+                    most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                 }
                 const float top = fmaxf(reference, most * scale);
                 const bool above = top > reference + kSlack || (!started && top > reference);
                 if (__any_sync(0xffffffffu, above)) {
                     const float now = above ? top : reference, factor = now == reference ? 1.0f : exp2_fast(reference - now);
                     reference = now;
-                    sum0 *= factor, sum1 *= factor;
+                    sum[0] *= factor, sum[1] *= factor, sum[2] *= factor, sum[3] *= factor;
                     if (started) {
                         // the stream's tile before has to be through
                         const uint32_t earlier = count - S::kStreams;
@@ -358,23 +384,23 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
                 if (!started) first_key = key;
                 started = true;
                 const float minus = reference == -INFINITY ? 0.0f : -reference;
-#pragma unroll 1
+#pragma unroll
                 for (uint32_t c = 0; c < kTile; c += 32) {
-                    uint32_t v[32], packed[16];
-                    tc_load32(from + c, v);
-                    tc_wait_ld();
-                    const uint32_t bits = masked ? seen(c) : 0xffffffffu;
+                    uint32_t packed[16];
 #pragma unroll
-                    for (uint32_t i = 0; i < 32; ++i) v[i] = __float_as_uint(exp2_fast(fmaf(__uint_as_float(v[i]), scale, minus)));
+                    for (uint32_t i = 0; i < 32; i += 2) fma2(v[c + i], v[c + i + 1], scale, minus);
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; ++i) v[c + i] = __float_as_uint(exp2_fast(__uint_as_float(v[c + i])));
                     if (masked) {
+                        const uint32_t bits = seen(c);   // (again: with a scale of zero the exponential is not zero)
 #pragma unroll
-                        for (uint32_t i = 0; i < 32; ++i) v[i] = bits >> i & 1 ? v[i] : 0;
+                        for (uint32_t i = 0; i < 32; ++i) v[c + i] = bits >> i & 1 ? v[c + i] : 0;
                     }
 #pragma unroll
                     for (uint32_t i = 0; i < 16; ++i) {
-                        const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                        const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(v[c + 2 * i]), __uint_as_float(v[c + 2 * i + 1]));
                         packed[i] = *reinterpret_cast<const uint32_t*>(&two);
-                        sum0 += __uint_as_float(packed[i] << 16), sum1 += __uint_as_float(packed[i] & 0xffff0000u);
+                        add2(sum[2 * (i % 2)], sum[2 * (i % 2) + 1], packed[i] << 16, packed[i] & 0xffff0000u);
                     }
                     store_columns16(from + c / 2, packed);
                 }
@@ -405,7 +431,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
             }
             // (a part all of whose scores are NaN or -infinity has the reference -infinity too, but counts: its sums may be NaN)
             if (started && reference == -INFINITY && limit > first_key) reference = kNoNumber;
-            reinterpret_cast<float2*>(p.parts + p.max_items * S::kStreams * kRowsM * kHeadDim)[part * kRowsM + thread] = make_float2(reference, sum0 + sum1);
+            reinterpret_cast<float2*>(p.parts + static_cast<uint64_t>(p.max_items) * S::kStreams * kRowsM * kHeadDim)[part * kRowsM + thread] = make_float2(reference, (sum[0] + sum[1]) + (sum[2] + sum[3]));
         }
     }
     tc_fence_before();
@@ -416,21 +442,262 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
     }
 }
 
-// Joins the parts of the prefix, in their order, and the sums over the row's own tokens. A CTA takes eight queries of an item's 128.
+// ---- a sequence's own tokens ----------------------------------------------------------------------
+// These are few next to the prefix, and often very few: what counts is how many are under way at once. So small CTAs, several an SM, each a chunk of the tokens
+// of a (sequence, key-value head), 64 at a time through shared memory and mma.sync (m16n8k16): a warp forms the scores of 16 of the 64 keys and then the
+// outputs of a quarter of the dims. (The paged attention's kernel, one CTA an SM, took 4.4 us for every pair of some 40 tokens: 171 sequences of 8 heads 41 us.)
+constexpr uint32_t kOwnThreads = 128, kOwnTile = 64;
+
+template <uint32_t kHeadDim, uint32_t kM>
+struct OwnShape {
+    static constexpr uint32_t kQueries = 16 * kM, kRowBytes = kHeadDim * 2;
+    static constexpr uint32_t kKeysAt = kQueries * kRowBytes, kValuesAt = kKeysAt + kOwnTile * kRowBytes, kWeightsAt = kValuesAt + kOwnTile * kRowBytes;
+    static constexpr uint32_t kMostAt = kWeightsAt + kQueries * kOwnTile * 2, kSmem = kMostAt + 4 * kQueries * 4;
+};
+// 16 bytes `piece` of a row: pieces of eight rows that follow one another lie in different banks.
+template <uint32_t kRowBytes>
+__device__ __forceinline__ uint32_t own_at(uint32_t row, uint32_t piece) { return row * kRowBytes + ((piece ^ (row & 7)) << 4); }
+__device__ __forceinline__ void ldmatrix4(uint32_t (&v)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_turned(uint32_t (&v)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <uint32_t kHeadDim, uint32_t kM>
+__global__ void __launch_bounds__(kOwnThreads) own_attention_kernel(const __nv_bfloat16* keys, const __nv_bfloat16* values, const __grid_constant__ PrefixParams p) {
+    using S = OwnShape<kHeadDim, kM>;
+    constexpr uint32_t kPieces = kHeadDim / 8, kDims = kHeadDim / 4;   // 16-byte pieces of a row, dims of a warp
+    extern __shared__ __align__(128) uint8_t own_smem[];
+    const uint32_t smem = smem_u32(own_smem), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float* const wide = reinterpret_cast<float*>(own_smem + S::kMostAt);   // [warp][query]
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t chunk = blockIdx.x % p.chunks, pair = blockIdx.x / p.chunks, head = pair % p.a.kv_heads, b = pair / p.a.kv_heads;
+    const int32_t first_row = p.a.token_starts[b], end_row = p.a.token_starts[b + 1];
+    int32_t length = p.a.lengths[b];
+    const uint32_t shared = shared_tokens(p);
+    if (first_row < 0 || end_row > static_cast<int32_t>(p.a.rows) || end_row < first_row || end_row - first_row > static_cast<int32_t>(p.a.max_new)) {
+        if (threadIdx.x == 0) atomicCAS(p.a.status_word, 0u, kStatusRows);
+        return;
+    }
+    const int32_t room = static_cast<int32_t>(p.a.table_pages << p.a.page_shift);
+    if (length > room) {
+        length = room;
+        if (threadIdx.x == 0) atomicCAS(p.a.status_word, 0u, kStatusPage);
+    }
+    const uint32_t tokens = static_cast<uint32_t>(end_row - first_row), group = p.a.query_heads / p.a.kv_heads, queries = tokens * group;
+    if (!tokens) return;
+    const int32_t own = length - static_cast<int32_t>(shared);   // below zero: the sequence ends in the prefix
+    const uint32_t tiles = own > 0 ? (static_cast<uint32_t>(own) + kOwnTile - 1) / kOwnTile : 0, per = (tiles + p.chunks - 1) / p.chunks;
+    const uint32_t tile0 = chunk * per, tile1 = tile0 + per < tiles ? tile0 + per : tiles;
+    auto place_of = [&](uint32_t query) { return (static_cast<uint64_t>(first_row) + query / group) * p.a.query_heads + head * group + query % group; };
+    if (tile0 >= tile1) {
+        if (threadIdx.x < queries) p.own_stats[place_of(threadIdx.x) * p.chunks + chunk] = make_float2(-INFINITY, 0.0f);
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < S::kQueries * kPieces; i += kOwnThreads) {
+        const uint32_t query = i / kPieces, piece = i % kPieces;
+        const bool live = query < queries;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                     ::"r"(smem + own_at<S::kRowBytes>(query, piece)), "l"(p.a.query + place_of(live ? query : 0) * kHeadDim + piece * 8), "r"(live ? 16 : 0)
+                     : "memory");
+    }
+    // Of this thread's rows (of each 16: lane / 4 and 8 further): tokens seen, reference maximum, part of the denominator. And a quarter of the dims of the output.
+    int32_t limit[kM][2];
+    float reference[kM][2], sum[kM][2], out[kM][kDims / 8][4];
+#pragma unroll
+    for (uint32_t m = 0; m < kM; ++m) {
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            const uint32_t query = 16 * m + 8 * h + lane / 4;
+            limit[m][h] = query < queries ? own - static_cast<int32_t>(tokens) + static_cast<int32_t>(query / group) + 1 : 0;
+            reference[m][h] = -INFINITY, sum[m][h] = 0.0f;
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < kDims / 8; ++n) out[m][n][0] = out[m][n][1] = out[m][n][2] = out[m][n][3] = 0.0f;
+    }
+    const int32_t* const table = p.a.page_table + static_cast<uint64_t>(b) * p.a.table_pages + (shared >> p.a.page_shift);
+    // A warp copies 16 of a tile's keys and values; a lane looks up the place of one of the 16.
+    auto slot_of = [&](uint32_t tile) -> int64_t {
+        const uint32_t key = tile * kOwnTile + warp * 16 + lane % 16;
+        if (tile >= tile1 || key >= static_cast<uint32_t>(own)) return -1;
+        const int32_t page = __ldg(table + (key >> p.a.page_shift));
+        if (page < 0 || static_cast<uint32_t>(page) >= p.a.pages) {
+            atomicCAS(p.a.status_word, 0u, kStatusPage);
+            return -1;
+        }
+        return ((static_cast<int64_t>(page) * p.a.kv_heads + head) << p.a.page_shift) + (key & ((1u << p.a.page_shift) - 1));
+    };
+    int64_t slot = slot_of(tile0);
+    for (uint32_t tile = tile0; tile < tile1; ++tile) {
+        if (tile != tile0) __syncthreads();   // the tile before is no longer read
+        auto copy = [&](const __nv_bfloat16* from, uint32_t to) {
+#pragma unroll
+            for (uint32_t i = 0; i < 16 * kPieces / 32; ++i) {
+                const uint32_t at = i * 32 + lane, row = at / kPieces, piece = at % kPieces;
+                const int64_t here = __shfl_sync(0xffffffffu, slot, row);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                             ::"r"(to + own_at<S::kRowBytes>(warp * 16 + row, piece)), "l"(from + (here < 0 ? 0 : here) * kHeadDim + piece * 8), "r"(here < 0 ? 0 : 16)
+                             : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        copy(keys, smem + S::kKeysAt);
+        copy(values, smem + S::kValuesAt);
+        const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);   // (keys without a page count as not there)
+        slot = slot_of(tile + 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        if (tile == tile0) __syncthreads();   // the queries; a warp's own keys it waits for itself
+        else __syncwarp();
+        // ---- scores of the warp's 16 keys ----
+        float s[kM][2][4];
+#pragma unroll
+        for (uint32_t m = 0; m < kM; ++m) {
+#pragma unroll
+            for (uint32_t n = 0; n < 2; ++n) s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.0f;
+        }
+#pragma unroll 4
+        for (uint32_t k = 0; k < kHeadDim / 16; ++k) {
+            uint32_t key[4];
+            ldmatrix4(key, smem + S::kKeysAt + own_at<S::kRowBytes>(warp * 16 + (lane & 7) + (lane >> 4) * 8, 2 * k + (lane >> 3 & 1)));
+#pragma unroll
+            for (uint32_t m = 0; m < kM; ++m) {
+                uint32_t query[4];
+                ldmatrix4(query, smem + own_at<S::kRowBytes>(16 * m + (lane & 15), 2 * k + (lane >> 4)));
+                mma_16816(s[m][0], query, key[0], key[1]);
+                mma_16816(s[m][1], query, key[2], key[3]);
+            }
+        }
+        const int32_t key0 = static_cast<int32_t>(tile * kOwnTile + warp * 16 + 2 * (lane & 3));
+#pragma unroll
+        for (uint32_t m = 0; m < kM; ++m) {
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                float most = -INFINITY;
+#pragma unroll
+                for (uint32_t n = 0; n < 2; ++n) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+                        float& x = s[m][n][2 * h + e];
+                        x = key0 + static_cast<int32_t>(8 * n + e) < limit[m][h] && (there >> (8 * n + 2 * (lane & 3) + e) & 1) ? x * p.a.scale_log2 : -INFINITY;
+                        most = fmaxf(most, x);
+                    }
+                }
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                if ((lane & 3) == 0) wide[warp * S::kQueries + 16 * m + 8 * h + lane / 4] = most;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t m = 0; m < kM; ++m) {
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                const uint32_t query = 16 * m + 8 * h + lane / 4;
+                float now = reference[m][h];
+#pragma unroll
+                for (uint32_t w = 0; w < 4; ++w) now = fmaxf(now, wide[w * S::kQueries + query]);
+                const float factor = now == reference[m][h] ? 1.0f : exp2_fast(reference[m][h] - now), minus = now == -INFINITY ? 0.0f : now;
+                reference[m][h] = now;
+                sum[m][h] *= factor;
+#pragma unroll
+                for (uint32_t n = 0; n < kDims / 8; ++n) out[m][n][2 * h] *= factor, out[m][n][2 * h + 1] *= factor;
+#pragma unroll
+                for (uint32_t n = 0; n < 2; ++n) {
+                    const __nv_bfloat162 two = __floats2bfloat162_rn(exp2_fast(s[m][n][2 * h] - minus), exp2_fast(s[m][n][2 * h + 1] - minus));
+                    const uint32_t bits = *reinterpret_cast<const uint32_t*>(&two);
+                    sum[m][h] += __uint_as_float(bits << 16) + __uint_as_float(bits & 0xffff0000u);
+                    *reinterpret_cast<uint32_t*>(own_smem + S::kWeightsAt + own_at<kOwnTile * 2>(query, warp * 2 + n) + (lane & 3) * 4) = bits;
+                }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        // ---- outputs of the warp's dims ----
+#pragma unroll
+        for (uint32_t k = 0; k < kOwnTile / 16; ++k) {
+            uint32_t weights[kM][4];
+#pragma unroll
+            for (uint32_t m = 0; m < kM; ++m) ldmatrix4(weights[m], smem + S::kWeightsAt + own_at<kOwnTile * 2>(16 * m + (lane & 15), 2 * k + (lane >> 4)));
+#pragma unroll
+            for (uint32_t n = 0; n < kDims / 8; n += 2) {
+                uint32_t value[4];
+                ldmatrix4_turned(value, smem + S::kValuesAt + own_at<S::kRowBytes>(16 * k + (lane & 15), (warp * kDims) / 8 + n + (lane >> 4)));
+#pragma unroll
+                for (uint32_t m = 0; m < kM; ++m) {
+                    mma_16816(out[m][n], weights[m], value[0], value[1]);
+                    mma_16816(out[m][n + 1], weights[m], value[2], value[3]);
+                }
+            }
+        }
+    }
+    // ---- the chunk's part ----
+#pragma unroll
+    for (uint32_t m = 0; m < kM; ++m) {
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 1);
+            sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 2);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t m = 0; m < kM; ++m) {
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            if ((lane & 3) == 0) wide[warp * S::kQueries + 16 * m + 8 * h + lane / 4] = sum[m][h];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t m = 0; m < kM; ++m) {
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            const uint32_t query = 16 * m + 8 * h + lane / 4;
+            if (query >= queries) continue;
+            const uint64_t part = place_of(query) * p.chunks + chunk;
+            if (warp == 0 && (lane & 3) == 0) {
+                // (a part all of whose scores are NaN or -infinity has the reference -infinity too, but counts: its sums may be NaN)
+                const bool none = reference[m][h] == -INFINITY && limit[m][h] > static_cast<int32_t>(tile0 * kOwnTile);
+                float all = 0.0f;
+#pragma unroll
+                for (uint32_t w = 0; w < 4; ++w) all += wide[w * S::kQueries + query];
+                p.own_stats[part] = make_float2(none ? kNoNumber : reference[m][h], all);
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < kDims / 8; ++n) {
+                *reinterpret_cast<float2*>(p.own_parts + part * kHeadDim + warp * kDims + n * 8 + 2 * (lane & 3)) = make_float2(out[m][n][2 * h], out[m][n][2 * h + 1]);
+            }
+        }
+    }
+}
+
+// Joins the parts of the prefix and of the rows' own tokens, in their order. A CTA takes eight queries of an item's 128, a warp the weights of one of them.
 constexpr uint32_t kMergeThreads = 256, kMergeQueries = 8;
 template <uint32_t kHeadDim>
 __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const __grid_constant__ PrefixParams p, uint32_t ctas) {
     using S = PrefixShape<kHeadDim>;
-    constexpr uint32_t kEach = kHeadDim / 4 / 32;   // float4 of a thread
+    constexpr uint32_t kEach = kHeadDim / 4 / 32, kAhead = 4;   // float4 of a thread, parts under way at once
+    constexpr uint32_t kMost = kMaxSplit * S::kStreams + kMaxChunks;
+    __shared__ float weight[kMergeQueries][kMost + 4], total[kMergeQueries];
     __shared__ uint32_t live[kMergeQueries];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Items items = items_of(p, ctas);
-    const uint32_t group = p.a.query_heads / p.a.kv_heads, all_queries = p.a.rows * group;
+    const uint32_t group = p.a.query_heads / p.a.kv_heads, all_queries = p.a.rows * group, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     constexpr uint32_t kSlices = kRowsM / kMergeQueries;
     const uint32_t slice = blockIdx.x % kSlices, tile = blockIdx.x / kSlices % p.tiles, head = blockIdx.x / kSlices / p.tiles;
     const uint32_t query0 = tile * kRowsM + slice * kMergeQueries;
     if (query0 >= all_queries) return;
+    const uint32_t shared_parts = items.key_tiles ? items.split * S::kStreams : 0, parts = shared_parts + p.chunks;
+    auto part_of = [&](uint32_t n) { return ((static_cast<uint64_t>(head) * items.split + n / S::kStreams) * p.tiles + tile) * S::kStreams + n % S::kStreams; };
+    auto place_of = [&](uint32_t query) { return static_cast<uint64_t>(query / group) * p.a.query_heads + head * group + query % group; };
     // The rows that belong to a sequence.
     if (threadIdx.x < kMergeQueries) live[threadIdx.x] = 0;
     __syncthreads();
@@ -443,59 +710,88 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const __gri
         }
     }
     __syncthreads();
+    // A warp's query: the weights 2^(reference - largest reference) of its parts, and the denominator. Parts of which it sees nothing are passed over (-1).
+    // All others count, with a weight of zero too: zero times a NaN is one.
+    if (live[warp] && query0 + warp < all_queries) {
+        const float2* const stats = reinterpret_cast<const float2*>(p.parts + static_cast<uint64_t>(p.max_items) * S::kStreams * kRowsM * kHeadDim);
+        const uint64_t own = place_of(query0 + warp) * p.chunks;
+        auto stat_of = [&](uint32_t n) { return n < shared_parts ? stats[part_of(n) * kRowsM + slice * kMergeQueries + warp] : p.own_stats[own + n - shared_parts]; };
+        float most = -INFINITY, all = 0.0f;
+        for (uint32_t n = lane; n < parts; n += 32) {
+            const float x = stat_of(n).x;
+            weight[warp][n] = x;
+            most = fmaxf(most, x);
+        }
+#pragma unroll
+        for (uint32_t step = 16; step; step /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, step));
+        for (uint32_t n = lane; n < parts; n += 32) {
+            const float x = weight[warp][n], w = x == -INFINITY ? -1.0f : exp2_fast(x - most);
+            weight[warp][n] = w;
+            if (!(w < 0.0f)) all = fmaf(w, stat_of(n).y, all);
+        }
+#pragma unroll
+        for (uint32_t step = 16; step; step /= 2) all += __shfl_xor_sync(0xffffffffu, all, step);
+        if (lane == 0) total[warp] = all;
+    }
+    __syncthreads();
     // lanes: eight queries, four neighbouring float4 of each
-    const uint32_t i = threadIdx.x % kMergeQueries, query = query0 + i, column = threadIdx.x / kMergeQueries;
+    const uint32_t i = threadIdx.x % kMergeQueries, query = query0 + i, column = threadIdx.x / kMergeQueries, row = slice * kMergeQueries + i;
     if (!live[i] || query >= all_queries) return;
-    const uint32_t token = query / group;
-    const uint64_t place = static_cast<uint64_t>(token) * p.a.query_heads + head * group + (query - token * group);
-    const uint32_t row = slice * kMergeQueries + i, parts = items.key_tiles ? items.split * S::kStreams : 0;
-    auto part_of = [&](uint32_t n) { return ((static_cast<uint64_t>(head) * items.split + n / S::kStreams) * p.tiles + tile) * S::kStreams + n % S::kStreams; };
-    const float2* const stats = reinterpret_cast<const float2*>(p.parts + p.max_items * S::kStreams * kRowsM * kHeadDim);
-    const float2 own = p.a.own_stats[place];
-    float most = own.x;
-    for (uint32_t n = 0; n < parts; ++n) most = fmaxf(most, stats[part_of(n) * kRowsM + row].x);
+    const uint64_t place = place_of(query);
     float4 sum[kEach];
-    float all = 0.0f;
 #pragma unroll
     for (uint32_t e = 0; e < kEach; ++e) sum[e] = make_float4(0, 0, 0, 0);
-    auto add = [&](float2 stat, const float4* from, uint32_t stride) {
-        // Parts of which the query sees nothing are passed over. All others count, with a weight of zero too: zero times a NaN is one.
-        if (stat.x == -INFINITY) return;
-        const float w = exp2_fast(stat.x - most);
-        all = fmaf(w, stat.y, all);
+    for (uint32_t first = 0; first < parts; first += kAhead) {
+        float4 v[kAhead][kEach];
+        float w[kAhead];
 #pragma unroll
-        for (uint32_t e = 0; e < kEach; ++e) {
-            const float4 x = from[e * 32 * stride];
-            sum[e].x = fmaf(w, x.x, sum[e].x), sum[e].y = fmaf(w, x.y, sum[e].y), sum[e].z = fmaf(w, x.z, sum[e].z), sum[e].w = fmaf(w, x.w, sum[e].w);
+        for (uint32_t a = 0; a < kAhead; ++a) {
+            const uint32_t n = first + a;
+            w[a] = n < parts ? weight[i][n] : -1.0f;
+            if (w[a] < 0.0f) continue;
+            const float4* const from = n < shared_parts ? reinterpret_cast<const float4*>(p.parts) + (part_of(n) * (kHeadDim / 4) + column) * kRowsM + row
+                                                        : reinterpret_cast<const float4*>(p.own_parts + (place * p.chunks + n - shared_parts) * kHeadDim) + column;
+            const uint32_t stride = n < shared_parts ? 32 * kRowsM : 32;
+#pragma unroll
+            for (uint32_t e = 0; e < kEach; ++e) v[a][e] = from[e * stride];
         }
-    };
-    for (uint32_t n = 0; n < parts; ++n) {
-        const uint64_t part = part_of(n);
-        add(stats[part * kRowsM + row], reinterpret_cast<const float4*>(p.parts) + (part * (kHeadDim / 4) + column) * kRowsM + row, kRowsM);
+#pragma unroll
+        for (uint32_t a = 0; a < kAhead; ++a) {
+            if (w[a] < 0.0f) continue;
+#pragma unroll
+            for (uint32_t e = 0; e < kEach; ++e) {
+                sum[e].x = fmaf(w[a], v[a][e].x, sum[e].x), sum[e].y = fmaf(w[a], v[a][e].y, sum[e].y);
+                sum[e].z = fmaf(w[a], v[a][e].z, sum[e].z), sum[e].w = fmaf(w[a], v[a][e].w, sum[e].w);
+            }
+        }
     }
-    add(own, reinterpret_cast<const float4*>(p.a.own_sums + place * kHeadDim) + column, 1);
-    const float inverse = 1.0f / all;
+    const float all = total[i], inverse = 1.0f / all;
 #pragma unroll
     for (uint32_t e = 0; e < kEach; ++e) {
         const __nv_bfloat162 a = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum[e].x * inverse, all == 0.0f ? 0.0f : sum[e].y * inverse);
-        const __nv_bfloat162 b = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum[e].z * inverse, all == 0.0f ? 0.0f : sum[e].w * inverse);
-        reinterpret_cast<uint2*>(p.a.output + place * kHeadDim)[column + e * 32] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        const __nv_bfloat162 c = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum[e].z * inverse, all == 0.0f ? 0.0f : sum[e].w * inverse);
+        reinterpret_cast<uint2*>(p.a.output + place * kHeadDim)[column + e * 32] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
     }
 }
 
 // What the plan's scratch holds, in bytes from its start.
 struct Layout {
-    uint64_t own_sums, own_stats, parts, max_items, bytes;
+    uint64_t own_parts, own_stats, parts, bytes;
+    uint32_t max_items, tiles, chunks;
 };
 Layout layout_of(uint32_t query_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t rows, uint32_t max_new, uint32_t sm_count) {
-    const uint64_t spans = launch_spans(sm_count), columns = query_columns(query_heads, kv_heads, max_new), outputs = static_cast<uint64_t>(rows) * query_heads;
-    const uint64_t pairs = kv_heads * ((static_cast<uint64_t>(rows) * (query_heads / kv_heads) + kRowsM - 1) / kRowsM), streams = head_dim == 128 ? 2 : 1;
-    Layout l;
     auto aligned = [](uint64_t x) { return (x + 255) / 256 * 256; };
-    l.own_sums = aligned(kCounterBytes + spans * sizeof(JoinRecord) + 2 * spans * columns * (head_dim + 2) * sizeof(float));   // (behind the paged attention's)
-    l.own_stats = aligned(l.own_sums + outputs * head_dim * sizeof(float));
-    l.parts = aligned(l.own_stats + outputs * sizeof(float2));
-    l.max_items = pairs > kRounds * static_cast<uint64_t>(sm_count) ? pairs : kRounds * static_cast<uint64_t>(sm_count);
+    const uint64_t outputs = static_cast<uint64_t>(rows) * query_heads, streams = head_dim == 128 ? 2 : 1;
+    Layout l;
+    l.tiles = static_cast<uint32_t>((static_cast<uint64_t>(rows) * (query_heads / kv_heads) + kRowsM - 1) / kRowsM);
+    const uint64_t pairs = static_cast<uint64_t>(kv_heads) * l.tiles, most = kRounds * static_cast<uint64_t>(sm_count);   // (of queries and heads; below 2^30)
+    l.max_items = static_cast<uint32_t>(pairs > most ? pairs : most);
+    // The sequences' own tokens in as many chunks as give an SM about eight CTAs.
+    const uint64_t sequences = (rows + max_new - 1) / max_new, chunks = 8 * static_cast<uint64_t>(sm_count) / (sequences * kv_heads);
+    l.chunks = static_cast<uint32_t>(chunks < 1 ? 1 : chunks < kMaxChunks ? chunks : kMaxChunks);
+    l.own_parts = kCounterBytes;
+    l.own_stats = aligned(l.own_parts + outputs * l.chunks * head_dim * sizeof(float));
+    l.parts = aligned(l.own_stats + outputs * l.chunks * sizeof(float2));
     l.bytes = l.parts + l.max_items * streams * kRowsM * (head_dim + 2) * sizeof(float);
     return l;
 }
@@ -517,21 +813,37 @@ bool check_shared(int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm100
     return !full || inspect_device_ranges(d, ranges, count - 1, failure);
 }
 
+template <uint32_t kHeadDim, uint32_t kM>
+void launch_own(cudaStream_t stream, const __nv_bfloat16* keys, const __nv_bfloat16* values, const PrefixParams& p) {
+    launch_dependent(stream, own_attention_kernel<kHeadDim, kM>, p.a.sequences * p.a.kv_heads * p.chunks, kOwnThreads, OwnShape<kHeadDim, kM>::kSmem, keys, values, p);
+}
+
 template <uint32_t kHeadDim>
-void launch_prefix(cudaStream_t stream, const CUtensorMap& keys, const CUtensorMap& values, const PrefixParams& p, uint32_t sm_count, uint32_t columns) {
+void launch_prefix(cudaStream_t stream, const CUtensorMap& map_keys, const CUtensorMap& map_values, const __nv_bfloat16* keys, const __nv_bfloat16* values, const PrefixParams& p,
+                   uint32_t sm_count) {
     using S = PrefixShape<kHeadDim>;
-    launch_dependent(stream, prefix_attention_kernel<kHeadDim>, sm_count, S::kThreads, S::kSmem, keys, values, p);
-    launch_own_attention(stream, kHeadDim, columns, keys, values, p.a);
+    launch_dependent(stream, prefix_attention_kernel<kHeadDim>, sm_count, S::kThreads, S::kSmem, map_keys, map_values, p);
+    const uint32_t queries = p.a.query_heads / p.a.kv_heads * p.a.max_new;
+    (queries <= 16 ? launch_own<kHeadDim, 1> : queries <= 32 ? launch_own<kHeadDim, 2> : launch_own<kHeadDim, 4>)(stream, keys, values, p);
     launch_dependent(stream, prefix_merge_kernel<kHeadDim>, p.a.kv_heads * p.tiles * (kRowsM / kMergeQueries), kMergeThreads, 0, p, sm_count);
-    count_launch(2);
+    count_launch(3);
+}
+
+template <uint32_t kHeadDim>
+cudaError_t configure() {
+    constexpr cudaFuncAttribute kSmem = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    cudaError_t e = cudaFuncSetAttribute(prefix_attention_kernel<kHeadDim>, kSmem, PrefixShape<kHeadDim>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(own_attention_kernel<kHeadDim, 1>, kSmem, OwnShape<kHeadDim, 1>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(own_attention_kernel<kHeadDim, 2>, kSmem, OwnShape<kHeadDim, 2>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(own_attention_kernel<kHeadDim, 4>, kSmem, OwnShape<kHeadDim, 4>::kSmem);
+    return e;
 }
 
 }  // namespace
 
 cudaError_t shared_prefix_configure_device() {
-    constexpr cudaFuncAttribute kSmem = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    const cudaError_t e = cudaFuncSetAttribute(prefix_attention_kernel<128>, kSmem, PrefixShape<128>::kSmem);
-    return e == cudaSuccess ? cudaFuncSetAttribute(prefix_attention_kernel<256>, kSmem, PrefixShape<256>::kSmem) : e;
+    const cudaError_t e = configure<128>();
+    return e == cudaSuccess ? configure<256>() : e;
 }
 
 }  // namespace augur_sm100
@@ -562,21 +874,20 @@ extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_shared_pr
     const Layout l = layout_of(a->query_heads, kv_heads, head_dim, a->batch.rows, a->max_new_tokens, plan->sm_count);
     PrefixParams p{};
     p.a = attention_params(plan, a);
-    p.a.prefix_tokens = reinterpret_cast<const int32_t*>(a->prefix_tokens);
-    p.a.prefix_pages = static_cast<uint32_t>(a->prefix_pages_len_bytes / 4);
-    p.a.own_sums = reinterpret_cast<float*>(plan->scratch + l.own_sums);
-    p.a.own_stats = reinterpret_cast<float2*>(plan->scratch + l.own_stats);
     p.prefix_table = reinterpret_cast<const int32_t*>(a->prefix_pages);
+    p.prefix_tokens = reinterpret_cast<const int32_t*>(a->prefix_tokens);
+    p.prefix_pages = static_cast<uint32_t>(a->prefix_pages_len_bytes / 4);
+    p.own_parts = reinterpret_cast<float*>(plan->scratch + l.own_parts);
+    p.own_stats = reinterpret_cast<float2*>(plan->scratch + l.own_stats);
     p.parts = reinterpret_cast<float*>(plan->scratch + l.parts);
-    p.max_items = l.max_items;
-    p.tiles = static_cast<uint32_t>((static_cast<uint64_t>(a->batch.rows) * (a->query_heads / kv_heads) + kRowsM - 1) / kRowsM);
+    p.max_items = l.max_items, p.tiles = l.tiles, p.chunks = l.chunks;
     const uint64_t cache_rows = static_cast<uint64_t>(a->layer.pages) * kv_heads * a->layer.page_tokens;
     CUtensorMap keys, values;
     if (!make_code_map(&keys, a->layer.keys, cache_rows, head_dim * 4, box) || !make_code_map(&values, a->layer.values, cache_rows, head_dim * 4, box)) {
         return make_result(AUGUR_CUDA_STATUS_RUNTIME_FAILURE);
     }
-    const uint32_t columns = query_columns(a->query_heads, kv_heads, a->max_new_tokens);
-    if (head_dim == 256) launch_prefix<256>(s->stream, keys, values, p, plan->sm_count, columns);
-    else launch_prefix<128>(s->stream, keys, values, p, plan->sm_count, columns);
+    const auto* const key_data = reinterpret_cast<const __nv_bfloat16*>(a->layer.keys);
+    const auto* const value_data = reinterpret_cast<const __nv_bfloat16*>(a->layer.values);
+    (head_dim == 256 ? launch_prefix<256> : launch_prefix<128>)(s->stream, keys, values, key_data, value_data, p, plan->sm_count);
     return submitted();
 }
