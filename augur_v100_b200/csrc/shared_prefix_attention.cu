@@ -25,8 +25,7 @@ static_assert(sizeof(augur_cuda_nvfp4_sm100_shared_prefix_attention_args_v1) == 
 
 constexpr uint32_t kRowsM = 128;               // queries of a CTA
 constexpr uint32_t kRounds = 3;                // a device's worth of CTAs, at most so many times, where the prefix is split for it
-constexpr uint32_t kMaxSplit = 512;             // of the prefix, and of a sequence's own tokens
-constexpr uint32_t kMaxChunks = 32;
+constexpr uint32_t kMaxSplit = 256, kMaxChunks = 32;   // of the prefix, and of a sequence's own tokens
 constexpr uint32_t kInfoRing = 8;
 constexpr uint32_t kStatusPrefixLoad = 0x421, kStatusPrefixMma = 0x422, kStatusPrefixScores = 0x423, kStatusPrefixQuery = 0x424, kStatusPrefixProduct = 0x425, kStatusPrefixInfo = 0x426;
 
@@ -52,7 +51,7 @@ __device__ __forceinline__ uint32_t shared_tokens(const PrefixParams& p) {
 template <uint32_t kHeadDim>
 struct PrefixShape {
     static constexpr uint32_t kChunks = kHeadDim / 64, kStreams = kHeadDim == 128 ? 2 : 1;
-    static constexpr uint32_t kThreads = 128 + 128 * kStreams;   // warp 0 loads keys, 1 MMA, 2 queries, 3 values, then the softmax
+    static constexpr uint32_t kThreads = 128 + 128 * kStreams;   // warp 0 loads keys, 1 MMA, 3 values, then the softmax
     static constexpr uint32_t kQueryBytes = kRowsM * kHeadDim * 2, kSlots = (224 * 1024 - kQueryBytes) / kSlotBytes;
     // A ring each for the keys and the values, so that two warps deal out the copies: one alone took 80 cycles a copy, and pages of 16 tokens are eight copies a slot.
     static constexpr uint32_t kValueSlots = (kSlots / 2 + 1) / 2 * 2, kKeySlots = kSlots - kValueSlots;   // (pairs of value slots are one operand)
@@ -71,13 +70,13 @@ static_assert(sizeof(PrefixState) <= 1024, "the state's room");
 // another, so that the keys come from L2 for all but the first.
 struct Items {
     uint32_t key_tiles, split, tokens;
-    uint64_t count;
-    __device__ __forceinline__ void locate(const PrefixParams& p, uint64_t item, uint32_t* head, uint32_t* tile, uint32_t* first, uint32_t* last) const {
-        const uint64_t rest = item / p.tiles;
-        *tile = static_cast<uint32_t>(item - rest * p.tiles);
-        *head = static_cast<uint32_t>(rest / split);
-        const uint32_t part = static_cast<uint32_t>(rest - static_cast<uint64_t>(*head) * split);
-        *first = static_cast<uint32_t>(static_cast<uint64_t>(part) * key_tiles / split), *last = static_cast<uint32_t>(static_cast<uint64_t>(part + 1) * key_tiles / split);
+    uint32_t count;
+    __device__ __forceinline__ void locate(const PrefixParams& p, uint32_t item, uint32_t* head, uint32_t* tile, uint32_t* first, uint32_t* last) const {
+        const uint32_t rest = item / p.tiles;
+        *tile = item - rest * p.tiles;
+        *head = rest / split;
+        const uint32_t part = rest - *head * split;
+        *first = part * key_tiles / split, *last = (part + 1) * key_tiles / split;   // (below 2^9 * 2^17)
     }
 };
 // The split that a simple model takes for quickest: rounds of items, each its tiles and four for beginning and end, and a 32nd of a tile for every part to
@@ -86,12 +85,13 @@ __device__ __forceinline__ Items items_of(const PrefixParams& p, uint32_t ctas) 
     Items x;
     x.tokens = shared_tokens(p);
     x.key_tiles = (x.tokens + kTile - 1) / kTile;
-    const uint64_t pairs = static_cast<uint64_t>(p.a.kv_heads) * p.tiles, room = p.max_items / pairs;
-    uint32_t most = x.key_tiles < room ? x.key_tiles : static_cast<uint32_t>(room);
+    const uint32_t pairs = p.a.kv_heads * p.tiles, room = p.max_items / pairs;
+    uint32_t most = x.key_tiles < room ? x.key_tiles : room;
     most = most < kMaxSplit ? most : kMaxSplit;
     uint64_t best = UINT64_MAX;
     for (uint32_t split = 1 + threadIdx.x % 32; split <= most; split += 32) {
-        const uint64_t items = pairs * split, cost = (items + ctas - 1) / ctas * ((x.key_tiles + split - 1) / split + 4) * 32 + items, key = cost << 16 | split;
+        const uint32_t items = pairs * split;   // at most max_items
+        const uint64_t cost = static_cast<uint64_t>((items + ctas - 1) / ctas) * ((x.key_tiles + split - 1) / split + 4) * 32 + items, key = cost << 16 | split;
         if (key < best) best = key;
     }
 #pragma unroll
@@ -148,7 +148,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
         for (uint32_t s = 0; s < S::kSlots; ++s) mbar_init(full + 8 * s, 1), mbar_init(empty + 8 * s, 1);
         for (uint32_t b = 0; b < 2; ++b) mbar_init(scores_full + 8 * b, 1), mbar_init(weights_full + 8 * b, 4), mbar_init(products + 8 * b, 1);
         for (uint32_t i = 0; i < kInfoRing; ++i) mbar_init(info_full + 8 * i, 1);
-        mbar_init(query_full, 1), mbar_init(query_empty, 1);
+        mbar_init(query_full, 4 * S::kStreams), mbar_init(query_empty, 1);
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_keys) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_values) : "memory");
         for (uint32_t i = 0; i < 1 + 12; ++i) st->abort[i] = 0;
@@ -173,8 +173,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
         ends_within |= to > from && static_cast<int64_t>(min(p.a.lengths[b], room)) - to + from + 1 < static_cast<int64_t>(items.tokens);
     }
     ends_within = __syncthreads_or(ends_within);
-    const uint32_t tmem = st->tmem, group = p.a.query_heads / p.a.kv_heads;
-    const uint32_t all_queries = p.a.rows * group;   // of a key-value head; below 2^26
+    const uint32_t tmem = st->tmem, group = p.a.query_heads / p.a.kv_heads, all_queries = p.a.rows * group;   // (of a key-value head; below 2^26)
 
     if (warp == 0 || warp == 3) {
         // ---------------- pages: warp 0 the keys, warp 3 the values ----------------
@@ -184,7 +183,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
         const uint32_t first_slot = warp == 0 ? 0 : S::kKeySlots, end_slot = warp == 0 ? S::kKeySlots : S::kSlots;
         uint32_t slot = first_slot, phase = 1, count = 0;
         bool alive = true;
-        for (uint64_t item = blockIdx.x; alive && item < items.count; item += gridDim.x) {
+        for (uint32_t item = blockIdx.x; alive && item < items.count; item += gridDim.x) {
             uint32_t head, tile, first, last;
             items.locate(p, item, &head, &tile, &first, &last);
             auto page_of = [&](uint32_t t) {
@@ -233,7 +232,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
             ++scores;
             return true;
         };
-        for (uint64_t item = blockIdx.x; alive && item < items.count; item += gridDim.x, ++round) {
+        for (uint32_t item = blockIdx.x; alive && item < items.count; item += gridDim.x, ++round) {
             uint32_t head, tile, first, last;
             items.locate(p, item, &head, &tile, &first, &last);
             if (!warp_look_wait(query_full, round & 1, abort_flag, status, kStatusPrefixMma)) break;
@@ -264,38 +263,40 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
                 ++done;
             }
         }
-    } else if (warp == 2) {
-        // ---------------- queries of an item, in the 128-byte swizzle of the operand; past the last they are zero ----------------
-        constexpr uint32_t kPieces = kHeadDim / 8;   // of 16 bytes
-        uint32_t round = 0;
-        for (uint64_t item = blockIdx.x; item < items.count; item += gridDim.x, ++round) {
-            uint32_t head, tile, first, last;
-            items.locate(p, item, &head, &tile, &first, &last);
-            if (!warp_look_wait(query_empty, (round & 1) ^ 1, abort_flag, status, kStatusPrefixQuery)) break;
-            for (uint32_t i = lane; i < kRowsM * kPieces; i += 32) {
-                const uint32_t row = i / kPieces, piece = i % kPieces, query = tile * kRowsM + row, token = query / group;
-                const bool live = query < all_queries;
-                const __nv_bfloat16* const at = p.a.query + (static_cast<uint64_t>(live ? token : 0) * p.a.query_heads + head * group + (live ? query - token * group : 0)) * kHeadDim + piece * 8;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                             ::"r"(smem_u32(query_smem) + (piece >> 3) * kSlotBytes + row * 128 + (((piece & 7) ^ (row & 7)) << 4)), "l"(at), "r"(live ? 16 : 0)
-                             : "memory");
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(query_full);
-        }
-    } else {
-        // ---------------- softmax: a query a thread ----------------
+    } else if (warp >= 4) {
+        // ---------------- queries of an item, then the softmax: a query a thread ----------------
         const uint32_t stream = (warp - 4) / 4, thread = threadIdx.x & 127, lanes = ((warp & 3) * 32) << 16;
         const uint32_t box_shift = p.a.page_shift < 6 ? p.a.page_shift : 6, all_boxes = (1u << (kTile >> box_shift)) - 1;
         const uint32_t out = tmem + S::kOutAt + stream * (S::kStreams == 2 ? kHeadDim : 0) + lanes;
         const float scale = p.a.scale_log2;
-        uint32_t count = 0;   // tiles of this CTA
+        uint32_t count = 0, round = 0;   // tiles and items of this CTA
         bool alive = true;
-        for (uint64_t item = blockIdx.x; alive && item < items.count; item += gridDim.x) {
+        for (uint32_t item = blockIdx.x; alive && item < items.count; item += gridDim.x, ++round) {
             uint32_t head, tile, first, last;
             items.locate(p, item, &head, &tile, &first, &last);
+            // The item's queries in the 128-byte swizzle of the operand, once the products of the item before are through; past the last they are zero. (All of these warps: by
+            // one alone they were there after 5.4 us.)
+            if (!warp_look_wait(query_empty, (round & 1) ^ 1, abort_flag, status, kStatusPrefixQuery)) break;
+            {
+                // a lane's piece of every (kWarps * 32 / kPieces)-th row; its token and the head among those that share the key-value head go along
+                constexpr uint32_t kPieces = kHeadDim / 8, kWarps = 4 * S::kStreams, kStep = kWarps * 32 / kPieces;
+                const uint32_t piece = lane % kPieces, row0 = ((warp - 4) * 32 + lane) / kPieces, query0 = tile * kRowsM + row0;
+                uint32_t token = query0 / group, within = query0 - token * group;
+                const uint32_t to = smem_u32(query_smem) + (piece >> 3) * kSlotBytes;
+#pragma unroll 4
+                for (uint32_t row = row0; row < kRowsM; row += kStep, within += kStep) {
+                    while (within >= group) within -= group, ++token;
+                    const bool live = token < p.a.rows;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                                 ::"r"(to + row * 128 + (((piece & 7) ^ (row & 7)) << 4)),
+                                 "l"(p.a.query + (static_cast<uint64_t>(live ? token : 0) * p.a.query_heads + head * group + within) * kHeadDim + piece * 8), "r"(live ? 16 : 0)
+                                 : "memory");
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(query_full);
+            }
             // How many tokens of the prefix this row sees.
             uint32_t limit = items.tokens;
             if (ends_within) {
@@ -411,7 +412,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
             }
             if (!alive) break;
             // ---- the item's part ----
-            const uint64_t part = item * S::kStreams + stream;
+            const uint64_t part = static_cast<uint64_t>(item) * S::kStreams + stream;
             if (started) {
                 const uint32_t final = count - 1 - (S::kStreams == 2 && ((count - 1) & 1) != stream ? 1 : 0);   // the stream's last tile
                 if (!warp_look_wait(products + 8 * (final & 1), final >> 1 & 1, abort_flag, status, kStatusPrefixProduct)) break;
@@ -424,7 +425,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
                     tc_wait_ld();
 #pragma unroll
                     for (uint32_t i = 0; i < 32; i += 4) {
-                        to[(c + i) / 4 * kRowsM] = make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+                        if (tile * kRowsM + thread < all_queries) to[(c + i) / 4 * kRowsM] = make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
                     }
                 }
                 tc_fence_before();
@@ -678,100 +679,104 @@ __global__ void __launch_bounds__(kOwnThreads) own_attention_kernel(const __nv_b
     }
 }
 
-// Joins the parts of the prefix and of the rows' own tokens, in their order. A CTA takes eight queries of an item's 128, a warp the weights of one of them.
-constexpr uint32_t kMergeThreads = 256, kMergeQueries = 8;
+// Joins the parts of the prefix and of the rows' own tokens, in their order: a float4 a thread, and a warp (some warps) the weights of one of a CTA's queries.
+constexpr uint32_t kMergeThreads = 256;
+template <uint32_t kHeadDim>
+constexpr uint32_t kMergeQueries = kMergeThreads / (kHeadDim / 4);
 template <uint32_t kHeadDim>
 __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const __grid_constant__ PrefixParams p, uint32_t ctas) {
     using S = PrefixShape<kHeadDim>;
-    constexpr uint32_t kEach = kHeadDim / 4 / 32, kAhead = 4;   // float4 of a thread, parts under way at once
-    constexpr uint32_t kMost = kMaxSplit * S::kStreams + kMaxChunks;
-    __shared__ float weight[kMergeQueries][kMost + 4], total[kMergeQueries];
-    __shared__ uint32_t live[kMergeQueries];
+    constexpr uint32_t kQueries = kMergeQueries<kHeadDim>, kAhead = 8, kSlices = kRowsM / kQueries;
+    constexpr uint32_t kMost = (kMaxSplit * S::kStreams + kMaxChunks + kAhead - 1) / kAhead * kAhead;
+    __shared__ float2 stat[kQueries][kMost];   // reference maximum and denominator of a part; then, of those that count, the weight and the part's number
+    __shared__ float total[kQueries];
+    __shared__ uint32_t live[kQueries], count[kQueries];
+    if (threadIdx.x < kQueries) live[threadIdx.x] = 0;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Items items = items_of(p, ctas);
     const uint32_t group = p.a.query_heads / p.a.kv_heads, all_queries = p.a.rows * group, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    constexpr uint32_t kSlices = kRowsM / kMergeQueries;
     const uint32_t slice = blockIdx.x % kSlices, tile = blockIdx.x / kSlices % p.tiles, head = blockIdx.x / kSlices / p.tiles;
-    const uint32_t query0 = tile * kRowsM + slice * kMergeQueries;
+    const uint32_t query0 = tile * kRowsM + slice * kQueries;
     if (query0 >= all_queries) return;
-    const uint32_t shared_parts = items.key_tiles ? items.split * S::kStreams : 0, parts = shared_parts + p.chunks;
-    auto part_of = [&](uint32_t n) { return ((static_cast<uint64_t>(head) * items.split + n / S::kStreams) * p.tiles + tile) * S::kStreams + n % S::kStreams; };
+    const uint32_t shared_parts = items.key_tiles ? items.split * S::kStreams : 0, parts = shared_parts + p.chunks, padded = (parts + kAhead - 1) / kAhead * kAhead;
+    // part n of the prefix: item (head, n / streams, tile), stream n % streams
+    const uint64_t first_part = (static_cast<uint64_t>(head) * items.split * p.tiles + tile) * S::kStreams, next_item = static_cast<uint64_t>(p.tiles) * S::kStreams;
+    auto part_of = [&](uint32_t n) { return first_part + n / S::kStreams * next_item + n % S::kStreams; };
     auto place_of = [&](uint32_t query) { return static_cast<uint64_t>(query / group) * p.a.query_heads + head * group + query % group; };
-    // The rows that belong to a sequence.
-    if (threadIdx.x < kMergeQueries) live[threadIdx.x] = 0;
     __syncthreads();
+    // The rows that belong to a sequence; meanwhile the parts' statistics.
+    const float2* const stats = reinterpret_cast<const float2*>(p.parts + static_cast<uint64_t>(p.max_items) * S::kStreams * kRowsM * kHeadDim);
+    for (uint32_t i = threadIdx.x; i < kQueries * padded; i += kMergeThreads) {
+        const uint32_t n = i / kQueries, query = i % kQueries;
+        float2 x = make_float2(-INFINITY, 0.0f);
+        if (n < shared_parts) x = stats[part_of(n) * kRowsM + slice * kQueries + query];
+        else if (n < parts && query0 + query < all_queries) x = p.own_stats[place_of(query0 + query) * p.chunks + n - shared_parts];
+        stat[query][n] = x;
+    }
     for (uint32_t b = threadIdx.x; b < p.a.sequences; b += kMergeThreads) {
         const int32_t from = p.a.token_starts[b], to = p.a.token_starts[b + 1];
         if (from < 0 || to > static_cast<int32_t>(p.a.rows) || to < from || to - from > static_cast<int32_t>(p.a.max_new)) continue;
-        for (uint32_t i = 0; i < kMergeQueries; ++i) {
+        for (uint32_t i = 0; i < kQueries; ++i) {
             const int32_t row = static_cast<int32_t>((query0 + i) / group);
             if (from <= row && row < to) live[i] = 1;
         }
     }
     __syncthreads();
-    // A warp's query: the weights 2^(reference - largest reference) of its parts, and the denominator. Parts of which it sees nothing are passed over (-1).
-    // All others count, with a weight of zero too: zero times a NaN is one.
-    if (live[warp] && query0 + warp < all_queries) {
-        const float2* const stats = reinterpret_cast<const float2*>(p.parts + static_cast<uint64_t>(p.max_items) * S::kStreams * kRowsM * kHeadDim);
-        const uint64_t own = place_of(query0 + warp) * p.chunks;
-        auto stat_of = [&](uint32_t n) { return n < shared_parts ? stats[part_of(n) * kRowsM + slice * kMergeQueries + warp] : p.own_stats[own + n - shared_parts]; };
+    // A query's weights 2^(reference - largest reference), and its denominator. Parts of which it sees nothing are passed over. All others count, with a
+    // weight of zero too: zero times a NaN is one.
+    if (warp < kQueries) {
         float most = -INFINITY, all = 0.0f;
-        for (uint32_t n = lane; n < parts; n += 32) {
-            const float x = stat_of(n).x;
-            weight[warp][n] = x;
-            most = fmaxf(most, x);
-        }
+        for (uint32_t n = lane; n < parts; n += 32) most = fmaxf(most, stat[warp][n].x);
 #pragma unroll
         for (uint32_t step = 16; step; step /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, step));
-        for (uint32_t n = lane; n < parts; n += 32) {
-            const float x = weight[warp][n], w = x == -INFINITY ? -1.0f : exp2_fast(x - most);
-            weight[warp][n] = w;
-            if (!(w < 0.0f)) all = fmaf(w, stat_of(n).y, all);
+        uint32_t kept = 0;
+        for (uint32_t first = 0; first < padded; first += 32) {
+            const uint32_t n = first + lane;
+            const float2 x = n < parts ? stat[warp][n] : make_float2(-INFINITY, 0.0f);
+            const uint32_t counts = __ballot_sync(0xffffffffu, x.x != -INFINITY);
+            if (x.x != -INFINITY) {
+                const float w = exp2_fast(x.x - most);
+                all = fmaf(w, x.y, all);
+                stat[warp][kept + __popc(counts & ((1u << lane) - 1))] = make_float2(w, __uint_as_float(n));   // (at or before its own place, which all lanes have read)
+            }
+            kept += __popc(counts);
+            __syncwarp();
         }
 #pragma unroll
         for (uint32_t step = 16; step; step /= 2) all += __shfl_xor_sync(0xffffffffu, all, step);
-        if (lane == 0) total[warp] = all;
+        if (lane == 0) total[warp] = all, count[warp] = kept;
     }
     __syncthreads();
-    // lanes: eight queries, four neighbouring float4 of each
-    const uint32_t i = threadIdx.x % kMergeQueries, query = query0 + i, column = threadIdx.x / kMergeQueries, row = slice * kMergeQueries + i;
-    if (!live[i] || query >= all_queries) return;
+    const uint32_t i = threadIdx.x % kQueries, query = query0 + i, column = threadIdx.x / kQueries, row = slice * kQueries + i;
+    if (query >= all_queries || !live[i]) return;
     const uint64_t place = place_of(query);
-    float4 sum[kEach];
-#pragma unroll
-    for (uint32_t e = 0; e < kEach; ++e) sum[e] = make_float4(0, 0, 0, 0);
-    for (uint32_t first = 0; first < parts; first += kAhead) {
-        float4 v[kAhead][kEach];
+    const float4* const shared_from = reinterpret_cast<const float4*>(p.parts) + column * kRowsM + row;
+    const float4* const own_from = reinterpret_cast<const float4*>(p.own_parts + place * p.chunks * kHeadDim) + column;
+    const uint32_t kept = count[i];
+    float4 sum = make_float4(0, 0, 0, 0);
+    for (uint32_t first = 0; first < kept; first += kAhead) {
+        float4 v[kAhead];
         float w[kAhead];
 #pragma unroll
         for (uint32_t a = 0; a < kAhead; ++a) {
-            const uint32_t n = first + a;
-            w[a] = n < parts ? weight[i][n] : -1.0f;
-            if (w[a] < 0.0f) continue;
-            const float4* const from = n < shared_parts ? reinterpret_cast<const float4*>(p.parts) + (part_of(n) * (kHeadDim / 4) + column) * kRowsM + row
-                                                        : reinterpret_cast<const float4*>(p.own_parts + (place * p.chunks + n - shared_parts) * kHeadDim) + column;
-            const uint32_t stride = n < shared_parts ? 32 * kRowsM : 32;
-#pragma unroll
-            for (uint32_t e = 0; e < kEach; ++e) v[a][e] = from[e * stride];
+            v[a] = make_float4(0, 0, 0, 0), w[a] = 0.0f;
+            if (first + a < kept) {
+                const float2 x = stat[i][first + a];
+                const uint32_t n = __float_as_uint(x.y);
+                w[a] = x.x;
+                v[a] = n < shared_parts ? shared_from[part_of(n) * (kHeadDim / 4 * kRowsM)] : own_from[(n - shared_parts) * (kHeadDim / 4)];
+            }
         }
 #pragma unroll
         for (uint32_t a = 0; a < kAhead; ++a) {
-            if (w[a] < 0.0f) continue;
-#pragma unroll
-            for (uint32_t e = 0; e < kEach; ++e) {
-                sum[e].x = fmaf(w[a], v[a][e].x, sum[e].x), sum[e].y = fmaf(w[a], v[a][e].y, sum[e].y);
-                sum[e].z = fmaf(w[a], v[a][e].z, sum[e].z), sum[e].w = fmaf(w[a], v[a][e].w, sum[e].w);
-            }
+            sum.x = fmaf(w[a], v[a].x, sum.x), sum.y = fmaf(w[a], v[a].y, sum.y), sum.z = fmaf(w[a], v[a].z, sum.z), sum.w = fmaf(w[a], v[a].w, sum.w);
         }
     }
     const float all = total[i], inverse = 1.0f / all;
-#pragma unroll
-    for (uint32_t e = 0; e < kEach; ++e) {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum[e].x * inverse, all == 0.0f ? 0.0f : sum[e].y * inverse);
-        const __nv_bfloat162 c = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum[e].z * inverse, all == 0.0f ? 0.0f : sum[e].w * inverse);
-        reinterpret_cast<uint2*>(p.a.output + place * kHeadDim)[column + e * 32] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
-    }
+    const __nv_bfloat162 a = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum.x * inverse, all == 0.0f ? 0.0f : sum.y * inverse);
+    const __nv_bfloat162 c = __floats2bfloat162_rn(all == 0.0f ? 0.0f : sum.z * inverse, all == 0.0f ? 0.0f : sum.w * inverse);
+    reinterpret_cast<uint2*>(p.a.output + place * kHeadDim)[column] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
 }
 
 // What the plan's scratch holds, in bytes from its start.
@@ -822,10 +827,11 @@ template <uint32_t kHeadDim>
 void launch_prefix(cudaStream_t stream, const CUtensorMap& map_keys, const CUtensorMap& map_values, const __nv_bfloat16* keys, const __nv_bfloat16* values, const PrefixParams& p,
                    uint32_t sm_count) {
     using S = PrefixShape<kHeadDim>;
-    launch_dependent(stream, prefix_attention_kernel<kHeadDim>, sm_count, S::kThreads, S::kSmem, map_keys, map_values, p);
+    // The prefix behind the own tokens: its parts are the many, and still in L2 when they are joined. (The other way round the join of 64 sequences took 14 us, not NN.)
     const uint32_t queries = p.a.query_heads / p.a.kv_heads * p.a.max_new;
     (queries <= 16 ? launch_own<kHeadDim, 1> : queries <= 32 ? launch_own<kHeadDim, 2> : launch_own<kHeadDim, 4>)(stream, keys, values, p);
-    launch_dependent(stream, prefix_merge_kernel<kHeadDim>, p.a.kv_heads * p.tiles * (kRowsM / kMergeQueries), kMergeThreads, 0, p, sm_count);
+    launch_dependent(stream, prefix_attention_kernel<kHeadDim>, sm_count, S::kThreads, S::kSmem, map_keys, map_values, p);
+    launch_dependent(stream, prefix_merge_kernel<kHeadDim>, p.a.kv_heads * p.tiles * (kRowsM / kMergeQueries<kHeadDim>), kMergeThreads, 0, p, sm_count);
     count_launch(3);
 }
 
