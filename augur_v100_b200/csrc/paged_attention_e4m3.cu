@@ -15,12 +15,11 @@
 //   w = 2^(s_j + f_j - m), rounded to half precision (2^-11), in three, each in units a sixteenth of the one before it: exact. Side by side on the
 //     narrow operand, whose terms' sums are added at the end. With two the rounding (2^-9) would be as large an error as the output's own.
 // A scale is a power of two, so that a value's is part of the weight's exponent: the reference m follows the largest s_j + f_j, and the weights that enter the
-// product lie below 2^8 whatever the scales are. The denominator sums w 2^-f_j in F32, a part of it in each softmax thread. As the scales lie
-// within 2^-60..2^60, it cannot leave the range.
+// product lie below 2^8 whatever the scales are. The denominator sums w 2^-f_j in F32, a part of it in each softmax thread.
 //
 // A thread of the four softmax warps holds one key and, up to 16 at a time, the queries of S^T; it writes 16 weights' terms as three
-// 16-byte stores (W^T is MN-major: a key's row holds all queries). The reference moves only when a weight would pass 2^8; then O^T is scaled
-// down in tensor memory. Spans, parts and their join are those of the BF16 cache's kernel.
+// 16-byte stores (W^T is MN-major: a key's row holds all queries). The reference moves only when a weight would pass 2^8, which is found out while the weights are
+// formed; then O^T is scaled down in tensor memory. Spans, parts and their join are those of the BF16 cache's kernel.
 #include "paged_attention.cuh"
 
 namespace augur_sm100 {
@@ -28,8 +27,11 @@ namespace {
 
 static_assert(sizeof(augur_cuda_nvfp4_sm100_paged_attention_e4m3_args_v1) == 176, "attention ABI");
 
-// How far, in powers of two, a weight may pass 1, and how far all of them are shifted up: weights of 2^3 for the largest, 2^8 at most.
-constexpr float kRoom = 5.0f, kShift = 3.0f;
+// Weights are formed 2^kLift times too large and brought down where they become half precision: the denominator divides by the value's scale again, and wants those of
+// small scales down to 2^-30 of the largest. 2^(8 + kLift) * 2^60 and 2^-126 are 2^(30 + 60 + 60 + 8) apart at least, and as much lies between.
+constexpr float kLift = 48.0f;
+constexpr float kNoReference = 1e30f;         // where a query has seen no key yet: whatever is added, but -infinity, passes
+constexpr float kRoom = 8.0f;                  // how far, in powers of two, a weight may pass 1, which was the largest when the reference moved
 constexpr uint32_t kTileInfos = 16;            // tiles that the loader is ahead of the softmax at most (a ring of keys and three more), rounded up
 constexpr uint32_t kWeightAtom = kTile * 32;   // 32 columns of a tile's weights
 
@@ -41,6 +43,7 @@ struct StateE4m3 : BatchState {
     uint32_t needs[2];                 // a byte per softmax warp: a reference has to move
     uint32_t info[kTileInfos];         // of a tile: pages that are there, a bit per box
     float reference[kMaxQueries], factor[kMaxQueries], total[kMaxQueries];
+    alignas(16) float minus[kMaxQueries];            // the references with the sign changed, kNoReference for -infinity
     alignas(16) float query_scale[2][kMaxQueries];   // (read four at a time)
     float4 wide[kMaxQueries];          // by softmax warp: the largest score, or the sum of the weights
     int32_t limit[kMaxQueries];        // keys that a query sees
@@ -90,6 +93,17 @@ __device__ __forceinline__ void mma_block_e4m3(uint32_t d, uint32_t a, uint32_t 
         : "memory");
 }
 
+template <uint32_t kCount>
+__device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t* v) {
+    if constexpr (kCount == 16) {
+        store_columns16(taddr, v);
+    } else {
+        static_assert(kCount == 8, "columns at a time");
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
+                     ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(taddr)
+                     : "memory");
+    }
+}
 __device__ __forceinline__ uint32_t half2_of(float low, float high) {
     uint32_t x;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(high), "f"(low));
@@ -339,10 +353,14 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
         uint32_t tile = 0, meetings = 0, pair = 0;
         JoinRecord record{};
         // The four warps meet (a bounded wait, where a named barrier would hang on a warp that gave up).
-        auto meet = [&]() {
+        auto come = [&]() {
             __syncwarp();
             if (lane == 0) mbar_arrive(group_bar);
-            return warp_look_wait(group_bar, meetings++ & 1, abort_flag, status, kStatusGroup);
+        };
+        auto all_came = [&]() { return warp_look_wait(group_bar, meetings++ & 1, abort_flag, status, kStatusGroup); };
+        auto meet = [&]() {
+            come();
+            return all_came();
         };
         Walk walk;
         walk.open(st, p, from, to);
@@ -378,156 +396,196 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                 const uint32_t bytes = my_key ? st->scales[at][thread] : 0x7f7fu, key_byte = scale_byte(bytes & 0xff), value_byte = scale_byte(bytes >> 8);
                 const float key_scale = (bytes & 0xff) == 0xff ? __uint_as_float(0x7fc00000u) : __uint_as_float(key_byte << 23) * p.scale_log2;
                 const float value_power = bytes >> 8 == 0xff ? __uint_as_float(0x7fc00000u) : static_cast<float>(static_cast<int32_t>(value_byte) - 127);
-                const float value_inverse = __uint_as_float((254 - value_byte) << 23);
-                // 16 queries' s + f of this thread's key. Every step below goes through them again from tensor memory in a rolled loop (up to 16 queries' stay in registers).
+                const float value_inverse = __uint_as_float((254 - 60 - value_byte) << 23);   // 2^-60 of it, which the total makes up for
+                // 16 queries' s + f of this thread's key. More than 16 queries are gone through 16 at a time, in rolled loops, from tensor memory each time; up to 16
+                // queries' stay in registers.
                 float s[kBlock];
                 auto scores = [&](uint32_t c0) {
-                    if (kOneBlock && c0 != 0) return;   // (there already)
-                    load_columns<kBlock>(tmem + lanes + buffer * S::kScores + c0 % kN, reinterpret_cast<uint32_t*>(s));
+                    load_columns<kBlock>(tmem + lanes + buffer * S::kScores + c0, reinterpret_cast<uint32_t*>(s));
                     float scale[kBlock];
 #pragma unroll
-                    for (uint32_t i = 0; i < kBlock; i += 4) *reinterpret_cast<float4*>(scale + i) = *reinterpret_cast<const float4*>(query_scale + c0 % kN + i);
+                    for (uint32_t i = 0; i < kBlock; i += 4) *reinterpret_cast<float4*>(scale + i) = *reinterpret_cast<const float4*>(query_scale + c0 + i);
                     tc_wait_ld();
 #pragma unroll
                     for (uint32_t i = 0; i < kBlock; ++i) s[i] = fmaf(s[i] * scale[i], key_scale, value_power);
                     if (masked) {
 #pragma unroll
-                        for (uint32_t i = 0; i < kBlock; ++i) s[i] = my_key && static_cast<int32_t>(key + thread) < st->limit[c0 % kN + i] ? s[i] : -INFINITY;
+                        for (uint32_t i = 0; i < kBlock; ++i) s[i] = my_key && static_cast<int32_t>(key + thread) < st->limit[c0 + i] ? s[i] : -INFINITY;
                     }
                 };
-                constexpr uint32_t kAgain = kOneBlock ? kN : 0;
-                bool above = key == walk.key;   // a pair's first tile sets the references
-                if (!above) {
-#pragma unroll 1
-                    for (uint32_t c = 0; c < kN; c += kBlock) {
-                        scores(c);
+                // Their weights under the references as they stand, and whether one of them would pass 2^kRoom (it is held there).
+                auto weights = [&](uint32_t c0, float (&w)[kBlock]) {
+                    bool passes = false;
 #pragma unroll
-                        for (uint32_t i = 0; i < kBlock; ++i) above |= s[i] > st->reference[c + i] + kRoom;
-                    }
-                    above = __any_sync(0xffffffffu, above);
-                    if (lane == 0) reinterpret_cast<uint8_t*>(&st->needs[buffer])[quadrant] = above;
-                    if (!meet()) {
-                        alive = false;
-                        break;
-                    }
-                    above = *const_cast<volatile uint32_t*>(&st->needs[buffer]) != 0;
-                } else {
-                    scores(0);
-                }
-                if (above) {
-                    // The references move up to the largest so far.
-#pragma unroll 1
-                    for (uint32_t c = 0; c < kN; c += kBlock) {
-                        scores(c + kAgain);
-                        float most = -INFINITY;
+                    for (uint32_t i = 0; i < kBlock; i += 4) *reinterpret_cast<float4*>(w + i) = *reinterpret_cast<const float4*>(st->minus + c0 + i);
 #pragma unroll
-                        for (uint32_t i = 0; i < kBlock; ++i) {
-                            const float x = warp_max(s[i]);
-                            if (lane == i) most = x;
-                        }
-                        if (lane < kBlock) reinterpret_cast<float*>(&st->wide[c + lane])[quadrant] = most;
+                    for (uint32_t i = 0; i < kBlock; ++i) {
+                        w[i] += s[i];
+                        passes |= w[i] > kRoom + kLift;
+                        asm("min.NaN.f32 %0, %0, %1;" : "+f"(w[i]) : "f"(kRoom + kLift));
                     }
-                    if (!meet()) {
-                        alive = false;
-                        break;
-                    }
-                    if (thread < kN) {
-                        const float old = st->reference[thread];
-                        const float4 w = st->wide[thread];
-                        const float now = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), old);
-                        st->factor[thread] = now == old ? 1.0f : exp2_fast(old - now);
-                        st->reference[thread] = now;
-                    }
-                    if (!meet()) {
-                        alive = false;
-                        break;
-                    }
-                    if (key != walk.key) {
-                        if (!warp_look_wait(weights_empty + 8 * (buffer ^ 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) {
-                            alive = false;
-                            break;
-                        }
-                        tc_fence_after();
-#pragma unroll 1
-                        for (uint32_t h = 0; h < S::kChunks; ++h) {
-#pragma unroll 1
-                            for (uint32_t c = 0; c < S::kTerms; c += 16) {
-                                uint32_t v[16];
-                                load_columns<16>(tmem_out + lanes + h * S::kTerms + c, v);
-                                tc_wait_ld();
-#pragma unroll
-                                for (uint32_t i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * st->factor[kN < 16 ? i % kN : c % kN + i]);
-                                store_columns16(tmem_out + lanes + h * S::kTerms + c, v);
-                            }
-                        }
-                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                        tc_fence_before();
-                        if constexpr (kOneBlock) {
-#pragma unroll
-                            for (uint32_t i = 0; i < kBlock; ++i) sum[i] *= st->factor[i];
-                        } else {
-#pragma unroll 1
-                            for (uint32_t c = 0; c < kN; c += 4) {
-                                float4& x = sum_smem[c / 4 * kTile + thread];
-                                x = make_float4(x.x * st->factor[c], x.y * st->factor[c + 1], x.z * st->factor[c + 2], x.w * st->factor[c + 3]);
-                            }
-                        }
-                    }
-                }
+                    return passes;
+                };
                 if (!warp_look_wait(weights_empty + 8 * buffer, (tile >> 1 & 1) ^ 1, abort_flag, status, kStatusProduct)) {
                     alive = false;
                     break;
                 }
-                // a key's row of a column's atom, and the halves of it in the 32-byte swizzle
-                uint8_t* const to_weights = weight_smem + buffer * S::kWeightBytes + thread * 32;
-                const uint32_t turned = (thread & 7) >> 2;
-                auto store = [&](uint32_t column, uint4 sixteen) { *reinterpret_cast<uint4*>(to_weights + column / 32 * kWeightAtom + ((column / 16 % 2 ^ turned) << 4)) = sixteen; };
+                if (kOneBlock) scores(0);
+                // The weights are formed and stored under the references as they stand, and stand if no warp finds one that passes 2^kRoom; else the references
+                // move and the weights are formed anew. (Asked first and formed then, a tile of eight queries took 400 cycles more, which the warps waited for one another.)
+                bool move = key == walk.key;   // a pair's first tile sets the references
+                for (bool again = false;; again = true) {
+                    if (move) {
+                        if (again) {   // the sums as they were
 #pragma unroll 1
-                for (uint32_t c = 0; c < kN; c += kBlock) {
-                    scores(c + kAgain);
-                    if constexpr (!kOneBlock) {
-                        if (key != walk.key) {
+                            for (uint32_t c = 0; c < kN; c += kBlock) {
+                                if (!kOneBlock) scores(c);
+                                float w[kBlock];
+                                weights(c, w);
 #pragma unroll
-                            for (uint32_t i = 0; i < kBlock; i += 4) *reinterpret_cast<float4*>(sum + i) = sum_smem[(c + i) / 4 * kTile + thread];
+                                for (uint32_t i = 0; i < kBlock; ++i) w[i] = exp2_fast(w[i]);
+                                if constexpr (kOneBlock) {
+#pragma unroll
+                                    for (uint32_t i = 0; i < kBlock; ++i) sum[i] = fmaf(-w[i], value_inverse, sum[i]);
+                                } else {
+#pragma unroll
+                                    for (uint32_t i = 0; i < kBlock; i += 4) {
+                                        float4& x = sum_smem[(c + i) / 4 * kTile + thread];
+                                        x = make_float4(fmaf(-w[i], value_inverse, x.x), fmaf(-w[i + 1], value_inverse, x.y), fmaf(-w[i + 2], value_inverse, x.z), fmaf(-w[i + 3], value_inverse, x.w));
+                                    }
+                                }
+                            }
+                        }
+                        // The references move up to the largest so far.
+#pragma unroll 1
+                        for (uint32_t c = 0; c < kN; c += kBlock) {
+                            if (!kOneBlock) scores(c);
+                            float most = -INFINITY;
+#pragma unroll
+                            for (uint32_t i = 0; i < kBlock; ++i) {
+                                const float x = warp_max(s[i]);
+                                if (lane == i) most = x;
+                            }
+                            if (lane < kBlock) reinterpret_cast<float*>(&st->wide[c + lane])[quadrant] = most;
+                        }
+                        if (!meet()) {
+                            alive = false;
+                            break;
+                        }
+                        if (thread < kN) {
+                            const float old = st->reference[thread];
+                            const float4 w = st->wide[thread];
+                            const float now = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), old);
+                            st->factor[thread] = now == old ? 1.0f : exp2_fast(old - now);
+                            st->reference[thread] = now;
+                            st->minus[thread] = now == -INFINITY ? kNoReference : kLift - now;
+                        }
+                        if (!meet()) {
+                            alive = false;
+                            break;
+                        }
+                        if (again) {
+                            if (!warp_look_wait(weights_empty + 8 * (buffer ^ 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) {
+                                alive = false;
+                                break;
+                            }
+                            tc_fence_after();
+#pragma unroll 1
+                            for (uint32_t c = 0; c < kN; c += kBlock) {   // 16 queries' columns (or eight), if one of them has moved
+                                float factor[kBlock];
+                                bool moved = false;
+#pragma unroll
+                                for (uint32_t i = 0; i < kBlock; ++i) factor[i] = st->factor[c + i], moved |= factor[i] != 1.0f;
+                                if (!moved) continue;
+#pragma unroll 1
+                                for (uint32_t column = c; column < S::kChunks * S::kTerms; column = column % S::kTerms + kN < 3 * kN ? column + kN : column / S::kTerms * S::kTerms + S::kTerms + c) {
+                                    uint32_t v[kBlock];
+                                    load_columns<kBlock>(tmem_out + lanes + column, v);
+                                    tc_wait_ld();
+#pragma unroll
+                                    for (uint32_t i = 0; i < kBlock; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * factor[i]);
+                                    store_columns<kBlock>(tmem_out + lanes + column, v);
+                                }
+                                if constexpr (kOneBlock) {
+#pragma unroll
+                                    for (uint32_t i = 0; i < kBlock; ++i) sum[i] *= factor[i];
+                                } else {
+#pragma unroll
+                                    for (uint32_t i = 0; i < kBlock; i += 4) {
+                                        float4& x = sum_smem[(c + i) / 4 * kTile + thread];
+                                        x = make_float4(x.x * factor[i], x.y * factor[i + 1], x.z * factor[i + 2], x.w * factor[i + 3]);
+                                    }
+                                }
+                            }
+                            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                            tc_fence_before();
+                        }
+                    }
+                    // a key's row of a column's atom, and the halves of it in the 32-byte swizzle
+                    uint8_t* const to_weights = weight_smem + buffer * S::kWeightBytes + thread * 32;
+                    const uint32_t turned = (thread & 7) >> 2;
+                    auto store = [&](uint32_t column, uint4 sixteen) { *reinterpret_cast<uint4*>(to_weights + column / 32 * kWeightAtom + ((column / 16 % 2 ^ turned) << 4)) = sixteen; };
+                    bool passes = false;
+#pragma unroll 1
+                    for (uint32_t c = 0; c < kN; c += kBlock) {
+                        if (!kOneBlock) scores(c);
+                        if constexpr (!kOneBlock) {
+                            if (key != walk.key) {
+#pragma unroll
+                                for (uint32_t i = 0; i < kBlock; i += 4) *reinterpret_cast<float4*>(sum + i) = sum_smem[(c + i) / 4 * kTile + thread];
+                            } else {
+#pragma unroll
+                                for (uint32_t i = 0; i < kBlock; ++i) sum[i] = 0.0f;
+                            }
+                        }
+                        float w[kBlock];
+                        passes |= weights(c, w);
+                        if (!move && c + kBlock == kN) {   // say so, and go on
+                            passes = __any_sync(0xffffffffu, passes);
+                            if (lane == 0) reinterpret_cast<uint8_t*>(&st->needs[buffer])[quadrant] = passes;
+                            come();
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < kBlock; ++i) w[i] = exp2_fast(w[i]);
+                        constexpr float kDown = 1.0f / (1ull << static_cast<int>(kLift));
+                        uint32_t term[3][kBlock / 4];   // four codes each
+#pragma unroll
+                        for (uint32_t i = 0; i < kBlock; i += 4) {
+                            uint16_t code[3][2];
+#pragma unroll
+                            for (uint32_t j = 0; j < 2; ++j) {
+                                uint32_t x = half2_of(w[i + 2 * j] * kDown, w[i + 2 * j + 1] * kDown);
+                                code[0][j] = codes_of(x);
+                                x = rest16(x, halves_of(code[0][j]));
+                                code[1][j] = codes_of(x);
+                                code[2][j] = codes_of(rest16(x, halves_of(code[1][j])));
+                            }
+#pragma unroll
+                            for (uint32_t t = 0; t < 3; ++t) term[t][i / 4] = code[t][0] | static_cast<uint32_t>(code[t][1]) << 16;
+                        }
+                        if constexpr (kBlock == 16) {
+#pragma unroll
+                            for (uint32_t t = 0; t < 3; ++t) store(t * kN + c, make_uint4(term[t][0], term[t][1], term[t][2], term[t][3]));
                         } else {
-#pragma unroll
-                            for (uint32_t i = 0; i < kBlock; ++i) sum[i] = 0.0f;
-                        }
-                    }
-                    float w[kBlock];
-#pragma unroll
-                    for (uint32_t i = 0; i < kBlock; ++i) w[i] = st->reference[c + i];
-#pragma unroll
-                    for (uint32_t i = 0; i < kBlock; ++i) w[i] = exp2_fast(s[i] - (w[i] == -INFINITY ? 0.0f : w[i] - kShift));
-                    uint32_t term[3][kBlock / 4];   // four codes each
-#pragma unroll
-                    for (uint32_t i = 0; i < kBlock; i += 4) {
-                        uint16_t code[3][2];
-#pragma unroll
-                        for (uint32_t j = 0; j < 2; ++j) {
-                            uint32_t x = half2_of(w[i + 2 * j], w[i + 2 * j + 1]);
-                            code[0][j] = codes_of(x);
-                            x = rest16(x, halves_of(code[0][j]));
-                            code[1][j] = codes_of(x);
-                            code[2][j] = codes_of(rest16(x, halves_of(code[1][j])));
+                            store(0, make_uint4(term[0][0], term[0][1], term[1][0], term[1][1]));
+                            store(16, make_uint4(term[2][0], term[2][1], 0, 0));
                         }
 #pragma unroll
-                        for (uint32_t t = 0; t < 3; ++t) term[t][i / 4] = code[t][0] | static_cast<uint32_t>(code[t][1]) << 16;
-                    }
-                    if constexpr (kBlock == 16) {
+                        for (uint32_t i = 0; i < kBlock; ++i) sum[i] = fmaf(w[i], value_inverse, sum[i]);
+                        if constexpr (!kOneBlock) {
 #pragma unroll
-                        for (uint32_t t = 0; t < 3; ++t) store(t * kN + c, make_uint4(term[t][0], term[t][1], term[t][2], term[t][3]));
-                    } else {
-                        store(0, make_uint4(term[0][0], term[0][1], term[1][0], term[1][1]));
-                        store(16, make_uint4(term[2][0], term[2][1], 0, 0));
+                            for (uint32_t i = 0; i < kBlock; i += 4) sum_smem[(c + i) / 4 * kTile + thread] = *reinterpret_cast<const float4*>(sum + i);
+                        }
                     }
-#pragma unroll
-                    for (uint32_t i = 0; i < kBlock; ++i) sum[i] = fmaf(w[i], value_inverse, sum[i]);
-                    if constexpr (!kOneBlock) {
-#pragma unroll
-                        for (uint32_t i = 0; i < kBlock; i += 4) sum_smem[(c + i) / 4 * kTile + thread] = *reinterpret_cast<const float4*>(sum + i);
+                    if (move) break;
+                    if (!all_came()) {
+                        alive = false;
+                        break;
                     }
+                    move = *const_cast<volatile uint32_t*>(&st->needs[buffer]) != 0;
+                    if (!move) break;
                 }
+                if (!alive) break;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(scores_empty + 8 * buffer);
@@ -590,7 +648,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                     if (lane % (32 / kBlock) == 0) reinterpret_cast<float*>(&st->wide[c + query])[quadrant] = sum[0];
                 }
                 if (!meet()) break;
-                if (thread < kN) st->total[thread] = (st->wide[thread].x + st->wide[thread].y) + (st->wide[thread].z + st->wide[thread].w);
+                if (thread < kN) st->total[thread] = ((st->wide[thread].x + st->wide[thread].y) + (st->wide[thread].z + st->wide[thread].w)) * static_cast<float>(1ull << (60 - static_cast<int>(kLift)));
                 if (!meet()) break;
                 if (!warp_look_wait(weights_empty + 8 * ((tile - 1) & 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) break;
                 tc_fence_after();

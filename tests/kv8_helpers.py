@@ -53,9 +53,9 @@ def e4m3_attention_reference(batch, scale, layer=0, q=None):
     The bound, for outputs o = sum w_j v_j: the result is rounded to BF16 once (2^-8 |o|). A query enters as two E4M3 terms in units in which its largest
     element is 224 at least: together they are off by 2^-10 of a unit at most, below 2^-17 of the largest element. A score's F32 sums of
     head_dim products for either term, in any order and with truncation, are off by 2 head_dim 2^-23 sum |q_i k_ji|. What a score is off by is a
-    relative error of its weight, in numerator and denominator, with 2^-22 for the exponential. A weight times its value's scale enters the product in
-    half precision (2^-11 of it) as three E4M3 terms, exact above their units: those are 2^-17, half of it the error, where the largest weight so
-    far is 2^3 or more: 2^-21 of the largest, for every code. Sums in F32, with truncation: the number of tokens times 2^-23."""
+    relative error of its weight, in numerator and denominator, with 2^-22 for the exponential and 2^-18 for its argument, which is up to 56. A weight times its value's scale enters the product in
+    half precision (2^-11 of it) as three E4M3 terms, exact above their units: the last one's is 2^-9 / 16^2 = 2^-17, half of it the error, where the
+    largest weight is 1 or more (the one that set the reference): 2^-18 of the largest, for every code. Sums in F32, with truncation: the number of tokens times 2^-23."""
     q = batch.q if q is None else q
     out = torch.full(q.shape, float("nan"), dtype=torch.float64, device=q.device)
     bound = torch.zeros_like(out)
@@ -75,10 +75,10 @@ def e4m3_attention_reference(batch, scale, layer=0, q=None):
         hidden = (torch.arange(length, device=q.device) > torch.arange(length - new, length, device=q.device)[:, None])[:, None, None]
         scores = scores.masked_fill(hidden, -float("inf"))
         w = torch.softmax(scores, -1).masked_fill(hidden.all(-1, keepdim=True), 0)      # a row that sees nothing gets zeros
-        score_error = (size * 2 * batch.head_dim * 2.0 ** -23 + rough).masked_fill(hidden, 0).amax(-1) + 2.0 ** -22
+        score_error = (size * 2 * batch.head_dim * 2.0 ** -23 + rough).masked_fill(hidden, 0).amax(-1) + 2.0 ** -22 + 2.0 ** -18
         value = torch.einsum("nhgj,hjd->nhgd", w, v * vs)
         spread = torch.einsum("nhgj,hjd->nhgd", w, (v * vs).abs())
-        units = (w * vs[None, :, None, :, 0]).amax(-1, keepdim=True) * v.abs().sum(1)[None, :, None] * 2.0 ** -21
+        units = (w * vs[None, :, None, :, 0]).amax(-1, keepdim=True) * v.abs().sum(1)[None, :, None] * 2.0 ** -18
         relative = 2.0 ** -11 + 2 * score_error[..., None] + 2 * length * 2.0 ** -23
         out[rows] = value.reshape(new, batch.query_heads, -1)
         bound[rows] = (BF16_HALF_ULP * value.abs() + (relative * spread + units) * (1 + BF16_HALF_ULP)).reshape(new, batch.query_heads, -1)
