@@ -296,7 +296,9 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             uint8_t* const to_here = query_smem + buffer * S::kQueryBytes + (piece >> 4) * (S::kScores * 128) + (piece & 1) * 8;
 #pragma unroll 1
             for (uint32_t first = 0; first < S::kScores; first += kRows * kAhead) {
+                static_assert(S::kScores % (kRows * kAhead) == 0, "rows of a round");
                 uint4 raw[kAhead];
+                uint32_t most[kAhead];   // of the magnitudes' bits
 #pragma unroll
                 for (uint32_t i = 0; i < kAhead; ++i) {
                     const uint32_t row = first + i * kRows + lane / kLanes, token = row / group;
@@ -305,26 +307,31 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                 }
 #pragma unroll
                 for (uint32_t i = 0; i < kAhead; ++i) {
-                    const uint32_t row = first + i * kRows + lane / kLanes;
-                    if (first + i * kRows >= S::kScores) break;
-                    const uint32_t word[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                    uint32_t most = 0;   // of the magnitudes' bits
+                    const uint32_t two = __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu), __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu));
+                    most[i] = max(two >> 16, two & 0xffffu);
+                }
+                if constexpr (kLanes == 32) {
 #pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) most = __vmaxu2(most, word[e] & 0x7fff7fffu);
-                    most = most >> 16 > (most & 0xffffu) ? most >> 16 : most & 0xffffu;
+                    for (uint32_t i = 0; i < kAhead; ++i) most[i] = __reduce_max_sync(0xffffffffu, most[i]);
+                } else {   // a row in either half of the warp: step by step, the rows side by side
 #pragma unroll
                     for (uint32_t step = kLanes / 2; step; step /= 2) {
-                        const uint32_t other = __shfl_xor_sync(0xffffffffu, most, step);
-                        most = most > other ? most : other;
+#pragma unroll
+                        for (uint32_t i = 0; i < kAhead; ++i) most[i] = max(most[i], __shfl_xor_sync(0xffffffffu, most[i], step));
                     }
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < kAhead; ++i) {
+                    const uint32_t row = first + i * kRows + lane / kLanes;
                     // the smallest power of two (a normal number) with which the largest is at most 448 = 1.75 * 2^8; a row that is not finite: codes of zero, a scale of NaN
-                    const bool finite = most < 0x7f80u;
-                    const uint32_t exponent = (most >> 7) + ((most & 0x7fu) > 0x60u ? 1 : 0), byte = exponent < 9 ? 1 : exponent - 8;
+                    const bool finite = most[i] < 0x7f80u;
+                    const uint32_t exponent = (most[i] >> 7) + ((most[i] & 0x7fu) > 0x60u ? 1 : 0), byte = exponent < 9 ? 1 : exponent - 8;
                     const float inverse = __uint_as_float((254 - byte) << 23);
+                    const uint32_t word[4] = {finite ? raw[i].x : 0, finite ? raw[i].y : 0, finite ? raw[i].z : 0, finite ? raw[i].w : 0};
                     uint32_t high[4], low[4];
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) {
-                        const float x0 = finite ? __uint_as_float(word[e] << 16) * inverse : 0.0f, x1 = finite ? __uint_as_float(word[e] & 0xffff0000u) * inverse : 0.0f;
+                        const float x0 = __uint_as_float(word[e] << 16) * inverse, x1 = __uint_as_float(word[e] & 0xffff0000u) * inverse;
                         uint16_t code;
                         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(code) : "f"(x1), "f"(x0));
                         const uint32_t back = halves_of(code);
