@@ -234,10 +234,11 @@ __device__ __forceinline__ float warp_max(float x) {
 // Joins the parts of one pair, in the order of their spans. A CTA takes queries blockIdx.y, blockIdx.y + gridDim.y, ...; four outputs a
 // thread, and the threads of a query's outputs as many times over as there are, each with every so many-th part.
 constexpr uint32_t kJoinThreads = 256, kJoinCtas = 1184;   // about as many as run at once
-// Few queries have few CTAs, and as many loads under way as the parts of one sequence want; many queries more CTAs at once.
-template <uint32_t kHeadDim, uint32_t kN>
-__global__ void __launch_bounds__(kJoinThreads, kN <= 16 ? 1 : 6) attention_join_kernel(const __grid_constant__ AttentionParams p) {
-    constexpr uint32_t kLanes = kHeadDim / 4, kShares = kJoinThreads / kLanes, kAhead = kN <= 16 ? 10 : 6;
+// Few CTAs have as many loads under way as the parts of one sequence want; of many (kMany) six run at once on an SM, and take their places while the attention's last CTAs
+// are still at work. (148 x 6 of eight columns, two an SM: the last of them began 4.7 us behind the attention.) Either sums in the same order.
+template <uint32_t kHeadDim, uint32_t kN, bool kMany>
+__global__ void __launch_bounds__(kJoinThreads, kMany ? 6 : 1) attention_join_kernel(const __grid_constant__ AttentionParams p) {
+    constexpr uint32_t kLanes = kHeadDim / 4, kShares = kJoinThreads / kLanes, kAhead = kMany ? 6 : 10;
     __shared__ float weight[kMaxCtas];
     __shared__ float4 sums[kShares][kLanes];
     __shared__ float wide[2][kJoinThreads / 32];
@@ -321,7 +322,8 @@ void launch_join(cudaStream_t stream, const AttentionParams& p) {
     config.stream = stream, config.attrs = &attribute, config.numAttrs = 1;
     const uint32_t rows = (kJoinCtas + p.joins - 1) / p.joins;
     config.gridDim = dim3(p.joins, queries < rows ? queries : rows), config.blockDim = dim3(kJoinThreads);
-    cudaLaunchKernelEx(&config, attention_join_kernel<kHeadDim, kN>, p);
+    const bool many = kN > 16 || config.gridDim.x * config.gridDim.y > 2 * p.spans;
+    cudaLaunchKernelEx(&config, many ? attention_join_kernel<kHeadDim, kN, true> : attention_join_kernel<kHeadDim, kN, kN <= 16 ? false : true>, p);
 }
 
 uint32_t query_columns(uint32_t query_heads, uint32_t kv_heads, uint32_t max_new) {
