@@ -63,8 +63,8 @@ struct ShapeE4m3 {
         const uint32_t fit = (kSmemLimit - fixed(buffers)) / kSlotBytes / 2 * 2;
         return fit < 16 ? fit : 16;
     }
-    // A ring each for the keys and the values, as many slots of 16 KB each as there is room for; the queries of a pair twice, so that the next pair's are there in
-    // time, where two tiles of both fit beside them.
+    // A ring each for the keys and the values, as many slots of 16 KB each as there is room for; the queries of a pair twice where two tiles of both fit beside them, so that a
+    // warp of its own can split the next pair's in time. Else the softmax warps split them, all four, once the last pair's are no longer read.
     static constexpr uint32_t kQueryBuffers = slots(2) < 4 * kChunks ? 1 : 2, kSlots = slots(kQueryBuffers), kFixed = fixed(kQueryBuffers);
     static constexpr uint32_t kKeySlots = kSlots / 2, kValueSlots = kSlots - kKeySlots;
     static constexpr uint32_t kSmem = kFixed + kSlots * kSlotBytes;
@@ -126,6 +126,91 @@ __device__ __forceinline__ uint32_t rest16(uint32_t x, uint32_t y) {
 }
 __device__ __forceinline__ uint32_t scale_byte(uint32_t byte) { return byte < kE4m3LeastScale ? kE4m3LeastScale : byte > kE4m3LargestScale ? kE4m3LargestScale : byte; }
 
+// A pair's queries as two terms, in the 128-byte swizzle of the operand; rows past the last are zero. Each of `warps` warps takes every so many-th round of kRows * kAhead rows.
+template <uint32_t kHeadDim, uint32_t kN>
+struct SplitQueries {
+    using S = ShapeE4m3<kHeadDim, kN>;
+    static constexpr uint32_t kLanes = kHeadDim / 8, kRows = 32 / kLanes, kAhead = S::kQueryBuffers == 1 ? 4 : 8;   // lanes for a row, rows at a time, loads under way
+    static_assert(S::kScores % (kRows * kAhead) == 0, "rows of a round");
+    // A round's rows are on their way while the round before is split, the first of them while the buffer's last pair is still in use. (The place of a row follows from
+    // the one before: a division for each made eight loads 1500 cycles.)
+    uint4 next[kAhead];
+    const __nv_bfloat16* ahead;
+    uint32_t row_ahead, within, queries, group, query_heads, first, step;
+
+    __device__ __forceinline__ void load() {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            next[i] = make_uint4(0, 0, 0, 0);
+            if (row_ahead < queries) next[i] = *reinterpret_cast<const uint4*>(ahead);
+            move(kRows);
+        }
+    }
+    __device__ __forceinline__ void move(uint32_t rows) {
+        row_ahead += rows, within += rows, ahead += rows * kHeadDim;
+        while (within >= group) within -= group, ahead += (query_heads - group) * kHeadDim;
+    }
+    __device__ __forceinline__ void open(const __nv_bfloat16* from, uint32_t pair_queries, uint32_t pair_group, uint32_t all_heads, uint32_t warp, uint32_t warps, uint32_t lane) {
+        queries = pair_queries, group = pair_group, query_heads = all_heads, first = warp * kRows * kAhead, step = warps * kRows * kAhead;
+        row_ahead = within = 0, ahead = from;
+        move(first + lane / kLanes);
+        load();
+    }
+    __device__ __forceinline__ void run(uint8_t* to, float* scales, uint32_t lane) {
+        const uint32_t piece = lane % kLanes, unit = (piece & 15) >> 1;
+        uint8_t* const to_here = to + (piece >> 4) * (S::kScores * 128) + (piece & 1) * 8;
+#pragma unroll 1
+        for (; first < S::kScores; first += step) {
+            uint4 raw[kAhead];
+            uint32_t most[kAhead];   // of the magnitudes' bits
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i) raw[i] = next[i];
+            if (step > kRows * kAhead) move(step - kRows * kAhead);
+            load();
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i) {
+                const uint32_t two = __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu), __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu));
+                most[i] = max(two >> 16, two & 0xffffu);
+            }
+            if constexpr (kLanes == 32) {
+#pragma unroll
+                for (uint32_t i = 0; i < kAhead; ++i) most[i] = __reduce_max_sync(0xffffffffu, most[i]);
+            } else {   // a row in either half of the warp: step by step, the rows side by side
+#pragma unroll
+                for (uint32_t step = kLanes / 2; step; step /= 2) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kAhead; ++i) most[i] = max(most[i], __shfl_xor_sync(0xffffffffu, most[i], step));
+                }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i) {
+                const uint32_t row = first + i * kRows + lane / kLanes;
+                // the smallest power of two (a normal number) with which the largest is at most 448 = 1.75 * 2^8; a row that is not finite: codes of zero, a scale of NaN
+                const bool finite = most[i] < 0x7f80u;
+                const uint32_t exponent = (most[i] >> 7) + ((most[i] & 0x7fu) > 0x60u ? 1 : 0), byte = exponent < 9 ? 1 : exponent - 8;
+                const float inverse = __uint_as_float((254 - byte) << 23);
+                const uint32_t word[4] = {finite ? raw[i].x : 0, finite ? raw[i].y : 0, finite ? raw[i].z : 0, finite ? raw[i].w : 0};
+                uint32_t high[4], low[4];
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    const float x0 = __uint_as_float(word[e] << 16) * inverse, x1 = __uint_as_float(word[e] & 0xffff0000u) * inverse;
+                    uint16_t code;
+                    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(code) : "f"(x1), "f"(x0));
+                    const uint32_t back = halves_of(code);
+                    const float2 met = __half22float2(*reinterpret_cast<const __half2*>(&back));
+                    high[e] = code;
+                    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(code) : "f"(x1 - met.y), "f"(x0 - met.x));
+                    low[e] = code;
+                }
+                uint8_t* const at = to_here + row * 128 + ((unit ^ (row & 7)) << 4);
+                *reinterpret_cast<uint2*>(at) = make_uint2(high[0] | high[1] << 16, high[2] | high[3] << 16);
+                *reinterpret_cast<uint2*>(at + S::kTermBytes) = make_uint2(low[0] | low[1] << 16, low[2] | low[3] << 16);
+                if (piece == 0 && row < kN) scales[row] = finite ? __uint_as_float(byte << 23) : __uint_as_float(0x7fc00000u);
+            }
+        }
+    }
+};
+
 template <uint32_t kHeadDim, uint32_t kN>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const __grid_constant__ CUtensorMap map_values, const __grid_constant__ AttentionParams p) {
@@ -149,7 +234,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
         for (uint32_t b = 0; b < 2; ++b) {
             mbar_init(scores_full + 8 * b, 1), mbar_init(scores_empty + 8 * b, 4);
             mbar_init(weights_full + 8 * b, 4), mbar_init(weights_empty + 8 * b, 1);
-            mbar_init(query_full + 8 * b, 1), mbar_init(query_empty + 8 * b, 5);   // the MMAs, and the softmax warps with the queries' scales
+            mbar_init(query_full + 8 * b, S::kQueryBuffers == 1 ? 4 : 1), mbar_init(query_empty + 8 * b, 5);   // the MMAs, and the softmax warps with the queries' scales
         }
         mbar_init(group_bar, 4), mbar_init(smem_u32(&st->keys_first), 1);
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_keys) : "memory");
@@ -262,7 +347,10 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
         };
         if (ahead.valid) alive = scores_of_tile();
         while (alive && now.valid) {
-            if (ahead.valid && !scores_of_tile()) break;
+            // (a new pair's scores before the old one's last product only if its queries are there: they may be waiting for that product)
+            const uint32_t query = S::kQueryBuffers == 2 ? pair & 1 : 0, query_phase = (S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1;
+            const bool scores_first = ahead.valid && (!ahead.first() || __all_sync(0xffffffffu, mbar_test(query_full + 8 * query, query_phase)));
+            if (scores_first && !scores_of_tile()) break;
             const uint32_t buffer = products & 1, steps = (now.keys() + 31) / 32;
             if (!warp_look_wait(weights_full + 8 * buffer, products >> 1 & 1, abort_flag, status, kStatusProduct)) break;
             for (uint32_t h = 0; alive && h < S::kChunks; ++h) {
@@ -278,12 +366,12 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             if (!alive) break;
             commit(weights_empty + 8 * buffer);
             ++products;
+            if (!scores_first && ahead.valid && !scores_of_tile()) break;
             now.advance(st, p);
         }
     } else if (warp == 2) {
         // ---------------- queries of a pair as two terms, in the 128-byte swizzle of the operand; rows past the last are zero ----------------
-        constexpr uint32_t kLanes = kHeadDim / 8, kRows = 32 / kLanes, kAhead = 8;   // lanes for a row, rows at a time, loads under way
-        const uint32_t piece = lane % kLanes, unit = (piece & 15) >> 1;
+        constexpr uint32_t kLanes = kHeadDim / 8, kRows = 32 / kLanes;   // lanes for a row, rows at a time
         Walk walk;
         walk.open(st, p, from, to);
         uint32_t pair = 0;
@@ -291,74 +379,17 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             if (walk.key >= walk.key_end) continue;
             const uint32_t buffer = S::kQueryBuffers == 2 ? pair & 1 : 0;
             const uint32_t first_row = st->row[walk.sequence], queries = walk.tokens * group;
-            const __nv_bfloat16* const from_here = p.query + (static_cast<uint64_t>(first_row) * p.query_heads + walk.head * group) * kHeadDim + piece * 8;
-            // A round's rows are on their way while the round before is split (from memory, one round behind the other, 48 rows took 10 us); the first of them while
-            // the buffer's last pair is still in use.
-            // (The place of a row follows from the one before: a division for each made eight loads 1500 cycles.)
-            uint4 next[kAhead];
-            uint32_t row_ahead = lane / kLanes, within = row_ahead % group;
-            const __nv_bfloat16* ahead = from_here + (static_cast<uint64_t>(row_ahead / group) * p.query_heads + within) * kHeadDim;
-            auto load = [&]() {
-#pragma unroll
-                for (uint32_t i = 0; i < kAhead; ++i) {
-                    next[i] = make_uint4(0, 0, 0, 0);
-                    if (row_ahead < queries) next[i] = *reinterpret_cast<const uint4*>(ahead);
-                    row_ahead += kRows, within += kRows, ahead += kRows * kHeadDim;
-                    while (within >= group) within -= group, ahead += (p.query_heads - group) * kHeadDim;
+            const __nv_bfloat16* const from_here = p.query + (static_cast<uint64_t>(first_row) * p.query_heads + walk.head * group) * kHeadDim + lane % kLanes * 8;
+            if constexpr (S::kQueryBuffers == 1) {   // the softmax warps split them; here they are only brought nearer
+                for (uint32_t row = lane / kLanes; row < queries; row += kRows) {
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(from_here + (static_cast<uint64_t>(row / group) * p.query_heads + row % group) * kHeadDim));
                 }
-            };
-            load();
-            if (!warp_look_wait(query_empty + 8 * buffer, ((S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1) ^ 1, abort_flag, status, kStatusQuery)) break;
-            uint8_t* const to_here = query_smem + buffer * S::kQueryBytes + (piece >> 4) * (S::kScores * 128) + (piece & 1) * 8;
-#pragma unroll 1
-            for (uint32_t first = 0; first < S::kScores; first += kRows * kAhead) {
-                static_assert(S::kScores % (kRows * kAhead) == 0, "rows of a round");
-                uint4 raw[kAhead];
-                uint32_t most[kAhead];   // of the magnitudes' bits
-#pragma unroll
-                for (uint32_t i = 0; i < kAhead; ++i) raw[i] = next[i];
-                load();
-#pragma unroll
-                for (uint32_t i = 0; i < kAhead; ++i) {
-                    const uint32_t two = __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu), __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu));
-                    most[i] = max(two >> 16, two & 0xffffu);
-                }
-                if constexpr (kLanes == 32) {
-#pragma unroll
-                    for (uint32_t i = 0; i < kAhead; ++i) most[i] = __reduce_max_sync(0xffffffffu, most[i]);
-                } else {   // a row in either half of the warp: step by step, the rows side by side
-#pragma unroll
-                    for (uint32_t step = kLanes / 2; step; step /= 2) {
-#pragma unroll
-                        for (uint32_t i = 0; i < kAhead; ++i) most[i] = max(most[i], __shfl_xor_sync(0xffffffffu, most[i], step));
-                    }
-                }
-#pragma unroll
-                for (uint32_t i = 0; i < kAhead; ++i) {
-                    const uint32_t row = first + i * kRows + lane / kLanes;
-                    // the smallest power of two (a normal number) with which the largest is at most 448 = 1.75 * 2^8; a row that is not finite: codes of zero, a scale of NaN
-                    const bool finite = most[i] < 0x7f80u;
-                    const uint32_t exponent = (most[i] >> 7) + ((most[i] & 0x7fu) > 0x60u ? 1 : 0), byte = exponent < 9 ? 1 : exponent - 8;
-                    const float inverse = __uint_as_float((254 - byte) << 23);
-                    const uint32_t word[4] = {finite ? raw[i].x : 0, finite ? raw[i].y : 0, finite ? raw[i].z : 0, finite ? raw[i].w : 0};
-                    uint32_t high[4], low[4];
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) {
-                        const float x0 = __uint_as_float(word[e] << 16) * inverse, x1 = __uint_as_float(word[e] & 0xffff0000u) * inverse;
-                        uint16_t code;
-                        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(code) : "f"(x1), "f"(x0));
-                        const uint32_t back = halves_of(code);
-                        const float2 met = __half22float2(*reinterpret_cast<const __half2*>(&back));
-                        high[e] = code;
-                        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(code) : "f"(x1 - met.y), "f"(x0 - met.x));
-                        low[e] = code;
-                    }
-                    uint8_t* const at = to_here + row * 128 + ((unit ^ (row & 7)) << 4);
-                    *reinterpret_cast<uint2*>(at) = make_uint2(high[0] | high[1] << 16, high[2] | high[3] << 16);
-                    *reinterpret_cast<uint2*>(at + S::kTermBytes) = make_uint2(low[0] | low[1] << 16, low[2] | low[3] << 16);
-                    if (piece == 0 && row < kN) st->query_scale[buffer][row] = finite ? __uint_as_float(byte << 23) : __uint_as_float(0x7fc00000u);
-                }
+                continue;
             }
+            SplitQueries<kHeadDim, kN> split;
+            split.open(from_here, queries, group, p.query_heads, 0, 1, lane);
+            if (!warp_look_wait(query_empty + 8 * buffer, (pair >> 1 & 1) ^ 1, abort_flag, status, kStatusQuery)) break;
+            split.run(query_smem + buffer * S::kQueryBytes, st->query_scale[buffer], lane);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(query_full + 8 * buffer);
@@ -396,6 +427,15 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             if (!meet()) break;
             const uint32_t query_buffer = S::kQueryBuffers == 2 ? pair & 1 : 0;
             const float* const query_scale = st->query_scale[query_buffer];
+            if (S::kQueryBuffers == 1 && any) {
+                SplitQueries<kHeadDim, kN> split;
+                split.open(p.query + (static_cast<uint64_t>(first_row) * p.query_heads + walk.head * group) * kHeadDim + lane % (kHeadDim / 8) * 8, queries, group, p.query_heads, quadrant, 4, lane);
+                if (!warp_look_wait(query_empty, (pair & 1) ^ 1, abort_flag, status, kStatusQuery)) break;
+                split.run(query_smem, st->query_scale[0], lane);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(query_full);
+            }
             if (any && !warp_look_wait(query_full + 8 * query_buffer, (S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1, abort_flag, status, kStatusQuery)) break;
             const int32_t seen_by_all = static_cast<int32_t>(walk.length) - static_cast<int32_t>(walk.tokens) + 1;
             float sum[kBlock];   // this thread's part of the denominators
