@@ -39,6 +39,7 @@ struct AttentionParams {
     uint32_t rows, sequences, table_pages, pages, query_heads, kv_heads, page_shift, max_new, spans, joins;
     float scale_log2;             // scale * log2(e)
     const uint8_t* scales;        // of an E4M3 cache
+    uint32_t pair_units;          // what a pair costs beside its units, in units: its beginning and end
 };
 
 namespace {
@@ -70,7 +71,7 @@ __device__ __forceinline__ void scan_units(BatchState* st, const AttentionParams
         if (!tokens && p.joins < p.spans && blockIdx.x == b % p.spans) {
             for (uint32_t h = 0; h < p.kv_heads; ++h) p.records[b * p.kv_heads + h] = JoinRecord{};   // an idle slot's
         }
-        return !tokens ? 0 : length ? (static_cast<uint32_t>(length) + kUnit - 1) / kUnit : 1;   // a row that sees nothing is written too
+        return !tokens ? 0 : (length ? (static_cast<uint32_t>(length) + kUnit - 1) / kUnit : 1) + p.pair_units;   // a row that sees nothing is written too
     };
     if (p.sequences <= 32) {   // every warp for itself, all with the same result
         const uint32_t count = lane < p.sequences ? units_of(lane) : 0;
@@ -119,15 +120,23 @@ struct Walk {
     uint32_t unit, end, sequence, head, key, key_end, length, tokens;
     bool starts, ends;   // the pair's first and last key are in the span
 
-    __device__ void open(const BatchState* st, const AttentionParams& p, uint32_t from, uint32_t to) {
-        unit = from, end = to;
-        uint32_t low = 0, high = p.sequences;   // the last sequence whose units start at or before `from`
+    __device__ static uint32_t sequence_of(const BatchState* st, const AttentionParams& p, uint32_t at) {
+        uint32_t low = 0, high = p.sequences;   // the last sequence whose units start at or before it
         while (high - low > 1) {
             const uint32_t middle = (low + high) / 2;
-            if (st->units[middle] * p.kv_heads <= from) low = middle;
+            if (st->units[middle] * p.kv_heads <= at) low = middle;
             else high = middle;
         }
-        sequence = low;
+        return low;
+    }
+    // Where a span is cut: behind the pair, if the cut falls on what it costs beside its units.
+    __device__ static uint32_t cut(const BatchState* st, const AttentionParams& p, uint32_t at) {
+        if (!p.pair_units || at >= st->units[p.sequences] * p.kv_heads) return at;
+        const uint32_t sequence = sequence_of(st, p, at), count = st->units[sequence + 1] - st->units[sequence], within = (at - st->units[sequence] * p.kv_heads) % count;
+        return within + p.pair_units >= count ? at + count - within : at;
+    }
+    __device__ void open(const BatchState* st, const AttentionParams& p, uint32_t from, uint32_t to) {
+        unit = from, end = to, sequence = sequence_of(st, p, from);
     }
     __device__ bool next(const BatchState* st, const AttentionParams& p) {
         if (unit >= end) return false;
@@ -138,9 +147,10 @@ struct Walk {
         const uint32_t first = at - head * count;
         const uint32_t take = end - unit < count - first ? end - unit : count - first;
         length = st->length[sequence] & ((1u << (kMaxTokensLog2 + 1)) - 1), tokens = st->length[sequence] >> (kMaxTokensLog2 + 1);
-        starts = first == 0, ends = first + take == count;
+        const uint32_t units = count - p.pair_units;
+        starts = first == 0, ends = first + take >= units;
         key = first * kUnit;
-        const uint32_t stop = (first + take) * kUnit;
+        const uint32_t stop = (first + take < units ? first + take : units) * kUnit;
         key_end = stop < length ? stop : length;
         unit += take;
         return true;
@@ -375,7 +385,7 @@ bool check_attention(int32_t d, augur_cuda_stream_t s, const augur_cuda_nvfp4_sm
 // What the launches get of a descriptor that passed.
 template <class Args>
 AttentionParams attention_params(const augur_cuda_nvfp4_sm100_plan_v1* plan, const Args* a) {
-    AttentionParams p{};
+    AttentionParams p{};   // (pair_units stays 0 where the launch does not say more)
     p.query = reinterpret_cast<const __nv_bfloat16*>(a->query);
     p.output = reinterpret_cast<__nv_bfloat16*>(a->output);
     p.page_table = reinterpret_cast<const int32_t*>(a->batch.page_table);

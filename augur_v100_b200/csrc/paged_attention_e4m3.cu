@@ -254,7 +254,8 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
     scan_units(st, p, warp, lane);
     const uint32_t total = st->units[p.sequences] * p.kv_heads, spans = total < p.spans ? total : p.spans;
     const uint32_t base = spans ? total / spans : 0, extra = total - base * spans;   // spans of `base` units, the first `extra` of one more
-    const uint32_t from = blockIdx.x * base + (blockIdx.x < extra ? blockIdx.x : extra), to = blockIdx.x < spans ? from + base + (blockIdx.x < extra ? 1 : 0) : from;
+    const auto cut = [&](uint32_t span) { return Walk::cut(st, p, span * base + (span < extra ? span : extra)); };
+    const uint32_t from = blockIdx.x < spans ? cut(blockIdx.x) : 0, to = blockIdx.x < spans ? cut(blockIdx.x + 1) : 0;
     const uint32_t tmem = st->tmem, tmem_out = tmem + 2 * S::kScores;
     const uint32_t group = p.query_heads / p.kv_heads;
 
@@ -783,7 +784,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             if (!alone) {
                 if (walk.starts) {
                     const uint32_t units = st->units[walk.sequence + 1] - st->units[walk.sequence], longer = extra * (base + 1);
-                    const uint32_t last = st->units[walk.sequence] * p.kv_heads + (walk.head + 1) * units - 1;   // the pair's last unit
+                    const uint32_t last = st->units[walk.sequence] * p.kv_heads + (walk.head + 1) * units - p.pair_units - 1;   // the pair's last unit
                     record.row = first_row, record.tokens = walk.tokens, record.head = walk.head, record.first = blockIdx.x;
                     record.last = last < longer ? last / (base + 1) : extra + (last - longer) / base;
                 }
@@ -856,13 +857,16 @@ extern "C" augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_paged_att
     if (e != cudaSuccess) return make_result(AUGUR_CUDA_STATUS_RUNTIME_FAILURE, e);
     AttentionParams p = attention_params(plan, a);
     p.scales = reinterpret_cast<const uint8_t*>(a->layer.scales);
+    const uint32_t columns = query_columns(a->query_heads, a->layer.kv_heads, a->max_new_tokens);
+    // A pair's beginning and end take about 2 us where a unit of head size 256 streams in 0.7 us, of 128 in 0.4; of many queries about 6 us. (64 ragged sequences, spans of as
+    // many units each: those of one pair done after 72 us, those of six after 84.)
+    p.pair_units = columns > 16 ? 8 : a->layer.head_dim == 256 ? 3 : 5;
     const uint32_t head_dim = a->layer.head_dim, box = a->layer.page_tokens < kUnit ? a->layer.page_tokens : kUnit;
     const uint64_t cache_rows = static_cast<uint64_t>(a->layer.pages) * a->layer.kv_heads * a->layer.page_tokens;
     CUtensorMap keys, values;   // rows of head_dim bytes, as a map of packed codes with twice the columns
     if (!make_code_map(&keys, a->layer.keys, cache_rows, head_dim * 2, box) || !make_code_map(&values, a->layer.values, cache_rows, head_dim * 2, box)) {
         return make_result(AUGUR_CUDA_STATUS_RUNTIME_FAILURE);
     }
-    const uint32_t columns = query_columns(a->query_heads, a->layer.kv_heads, a->max_new_tokens);
     auto launch = head_dim == 256 ? launch_of<256>(columns) : launch_of<128>(columns);
     launch(s->stream, keys, values, p);
     return submitted();
