@@ -346,17 +346,11 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             ahead.advance(st, p);
             return true;
         };
-        if (ahead.valid) alive = scores_of_tile();
-        while (alive && now.valid) {
-            // (a new pair's scores before the old one's last product only if its queries are there: they may be waiting for that product)
-            const uint32_t query = S::kQueryBuffers == 2 ? pair & 1 : 0, query_phase = (S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1;
-            const bool scores_first = ahead.valid && (!ahead.first() || __all_sync(0xffffffffu, mbar_test(query_full + 8 * query, query_phase)));
-            if (scores_first && !scores_of_tile()) break;
+        auto product_of_tile = [&]() {
             const uint32_t buffer = products & 1, steps = (now.keys() + 31) / 32;
-            if (!warp_look_wait(weights_full + 8 * buffer, products >> 1 & 1, abort_flag, status, kStatusProduct)) break;
-            for (uint32_t h = 0; alive && h < S::kChunks; ++h) {
-                alive = warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusProduct);
-                if (!alive) break;
+            if (!warp_look_wait(weights_full + 8 * buffer, products >> 1 & 1, abort_flag, status, kStatusProduct)) return false;
+            for (uint32_t h = 0; h < S::kChunks; ++h) {
+                if (!warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusProduct)) return false;
                 tc_fence_after();
                 // 32 keys: 32 rows of 128 bytes of V, of 32 bytes of W
                 mma_block_e4m3<kHighWeights, (32 * 128 >> 4), (32 * 32 >> 4)>(tmem_out + h * S::kTerms, slots + slot * (kSlotBytes >> 4), weights + ((buffer * S::kWeightBytes) >> 4),
@@ -364,11 +358,22 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                 commit(empty + 8 * slot);
                 if (++slot == S::kSlots) slot = S::kKeySlots, phase ^= 1;
             }
-            if (!alive) break;
             commit(weights_empty + 8 * buffer);
             ++products;
-            if (!scores_first && ahead.valid && !scores_of_tile()) break;
             now.advance(st, p);
+            return true;
+        };
+        // The scores of a tile are formed once the softmax is done with those of two tiles before, ahead of that tile's product: behind it, the softmax waited for them. (Whichever
+        // can go next, found out by polling, was worse: 120 us where this order takes NN.) A new pair's queries may be waiting for the products of the pair before.
+        while (alive && now.valid) {
+            while (alive && ahead.valid && scores < products + 3) {
+                if (ahead.first() && scores != products) {
+                    const uint32_t query = S::kQueryBuffers == 2 ? pair & 1 : 0, query_phase = (S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1;
+                    if (!__all_sync(0xffffffffu, mbar_test(query_full + 8 * query, query_phase))) break;
+                }
+                alive = scores_of_tile();
+            }
+            alive = alive && product_of_tile();
         }
     } else if (warp == 2) {
         // ---------------- queries of a pair as two terms, in the 128-byte swizzle of the operand; rows past the last are zero ----------------
