@@ -447,19 +447,21 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             float sum[kBlock];   // this thread's part of the denominators
 #pragma unroll
             for (uint32_t i = 0; i < kBlock; ++i) sum[i] = 0.0f;
+            // A tile's pages and scales, asked for while the warps wait for one another over the tile before.
+            uint32_t next_there = 0, next_bytes = 0;
+            auto fetch = [&](uint32_t t) {
+                const uint32_t at = t % kTileInfos;
+                if (!warp_look_wait(scales_full + 8 * at, t / kTileInfos & 1, abort_flag, status, kStatusScores)) return false;
+                next_there = st->info[at], next_bytes = st->scales[at][thread];
+                return true;
+            };
+            if (any && !fetch(tile)) break;
             for (uint32_t key = walk.key; key < walk.key_end; key += kTile, ++tile) {
-                const uint32_t buffer = tile & 1, at = tile % kTileInfos;
-                if (!warp_look_wait(scales_full + 8 * at, tile / kTileInfos & 1, abort_flag, status, kStatusScores) ||
-                    !warp_look_wait(scores_full + 8 * buffer, tile >> 1 & 1, abort_flag, status, kStatusScores)) {
-                    alive = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t there = st->info[at];
+                const uint32_t buffer = tile & 1, there = next_there;
                 const uint32_t count = walk.key_end - key < kTile ? walk.key_end - key : kTile;
                 const bool whole = count == kTile && there == all_boxes, masked = !whole || static_cast<int32_t>(key + kTile) > seen_by_all;
                 const bool my_key = thread < count && (there >> (thread >> box_shift) & 1);
-                const uint32_t bytes = my_key ? st->scales[at][thread] : 0x7f7fu, key_byte = scale_byte(bytes & 0xff), value_byte = scale_byte(bytes >> 8);
+                const uint32_t bytes = my_key ? next_bytes : 0x7f7fu, key_byte = scale_byte(bytes & 0xff), value_byte = scale_byte(bytes >> 8);
                 const float key_scale = (bytes & 0xff) == 0xff ? __uint_as_float(0x7fc00000u) : __uint_as_float(key_byte << 23) * p.scale_log2;
                 const float value_power = bytes >> 8 == 0xff ? __uint_as_float(0x7fc00000u) : static_cast<float>(static_cast<int32_t>(value_byte) - 127);
                 const float value_inverse = __uint_as_float((254 - 60 - value_byte) << 23);   // 2^-60 of it, which the total makes up for
@@ -492,10 +494,12 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                     }
                     return passes;
                 };
-                if (!warp_look_wait(weights_empty + 8 * buffer, (tile >> 1 & 1) ^ 1, abort_flag, status, kStatusProduct)) {
+                if (!warp_look_wait(weights_empty + 8 * buffer, (tile >> 1 & 1) ^ 1, abort_flag, status, kStatusProduct) ||
+                    !warp_look_wait(scores_full + 8 * buffer, tile >> 1 & 1, abort_flag, status, kStatusScores)) {
                     alive = false;
                     break;
                 }
+                tc_fence_after();
                 if (kOneBlock) scores(0);
                 // The weights are formed and stored under the references as they stand, and stand if no warp finds one that passes 2^kRoom; else the references
                 // move and the weights are formed anew. (Asked first and formed then, a tile of eight queries took 400 cycles more, which the warps waited for one another.)
@@ -643,6 +647,11 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                             for (uint32_t i = 0; i < kBlock; i += 4) sum_smem[(c + i) / 4 * kTile + thread] = *reinterpret_cast<const float4*>(sum + i);
                         }
                     }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    if (!again && key + kTile < walk.key_end && !fetch(tile + 1)) {
+                        alive = false;
+                        break;
+                    }
                     if (move) break;
                     if (!all_came()) {
                         alive = false;
@@ -677,8 +686,8 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                         if (++slot == S::kSlots) slot = S::kKeySlots, phase ^= 1;
                     }
                     if (!alive) break;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(weights_full + 8 * buffer);
             }
