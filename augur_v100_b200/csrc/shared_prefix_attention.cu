@@ -26,7 +26,7 @@ static_assert(sizeof(augur_cuda_nvfp4_sm100_shared_prefix_attention_args_v1) == 
 constexpr uint32_t kRowsM = 128;               // queries of a CTA
 constexpr uint32_t kRounds = 3;                // a device's worth of CTAs, at most so many times, where the prefix is split for it
 constexpr uint32_t kMaxSplit = 256, kMaxChunks = 32;   // of the prefix, and of a sequence's own tokens
-constexpr uint32_t kInfoRing = 8;
+constexpr uint32_t kInfoRing = 16, kMaxSlots = 24, kMaxBuffers = 4;
 constexpr uint32_t kStatusPrefixLoad = 0x421, kStatusPrefixMma = 0x422, kStatusPrefixScores = 0x423, kStatusPrefixQuery = 0x424, kStatusPrefixProduct = 0x425, kStatusPrefixInfo = 0x426;
 
 struct PrefixParams {
@@ -51,17 +51,20 @@ __device__ __forceinline__ uint32_t shared_tokens(const PrefixParams& p) {
 template <uint32_t kHeadDim>
 struct PrefixShape {
     static constexpr uint32_t kChunks = kHeadDim / 64, kStreams = kHeadDim == 128 ? 2 : 1;
+    // Keys of a tile, and S in tensor memory: 256 columns of it. With two streams each has two, so that the next scores are formed while its softmax is at work (of 128 keys
+    // and one each, the weights' product and the next scores behind it were waited for: 2300 cycles for 128 keys, NN now).
+    static constexpr uint32_t kKeys = kHeadDim == 128 ? 64 : 128, kBuffers = 256 / kKeys, kSlot = kKeys * 128;
     static constexpr uint32_t kThreads = 128 + 128 * kStreams;   // warp 0 loads keys, 1 MMA, 3 values, then the softmax
-    static constexpr uint32_t kQueryBytes = kRowsM * kHeadDim * 2, kSlots = (224 * 1024 - kQueryBytes) / kSlotBytes;
+    static constexpr uint32_t kQueryBytes = kRowsM * kHeadDim * 2, kSlots = (224 * 1024 - kQueryBytes) / kSlot;
     // A ring each for the keys and the values, so that two warps deal out the copies: one alone took 80 cycles a copy, and pages of 16 tokens are eight copies a slot.
     static constexpr uint32_t kValueSlots = (kSlots / 2 + 1) / 2 * 2, kKeySlots = kSlots - kValueSlots;   // (pairs of value slots are one operand)
-    static constexpr uint32_t kSmem = 1024 + kQueryBytes + kSlots * kSlotBytes + 1024;
-    static constexpr uint32_t kScoresAt = 0, kOutAt = 256;       // tensor memory: two of S, one O per stream
-    static_assert(kKeySlots >= kChunks && kValueSlots >= kChunks && kChunks % 2 == 0 && kSmem <= kSmemLimit && kOutAt + kStreams * kHeadDim == 512, "a CTA's memory");
+    static constexpr uint32_t kSmem = 1024 + kQueryBytes + kSlots * kSlot + 1024;
+    static constexpr uint32_t kScoresAt = 0, kOutAt = 256;       // tensor memory: S, then one O per stream
+    static_assert(kSlots <= kMaxSlots && kKeySlots / kChunks + kBuffers + 1 <= kInfoRing && kKeySlots >= kChunks && kValueSlots >= kChunks && kChunks % 2 == 0 && kSmem <= kSmemLimit && kOutAt + kStreams * kHeadDim == 512, "a CTA's memory");
 };
 
 struct PrefixState {
-    uint64_t full[16], empty[16], scores_full[2], weights_full[2], products[2], query_full, query_empty, info_full[kInfoRing];
+    uint64_t full[kMaxSlots], empty[kMaxSlots], scores_full[kMaxBuffers], weights_full[kMaxBuffers], products[kMaxBuffers], query_full, query_empty, info_full[kInfoRing];
     uint32_t tmem, abort[1 + 12], info[kInfoRing];
 };
 static_assert(sizeof(PrefixState) <= 1024, "the state's room");
@@ -79,19 +82,19 @@ struct Items {
         *first = part * key_tiles / split, *last = (part + 1) * key_tiles / split;   // (below 2^9 * 2^17)
     }
 };
-// The split that a simple model takes for quickest: rounds of items, each its tiles and four for beginning and end, and a 32nd of a tile for every part to
-// be joined. A warp together.
+// The split that a simple model takes for quickest: rounds of items, each its keys and 512 for beginning and end, and four keys for every part to be joined. A warp together.
+template <uint32_t kKeys>
 __device__ __forceinline__ Items items_of(const PrefixParams& p, uint32_t ctas) {
     Items x;
     x.tokens = shared_tokens(p);
-    x.key_tiles = (x.tokens + kTile - 1) / kTile;
+    x.key_tiles = (x.tokens + kKeys - 1) / kKeys;
     const uint32_t pairs = p.a.kv_heads * p.tiles, room = p.max_items / pairs;
     uint32_t most = x.key_tiles < room ? x.key_tiles : room;
     most = most < kMaxSplit ? most : kMaxSplit;
     uint64_t best = UINT64_MAX;
     for (uint32_t split = 1 + threadIdx.x % 32; split <= most; split += 32) {
         const uint32_t items = pairs * split;   // at most max_items
-        const uint64_t cost = static_cast<uint64_t>((items + ctas - 1) / ctas) * ((x.key_tiles + split - 1) / split + 4) * 32 + items, key = cost << 16 | split;
+        const uint64_t cost = static_cast<uint64_t>((items + ctas - 1) / ctas) * ((x.key_tiles + split - 1) / split + 512 / kKeys) * kKeys + items * 4, key = cost << 16 | split;
         if (key < best) best = key;
     }
 #pragma unroll
@@ -136,7 +139,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
     using S = PrefixShape<kHeadDim>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* const query_smem = smem + S::kSlots * kSlotBytes;
+    uint8_t* const query_smem = smem + S::kSlots * S::kSlot;
     PrefixState* const st = reinterpret_cast<PrefixState*>(query_smem + S::kQueryBytes);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full = smem_u32(st->full), empty = smem_u32(st->empty), scores_full = smem_u32(st->scores_full), weights_full = smem_u32(st->weights_full);
@@ -146,7 +149,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < S::kSlots; ++s) mbar_init(full + 8 * s, 1), mbar_init(empty + 8 * s, 1);
-        for (uint32_t b = 0; b < 2; ++b) mbar_init(scores_full + 8 * b, 1), mbar_init(weights_full + 8 * b, 4), mbar_init(products + 8 * b, 1);
+        for (uint32_t b = 0; b < S::kBuffers; ++b) mbar_init(scores_full + 8 * b, 1), mbar_init(weights_full + 8 * b, 4), mbar_init(products + 8 * b, 1);
         for (uint32_t i = 0; i < kInfoRing; ++i) mbar_init(info_full + 8 * i, 1);
         mbar_init(query_full, 4 * S::kStreams), mbar_init(query_empty, 1);
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_keys) : "memory");
@@ -163,7 +166,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
     tc_fence_after();
     // Everything above runs while the launch before this one drains; from here on its results are read.
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const Items items = items_of(p, gridDim.x);
+    const Items items = items_of<S::kKeys>(p, gridDim.x);
     if (blockIdx.x == 0 && threadIdx.x == 0 && *p.prefix_tokens > static_cast<int32_t>(p.prefix_pages << p.a.page_shift)) atomicCAS(status, 0u, kStatusPage);
     // Does any row end within the prefix?
     bool ends_within = false;
@@ -177,7 +180,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
 
     if (warp == 0 || warp == 3) {
         // ---------------- pages: warp 0 the keys, warp 3 the values ----------------
-        const uint32_t box_shift = p.a.page_shift < 6 ? p.a.page_shift : 6, boxes = kTile >> box_shift, box_bytes = 128u << box_shift;
+        const uint32_t box_shift = p.a.page_shift < 6 ? p.a.page_shift : 6, boxes = S::kKeys >> box_shift, box_bytes = 128u << box_shift;
         const uint32_t beyond = (p.a.pages * p.a.kv_heads) << p.a.page_shift;   // a row behind the cache: TMA reads zeros there
         const CUtensorMap* const map = warp == 0 ? &map_keys : &map_values;
         const uint32_t first_slot = warp == 0 ? 0 : S::kKeySlots, end_slot = warp == 0 ? S::kKeySlots : S::kSlots;
@@ -187,27 +190,27 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
             uint32_t head, tile, first, last;
             items.locate(p, item, &head, &tile, &first, &last);
             auto page_of = [&](uint32_t t) {
-                const uint32_t key = t * kTile + (lane << box_shift);
+                const uint32_t key = t * S::kKeys + (lane << box_shift);
                 return t < last && lane < boxes && key < items.tokens ? __ldg(p.prefix_table + (key >> p.a.page_shift)) : INT32_MIN;
             };
             int32_t page = page_of(first);
             for (uint32_t t = first; alive && t < last; ++t, ++count) {
-                const uint32_t key = t * kTile + (lane << box_shift);
+                const uint32_t key = t * S::kKeys + (lane << box_shift);
                 const bool there = page >= 0 && static_cast<uint32_t>(page) < p.a.pages;
                 if (!there && page != INT32_MIN) atomicCAS(status, 0u, kStatusPage);
                 const uint32_t row = there ? ((static_cast<uint32_t>(page) * p.a.kv_heads + head) << p.a.page_shift) + (key & ((1u << p.a.page_shift) - 1)) : beyond;
                 const uint32_t mask = __ballot_sync(0xffffffffu, there);
                 page = page_of(t + 1);
-                if (warp == 0 && lane == 0) {   // (the ring is that long: keys are loaded three tiles ahead at most of those whose scores the softmax has)
+                if (warp == 0 && lane == 0) {   // (the ring is that long: a ring of keys, and the tiles whose scores are formed, ahead of the softmax)
                     st->info[count % kInfoRing] = mask;
                     mbar_arrive(info_full + 8 * (count % kInfoRing));
                 }
                 __syncwarp();
                 for (uint32_t c = 0; c < S::kChunks; ++c) {
                     if (!(alive = warp_look_wait(empty + 8 * slot, phase, abort_flag, status, kStatusPrefixLoad))) break;
-                    if (lane == 0) mbar_expect_tx(full + 8 * slot, kSlotBytes);
+                    if (lane == 0) mbar_expect_tx(full + 8 * slot, S::kSlot);
                     __syncwarp();
-                    if (lane < boxes) tma_load_2d(smem_u32(smem) + slot * kSlotBytes + lane * box_bytes, map, c * 128, row, full + 8 * slot);
+                    if (lane < boxes) tma_load_2d(smem_u32(smem) + slot * S::kSlot + lane * box_bytes, map, c * 128, row, full + 8 * slot);
                     __syncwarp();
                     if (++slot == end_slot) slot = first_slot, phase ^= 1;
                 }
@@ -216,19 +219,19 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
     } else if (warp == 1) {
         // ---------------- MMA issuer: S of a tile, then O of the tile before it ----------------
         constexpr uint32_t idesc_any = (1u << 4) | (1u << 7) | (1u << 10) | ((kRowsM >> 4) << 24);   // F32 += BF16 x BF16
-        constexpr uint32_t idesc = idesc_any | ((kTile >> 3) << 17), idesc_values = idesc_any | ((128 >> 3) << 17) | (1u << 16);   // V is MN-major
-        const uint32_t slots = low_word(smem_u32(smem), 16), slots_values = low_word(smem_u32(smem), kSlotBytes), queries = low_word(smem_u32(query_smem), 16);
+        constexpr uint32_t idesc = idesc_any | ((S::kKeys >> 3) << 17), idesc_values = idesc_any | ((128 >> 3) << 17) | (1u << 16);   // V is MN-major
+        const uint32_t slots = low_word(smem_u32(smem), 16), slots_values = low_word(smem_u32(smem), S::kSlot), queries = low_word(smem_u32(query_smem), 16);
         uint32_t key_slot = 0, key_phase = 0, slot = S::kKeySlots, phase = 0, scores = 0, done = 0, round = 0;
         bool alive = true;
         auto scores_of_tile = [&]() {
             for (uint32_t c = 0; c < S::kChunks; ++c) {
                 if (!warp_look_wait(full + 8 * key_slot, key_phase, abort_flag, status, kStatusPrefixMma)) return false;
                 tc_fence_after();
-                mma_block<kHighSwizzled, 2>(tmem + S::kScoresAt + (scores & 1) * kTile, queries + c * (kSlotBytes >> 4), slots + key_slot * (kSlotBytes >> 4), idesc, c, 4);
+                mma_block<kHighSwizzled, 2>(tmem + S::kScoresAt + scores % S::kBuffers * S::kKeys, queries + c * (kSlotBytes >> 4), slots + key_slot * (S::kSlot >> 4), idesc, c, 4);
                 commit(empty + 8 * key_slot);
                 if (++key_slot == S::kKeySlots) key_slot = 0, key_phase ^= 1;
             }
-            commit(scores_full + 8 * (scores & 1));
+            commit(scores_full + 8 * (scores % S::kBuffers));
             ++scores;
             return true;
         };
@@ -236,23 +239,24 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
             uint32_t head, tile, first, last;
             items.locate(p, item, &head, &tile, &first, &last);
             if (!warp_look_wait(query_full, round & 1, abort_flag, status, kStatusPrefixMma)) break;
-            // (S of a tile goes where the weights of two tiles before were read by MMAs that were issued earlier; a new item's where the last one's were)
-            alive = scores_of_tile();
+            // (S of a tile goes where the weights of kBuffers tiles before were read by MMAs that were issued earlier; a new item's where the last one's were)
+            uint32_t formed = first;
             for (uint32_t t = first; alive && t < last; ++t) {
-                if (t + 1 < last) {
-                    if (!(alive = scores_of_tile())) break;
+                for (; alive && formed < last && formed < t + S::kBuffers; ++formed) {
+                    alive = scores_of_tile();
+                    if (formed + 1 == last) commit(query_empty);
                 }
-                if (t + 1 >= last) commit(query_empty);
-                const uint32_t buffer = done & 1, d = tmem + S::kOutAt + (S::kStreams == 2 ? buffer * kHeadDim : 0);
+                if (!alive) break;
+                const uint32_t buffer = done % S::kBuffers, d = tmem + S::kOutAt + (S::kStreams == 2 ? (done & 1) * kHeadDim : 0);
                 const uint32_t follows = t >= first + S::kStreams;
-                if (!(alive = warp_look_wait(weights_full + 8 * buffer, done >> 1 & 1, abort_flag, status, kStatusPrefixProduct))) break;
+                if (!(alive = warp_look_wait(weights_full + 8 * buffer, done / S::kBuffers & 1, abort_flag, status, kStatusPrefixProduct))) break;
                 for (uint32_t c = 0; c < S::kChunks; c += 2) {   // 128 dims: two slots, side by side
                     alive = warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusPrefixProduct) && warp_look_wait(full + 8 * (slot + 1), phase, abort_flag, status, kStatusPrefixProduct);
                     if (!alive) break;
                     tc_fence_after();
-                    const uint32_t a = tmem + S::kScoresAt + buffer * kTile, b = slots_values + slot * (kSlotBytes >> 4);   // 16 keys: 8 columns of P, 16 rows of V
+                    const uint32_t a = tmem + S::kScoresAt + buffer * S::kKeys, b = slots_values + slot * (S::kSlot >> 4);   // 16 keys: 8 columns of P, 16 rows of V
                     mma_block_from_tmem<(16 * 128 >> 4)>(d + c * 64, a, b, idesc_values, follows);
-                    mma_block_from_tmem<(16 * 128 >> 4)>(d + c * 64, a + 32, b + 4 * (16 * 128 >> 4), idesc_values, 1);
+                    if (S::kKeys == 128) mma_block_from_tmem<(16 * 128 >> 4)>(d + c * 64, a + 32, b + 4 * (16 * 128 >> 4), idesc_values, 1);
                     commit(empty + 8 * slot);
                     commit(empty + 8 * (slot + 1));
                     slot += 2;
@@ -266,7 +270,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
     } else if (warp >= 4) {
         // ---------------- queries of an item, then the softmax: a query a thread ----------------
         const uint32_t stream = (warp - 4) / 4, thread = threadIdx.x & 127, lanes = ((warp & 3) * 32) << 16;
-        const uint32_t box_shift = p.a.page_shift < 6 ? p.a.page_shift : 6, all_boxes = (1u << (kTile >> box_shift)) - 1;
+        const uint32_t box_shift = p.a.page_shift < 6 ? p.a.page_shift : 6, all_boxes = (1u << (S::kKeys >> box_shift)) - 1;
         const uint32_t out = tmem + S::kOutAt + stream * (S::kStreams == 2 ? kHeadDim : 0) + lanes;
         const float scale = p.a.scale_log2;
         uint32_t count = 0, round = 0;   // tiles and items of this CTA
@@ -315,16 +319,16 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
             bool started = false;
             uint32_t first_key = 0;
             for (uint32_t t = first; t < last; ++t, ++count) {
-                const uint32_t buffer = count & 1;
-                if (S::kStreams == 2 && buffer != stream) continue;
+                const uint32_t buffer = count % S::kBuffers;
+                if (S::kStreams == 2 && (count & 1) != stream) continue;
                 if (!warp_look_wait(info_full + 8 * (count % kInfoRing), count / kInfoRing & 1, abort_flag, status, kStatusPrefixInfo) ||
-                    !warp_look_wait(scores_full + 8 * buffer, count >> 1 & 1, abort_flag, status, kStatusPrefixScores)) {
+                    !warp_look_wait(scores_full + 8 * buffer, count / S::kBuffers & 1, abort_flag, status, kStatusPrefixScores)) {
                     alive = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t there = st->info[count % kInfoRing], key = t * kTile, from = tmem + S::kScoresAt + buffer * kTile + lanes;
-                const bool masked = there != all_boxes || key + kTile > seen_by_all;
+                const uint32_t there = st->info[count % kInfoRing], key = t * S::kKeys, from = tmem + S::kScoresAt + buffer * S::kKeys + lanes;
+                const bool masked = there != all_boxes || key + S::kKeys > seen_by_all;
                 // Which of 32 keys from c on this row sees.
                 auto seen = [&](uint32_t c) {
                     uint32_t bits = limit <= key + c ? 0 : limit - key - c >= 32 ? 0xffffffffu : (1u << (limit - key - c)) - 1;
@@ -332,13 +336,13 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
                     else bits &= (there >> (c >> 4) & 1 ? 0xffffu : 0) | (there >> ((c >> 4) + 1) & 1 ? 0xffff0000u : 0);
                     return bits;
                 };
-                uint32_t v[kTile];
+                uint32_t v[S::kKeys];
 #pragma unroll
-                for (uint32_t c = 0; c < kTile; c += 32) tc_load32(from + c, reinterpret_cast<uint32_t(&)[32]>(v[c]));
+                for (uint32_t c = 0; c < S::kKeys; c += 32) tc_load32(from + c, reinterpret_cast<uint32_t(&)[32]>(v[c]));
                 tc_wait_ld();
                 if (masked) {
 #pragma unroll
-                    for (uint32_t c = 0; c < kTile; c += 32) {
+                    for (uint32_t c = 0; c < S::kKeys; c += 32) {
                         const uint32_t bits = seen(c);
 #pragma unroll
                         for (uint32_t i = 0; i < 32; ++i) v[c + i] = bits >> i & 1 ? v[c + i] : __float_as_uint(scale < 0.0f ? INFINITY : -INFINITY);
@@ -349,12 +353,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
                 if (scale < 0.0f) {
                     float m[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
 #pragma unroll
-                    for (uint32_t i = 0; i < kTile; i += 2) m[i / 2 % 4] = fminf(fminf(m[i / 2 % 4], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
+                    for (uint32_t i = 0; i < S::kKeys; i += 2) m[i / 2 % 4] = fminf(fminf(m[i / 2 % 4], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
                     most = fminf(fminf(m[0], m[1]), fminf(m[2], m[3]));
                 } else {
                     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (uint32_t i = 0; i < kTile; i += 2) m[i / 2 % 4] = fmaxf(fmaxf(m[i / 2 % 4], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
+                    for (uint32_t i = 0; i < S::kKeys; i += 2) m[i / 2 % 4] = fmaxf(fmaxf(m[i / 2 % 4], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
                     most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                 }
                 const float top = fmaxf(reference, most * scale);
@@ -366,7 +370,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
                     if (started) {
                         // the stream's tile before has to be through
                         const uint32_t earlier = count - S::kStreams;
-                        if (!warp_look_wait(products + 8 * (earlier & 1), earlier >> 1 & 1, abort_flag, status, kStatusPrefixProduct)) {
+                        if (!warp_look_wait(products + 8 * (earlier % S::kBuffers), earlier / S::kBuffers & 1, abort_flag, status, kStatusPrefixProduct)) {
                             alive = false;
                             break;
                         }
@@ -386,7 +390,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
                 started = true;
                 const float minus = reference == -INFINITY ? 0.0f : -reference;
 #pragma unroll
-                for (uint32_t c = 0; c < kTile; c += 32) {
+                for (uint32_t c = 0; c < S::kKeys; c += 32) {
                     uint32_t packed[16];
 #pragma unroll
                     for (uint32_t i = 0; i < 32; i += 2) fma2(v[c + i], v[c + i + 1], scale, minus);
@@ -415,7 +419,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
             const uint64_t part = static_cast<uint64_t>(item) * S::kStreams + stream;
             if (started) {
                 const uint32_t final = count - 1 - (S::kStreams == 2 && ((count - 1) & 1) != stream ? 1 : 0);   // the stream's last tile
-                if (!warp_look_wait(products + 8 * (final & 1), final >> 1 & 1, abort_flag, status, kStatusPrefixProduct)) break;
+                if (!warp_look_wait(products + 8 * (final % S::kBuffers), final / S::kBuffers & 1, abort_flag, status, kStatusPrefixProduct)) break;
                 tc_fence_after();
                 float4* const to = reinterpret_cast<float4*>(p.parts) + part * (kHeadDim / 4) * kRowsM + thread;
 #pragma unroll 1
@@ -694,7 +698,7 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const __gri
     if (threadIdx.x < kQueries) live[threadIdx.x] = 0;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const Items items = items_of(p, ctas);
+    const Items items = items_of<S::kKeys>(p, ctas);
     const uint32_t group = p.a.query_heads / p.a.kv_heads, all_queries = p.a.rows * group, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t slice = blockIdx.x % kSlices, tile = blockIdx.x / kSlices % p.tiles, head = blockIdx.x / kSlices / p.tiles;
     const uint32_t query0 = tile * kRowsM + slice * kQueries;
