@@ -120,6 +120,11 @@ static __device__ __noinline__ bool warp_wait_suspended(uint32_t bar, uint32_t p
     return mbar_wait_suspended(bar, parity, abort_flag, status_word, code) || !warp_gives_up(bar, parity, abort_flag);
 }
 
+// A look, then the suspended wait: for kernels many of whose warps wait at the same time, where those that poll make every look of the others slow.
+__device__ __forceinline__ bool warp_look_suspended(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* status_word, uint32_t code) {
+    return mbar_test(bar, parity) || warp_wait_suspended(bar, parity, abort_flag, status_word, code);
+}
+
 // One lane of a converged warp. The threads that issue tcgen05 and TMA operations run their loops as whole warps and elect
 // a lane around the operations only: addresses and descriptors then live in uniform registers, where those instructions
 // want them. (In a loop that a single thread runs every operand is moved there first: 70 cycles per MMA or copy.)

@@ -275,7 +275,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
         int32_t page = page_of();
         // The first tile's keys go before its values: the scores can be worked on while the values come.
         const uint32_t keys_first = smem_u32(&st->keys_first);
-        if (warp == 3 && tiles.valid) alive = warp_look_wait(keys_first, 0, abort_flag, status, kStatusLoad);
+        if (warp == 3 && tiles.valid) alive = warp_look_suspended(keys_first, 0, abort_flag, status, kStatusLoad);
         for (uint32_t tile = 0; alive && tiles.valid; ++tile) {
             // the row of the cache where this lane's box of the tile starts, and which lanes have one
             const bool there = page >= 0 && static_cast<uint32_t>(page) < p.pages;
@@ -297,7 +297,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             const uint32_t first_slot = warp == 0 ? 0 : S::kKeySlots, slots = warp == 0 ? S::kKeySlots : S::kValueSlots, use = S::kChunks * tile;
             uint32_t slot = first_slot + use % slots, phase = use / slots & 1 ^ 1;
             for (uint32_t c = 0; c < S::kChunks; ++c) {
-                if (!warp_look_wait(empty + 8 * slot, phase, abort_flag, status, kStatusLoad)) {
+                if (!warp_look_suspended(empty + 8 * slot, phase, abort_flag, status, kStatusLoad)) {
                     alive = false;
                     break;
                 }
@@ -326,10 +326,10 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
         bool alive = true;
         auto scores_of_tile = [&]() {
             const uint32_t buffer = scores & 1, query = S::kQueryBuffers == 2 ? pair & 1 : 0;
-            if (ahead.first() && !warp_look_wait(query_full + 8 * query, (S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1, abort_flag, status, kStatusMma)) return false;
-            if (!warp_look_wait(scores_empty + 8 * buffer, (scores >> 1 & 1) ^ 1, abort_flag, status, kStatusMma)) return false;
+            if (ahead.first() && !warp_look_suspended(query_full + 8 * query, (S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1, abort_flag, status, kStatusMma)) return false;
+            if (!warp_look_suspended(scores_empty + 8 * buffer, (scores >> 1 & 1) ^ 1, abort_flag, status, kStatusMma)) return false;
             for (uint32_t c = 0; c < S::kChunks; ++c) {
-                if (!warp_look_wait(full + 8 * key_slot, key_phase, abort_flag, status, kStatusMma)) return false;
+                if (!warp_look_suspended(full + 8 * key_slot, key_phase, abort_flag, status, kStatusMma)) return false;
                 tc_fence_after();
                 const uint32_t a = slots + key_slot * (kSlotBytes >> 4), b = queries + ((query * S::kQueryBytes + c * S::kScores * 128) >> 4);
                 mma_block_e4m3<kHighSwizzled, 2, 2>(tmem + buffer * S::kScores, a, b, idesc, c, 4);
@@ -348,9 +348,9 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
         };
         auto product_of_tile = [&]() {
             const uint32_t buffer = products & 1, steps = (now.keys() + 31) / 32;
-            if (!warp_look_wait(weights_full + 8 * buffer, products >> 1 & 1, abort_flag, status, kStatusProduct)) return false;
+            if (!warp_look_suspended(weights_full + 8 * buffer, products >> 1 & 1, abort_flag, status, kStatusProduct)) return false;
             for (uint32_t h = 0; h < S::kChunks; ++h) {
-                if (!warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusProduct)) return false;
+                if (!warp_look_suspended(full + 8 * slot, phase, abort_flag, status, kStatusProduct)) return false;
                 tc_fence_after();
                 // 32 keys: 32 rows of 128 bytes of V, of 32 bytes of W
                 mma_block_e4m3<kHighWeights, (32 * 128 >> 4), (32 * 32 >> 4)>(tmem_out + h * S::kTerms, slots + slot * (kSlotBytes >> 4), weights + ((buffer * S::kWeightBytes) >> 4),
@@ -394,7 +394,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             }
             SplitQueries<kHeadDim, kN> split;
             split.open(from_here, queries, group, p.query_heads, 0, 1, lane);
-            if (!warp_look_wait(query_empty + 8 * buffer, (pair >> 1 & 1) ^ 1, abort_flag, status, kStatusQuery)) break;
+            if (!warp_look_suspended(query_empty + 8 * buffer, (pair >> 1 & 1) ^ 1, abort_flag, status, kStatusQuery)) break;
             split.run(query_smem + buffer * S::kQueryBytes, st->query_scale[buffer], lane);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -414,7 +414,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             __syncwarp();
             if (lane == 0) mbar_arrive(group_bar);
         };
-        auto all_came = [&]() { return warp_look_wait(group_bar, meetings++ & 1, abort_flag, status, kStatusGroup); };
+        auto all_came = [&]() { return warp_look_suspended(group_bar, meetings++ & 1, abort_flag, status, kStatusGroup); };
         auto meet = [&]() {
             come();
             return all_came();
@@ -436,13 +436,13 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             if (S::kQueryBuffers == 1 && any) {
                 SplitQueries<kHeadDim, kN> split;
                 split.open(p.query + (static_cast<uint64_t>(first_row) * p.query_heads + walk.head * group) * kHeadDim + lane % (kHeadDim / 8) * 8, queries, group, p.query_heads, quadrant, 4, lane);
-                if (!warp_look_wait(query_empty, (pair & 1) ^ 1, abort_flag, status, kStatusQuery)) break;
+                if (!warp_look_suspended(query_empty, (pair & 1) ^ 1, abort_flag, status, kStatusQuery)) break;
                 split.run(query_smem, st->query_scale[0], lane);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(query_full);
             }
-            if (any && !warp_look_wait(query_full + 8 * query_buffer, (S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1, abort_flag, status, kStatusQuery)) break;
+            if (any && !warp_look_suspended(query_full + 8 * query_buffer, (S::kQueryBuffers == 2 ? pair >> 1 : pair) & 1, abort_flag, status, kStatusQuery)) break;
             const int32_t seen_by_all = static_cast<int32_t>(walk.length) - static_cast<int32_t>(walk.tokens) + 1;
             float sum[kBlock];   // this thread's part of the denominators
 #pragma unroll
@@ -451,7 +451,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             uint32_t next_there = 0, next_bytes = 0;
             auto fetch = [&](uint32_t t) {
                 const uint32_t at = t % kTileInfos;
-                if (!warp_look_wait(scales_full + 8 * at, t / kTileInfos & 1, abort_flag, status, kStatusScores)) return false;
+                if (!warp_look_suspended(scales_full + 8 * at, t / kTileInfos & 1, abort_flag, status, kStatusScores)) return false;
                 next_there = st->info[at], next_bytes = st->scales[at][thread];
                 return true;
             };
@@ -494,8 +494,8 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                     }
                     return passes;
                 };
-                if (!warp_look_wait(weights_empty + 8 * buffer, (tile >> 1 & 1) ^ 1, abort_flag, status, kStatusProduct) ||
-                    !warp_look_wait(scores_full + 8 * buffer, tile >> 1 & 1, abort_flag, status, kStatusScores)) {
+                if (!warp_look_suspended(weights_empty + 8 * buffer, (tile >> 1 & 1) ^ 1, abort_flag, status, kStatusProduct) ||
+                    !warp_look_suspended(scores_full + 8 * buffer, tile >> 1 & 1, abort_flag, status, kStatusScores)) {
                     alive = false;
                     break;
                 }
@@ -555,7 +555,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                             break;
                         }
                         if (again) {
-                            if (!warp_look_wait(weights_empty + 8 * (buffer ^ 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) {
+                            if (!warp_look_suspended(weights_empty + 8 * (buffer ^ 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) {
                                 alive = false;
                                 break;
                             }
@@ -667,14 +667,14 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                 if (!whole) {
                     // Rows of V that are no token's are multiplied with weights of zero: whatever lies there, they must be numbers.
                     // These warps do not wait for every use of a slot, so they must not be more than one ahead: the tile before has to be through.
-                    if (tile && !warp_look_wait(weights_empty + 8 * (buffer ^ 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) {
+                    if (tile && !warp_look_suspended(weights_empty + 8 * (buffer ^ 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) {
                         alive = false;
                         break;
                     }
                     const uint32_t use = S::kChunks * tile;
                     uint32_t slot = S::kKeySlots + use % S::kValueSlots, phase = use / S::kValueSlots & 1;
                     for (uint32_t c = 0; alive && c < S::kChunks; ++c) {
-                        if (!warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusValues)) {
+                        if (!warp_look_suspended(full + 8 * slot, phase, abort_flag, status, kStatusValues)) {
                             alive = false;
                             break;
                         }
@@ -725,7 +725,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                 if (!meet()) break;
                 if (thread < kN) st->total[thread] = ((st->wide[thread].x + st->wide[thread].y) + (st->wide[thread].z + st->wide[thread].w)) * static_cast<float>(1ull << (60 - static_cast<int>(kLift)));
                 if (!meet()) break;
-                if (!warp_look_wait(weights_empty + 8 * ((tile - 1) & 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) break;
+                if (!warp_look_suspended(weights_empty + 8 * ((tile - 1) & 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) break;
                 tc_fence_after();
             }
             const bool alone = walk.starts && walk.ends;

@@ -26,7 +26,7 @@ static_assert(sizeof(augur_cuda_nvfp4_sm100_shared_prefix_attention_args_v1) == 
 constexpr uint32_t kRowsM = 128;               // queries of a CTA
 constexpr uint32_t kRounds = 3;                // a device's worth of CTAs, at most so many times, where the prefix is split for it
 constexpr uint32_t kMaxSplit = 256, kMaxChunks = 32;   // of the prefix, and of a sequence's own tokens
-constexpr uint32_t kInfoRing = 16, kMaxSlots = 24, kMaxBuffers = 4;
+constexpr uint32_t kInfoRing = 16, kMaxSlots = 12, kMaxBuffers = 4;
 constexpr uint32_t kStatusPrefixLoad = 0x421, kStatusPrefixMma = 0x422, kStatusPrefixScores = 0x423, kStatusPrefixQuery = 0x424, kStatusPrefixProduct = 0x425, kStatusPrefixInfo = 0x426;
 
 struct PrefixParams {
@@ -50,17 +50,17 @@ __device__ __forceinline__ uint32_t shared_tokens(const PrefixParams& p) {
 
 template <uint32_t kHeadDim>
 struct PrefixShape {
-    static constexpr uint32_t kChunks = kHeadDim / 64, kStreams = kHeadDim == 128 ? 2 : 1;
+    static constexpr uint32_t kParts = kHeadDim / 128, kStreams = kHeadDim == 128 ? 2 : 1;
     // Keys of a tile, and S in tensor memory: 256 columns of it. With two streams each has two, so that the next scores are formed while its softmax is at work (of 128 keys
     // and one each, the weights' product and the next scores behind it were waited for: 2300 cycles for 128 keys, NN now).
-    static constexpr uint32_t kKeys = kHeadDim == 128 ? 64 : 128, kBuffers = 256 / kKeys, kSlot = kKeys * 128;
-    static constexpr uint32_t kThreads = 128 + 128 * kStreams;   // warp 0 loads keys, 1 MMA, 3 values, then the softmax
+    static constexpr uint32_t kKeys = kHeadDim == 128 ? 64 : 128, kBuffers = 256 / kKeys, kSlot = kKeys * 256;   // a slot: 128 dims of a tile, as two halves of 128 bytes a key
+    static constexpr uint32_t kThreads = 128 + 128 * kStreams;   // warp 0 loads keys, 1 and 2 MMA, 3 values, then the softmax
     static constexpr uint32_t kQueryBytes = kRowsM * kHeadDim * 2, kSlots = (224 * 1024 - kQueryBytes) / kSlot;
-    // A ring each for the keys and the values, so that two warps deal out the copies: one alone took 80 cycles a copy, and pages of 16 tokens are eight copies a slot.
-    static constexpr uint32_t kValueSlots = (kSlots / 2 + 1) / 2 * 2, kKeySlots = kSlots - kValueSlots;   // (pairs of value slots are one operand)
+    // A ring each for the keys and the values, so that two warps deal out the copies: one alone took 80 cycles a copy, and pages of 16 tokens are up to 16 copies a slot.
+    static constexpr uint32_t kKeySlots = kSlots / 2, kValueSlots = kSlots - kKeySlots;
     static constexpr uint32_t kSmem = 1024 + kQueryBytes + kSlots * kSlot + 1024;
     static constexpr uint32_t kScoresAt = 0, kOutAt = 256;       // tensor memory: S, then one O per stream
-    static_assert(kSlots <= kMaxSlots && kKeySlots / kChunks + kBuffers + 1 <= kInfoRing && kKeySlots >= kChunks && kValueSlots >= kChunks && kChunks % 2 == 0 && kSmem <= kSmemLimit && kOutAt + kStreams * kHeadDim == 512, "a CTA's memory");
+    static_assert(kSlots <= kMaxSlots && kKeySlots / kParts + kBuffers + 1 <= kInfoRing && kKeySlots >= kParts && kValueSlots >= kParts && kSmem <= kSmemLimit && kOutAt + kStreams * kHeadDim == 512, "a CTA's memory");
 };
 
 struct PrefixState {
@@ -190,81 +190,85 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
             uint32_t head, tile, first, last;
             items.locate(p, item, &head, &tile, &first, &last);
             auto page_of = [&](uint32_t t) {
-                const uint32_t key = t * S::kKeys + (lane << box_shift);
-                return t < last && lane < boxes && key < items.tokens ? __ldg(p.prefix_table + (key >> p.a.page_shift)) : INT32_MIN;
+                const uint32_t key = t * S::kKeys + ((lane % boxes) << box_shift);   // (the second half of a slot by the lanes behind)
+                return t < last && lane < 2 * boxes && key < items.tokens ? __ldg(p.prefix_table + (key >> p.a.page_shift)) : INT32_MIN;
             };
             int32_t page = page_of(first);
             for (uint32_t t = first; alive && t < last; ++t, ++count) {
-                const uint32_t key = t * S::kKeys + (lane << box_shift);
+                const uint32_t key = t * S::kKeys + ((lane % boxes) << box_shift);
                 const bool there = page >= 0 && static_cast<uint32_t>(page) < p.a.pages;
                 if (!there && page != INT32_MIN) atomicCAS(status, 0u, kStatusPage);
                 const uint32_t row = there ? ((static_cast<uint32_t>(page) * p.a.kv_heads + head) << p.a.page_shift) + (key & ((1u << p.a.page_shift) - 1)) : beyond;
-                const uint32_t mask = __ballot_sync(0xffffffffu, there);
+                const uint32_t mask = __ballot_sync(0xffffffffu, there && lane < boxes);
                 page = page_of(t + 1);
                 if (warp == 0 && lane == 0) {   // (the ring is that long: a ring of keys, and the tiles whose scores are formed, ahead of the softmax)
                     st->info[count % kInfoRing] = mask;
                     mbar_arrive(info_full + 8 * (count % kInfoRing));
                 }
                 __syncwarp();
-                for (uint32_t c = 0; c < S::kChunks; ++c) {
-                    if (!(alive = warp_look_wait(empty + 8 * slot, phase, abort_flag, status, kStatusPrefixLoad))) break;
+                for (uint32_t c = 0; c < S::kParts; ++c) {
+                    if (!(alive = warp_look_suspended(empty + 8 * slot, phase, abort_flag, status, kStatusPrefixLoad))) break;
                     if (lane == 0) mbar_expect_tx(full + 8 * slot, S::kSlot);
                     __syncwarp();
-                    if (lane < boxes) tma_load_2d(smem_u32(smem) + slot * S::kSlot + lane * box_bytes, map, c * 128, row, full + 8 * slot);
+                    if (lane < 2 * boxes) tma_load_2d(smem_u32(smem) + slot * S::kSlot + lane * box_bytes, map, c * 256 + (lane < boxes ? 0 : 128), row, full + 8 * slot);
                     __syncwarp();
                     if (++slot == end_slot) slot = first_slot, phase ^= 1;
                 }
             }
         }
-    } else if (warp == 1) {
-        // ---------------- MMA issuer: S of a tile, then O of the tile before it ----------------
+    } else if (warp == 1 || (warp == 2 && S::kStreams == 2)) {
+        // ---------------- MMA issuer: S of a tile, then O of a tile before it. With two streams a warp for each: what one has to wait for, look at and say for a tile took
+        // 1370 cycles for 64 keys, more than the products or the softmax. ----------------
         constexpr uint32_t idesc_any = (1u << 4) | (1u << 7) | (1u << 10) | ((kRowsM >> 4) << 24);   // F32 += BF16 x BF16
         constexpr uint32_t idesc = idesc_any | ((S::kKeys >> 3) << 17), idesc_values = idesc_any | ((128 >> 3) << 17) | (1u << 16);   // V is MN-major
-        const uint32_t slots = low_word(smem_u32(smem), 16), slots_values = low_word(smem_u32(smem), S::kSlot), queries = low_word(smem_u32(query_smem), 16);
+        const uint32_t slots = low_word(smem_u32(smem), 16), slots_values = low_word(smem_u32(smem), S::kSlot / 2), queries = low_word(smem_u32(query_smem), 16);
+        const bool forms = warp == 1, multiplies = warp == 2 || S::kStreams == 1;
         uint32_t key_slot = 0, key_phase = 0, slot = S::kKeySlots, phase = 0, scores = 0, done = 0, round = 0;
         bool alive = true;
         auto scores_of_tile = [&]() {
-            for (uint32_t c = 0; c < S::kChunks; ++c) {
-                if (!warp_look_wait(full + 8 * key_slot, key_phase, abort_flag, status, kStatusPrefixMma)) return false;
+            const uint32_t buffer = scores % S::kBuffers;
+            // S goes where the weights of kBuffers tiles before were: of this warp's own MMAs those that read them are ahead in the pipe
+            if (S::kStreams == 2 && scores >= S::kBuffers && !warp_look_suspended(products + 8 * buffer, scores / S::kBuffers - 1 & 1, abort_flag, status, kStatusPrefixMma)) return false;
+            for (uint32_t c = 0; c < S::kParts; ++c) {
+                if (!warp_look_suspended(full + 8 * key_slot, key_phase, abort_flag, status, kStatusPrefixMma)) return false;
                 tc_fence_after();
-                mma_block<kHighSwizzled, 2>(tmem + S::kScoresAt + scores % S::kBuffers * S::kKeys, queries + c * (kSlotBytes >> 4), slots + key_slot * (S::kSlot >> 4), idesc, c, 4);
+                const uint32_t d = tmem + S::kScoresAt + buffer * S::kKeys, a = queries + 2 * c * (kSlotBytes >> 4), b = slots + key_slot * (S::kSlot >> 4);
+                mma_block<kHighSwizzled, 2>(d, a, b, idesc, c, 4);
+                mma_block<kHighSwizzled, 2>(d, a + (kSlotBytes >> 4), b + (S::kSlot >> 5), idesc, 1, 4);
                 commit(empty + 8 * key_slot);
                 if (++key_slot == S::kKeySlots) key_slot = 0, key_phase ^= 1;
             }
-            commit(scores_full + 8 * (scores % S::kBuffers));
+            commit(scores_full + 8 * buffer);
             ++scores;
+            return true;
+        };
+        auto product_of_tile = [&](bool follows) {
+            const uint32_t buffer = done % S::kBuffers, d = tmem + S::kOutAt + (S::kStreams == 2 ? (done & 1) * kHeadDim : 0);
+            if (!warp_look_suspended(weights_full + 8 * buffer, done / S::kBuffers & 1, abort_flag, status, kStatusPrefixProduct)) return false;
+            for (uint32_t c = 0; c < S::kParts; ++c) {
+                if (!warp_look_suspended(full + 8 * slot, phase, abort_flag, status, kStatusPrefixProduct)) return false;
+                tc_fence_after();
+                const uint32_t a = tmem + S::kScoresAt + buffer * S::kKeys, b = slots_values + slot * (S::kSlot >> 4);   // 16 keys: 8 columns of P, 16 rows of V
+                mma_block_from_tmem<(16 * 128 >> 4)>(d + c * 128, a, b, idesc_values, follows);
+                if (S::kKeys == 128) mma_block_from_tmem<(16 * 128 >> 4)>(d + c * 128, a + 32, b + 4 * (16 * 128 >> 4), idesc_values, 1);
+                commit(empty + 8 * slot);
+                if (++slot == S::kSlots) slot = S::kKeySlots, phase ^= 1;
+            }
+            commit(products + 8 * buffer);
+            ++done;
             return true;
         };
         for (uint32_t item = blockIdx.x; alive && item < items.count; item += gridDim.x, ++round) {
             uint32_t head, tile, first, last;
             items.locate(p, item, &head, &tile, &first, &last);
-            if (!warp_look_wait(query_full, round & 1, abort_flag, status, kStatusPrefixMma)) break;
-            // (S of a tile goes where the weights of kBuffers tiles before were read by MMAs that were issued earlier; a new item's where the last one's were)
+            if (forms && !warp_look_suspended(query_full, round & 1, abort_flag, status, kStatusPrefixMma)) break;
             uint32_t formed = first;
             for (uint32_t t = first; alive && t < last; ++t) {
-                for (; alive && formed < last && formed < t + S::kBuffers; ++formed) {
+                for (; alive && forms && formed < last && (!multiplies || formed < t + S::kBuffers); ++formed) {
                     alive = scores_of_tile();
                     if (formed + 1 == last) commit(query_empty);
                 }
-                if (!alive) break;
-                const uint32_t buffer = done % S::kBuffers, d = tmem + S::kOutAt + (S::kStreams == 2 ? (done & 1) * kHeadDim : 0);
-                const uint32_t follows = t >= first + S::kStreams;
-                if (!(alive = warp_look_wait(weights_full + 8 * buffer, done / S::kBuffers & 1, abort_flag, status, kStatusPrefixProduct))) break;
-                for (uint32_t c = 0; c < S::kChunks; c += 2) {   // 128 dims: two slots, side by side
-                    alive = warp_look_wait(full + 8 * slot, phase, abort_flag, status, kStatusPrefixProduct) && warp_look_wait(full + 8 * (slot + 1), phase, abort_flag, status, kStatusPrefixProduct);
-                    if (!alive) break;
-                    tc_fence_after();
-                    const uint32_t a = tmem + S::kScoresAt + buffer * S::kKeys, b = slots_values + slot * (S::kSlot >> 4);   // 16 keys: 8 columns of P, 16 rows of V
-                    mma_block_from_tmem<(16 * 128 >> 4)>(d + c * 64, a, b, idesc_values, follows);
-                    if (S::kKeys == 128) mma_block_from_tmem<(16 * 128 >> 4)>(d + c * 64, a + 32, b + 4 * (16 * 128 >> 4), idesc_values, 1);
-                    commit(empty + 8 * slot);
-                    commit(empty + 8 * (slot + 1));
-                    slot += 2;
-                    if (slot == S::kSlots) slot = S::kKeySlots, phase ^= 1;
-                }
-                if (!alive) break;
-                commit(products + 8 * buffer);
-                ++done;
+                if (multiplies) alive = alive && product_of_tile(t >= first + S::kStreams);
             }
         }
     } else if (warp >= 4) {
@@ -280,7 +284,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
             items.locate(p, item, &head, &tile, &first, &last);
             // The item's queries in the 128-byte swizzle of the operand, once the products of the item before are through; past the last they are zero. (All of these warps: by
             // one alone they were there after 5.4 us.)
-            if (!warp_look_wait(query_empty, (round & 1) ^ 1, abort_flag, status, kStatusPrefixQuery)) break;
+            if (!warp_look_suspended(query_empty, (round & 1) ^ 1, abort_flag, status, kStatusPrefixQuery)) break;
             {
                 // a lane's piece of every (kWarps * 32 / kPieces)-th row; its token and the head among those that share the key-value head go along
                 constexpr uint32_t kPieces = kHeadDim / 8, kWarps = 4 * S::kStreams, kStep = kWarps * 32 / kPieces;
@@ -321,8 +325,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
             for (uint32_t t = first; t < last; ++t, ++count) {
                 const uint32_t buffer = count % S::kBuffers;
                 if (S::kStreams == 2 && (count & 1) != stream) continue;
-                if (!warp_look_wait(info_full + 8 * (count % kInfoRing), count / kInfoRing & 1, abort_flag, status, kStatusPrefixInfo) ||
-                    !warp_look_wait(scores_full + 8 * buffer, count / S::kBuffers & 1, abort_flag, status, kStatusPrefixScores)) {
+                if (!warp_look_suspended(info_full + 8 * (count % kInfoRing), count / kInfoRing & 1, abort_flag, status, kStatusPrefixInfo) ||
+                    !warp_look_suspended(scores_full + 8 * buffer, count / S::kBuffers & 1, abort_flag, status, kStatusPrefixScores)) {
                     alive = false;
                     break;
                 }
@@ -370,7 +374,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
                     if (started) {
                         // the stream's tile before has to be through
                         const uint32_t earlier = count - S::kStreams;
-                        if (!warp_look_wait(products + 8 * (earlier % S::kBuffers), earlier / S::kBuffers & 1, abort_flag, status, kStatusPrefixProduct)) {
+                        if (!warp_look_suspended(products + 8 * (earlier % S::kBuffers), earlier / S::kBuffers & 1, abort_flag, status, kStatusPrefixProduct)) {
                             alive = false;
                             break;
                         }
@@ -419,7 +423,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_keys, const __gr
             const uint64_t part = static_cast<uint64_t>(item) * S::kStreams + stream;
             if (started) {
                 const uint32_t final = count - 1 - (S::kStreams == 2 && ((count - 1) & 1) != stream ? 1 : 0);   // the stream's last tile
-                if (!warp_look_wait(products + 8 * (final % S::kBuffers), final / S::kBuffers & 1, abort_flag, status, kStatusPrefixProduct)) break;
+                if (!warp_look_suspended(products + 8 * (final % S::kBuffers), final / S::kBuffers & 1, abort_flag, status, kStatusPrefixProduct)) break;
                 tc_fence_after();
                 float4* const to = reinterpret_cast<float4*>(p.parts) + part * (kHeadDim / 4) * kRowsM + thread;
 #pragma unroll 1
