@@ -30,27 +30,34 @@ struct AppendParams {
 };
 
 // The scale byte of the eight elements x of each of kLanes lanes and their codes: the scale is the smallest power of two, of the ones allowed, with which
-// the largest element that is a number is at most 448 = 1.75 * 2^8.
+// the largest element that is a number is at most 448 = 1.75 * 2^8. Elements that are looked at one by one only where one of the head's is infinite or
+// too large (a maximum passes over NaN, and the conversion keeps it).
 template <uint32_t kLanes>
 __device__ __forceinline__ uint2 quantise_head(float (&x)[8], unsigned mask, uint32_t* scale) {
     float most = 0.0f;
 #pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
+    for (uint32_t e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
 #pragma unroll
     for (uint32_t step = kLanes / 2; step; step /= 2) most = fmaxf(most, __shfl_xor_sync(mask, most, step));
+    constexpr float kLargest = 448.0f * (1ull << (kE4m3LargestScale - 127));
+    if (most > kLargest) {
+        most = 0.0f;
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            most = fmaxf(most, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
+            if (fabsf(x[e]) > kLargest) x[e] = __uint_as_float(0x7fc00000u);   // (the conversion would clamp it)
+        }
+#pragma unroll
+        for (uint32_t step = kLanes / 2; step; step /= 2) most = fmaxf(most, __shfl_xor_sync(mask, most, step));
+    }
     const uint32_t bits = __float_as_uint(most), exact = (bits >> 23) + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
     const uint32_t byte = exact < kE4m3LeastScale + 8 ? kE4m3LeastScale : exact > kE4m3LargestScale + 8 ? kE4m3LargestScale : exact - 8;
     const float inverse = __uint_as_float((254 - byte) << 23);
     uint32_t pair[4];
 #pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) {
-        x[e] *= inverse;
-        if (!(fabsf(x[e]) <= 448.0f)) x[e] = __uint_as_float(0x7fc00000u);   // (the conversion would clamp it)
-    }
-#pragma unroll
     for (uint32_t e = 0; e < 4; ++e) {
         uint16_t two;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(x[2 * e + 1]), "f"(x[2 * e]));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(x[2 * e + 1] * inverse), "f"(x[2 * e] * inverse));
         pair[e] = two;
     }
     *scale = byte;
@@ -167,10 +174,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
             for (uint32_t e = 0; e < 8; e += 4) {
                 const float4 c = *reinterpret_cast<const float4*>(cosine[r] + pair + e), n = *reinterpret_cast<const float4*>(sine[r] + pair + e);
                 const float cosines[4] = {c.x, c.y, c.z, c.w}, sines[4] = {n.x, n.y, n.z, n.w};
+                float other[4];
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const float other = __shfl_sync(mask, x[e + i], partner, kLanes);
-                    if (turns) x[e + i] = fmaf(x[e + i], cosines[i], (upper ? other : -other) * sines[i]);
+                for (uint32_t i = 0; i < 4; ++i) other[i] = __shfl_sync(mask, x[e + i], partner, kLanes);
+                if (turns) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) x[e + i] = fmaf(x[e + i], cosines[i], (upper ? other[i] : -other[i]) * sines[i]);
                 }
             }
             uint32_t packed[4];
