@@ -364,7 +364,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             return true;
         };
         // The scores of a tile are formed once the softmax is done with those of two tiles before, ahead of that tile's product: behind it, the softmax waited for them. (Whichever
-        // can go next, found out by polling, was worse: 120 us where this order takes NN.) A new pair's queries may be waiting for the products of the pair before.
+        // can go next, found out by polling: two documents of 131071 tokens 121 us, so 102.) A new pair's queries may be waiting for the products of the pair before.
         while (alive && now.valid) {
             while (alive && ahead.valid && scores < products + 3) {
                 if (ahead.first() && scores != products) {

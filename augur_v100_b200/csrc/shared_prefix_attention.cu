@@ -52,7 +52,8 @@ template <uint32_t kHeadDim>
 struct PrefixShape {
     static constexpr uint32_t kParts = kHeadDim / 128, kStreams = kHeadDim == 128 ? 2 : 1;
     // Keys of a tile, and S in tensor memory: 256 columns of it. With two streams each has two, so that the next scores are formed while its softmax is at work (of 128 keys
-    // and one each, the weights' product and the next scores behind it were waited for: 2300 cycles for 128 keys, NN now).
+    // and one each, the weights' product and the next scores behind it were waited for: 2300 cycles a tile. What bounds it now with pages of 16 tokens is
+    // the copies' issue, 100 cycles each: 1120 cycles for 64 keys).
     static constexpr uint32_t kKeys = kHeadDim == 128 ? 64 : 128, kBuffers = 256 / kKeys, kSlot = kKeys * 256;   // a slot: 128 dims of a tile, as two halves of 128 bytes a key
     static constexpr uint32_t kThreads = 128 + 128 * kStreams;   // warp 0 loads keys, 1 and 2 MMA, 3 values, then the softmax
     static constexpr uint32_t kQueryBytes = kRowsM * kHeadDim * 2, kSlots = (224 * 1024 - kQueryBytes) / kSlot;
@@ -835,7 +836,7 @@ template <uint32_t kHeadDim>
 void launch_prefix(cudaStream_t stream, const CUtensorMap& map_keys, const CUtensorMap& map_values, const __nv_bfloat16* keys, const __nv_bfloat16* values, const PrefixParams& p,
                    uint32_t sm_count) {
     using S = PrefixShape<kHeadDim>;
-    // The prefix behind the own tokens: its parts are the many, and still in L2 when they are joined. (The other way round the join of 64 sequences took 14 us, not NN.)
+    // The prefix behind the own tokens: its parts are the many, and still in L2 when they are joined. (The other way round the join of 64 sequences took 14 us, not 9.)
     const uint32_t queries = p.a.query_heads / p.a.kv_heads * p.a.max_new;
     (queries <= 16 ? launch_own<kHeadDim, 1> : queries <= 32 ? launch_own<kHeadDim, 2> : launch_own<kHeadDim, 4>)(stream, keys, values, p);
     launch_dependent(stream, prefix_attention_kernel<kHeadDim>, sm_count, S::kThreads, S::kSmem, map_keys, map_values, p);

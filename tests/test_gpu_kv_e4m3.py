@@ -424,3 +424,54 @@ def test_two_streams_and_graphs():
     torch.cuda.synchronize()
     for x, want in zip(bound, alone):
         assert torch.equal(x.out, want) and x.plan.device_status() == 0
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_random_batches(seed):
+    """Batches of any make-up: where the spans are cut, which pairs share one, and which lie in several differs from seed to seed."""
+    g = torch.Generator().manual_seed(100 + seed)
+    pick = lambda *values: values[int(torch.randint(len(values), (1,), generator=g))]  # noqa: E731
+    heads = pick((24, 4, 256), (16, 16, 128), (8, 1, 128), (16, 2, 256), (32, 8, 128), (4, 4, 256))
+    tokens = int(torch.randint(1, min(8, 64 // (heads[0] // heads[1])) + 1, (1,), generator=g))
+    count, longest = pick(1, 7, 33, 150), pick(20, 300, 3000)
+    shape = []
+    for _ in range(count):
+        new = int(torch.randint(0, tokens + 1, (1,), generator=g))
+        shape.append((max(int(torch.randint(0, longest, (1,), generator=g)), new), new))
+    batch = BatchE4m3(shape, *heads, pick(16, 32, 64, 128), seed=seed, spare_rows=1, fill=0xff)
+    check(_attend(batch, tokens), *e4m3_attention_reference(batch, batch.head_dim ** -0.5))
+
+
+def test_idle_slots_only():
+    batch = BatchE4m3([(0, 0), (300, 0), (5, 0)], 8, 2, 128, 16, spare_rows=3)
+    assert bool((_attend(batch, 1) == 0).all())
+    before = [x.view(torch.uint8).clone() for x in (batch.k, batch.v, batch.scales)]
+    x = torch.randn((batch.rows, 2, 128), device=DEVICE).to(torch.bfloat16)
+    _append(batch, _cache(batch), (x, x), None, False, 64, torch.zeros((3, batch.rows), dtype=torch.int32, device=DEVICE))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, (batch.k, batch.v, batch.scales)))
+
+
+def test_back_to_back_on_one_plan():
+    """Calls of other shapes right behind one another on one plan, which is as large as the largest wants: the same results as alone."""
+    batches = [BatchE4m3([(700, 2), (33, 1)], 24, 4, 256, 64, seed=1), BatchE4m3([(4000, 8)], 8, 1, 128, 16, seed=2), BatchE4m3([(9, 1)] * 50, 16, 16, 128, 32, seed=3)]
+    alone = [_attend(b, 8 if i == 1 else 2).clone() for i, b in enumerate(batches)]
+    plan = host.Plan(host.Stream(0), max(kv.paged_attention_scratch_bytes(b.query_heads, b.kv_heads, b.head_dim, 8 if i == 1 else 2) for i, b in enumerate(batches)))
+    bound = [kv.PagedAttention.bind(plan, _cache(b), 0, b.q, b.table, b.lengths, b.starts, tokens=8 if i == 1 else 2) for i, b in enumerate(batches)]
+    for _ in range(10):
+        for x in bound:
+            x.submit_for_plan()
+    torch.cuda.synchronize()
+    assert plan.device_status() == 0 and all(torch.equal(x.out, want) for x, want in zip(bound, alone))
+
+
+def test_refusals():
+    batch = BatchE4m3([(40, 1)], 8, 2, 128, 16)
+    cache, plan = _cache(batch), host.Plan(host.Stream(0), kv.paged_attention_scratch_bytes(8, 2, 128, 1))
+    good = dict(plan=plan, cache=cache, layer=0, q=batch.q, table=batch.table, lengths=batch.lengths, starts=batch.starts)
+    kv.PagedAttention.bind(**good)
+    for change, error in (({"layer": 1}, ValueError), ({"q": batch.q.float()}, ValueError), ({"table": batch.table.long()}, ValueError), ({"out": batch.q}, host.CudaRuntimeError),
+                          ({"tokens": 9}, host.CudaRuntimeError), ({"scale": float("nan")}, host.CudaRuntimeError), ({"lengths": batch.lengths.cpu()}, ValueError),
+                          ({"cache": object()}, (ValueError, AttributeError)), ({"plan": host.Plan(host.Stream(0), 1 << 12)}, host.CudaRuntimeError)):
+        with pytest.raises(error):
+            kv.PagedAttention.bind(**{**good, **change})

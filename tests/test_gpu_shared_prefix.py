@@ -255,3 +255,81 @@ def test_two_streams():
     torch.cuda.synchronize()
     for (plan, x), want in zip(bound, alone):
         assert torch.equal(x.out, want) and plan.device_status() == 0
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_random_batches(seed):
+    """Batches of any make-up: how the prefix and the own tokens are cut differs from seed to seed, and some sequences end in the prefix."""
+    g = torch.Generator().manual_seed(200 + seed)
+    pick = lambda *values: values[int(torch.randint(len(values), (1,), generator=g))]  # noqa: E731
+    heads = pick((24, 4, 256), (16, 16, 128), (8, 1, 128), (16, 2, 256), (32, 8, 128), (4, 4, 256))
+    tokens = int(torch.randint(1, min(8, 64 // (heads[0] // heads[1])) + 1, (1,), generator=g))
+    page, count, longest = pick(16, 32, 64, 128), pick(2, 9, 40, 130), pick(20, 300, 2000)
+    prefix = pick(1, 5, 30, 70) * page
+    shape = []
+    for _ in range(count):
+        new = int(torch.randint(0, tokens + 1, (1,), generator=g))
+        length = int(torch.randint(prefix // 2, prefix + longest, (1,), generator=g)) if seed % 2 else prefix + int(torch.randint(0, longest, (1,), generator=g)) + new
+        shape.append((max(length, new), new))
+    batch = PrefixBatch(shape, *heads, page, prefix, seed=seed, spare_rows=1, fill=float("nan"), spare_prefix=seed % 3)
+    check(_attend(batch, tokens), *prefix_attention_reference(batch, batch.head_dim ** -0.5))
+
+
+def test_long_own_tokens():
+    batch = PrefixBatch(_behind(128, [(20000, 2), (3, 1), (7777, 1)]), 24, 4, 256, 128, 128, seed=8)
+    check(_attend(batch, 2), *prefix_attention_reference(batch, 0.0625))
+
+
+def test_a_page_more_than_once():
+    """The prefix's list may name a page twice."""
+    batch = PrefixBatch(_behind(512, [(30, 1), (64, 1)]), 8, 2, 128, 64, 512, seed=6)
+    batch.prefix_pages[5] = batch.prefix_pages[2]
+    batch.prefix_pages[6] = batch.prefix_pages[2]
+    check(_attend(batch, 1), *prefix_attention_reference(batch, 128 ** -0.5))
+
+
+def test_idle_slots_only():
+    batch = PrefixBatch([(0, 0), (300, 0), (256, 0)], 8, 2, 128, 16, 256, spare_rows=3)
+    assert bool((_attend(batch, 1) == 0).all())
+
+
+def test_back_to_back_on_one_plan():
+    batches = [PrefixBatch(_behind(640, [(700, 2), (33, 1)]), 24, 4, 256, 64, 640, seed=1), PrefixBatch(_behind(2048, [(400, 8)]), 8, 1, 128, 16, 2048, seed=2),
+               PrefixBatch(_behind(96, [(9, 1)] * 150), 16, 16, 128, 32, 96, seed=3)]
+    tokens = [2, 8, 1]
+    alone = [_attend(b, t).clone() for b, t in zip(batches, tokens)]
+    plan = host.Plan(host.Stream(0), max(kv.shared_prefix_attention_scratch_bytes(b.query_heads, b.kv_heads, b.head_dim, b.rows, t) for b, t in zip(batches, tokens)))
+    bound = [kv.SharedPrefixAttention.bind(plan, kv.KvCache(b.k, b.v), 0, b.q, b.table, b.lengths, b.starts, b.prefix_pages, b.prefix_tokens, tokens=t)
+             for b, t in zip(batches, tokens)]
+    for _ in range(10):
+        for x in bound:
+            x.submit_for_plan()
+    torch.cuda.synchronize()
+    assert plan.device_status() == 0 and all(torch.equal(x.out, want) for x, want in zip(bound, alone))
+
+
+def test_offsets_beyond_32_bits():
+    """Pages whose elements lie behind 2^32 of the layer."""
+    pages, kv_heads, page, size = 4200, 8, 512, 256
+    batch = PrefixBatch(_behind(1536, [(700, 2), (1, 1)]), 16, kv_heads, size, page, 1536, seed=8, spare_pages=0)
+    cache = kv.KvCache.allocate(host.Stream(0), 1, pages, kv_heads, page, size)
+    count = batch.k.shape[1]
+    cache.keys[0, -count:], cache.values[0, -count:] = batch.k[0], batch.v[0]
+    batch.table = torch.where(batch.table >= 0, batch.table + (pages - count), -1)
+    batch.prefix_pages = batch.prefix_pages + (pages - count)
+    batch.k, batch.v = cache.keys, cache.values
+    check(_attend(batch, 2), *prefix_attention_reference(batch, 0.0625))
+
+
+def test_refusals():
+    batch = PrefixBatch(_behind(256, [(30, 1)]), 8, 2, 128, 64, 256)
+    plan = host.Plan(host.Stream(0), kv.shared_prefix_attention_scratch_bytes(8, 2, 128, batch.rows, 1))
+    good = dict(plan=plan, cache=kv.KvCache(batch.k, batch.v), layer=0, q=batch.q, table=batch.table, lengths=batch.lengths, starts=batch.starts,
+                prefix_pages=batch.prefix_pages, prefix_tokens=batch.prefix_tokens)
+    kv.SharedPrefixAttention.bind(**good)
+    for change, error in (({"layer": 1}, ValueError), ({"prefix_pages": batch.prefix_pages.long()}, ValueError), ({"prefix_pages": batch.prefix_pages[:0]}, ValueError),
+                          ({"prefix_pages": batch.prefix_pages.cpu()}, ValueError), ({"prefix_tokens": batch.starts}, ValueError), ({"out": batch.q}, host.CudaRuntimeError),
+                          ({"prefix_tokens": batch.lengths, "lengths": batch.lengths}, host.CudaRuntimeError), ({"tokens": 9}, host.CudaRuntimeError),
+                          ({"scale": float("inf")}, host.CudaRuntimeError), ({"plan": host.Plan(host.Stream(0), 1 << 12)}, host.CudaRuntimeError)):
+        with pytest.raises(error):
+            kv.SharedPrefixAttention.bind(**{**good, **change})
