@@ -9,7 +9,7 @@
 //   O^T[dim][query]  += V^T W^T        V as it lies in the pages (the key is the k dimension: MN-major)
 //
 // That unit takes two operands of 8 bits, so what goes with the codes is split into E4M3 terms:
-//   q in two, in units in which its largest element is 224 at least: a BF16 element above 2^-14 of the largest is met exactly, a smaller one to
+//   q in two, in units in which its largest element is 224 at least: a BF16 element above 2^-9 of the largest is met exactly, a smaller one to
 //     2^-18 of the largest. Both terms add into the same S^T: two passes over K, for which the pipe has the time (side by side they would double
 //     what the softmax reads);
 //   w = 2^(s_j + f_j - m), rounded to half precision (2^-11), in three, each in units a sixteenth of the one before it: exact. Side by side on the

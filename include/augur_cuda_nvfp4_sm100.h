@@ -855,7 +855,9 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append_e4m3_preva
     int32_t ordinal, augur_cuda_stream_t stream, const augur_cuda_nvfp4_sm100_kv_append_e4m3_args_v1* args);
 
 /* paged_attention over such a cache: the same formula on the values that codes and scales stand for, the same limits, scratch
- * (paged_attention_scratch_extent_host_v1) and status words. */
+ * (paged_attention_scratch_extent_host_v1) and status words. A query enters as two E4M3 terms: an element above 2^-9 of its head's largest exactly, a smaller
+ * one to 2^-17 of the largest; an infinite element gives NaN as a NaN does, in all outputs of that query head's row. A weight enters the product with the values
+ * good to 2^-11, and to 2^-18 of the row's largest product of weight and value scale; the denominator is F32. */
 typedef struct augur_cuda_nvfp4_sm100_paged_attention_e4m3_args_v1 {
     uint32_t abi_version;
     uint32_t struct_size;
@@ -902,13 +904,13 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_copy_e4m3_pr
 /* ---- attention of a batch whose sequences share a prefix ------------------------------------------ */
 /* paged_attention (BF16 cache) of sequences that all begin with the same P tokens, whose keys and values are read once for the batch.
  * P = prefix_tokens[0] (device memory, as the batch's), in whole pages: what is over is read from each sequence's own pages.
- * The pages of the first P tokens are those of prefix_pages, whatever a sequence's page-table row says there; lengths[b] counts them too, and a
- * row of a sequence that is shorter than P sees its own length of them. P <= 0 is a batch without a prefix. P beyond prefix_pages counts as
+ * The pages of the first P tokens are those of prefix_pages, whatever a sequence's page-table row says there (its columns for them stay); lengths[b] counts them
+ * too, and a row of a sequence that ends within them sees them up to its own token. P <= 0 is a batch without a prefix. P beyond prefix_pages counts as
  * those and sets the status word to 0x401, as does a page outside the cache, which counts as not there. All else is as for
  * paged_attention: limits on heads, tokens and table, rows that are not written, rows that see nothing, status words (the waits
- * of the prefix set 0x421..0x427). A value of the prefix that is not finite may reach every row of the batch, those too short to see it included.
- * The weights of the prefix enter their product with the values as one BF16 term (good to 2^-8 of each, and the denominator sums the
- * same terms): for a batch, these products are the bound. */
+ * of the prefix set 0x421..0x426). A value that is not finite may reach rows that do not see it: one of the prefix every row, one of a sequence's own tokens that
+ * sequence's rows. The weights enter their product with the values as one BF16 term (good to 2^-8 of each, and the denominator sums
+ * the same terms): for a batch, these products are the bound. The results depend on the inputs and the device's SM count alone. */
 typedef struct augur_cuda_nvfp4_sm100_shared_prefix_attention_args_v1 {
     uint32_t abi_version;
     uint32_t struct_size;
