@@ -62,7 +62,7 @@ struct PrefixShape {
     static constexpr uint32_t kThreads = 128 + 128 * kStreams;   // warp 0 loads keys, 1 and 2 MMA, 3 values, then the softmax
     static constexpr uint32_t kQueryBytes = kRowsM * kHeadDim * 2, kSlots = (224 * 1024 - kQueryBytes) / kSlot;
     // A ring each for the keys and the values, so that two warps deal out the copies: one alone took 80 cycles a copy, and pages of 16 tokens are up to 16 copies a slot.
-    static constexpr uint32_t kKeySlots = kSlots / 2, kValueSlots = kSlots - kKeySlots;
+    static constexpr uint32_t kValueSlots = kSlots / 2, kKeySlots = kSlots - kValueSlots;
     static constexpr uint32_t kSmem = 1024 + kQueryBytes + kSlots * kSlot + 1024;
     static constexpr uint32_t kScoresAt = 0, kOutAt = 256;       // tensor memory: S, then one O per stream
     static_assert(kSlots <= kMaxSlots && kKeySlots / kParts + kBuffers + 1 <= kInfoRing && kKeySlots >= kParts && kValueSlots >= kParts && kSmem <= kSmemLimit && kOutAt + kStreams * kHeadDim == 512, "a CTA's memory");
@@ -804,8 +804,9 @@ Layout layout_of(uint32_t query_heads, uint32_t kv_heads, uint32_t head_dim, uin
     l.tiles = static_cast<uint32_t>((static_cast<uint64_t>(rows) * (query_heads / kv_heads) + kRowsM - 1) / kRowsM);
     const uint64_t pairs = static_cast<uint64_t>(kv_heads) * l.tiles, most = kRounds * static_cast<uint64_t>(sm_count);   // (of queries and heads; below 2^30)
     l.max_items = static_cast<uint32_t>(pairs > most ? pairs : most);
-    // The sequences' own tokens in as many chunks as give an SM about eight CTAs.
-    const uint64_t sequences = (rows + max_new - 1) / max_new, chunks = 8 * static_cast<uint64_t>(sm_count) / (sequences * kv_heads);
+    // The sequences' own tokens in as many chunks as give an SM about so many CTAs.
+    constexpr uint64_t kOwnCtas = 8;
+    const uint64_t sequences = (rows + max_new - 1) / max_new, chunks = kOwnCtas * static_cast<uint64_t>(sm_count) / (sequences * kv_heads);
     l.chunks = static_cast<uint32_t>(chunks < 1 ? 1 : chunks < kMaxChunks ? chunks : kMaxChunks);
     l.own_parts = kCounterBytes;
     l.own_stats = aligned(l.own_parts + outputs * l.chunks * head_dim * sizeof(float));
