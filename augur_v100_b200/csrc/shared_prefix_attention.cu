@@ -15,10 +15,11 @@
 // O is scaled in tensor memory). P is one BF16 term (2^-8 of each weight at most; the denominator sums the same terms): a second one would
 // cost half as much again of the product that bounds the kernel.
 //
-// Head size 256: one group of softmax warps, 128 keys a tile, two S; 2900 cycles a tile (44 GB/s and SM from L2) where the products alone take 2048: Q and K of the first are both
-// read from shared memory, 128 bytes a cycle with the copies coming in, and a tile's scores wait for the product of two tiles before, whose P lies in their place.
+// Head size 256: one group of softmax warps, 128 keys a tile, two S; 2800 cycles a tile where the products alone take 2048 (84 GB/s and SM from L2): a tile's scores wait for the
+// product of two tiles before, whose P lies in their place, and that for 2050 cycles of softmax, 1024 of them exponentials; and Q and K of the first product are both read from
+// shared memory, 128 bytes a cycle with the copies coming in.
 // Head size 128: two groups that take tiles of 64 keys in turn, each with an O and two S of its own: one group's exponentials take as long as a tile's products.
-// Twelve sequences of eight tokens on 65536 tokens (24 / 4 heads of 256): 162 us, 0.96 PFLOP/s.
+// Twelve sequences of eight tokens on 65536 tokens (24 / 4 heads of 256): 160 us, 0.97 PFLOP/s.
 #include "paged_attention.cuh"
 
 namespace augur_sm100 {

@@ -2,7 +2,8 @@
 move them.
 
 A decoding step of a layer is: projections (``host``), `KvAppend` (rotary positions, optional head norms, the cache
-write), `PagedAttention`, output projection. `KvPagePool` is the host's book of pages: sequences share full pages after a
+write), `PagedAttention`, output projection. The cache is BF16 (`KvCache`) or in 8 bits (`KvCacheE4m3`); `SharedPrefixAttention` stands in
+`PagedAttention`'s place where the sequences begin with the same pages. `KvPagePool` is the host's book of pages: sequences share full pages after a
 fork, and what has to be copied (a fork's partly filled page, a compaction's moves) comes back as two lists for
 `KvPageCopy`. The reference keeps one contiguous cache per session instead (crates/augur-model-qwen35-runtime); owners
 and bindings follow the rules of :mod:`augur_v100_b200.host`: everything is checked once at ``bind``, ``submit`` only
