@@ -25,6 +25,7 @@ constexpr float kNoNumber = -FLT_MAX;     // a part's reference where a query se
 constexpr uint32_t kStatusPage = 0x401, kStatusRows = 0x402;
 constexpr uint32_t kStatusLoad = 0x411, kStatusMma = 0x412, kStatusScores = 0x413, kStatusValues = 0x414, kStatusQuery = 0x415, kStatusGroup = 0x416, kStatusProduct = 0x417;
 constexpr uint32_t kThreads = 256;        // warp 0 loads keys, 1 MMA, 2 queries, 3 values, 4..7 softmax
+constexpr uint32_t kMaxWarps = 12;        // (a launch may have a second group of softmax warps)
 constexpr uint32_t kSmemLimit = 227 * 1024;
 
 }  // namespace
@@ -46,7 +47,7 @@ namespace {
 
 // What a launch knows of its sequences.
 struct BatchState {
-    uint32_t scan[kThreads / 32];
+    uint32_t scan[kMaxWarps];
     uint32_t units[kMaxSequences + 1]; // before sequence b, of one head
     uint32_t length[kMaxSequences];    // | new tokens << 25
     uint32_t row[kMaxSequences];       // the first token row

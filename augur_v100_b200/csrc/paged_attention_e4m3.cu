@@ -38,9 +38,9 @@ constexpr uint32_t kWeightAtom = kTile * 32;   // 32 columns of a tile's weights
 // Small state of a CTA, behind the rings, the queries and the weights.
 struct StateE4m3 : BatchState {
     uint64_t full[16], empty[16], scales_full[kTileInfos];
-    uint64_t scores_full[2], scores_empty[2], weights_full[2], weights_empty[2], query_full[2], query_empty[2], group, keys_first;
-    uint32_t tmem, abort[1 + kThreads / 32];
-    uint32_t needs[2];                 // a byte per softmax warp: a reference has to move
+    uint64_t scores_full[2], scores_empty[2], weights_full[2], weights_empty[2], query_full[2], query_empty[2], group[2], keys_first;
+    uint32_t tmem, abort[1 + kMaxWarps];
+    uint32_t needs[2][2];              // by group, a byte per softmax warp: a reference has to move
     uint32_t info[kTileInfos];         // of a tile: pages that are there, a bit per box
     float reference[kMaxQueries], factor[kMaxQueries], total[kMaxQueries];
     alignas(16) float minus[kMaxQueries];            // the references with the sign changed, kNoReference for -infinity
@@ -53,11 +53,14 @@ struct StateE4m3 : BatchState {
 template <uint32_t kHeadDim, uint32_t kN>
 struct ShapeE4m3 {
     static constexpr uint32_t kChunks = kHeadDim / 128;
-    // Columns of S^T (the MMA wants 16 at least), and of W^T and O^T: three terms side by side, in steps of 16. kBlock queries are worked on at a time.
-    static constexpr uint32_t kScores = kN < 16 ? 16 : kN, kTerms = (3 * kN + 15) / 16 * 16, kAtoms = (kTerms + 31) / 32, kBlock = kN < 16 ? kN : 16;
+    // Columns of S^T (the MMA wants 16 at least), and of W^T and O^T: three terms side by side, in steps of 16. A softmax warp works on kBlock queries at a time.
+    static constexpr uint32_t kScores = kN < 16 ? 16 : kN, kTerms = (3 * kN + 15) / 16 * 16, kAtoms = (kTerms + 31) / 32;
+    // From 32 queries on two groups of softmax warps, each for half of them: independent of one another but for where they say that a tile's weights are there. (One group: 3200
+    // cycles a tile of 48 queries, more than HBM takes to bring it.)
+    static constexpr uint32_t kGroups = kN < 32 ? 1 : 2, kMine = kN / kGroups, kBlock = kMine % 16 == 0 ? 16 : 8, kThreads = 128 + 128 * kGroups;
     static constexpr uint32_t kTermBytes = kScores * kHeadDim, kQueryBytes = 2 * kTermBytes, kWeightBytes = kAtoms * kWeightAtom;
     // The denominators' sums: in registers for one block of queries, else in shared memory.
-    static constexpr uint32_t kSumBytes = kN == kBlock ? 0 : kN * kTile * 4;
+    static constexpr uint32_t kSumBytes = kMine == kBlock ? 0 : kN * kTile * 4;
     static constexpr uint32_t fixed(uint32_t buffers) { return 1024 + sizeof(StateE4m3) + buffers * kQueryBytes + 2 * kWeightBytes + kSumBytes; }
     static constexpr uint32_t slots(uint32_t buffers) {
         const uint32_t fit = (kSmemLimit - fixed(buffers)) / kSlotBytes / 2 * 2;
@@ -212,7 +215,7 @@ struct SplitQueries {
 };
 
 template <uint32_t kHeadDim, uint32_t kN>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(ShapeE4m3<kHeadDim, kN>::kThreads, 1)
 paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const __grid_constant__ CUtensorMap map_values, const __grid_constant__ AttentionParams p) {
     using S = ShapeE4m3<kHeadDim, kN>;
     extern __shared__ uint8_t smem_raw[];
@@ -224,7 +227,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full = smem_u32(st->full), empty = smem_u32(st->empty), scores_full = smem_u32(st->scores_full), scores_empty = smem_u32(st->scores_empty);
     const uint32_t weights_full = smem_u32(st->weights_full), weights_empty = smem_u32(st->weights_empty), scales_full = smem_u32(st->scales_full);
-    const uint32_t query_full = smem_u32(st->query_full), query_empty = smem_u32(st->query_empty), group_bar = smem_u32(&st->group);
+    const uint32_t query_full = smem_u32(st->query_full), query_empty = smem_u32(st->query_empty), group_bar = smem_u32(st->group);
     volatile uint32_t* abort_flag = st->abort;
     uint32_t* const status = p.status_word;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -232,14 +235,14 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
         for (uint32_t s = 0; s < S::kSlots; ++s) mbar_init(full + 8 * s, 1), mbar_init(empty + 8 * s, 1);
         for (uint32_t i = 0; i < kTileInfos; ++i) mbar_init(scales_full + 8 * i, 1);
         for (uint32_t b = 0; b < 2; ++b) {
-            mbar_init(scores_full + 8 * b, 1), mbar_init(scores_empty + 8 * b, 4);
-            mbar_init(weights_full + 8 * b, 4), mbar_init(weights_empty + 8 * b, 1);
-            mbar_init(query_full + 8 * b, S::kQueryBuffers == 1 ? 4 : 1), mbar_init(query_empty + 8 * b, 5);   // the MMAs, and the softmax warps with the queries' scales
+            mbar_init(scores_full + 8 * b, 1), mbar_init(scores_empty + 8 * b, 4 * S::kGroups), mbar_init(group_bar + 8 * b, 4);
+            mbar_init(weights_full + 8 * b, 4 * S::kGroups), mbar_init(weights_empty + 8 * b, 1);
+            mbar_init(query_full + 8 * b, S::kQueryBuffers == 1 ? 4 * S::kGroups : 1), mbar_init(query_empty + 8 * b, 1 + 4 * S::kGroups);   // the MMAs, and the softmax warps with the queries' scales
         }
-        mbar_init(group_bar, 4), mbar_init(smem_u32(&st->keys_first), 1);
+        mbar_init(smem_u32(&st->keys_first), 1);
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_keys) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_values) : "memory");
-        for (uint32_t i = 0; i < 1 + kThreads / 32; ++i) st->abort[i] = 0;
+        for (uint32_t i = 0; i < 1 + kMaxWarps; ++i) st->abort[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -403,18 +406,19 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
         }
     } else {
         // ---------------- softmax: thread = key of a tile, then dim of the output ----------------
-        const uint32_t thread = threadIdx.x - 128, quadrant = warp & 3, lanes = (quadrant * 32) << 16;
+        const uint32_t thread = threadIdx.x & 127, quadrant = warp & 3, lanes = (quadrant * 32) << 16;
+        const uint32_t half = S::kGroups == 1 ? 0 : (warp - 4) / 4, first = half * S::kMine, behind = first + S::kMine;   // the group, its queries
         const uint32_t box_shift = p.page_shift < 6 ? p.page_shift : 6, boxes = kTile >> box_shift, all_boxes = (1u << boxes) - 1;
         constexpr uint32_t kBlock = S::kBlock;
-        constexpr bool kOneBlock = kN == kBlock;
+        constexpr bool kOneBlock = S::kMine == kBlock;
         uint32_t tile = 0, meetings = 0, pair = 0;
         JoinRecord record{};
-        // The four warps meet (a bounded wait, where a named barrier would hang on a warp that gave up).
+        // The four warps of a group meet (a bounded wait, where a named barrier would hang on a warp that gave up).
         auto come = [&]() {
             __syncwarp();
-            if (lane == 0) mbar_arrive(group_bar);
+            if (lane == 0) mbar_arrive(group_bar + 8 * half);
         };
-        auto all_came = [&]() { return warp_look_suspended(group_bar, meetings++ & 1, abort_flag, status, kStatusGroup); };
+        auto all_came = [&]() { return warp_look_suspended(group_bar + 8 * half, meetings++ & 1, abort_flag, status, kStatusGroup); };
         auto meet = [&]() {
             come();
             return all_came();
@@ -426,16 +430,17 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             const uint32_t queries = walk.tokens * group;
             const uint32_t first_row = st->row[walk.sequence];
             const bool any = walk.key < walk.key_end;
-            if (thread < kN) {
-                st->reference[thread] = -INFINITY;
-                st->limit[thread] = thread < queries ? static_cast<int32_t>(walk.length) - static_cast<int32_t>(walk.tokens) + static_cast<int32_t>(thread / group) + 1 : 0;
+            const uint32_t mine = first + thread;   // the query whose reference this thread keeps
+            if (thread < S::kMine) {
+                st->reference[mine] = -INFINITY;
+                st->limit[mine] = mine < queries ? static_cast<int32_t>(walk.length) - static_cast<int32_t>(walk.tokens) + static_cast<int32_t>(mine / group) + 1 : 0;
             }
             if (!meet()) break;
             const uint32_t query_buffer = S::kQueryBuffers == 2 ? pair & 1 : 0;
             const float* const query_scale = st->query_scale[query_buffer];
             if (S::kQueryBuffers == 1 && any) {
                 SplitQueries<kHeadDim, kN> split;
-                split.open(p.query + (static_cast<uint64_t>(first_row) * p.query_heads + walk.head * group) * kHeadDim + lane % (kHeadDim / 8) * 8, queries, group, p.query_heads, quadrant, 4, lane);
+                split.open(p.query + (static_cast<uint64_t>(first_row) * p.query_heads + walk.head * group) * kHeadDim + lane % (kHeadDim / 8) * 8, queries, group, p.query_heads, warp - 4, 4 * S::kGroups, lane);
                 if (!warp_look_suspended(query_empty, (pair & 1) ^ 1, abort_flag, status, kStatusQuery)) break;
                 split.run(query_smem, st->query_scale[0], lane);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -500,7 +505,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                     break;
                 }
                 tc_fence_after();
-                if (kOneBlock) scores(0);
+                if (kOneBlock) scores(first);
                 // The weights are formed and stored under the references as they stand, and stand if no warp finds one that passes 2^kRoom; else the references
                 // move and the weights are formed anew. (Asked first and formed then, a tile of eight queries took 400 cycles more, which the warps waited for one another.)
                 bool move = key == walk.key;   // a pair's first tile sets the references
@@ -508,7 +513,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                     if (move) {
                         if (again) {   // the sums as they were
 #pragma unroll 1
-                            for (uint32_t c = 0; c < kN; c += kBlock) {
+                            for (uint32_t c = first; c < behind; c += kBlock) {
                                 if (!kOneBlock) scores(c);
                                 float w[kBlock];
                                 weights(c, w);
@@ -528,7 +533,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                         }
                         // The references move up to the largest so far.
 #pragma unroll 1
-                        for (uint32_t c = 0; c < kN; c += kBlock) {
+                        for (uint32_t c = first; c < behind; c += kBlock) {
                             if (!kOneBlock) scores(c);
                             float most = -INFINITY;
 #pragma unroll
@@ -542,13 +547,13 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                             alive = false;
                             break;
                         }
-                        if (thread < kN) {
-                            const float old = st->reference[thread];
-                            const float4 w = st->wide[thread];
+                        if (thread < S::kMine) {
+                            const float old = st->reference[mine];
+                            const float4 w = st->wide[mine];
                             const float now = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), old);
-                            st->factor[thread] = now == old ? 1.0f : exp2_fast(old - now);
-                            st->reference[thread] = now;
-                            st->minus[thread] = now == -INFINITY ? kNoReference : kLift - now;
+                            st->factor[mine] = now == old ? 1.0f : exp2_fast(old - now);
+                            st->reference[mine] = now;
+                            st->minus[mine] = now == -INFINITY ? kNoReference : kLift - now;
                         }
                         if (!meet()) {
                             alive = false;
@@ -561,7 +566,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                             }
                             tc_fence_after();
 #pragma unroll 1
-                            for (uint32_t c = 0; c < kN; c += kBlock) {   // 16 queries' columns (or eight), if one of them has moved
+                            for (uint32_t c = first; c < behind; c += kBlock) {   // 16 queries' columns (or eight), if one of them has moved
                                 float factor[kBlock];
                                 bool moved = false;
 #pragma unroll
@@ -597,7 +602,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                     auto store = [&](uint32_t column, uint4 sixteen) { *reinterpret_cast<uint4*>(to_weights + column / 32 * kWeightAtom + ((column / 16 % 2 ^ turned) << 4)) = sixteen; };
                     bool passes = false;
 #pragma unroll 1
-                    for (uint32_t c = 0; c < kN; c += kBlock) {
+                    for (uint32_t c = first; c < behind; c += kBlock) {
                         if (!kOneBlock) scores(c);
                         if constexpr (!kOneBlock) {
                             if (key != walk.key) {
@@ -610,9 +615,9 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                         }
                         float w[kBlock];
                         passes |= weights(c, w);
-                        if (!move && c + kBlock == kN) {   // say so, and go on
+                        if (!move && c + kBlock == behind) {   // say so, and go on
                             passes = __any_sync(0xffffffffu, passes);
-                            if (lane == 0) reinterpret_cast<uint8_t*>(&st->needs[buffer])[quadrant] = passes;
+                            if (lane == 0) reinterpret_cast<uint8_t*>(&st->needs[half][buffer])[quadrant] = passes;
                             come();
                         }
 #pragma unroll
@@ -636,9 +641,15 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                         if constexpr (kBlock == 16) {
 #pragma unroll
                             for (uint32_t t = 0; t < 3; ++t) store(t * kN + c, make_uint4(term[t][0], term[t][1], term[t][2], term[t][3]));
-                        } else {
+                        } else if constexpr (kN == 8) {
                             store(0, make_uint4(term[0][0], term[0][1], term[1][0], term[1][1]));
                             store(16, make_uint4(term[2][0], term[2][1], 0, 0));
+                        } else {
+#pragma unroll
+                            for (uint32_t t = 0; t < 3; ++t) {
+                                const uint32_t column = t * kN + c;
+                                *reinterpret_cast<uint2*>(to_weights + column / 32 * kWeightAtom + ((column / 16 % 2 ^ turned) << 4) + column % 16) = make_uint2(term[t][0], term[t][1]);
+                            }
                         }
 #pragma unroll
                         for (uint32_t i = 0; i < kBlock; ++i) sum[i] = fmaf(w[i], value_inverse, sum[i]);
@@ -657,7 +668,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                         alive = false;
                         break;
                     }
-                    move = *const_cast<volatile uint32_t*>(&st->needs[buffer]) != 0;
+                    move = *const_cast<volatile uint32_t*>(&st->needs[half][buffer]) != 0;
                     if (!move) break;
                 }
                 if (!alive) break;
@@ -678,7 +689,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                             alive = false;
                             break;
                         }
-                        if (!my_key && thread < (count + 31) / 32 * 32) {
+                        if (half == 0 && !my_key && thread < (count + 31) / 32 * 32) {
                             uint4* row = reinterpret_cast<uint4*>(smem + slot * kSlotBytes + thread * 128);
 #pragma unroll
                             for (uint32_t i = 0; i < 8; ++i) row[i] = make_uint4(0, 0, 0, 0);
@@ -698,7 +709,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                 ++pair;
                 // The denominators: over the lanes, halving the queries that a lane holds as long as it holds more than one, then over the warps.
 #pragma unroll 1
-                for (uint32_t c = 0; c < kN; c += kBlock) {
+                for (uint32_t c = first; c < behind; c += kBlock) {
                     if constexpr (!kOneBlock) {
 #pragma unroll
                         for (uint32_t i = 0; i < kBlock; i += 4) *reinterpret_cast<float4*>(sum + i) = sum_smem[(c + i) / 4 * kTile + thread];
@@ -723,7 +734,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                     if (lane % (32 / kBlock) == 0) reinterpret_cast<float*>(&st->wide[c + query])[quadrant] = sum[0];
                 }
                 if (!meet()) break;
-                if (thread < kN) st->total[thread] = ((st->wide[thread].x + st->wide[thread].y) + (st->wide[thread].z + st->wide[thread].w)) * static_cast<float>(1ull << (60 - static_cast<int>(kLift)));
+                if (thread < S::kMine) st->total[mine] = ((st->wide[mine].x + st->wide[mine].y) + (st->wide[mine].z + st->wide[mine].w)) * static_cast<float>(1ull << (60 - static_cast<int>(kLift)));
                 if (!meet()) break;
                 if (!warp_look_suspended(weights_empty + 8 * ((tile - 1) & 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) break;
                 tc_fence_after();
@@ -734,8 +745,8 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
             __nv_bfloat16* const out = p.output + (static_cast<uint64_t>(first_row) * p.query_heads + walk.head * group) * kHeadDim + thread;
             const uint32_t next_token = (p.query_heads - group) * kHeadDim;   // from behind a token's queries to the next token's
             float2* const stats = reinterpret_cast<float2*>(p.parts + static_cast<uint64_t>(2 * p.spans) * kN * kHeadDim) + part * kN;
-            uint32_t token_end = group;
-            uint64_t skipped = 0;
+            uint32_t token_end = (first / group + 1) * group;
+            uint64_t skipped = static_cast<uint64_t>(first / group) * next_token;
             auto write = [&](const uint32_t (&v)[S::kChunks][kBlock], uint32_t c0, uint32_t i) {
                 const uint32_t c = c0 + i;
                 if (c == token_end) token_end += group, skipped += next_token;
@@ -748,7 +759,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                 }
             };
 #pragma unroll 1
-            for (uint32_t c0 = 0; c0 < queries; c0 += kBlock) {
+            for (uint32_t c0 = first; c0 < (queries < behind ? queries : behind); c0 += kBlock) {
                 uint32_t v[S::kChunks][kBlock], middle[S::kChunks][kBlock], low[S::kChunks][kBlock];   // the terms' sums
 #pragma unroll
                 for (uint32_t h = 0; h < S::kChunks; ++h) {
@@ -788,11 +799,11 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                     }
                 }
             }
-            if (!alone && thread < queries) {
+            if (!alone && thread < S::kMine && mine < queries) {
                 // A part all of whose scores are NaN or -infinity has the reference -infinity too, but counts: its sums may be NaN.
-                float2 mine = make_float2(st->reference[thread], any ? st->total[thread] : 0.0f);
-                if (mine.x == -INFINITY && st->limit[thread] > static_cast<int32_t>(walk.key)) mine.x = kNoNumber;
-                stats[thread] = mine;
+                float2 stat = make_float2(st->reference[mine], any ? st->total[mine] : 0.0f);
+                if (stat.x == -INFINITY && st->limit[mine] > static_cast<int32_t>(walk.key)) stat.x = kNoNumber;
+                stats[mine] = stat;
             }
             if (any) tc_fence_before();
             if (!alone) {
@@ -803,9 +814,9 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                     record.last = last < longer ? last / (base + 1) : extra + (last - longer) / base;
                 }
             }
-            if (p.joins < p.spans && walk.starts && thread == 0) p.records[walk.sequence * p.kv_heads + walk.head] = alone ? JoinRecord{} : record;
+            if (p.joins < p.spans && walk.starts && thread == 0 && half == 0) p.records[walk.sequence * p.kv_heads + walk.head] = alone ? JoinRecord{} : record;
         }
-        if (p.joins == p.spans && thread == 0) p.records[blockIdx.x] = record;
+        if (p.joins == p.spans && thread == 0 && half == 0) p.records[blockIdx.x] = record;
     }
     tc_fence_before();
     __syncthreads();
@@ -817,7 +828,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
 
 template <uint32_t kHeadDim, uint32_t kN>
 void launch_attention(cudaStream_t stream, const CUtensorMap& keys, const CUtensorMap& values, const AttentionParams& p) {
-    launch_dependent(stream, paged_attention_e4m3_kernel<kHeadDim, kN>, p.spans, kThreads, ShapeE4m3<kHeadDim, kN>::kSmem, keys, values, p);
+    launch_dependent(stream, paged_attention_e4m3_kernel<kHeadDim, kN>, p.spans, ShapeE4m3<kHeadDim, kN>::kThreads, ShapeE4m3<kHeadDim, kN>::kSmem, keys, values, p);
     launch_join<kHeadDim, kN>(stream, p);
     count_launch(2);
 }
