@@ -475,3 +475,14 @@ def test_refusals():
                           ({"cache": object()}, (ValueError, AttributeError)), ({"plan": host.Plan(host.Stream(0), 1 << 12)}, host.CudaRuntimeError)):
         with pytest.raises(error):
             kv.PagedAttention.bind(**{**good, **change})
+
+
+def test_as_many_sequences_as_there_may_be():
+    batch = BatchE4m3([(1 + (37 * b) % 90, int(b % 5 != 3)) for b in range(1024)], 8, 2, 128, 32, seed=12, fill=0x7f)
+    check(_attend(batch, 1), *e4m3_attention_reference(batch, 128 ** -0.5))
+
+
+def test_a_scale_of_zero():
+    """Every key weighs the same."""
+    batch = BatchE4m3([(300, 2), (40, 1)], 24, 4, 256, 64, seed=13)
+    check(_attend(batch, 2, scale=0.0), *e4m3_attention_reference(batch, 0.0))

@@ -333,3 +333,49 @@ def test_refusals():
                           ({"scale": float("inf")}, host.CudaRuntimeError), ({"plan": host.Plan(host.Stream(0), 1 << 12)}, host.CudaRuntimeError)):
         with pytest.raises(error):
             kv.SharedPrefixAttention.bind(**{**good, **change})
+
+
+def test_as_many_sequences_as_there_may_be():
+    batch = PrefixBatch(_behind(256, [(1 + (37 * b) % 50, int(b % 5 != 3)) for b in range(1024)]), 8, 2, 128, 32, 256, seed=12, hide=True, fill=float("nan"))
+    check(_attend(batch, 1), *prefix_attention_reference(batch, 128 ** -0.5))
+
+
+@pytest.mark.parametrize("head_dim", [128, 256])
+def test_a_scale_of_zero(head_dim):
+    """Every key weighs the same; some rows end in the prefix."""
+    batch = PrefixBatch([(300, 2), (40, 1), (193, 2), (500, 1)], 8, 2, head_dim, 64, 192, seed=13)
+    check(_attend(batch, 2, scale=0.0), *prefix_attention_reference(batch, 0.0))
+
+
+def test_another_prefix_in_a_captured_call():
+    """A replay follows the prefix's count and pages, the lengths and the tables."""
+    batch = PrefixBatch(_behind(2048, [(100 + 9 * b, 1) for b in range(24)]), 24, 4, 256, 64, 2048, seed=15)
+    stream = torch.cuda.Stream()
+    plan, bound = _bind(batch, 1, stream=host.Stream(0, stream))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        bound.submit_for_plan()
+    pages, table, lengths = batch.prefix_pages.clone(), batch.table.clone(), batch.lengths.clone()
+    for prefix in (2048, 640, 64, 0, 1984):
+        # the first tokens of the prefix; what is left of it moves to the sequences' own pages
+        held = prefix // 64
+        batch.prefix, batch.shape = prefix, [(int(n), 1) for n in lengths]
+        batch.table.copy_(torch.cat([pages.expand(24, -1), table[:, 32:]], 1))
+        batch.prefix_tokens.fill_(prefix)
+        want, error = prefix_attention_reference(batch, 0.0625)
+        batch.table[:, :held] = -9
+        graph.replay()
+        torch.cuda.synchronize()
+        assert plan.device_status() == 0
+        check(bound.out, want, error)
+    batch.prefix_pages.copy_(pages.flip(0))
+    batch.prefix, batch.shape = 1024, [(int(n) - 1024, 1) for n in lengths]
+    batch.prefix_tokens.fill_(1024)
+    batch.table[:, 16:-16] = table[:, 32:][:, :batch.table.shape[1] - 32]
+    batch.lengths.sub_(1024)
+    want, error = prefix_attention_reference(batch, 0.0625)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert plan.device_status() == 0
+    check(bound.out, want, error)
