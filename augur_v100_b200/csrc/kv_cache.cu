@@ -76,7 +76,7 @@ constexpr uint32_t kAppendThreads = 256, kAppendCtas = 2368;   // two rounds of 
 template <uint32_t kHeadDim, uint32_t kRows, bool kE4m3>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
     constexpr uint32_t kLanes = kHeadDim / 8, kGroups = kAppendThreads / kLanes;
-    __shared__ __align__(16) float cosine[kRows][kHeadDim / 2], sine[kRows][kHeadDim / 2];
+    __shared__ __align__(16) float cosine[kE4m3 ? 2 * kRows : kRows][kHeadDim / 2], sine[kE4m3 ? 2 * kRows : kRows][kHeadDim / 2];   // (from kRows on the keys')
     __shared__ int32_t sequence_at[kRows], slot_page[kRows], slot_offset[kRows];
     const uint32_t row0 = blockIdx.x * kRows, heads = p.query_heads + 2 * p.kv_heads;
     const uint32_t h = blockIdx.y * kGroups + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
@@ -136,13 +136,20 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
             static_cast<double>(__ldg(p.positions + static_cast<uint64_t>(axis) * p.rows + row0 + r)) * static_cast<double>(__ldg(p.inv_freq + i)) * 0.15915494309189535;
         const float part_turn = static_cast<float>(turns - rint(turns));
         sincospif(2.0f * part_turn, &sine[r][i], &cosine[r][i]);
+        if constexpr (kE4m3) {
+            // Nothing rounds a key between here and its code: what the angle has lost in F32 (up to 2^-26 of a turn, more than the function's own error) is
+            // brought back to first order; the queries stay those of a write to BF16.
+            // (67 million elements of keys, positions to 2^20: 243 codes other than a computation in 64 bits gives, with it 221.)
+            const float rest = static_cast<float>(turns - rint(turns) - part_turn) * 6.2831853f;
+            sine[kRows + r][i] = fmaf(cosine[r][i], rest, sine[r][i]), cosine[kRows + r][i] = fmaf(-sine[r][i], rest, cosine[r][i]);
+        }
     }
     __syncthreads();
     if (!live) return;   // (whole groups; nothing is waited for below)
     const uint32_t half_lanes = p.half / 8;
     const bool turns = lane < 2 * half_lanes, upper = lane >= half_lanes;
     const uint32_t partner = !turns ? lane : upper ? lane - half_lanes : lane + half_lanes;
-    const uint32_t pair = turns ? 8 * (upper ? lane - half_lanes : lane) : 0;
+    const uint32_t pair = (turns ? 8 * (upper ? lane - half_lanes : lane) : 0) + (kE4m3 && !is_query ? kRows * (kHeadDim / 2) : 0);
     const unsigned mask = kLanes == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);   // the lanes of a head stay together
 #pragma unroll
     for (uint32_t r = 0; r < kRows; ++r) {
