@@ -8,12 +8,14 @@
 //   S^T[key][query]   = K Q^T          K as it lies in the pages (K-major), 128 keys a tile
 //   O^T[dim][query]  += V^T W^T        V as it lies in the pages (the key is the k dimension: MN-major)
 //
-// That unit takes two operands of 8 bits, so what goes with the codes is split into E4M3 terms:
-//   q in two, in units in which its largest element is 224 at least: a BF16 element above 2^-9 of the largest is met exactly, a smaller one to
-//     2^-18 of the largest. Both terms add into the same S^T: two passes over K, for which the pipe has the time (side by side they would double
+// That unit takes two operands of 8 bits, so what goes with the codes is split into terms of 8 bits:
+//   q in two E4M3 terms, in units in which its largest element is 224 at least: a BF16 element above 2^-9 of the largest is met exactly, a smaller one to
+//     2^-17 of the largest. Both terms add into the same S^T: two passes over K, for which the pipe has the time (side by side they would double
 //     what the softmax reads);
-//   w = 2^(s_j + f_j - m), rounded to half precision (2^-11), in three, each in units a sixteenth of the one before it: exact. Side by side on the
-//     narrow operand, whose terms' sums are added at the end. With two the rounding (2^-9) would be as large an error as the output's own.
+//   w = 2^(s_j + f_j - m), rounded to half precision, in three E5M2 terms, each in units a sixteenth of the one before it: exact, since a term has the half's exponents
+//     and takes four bits of its eleven, the sign's among them. Side by side on the narrow operand, whose terms' sums are added at the end. The weight that sets the
+//     reference is 2^7: weights down to 2^-21 of it are good to 2^-11 of themselves, smaller ones to 2^-32 of it, which 2^24 tokens add up to 2^-8. (E4M3 terms with the
+//     reference at 1 end at 2^-17 and lose every weight below 2^-18 from the numerator alone: one key and 131071 of 2^-18.5 of its weight, all values 1, gave 0.74.)
 // A scale is a power of two, so that a value's is part of the weight's exponent: the reference m follows the largest s_j + f_j, and the weights that enter the
 // product lie below 2^8 whatever the scales are. The denominator sums w 2^-f_j in F32, a part of it in each softmax thread.
 //
@@ -27,9 +29,10 @@ namespace {
 
 static_assert(sizeof(augur_cuda_nvfp4_sm100_paged_attention_e4m3_args_v1) == 176, "attention ABI");
 
-// Weights are formed 2^kLift times too large and brought down where they become half precision: the denominator divides by the value's scale again, and wants those of
+// Weights are formed 2^kLift times too large and brought down to 2^kTop times where they become half precision: the denominator divides by the value's scale again, and wants those of
 // small scales down to 2^-30 of the largest. 2^(8 + kLift) * 2^60 and 2^-126 are 2^(30 + 60 + 60 + 8) apart at least, and as much lies between.
 constexpr float kLift = 48.0f;
+constexpr int kTop = 7;                        // the product's weights reach 2^(kTop + kRoom) = 2^15: a half, and what a term leaves of it, times 16, an E5M2 number
 constexpr float kNoReference = 1e30f;         // where a query has seen no key yet: whatever is added, but -infinity, passes
 constexpr float kRoom = 8.0f;                  // how far, in powers of two, a weight may pass 1, which was the largest when the reference moved
 constexpr uint32_t kTileInfos = 16;            // tiles that the loader is ahead of the softmax at most (a ring of keys and three more), rounded up
@@ -112,9 +115,15 @@ __device__ __forceinline__ uint32_t half2_of(float low, float high) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(high), "f"(low));
     return x;
 }
-__device__ __forceinline__ uint16_t codes_of(uint32_t halves) {
+// A weight's term and what it stands for (E5M2).
+__device__ __forceinline__ uint16_t term_of(uint32_t halves) {
     uint16_t x;
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(x) : "r"(halves));
+    asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(x) : "r"(halves));
+    return x;
+}
+__device__ __forceinline__ uint32_t halves_of_term(uint16_t codes) {
+    uint32_t x;
+    asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(x) : "h"(codes));
     return x;
 }
 __device__ __forceinline__ uint32_t halves_of(uint16_t codes) {
@@ -122,7 +131,7 @@ __device__ __forceinline__ uint32_t halves_of(uint16_t codes) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(x) : "h"(codes));
     return x;
 }
-// (x - y) * 16 of both halves, exact where y is x to the nearest E4M3 number.
+// (x - y) * 16 of both halves, exact where y is x to the nearest E5M2 number and x at most 2^15.
 __device__ __forceinline__ uint32_t rest16(uint32_t x, uint32_t y) {
     const __half2 r = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y)), __float2half2_rn(16.0f));
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -318,8 +327,8 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer: S of a tile, then O of the tile before it ----------------
-        constexpr uint32_t idesc_any = (1u << 4) | ((kTile >> 4) << 24);   // F32 += E4M3 x E4M3
-        constexpr uint32_t idesc = idesc_any | ((S::kScores >> 3) << 17), idesc_values = idesc_any | ((S::kTerms >> 3) << 17) | (1u << 15) | (1u << 16);   // V and W MN-major
+        constexpr uint32_t idesc_any = (1u << 4) | ((kTile >> 4) << 24);   // F32 += E4M3 x E4M3, or (1 << 10) x E5M2
+        constexpr uint32_t idesc = idesc_any | ((S::kScores >> 3) << 17), idesc_values = idesc_any | (1u << 10) | ((S::kTerms >> 3) << 17) | (1u << 15) | (1u << 16);   // V and W MN-major
         const uint32_t slots = low_word(smem_u32(smem), 16);
         const uint32_t queries = low_word(smem_u32(query_smem), 16), weights = low_word(smem_u32(weight_smem), kWeightAtom);
         Tiles ahead, now;
@@ -622,7 +631,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                         }
 #pragma unroll
                         for (uint32_t i = 0; i < kBlock; ++i) w[i] = exp2_fast(w[i]);
-                        constexpr float kDown = 1.0f / (1ull << static_cast<int>(kLift));
+                        constexpr float kDown = 1.0f / (1ull << (static_cast<int>(kLift) - kTop));
                         uint32_t term[3][kBlock / 4];   // four codes each
 #pragma unroll
                         for (uint32_t i = 0; i < kBlock; i += 4) {
@@ -630,10 +639,10 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
 #pragma unroll
                             for (uint32_t j = 0; j < 2; ++j) {
                                 uint32_t x = half2_of(w[i + 2 * j] * kDown, w[i + 2 * j + 1] * kDown);
-                                code[0][j] = codes_of(x);
-                                x = rest16(x, halves_of(code[0][j]));
-                                code[1][j] = codes_of(x);
-                                code[2][j] = codes_of(rest16(x, halves_of(code[1][j])));
+                                code[0][j] = term_of(x);
+                                x = rest16(x, halves_of_term(code[0][j]));
+                                code[1][j] = term_of(x);
+                                code[2][j] = term_of(rest16(x, halves_of_term(code[1][j])));
                             }
 #pragma unroll
                             for (uint32_t t = 0; t < 3; ++t) term[t][i / 4] = code[t][0] | static_cast<uint32_t>(code[t][1]) << 16;
@@ -734,7 +743,7 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                     if (lane % (32 / kBlock) == 0) reinterpret_cast<float*>(&st->wide[c + query])[quadrant] = sum[0];
                 }
                 if (!meet()) break;
-                if (thread < S::kMine) st->total[mine] = ((st->wide[mine].x + st->wide[mine].y) + (st->wide[mine].z + st->wide[mine].w)) * static_cast<float>(1ull << (60 - static_cast<int>(kLift)));
+                if (thread < S::kMine) st->total[mine] = ((st->wide[mine].x + st->wide[mine].y) + (st->wide[mine].z + st->wide[mine].w)) * static_cast<float>(1ull << (60 + kTop - static_cast<int>(kLift)));
                 if (!meet()) break;
                 if (!warp_look_suspended(weights_empty + 8 * ((tile - 1) & 1), (tile - 1) >> 1 & 1, abort_flag, status, kStatusProduct)) break;
                 tc_fence_after();

@@ -856,8 +856,8 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_append_e4m3_preva
 
 /* paged_attention over such a cache: the same formula on the values that codes and scales stand for, the same limits, scratch
  * (paged_attention_scratch_extent_host_v1) and status words. A query enters as two E4M3 terms: an element above 2^-9 of its head's largest exactly, a smaller
- * one to 2^-17 of the largest; an infinite element gives NaN as a NaN does, in all outputs of that query head's row. A weight enters the product with the values
- * good to 2^-11, and to 2^-18 of the row's largest product of weight and value scale; the denominator is F32. */
+ * one to 2^-17 of the largest; an infinite element gives NaN as a NaN does, in all outputs of that query head's row. A weight times its value's scale enters the
+ * product with the values good to 2^-11 of itself, or, below 2^-21 of the row's largest, to 2^-32 of that; the denominator is F32. */
 typedef struct augur_cuda_nvfp4_sm100_paged_attention_e4m3_args_v1 {
     uint32_t abi_version;
     uint32_t struct_size;
