@@ -236,6 +236,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// y 2^x for x <= 0 down to 2^-226, where 2^x alone is zero below 2^-126. With values whose scales are part of the reference (an E4M3 cache's), a
+// denominator under a lower one may be 2^(2 * 60 + 8) times its number of keys, and that much more counts than its factor says.
+__device__ __forceinline__ float scaled_down(float y, float x) { return x < -100.0f ? y * exp2_fast(x + 100.0f) * 0x1p-100f : y * exp2_fast(x); }
 __device__ __forceinline__ float warp_max(float x) {
     float y;
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
@@ -287,7 +290,7 @@ __global__ void __launch_bounds__(kJoinThreads, kMany ? 6 : 1) attention_join_ke
         const bool sees = mine.x != -INFINITY;
         const float w = sees ? exp2_fast(mine.x - most) : 0.0f;
         weight[threadIdx.x] = sees ? w : -1.0f;
-        float all = sees ? w * mine.y : 0.0f;
+        float all = sees ? scaled_down(mine.y, mine.x - most) : 0.0f;
 #pragma unroll
         for (uint32_t step = 16; step; step /= 2) all += __shfl_xor_sync(0xffffffffu, all, step);
         if (threadIdx.x % 32 == 0) wide[1][warp] = all;

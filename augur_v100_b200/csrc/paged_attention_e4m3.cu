@@ -34,6 +34,7 @@ static_assert(sizeof(augur_cuda_nvfp4_sm100_paged_attention_e4m3_args_v1) == 176
 constexpr float kLift = 48.0f;
 constexpr int kTop = 7;                        // the product's weights reach 2^(kTop + kRoom) = 2^15: a half, and what a term leaves of it, times 16, an E5M2 number
 constexpr float kNoReference = 1e30f;         // where a query has seen no key yet: whatever is added, but -infinity, passes
+constexpr float kFar = -100.0f, kFarFactor = 0x1p-100f;   // the least first factor, where a reference moves further
 constexpr float kRoom = 8.0f;                  // how far, in powers of two, a weight may pass 1, which was the largest when the reference moved
 constexpr uint32_t kTileInfos = 16;            // tiles that the loader is ahead of the softmax at most (a ring of keys and three more), rounded up
 constexpr uint32_t kWeightAtom = kTile * 32;   // 32 columns of a tile's weights
@@ -45,7 +46,7 @@ struct StateE4m3 : BatchState {
     uint32_t tmem, abort[1 + kMaxWarps];
     uint32_t needs[2][2];              // by group, a byte per softmax warp: a reference has to move
     uint32_t info[kTileInfos];         // of a tile: pages that are there, a bit per box
-    float reference[kMaxQueries], factor[kMaxQueries], total[kMaxQueries];
+    float reference[kMaxQueries], factor[2][kMaxQueries], total[kMaxQueries];
     alignas(16) float minus[kMaxQueries];            // the references with the sign changed, kNoReference for -infinity
     alignas(16) float query_scale[2][kMaxQueries];   // (read four at a time)
     float4 wide[kMaxQueries];          // by softmax warp: the largest score, or the sum of the weights
@@ -560,7 +561,9 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                             const float old = st->reference[mine];
                             const float4 w = st->wide[mine];
                             const float now = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), old);
-                            st->factor[mine] = now == old ? 1.0f : exp2_fast(old - now);
+                            // What the sums shrink by, in two factors: denominators of values of small scales still count where 2^(old - now) is zero.
+                            st->factor[0][mine] = now == old ? 1.0f : exp2_fast(fmaxf(old - now, kFar));
+                            st->factor[1][mine] = now == old ? 1.0f : exp2_fast(fminf(old - now - kFar, 0.0f));
                             st->reference[mine] = now;
                             st->minus[mine] = now == -INFINITY ? kNoReference : kLift - now;
                         }
@@ -575,33 +578,36 @@ paged_attention_e4m3_kernel(const __grid_constant__ CUtensorMap map_keys, const 
                             }
                             tc_fence_after();
 #pragma unroll 1
-                            for (uint32_t c = first; c < behind; c += kBlock) {   // 16 queries' columns (or eight), if one of them has moved
-                                float factor[kBlock];
-                                bool moved = false;
-#pragma unroll
-                                for (uint32_t i = 0; i < kBlock; ++i) factor[i] = st->factor[c + i], moved |= factor[i] != 1.0f;
-                                if (!moved) continue;
+                            for (uint32_t part = 0, far = 0; part <= far; ++part) {   // by the second factor where the first is its least
 #pragma unroll 1
-                                for (uint32_t column = c; column < S::kChunks * S::kTerms; column = column % S::kTerms + kN < 3 * kN ? column + kN : column / S::kTerms * S::kTerms + S::kTerms + c) {
-                                    uint32_t v[kBlock];
-                                    load_columns<kBlock>(tmem_out + lanes + column, v);
-                                    tc_wait_ld();
+                                for (uint32_t c = first; c < behind; c += kBlock) {   // 16 queries' columns (or eight), if one of them has moved
+                                    float factor[kBlock];
+                                    bool moved = false;
 #pragma unroll
-                                    for (uint32_t i = 0; i < kBlock; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * factor[i]);
-                                    store_columns<kBlock>(tmem_out + lanes + column, v);
-                                }
-                                if constexpr (kOneBlock) {
+                                    for (uint32_t i = 0; i < kBlock; ++i) factor[i] = st->factor[part][c + i], moved |= factor[i] != 1.0f, far |= factor[i] <= kFarFactor;
+                                    if (!moved) continue;
+#pragma unroll 1
+                                    for (uint32_t column = c; column < S::kChunks * S::kTerms; column = column % S::kTerms + kN < 3 * kN ? column + kN : column / S::kTerms * S::kTerms + S::kTerms + c) {
+                                        uint32_t v[kBlock];
+                                        load_columns<kBlock>(tmem_out + lanes + column, v);
+                                        tc_wait_ld();
 #pragma unroll
-                                    for (uint32_t i = 0; i < kBlock; ++i) sum[i] *= factor[i];
-                                } else {
+                                        for (uint32_t i = 0; i < kBlock; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * factor[i]);
+                                        store_columns<kBlock>(tmem_out + lanes + column, v);
+                                    }
+                                    if constexpr (kOneBlock) {
 #pragma unroll
-                                    for (uint32_t i = 0; i < kBlock; i += 4) {
-                                        float4& x = sum_smem[(c + i) / 4 * kTile + thread];
-                                        x = make_float4(x.x * factor[i], x.y * factor[i + 1], x.z * factor[i + 2], x.w * factor[i + 3]);
+                                        for (uint32_t i = 0; i < kBlock; ++i) sum[i] *= factor[i];
+                                    } else {
+#pragma unroll
+                                        for (uint32_t i = 0; i < kBlock; i += 4) {
+                                            float4& x = sum_smem[(c + i) / 4 * kTile + thread];
+                                            x = make_float4(x.x * factor[i], x.y * factor[i + 1], x.z * factor[i + 2], x.w * factor[i + 3]);
+                                        }
                                     }
                                 }
+                                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                             }
-                            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                             tc_fence_before();
                         }
                     }

@@ -85,3 +85,23 @@ def test_a_key_that_outweighs_a_long_tail(length, where, group, head_dim):
     q[..., 0] = torch.tensor([20.0, 17.0, 12.0], device=DEVICE)[torch.arange(group, device=DEVICE) % 3] * math.log(2) / (448 * unit * scale)
     batch.q = q.to(torch.bfloat16)
     _check(batch, scale)
+
+
+@pytest.mark.parametrize("where", [0.0, 0.5, 1.0])
+@pytest.mark.parametrize("parts", [True, False])
+@pytest.mark.parametrize("group,head_dim", [(8, 128), (16, 256), (40, 128), (64, 256)])
+def test_value_scales_at_either_end(parts, where, group, head_dim):
+    """Values of the least scale under one of the largest, in other parts of the sequence than that one's or in other tiles of the one part: the key with
+    the largest has 2^7 times their weight, or 2^3, and 16384 others nearly all of the denominator; their references lie 2^127 apart, or 2^123."""
+    length, scale, unit = 16385, head_dim ** -0.5, 2.0 ** -7
+    batch = _batch(length, 1 if parts else host.sm_count(0), group, head_dim, seed=7)
+    batch.k.view(torch.uint8).zero_()
+    batch.scales.view(torch.uint8)[..., 0] = 120
+    batch.scales.view(torch.uint8)[..., 1] = 67
+    slot = _slot(batch, min(int(where * length), length - 1))
+    batch.k.view(torch.uint8)[slot][0] = 0x7e                           # 448
+    batch.scales.view(torch.uint8)[slot][1] = 187
+    q = batch.q.float()
+    q[..., 0] = torch.tensor([7.0, 3.0], device=DEVICE)[torch.arange(group, device=DEVICE) % 2] * math.log(2) / (448 * unit * scale)
+    batch.q = q.to(torch.bfloat16)
+    _check(batch, scale)
