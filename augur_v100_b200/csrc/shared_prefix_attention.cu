@@ -19,7 +19,8 @@
 // product of two tiles before, whose P lies in their place, and that for 2050 cycles of softmax, 1024 of them exponentials; and Q and K of the first product are both read from
 // shared memory, 128 bytes a cycle with the copies coming in.
 // Head size 128: two groups that take tiles of 64 keys in turn, each with an O and two S of its own: one group's exponentials take as long as a tile's products.
-// Twelve sequences of eight tokens on 65536 tokens (24 / 4 heads of 256): 160 us, 0.97 PFLOP/s.
+// Twelve sequences of eight tokens on 65536 tokens (24 / 4 heads of 256): 160 to 165 us in bursts of some ms (0.94 to 0.97 PFLOP/s), 188 to 194 without a pause, where the power cap leaves
+// 1537 MHz (0.81).
 #include "paged_attention.cuh"
 
 namespace augur_sm100 {
@@ -85,7 +86,7 @@ struct Items {
         *tile = item - rest * p.tiles;
         *head = rest / split;
         const uint32_t part = rest - *head * split;
-        *first = part * key_tiles / split, *last = (part + 1) * key_tiles / split;   // (below 2^9 * 2^17)
+        *first = part * key_tiles / split, *last = (part + 1) * key_tiles / split;   // (at most 2^8 * 2^18)
     }
 };
 // The split that a simple model takes for quickest: rounds of items, each its keys and 512 for beginning and end, and four keys for every part to be joined. A warp together.

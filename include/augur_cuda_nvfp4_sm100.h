@@ -799,7 +799,7 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_copy_prevali
 /* ---- the cache in 8 bits ------------------------------------------------------------------------- */
 /* One layer of it is two tensors of E4M3 codes [pages][kv_heads][page_tokens][head_dim] and one of scale bytes
  * [pages][kv_heads][page_tokens][2] (keys, values): an element is code * 2^(byte - 127), one scale for a token's head. Half of what the BF16
- * cache takes, and half of what a decoding step reads. Limits as for the BF16 cache. Scale bytes are 67..187 (2^-60..2^60); smaller ones
+ * cache takes, and half of what a decoding step reads; attention over it is the quicker one from some 300 to 1000 tokens a sequence on (one sequence alone: 4000). Limits as for the BF16 cache. Scale bytes are 67..187 (2^-60..2^60); smaller ones
  * count as 67, larger ones as 187, and 255 as NaN. The reference's 8-bit cache holds whole numbers with a scale for 32 of them; here the matrix
  * units multiply the codes as they lie in the pages, which a scale within a token's head would not allow. */
 typedef struct augur_cuda_nvfp4_sm100_kv_e4m3_layer_v1 {
@@ -910,7 +910,8 @@ augur_cuda_result_v1 AUGUR_CUDA_CALL augur_cuda_nvfp4_sm100_kv_page_copy_e4m3_pr
  * paged_attention: limits on heads, tokens and table, rows that are not written, rows that see nothing, status words (the waits
  * of the prefix set 0x421..0x426). A value that is not finite may reach rows that do not see it: one of the prefix every row, one of a sequence's own tokens that
  * sequence's rows. The weights enter their product with the values as one BF16 term (good to 2^-8 of each, and the denominator sums
- * the same terms): for a batch, these products are the bound. The results depend on the inputs and the device's SM count alone. */
+ * the same terms; paged_attention has two): for a batch, these products are the bound. The time goes with batch.rows, whether a sequence has them or not. Against paged_attention it
+ * pays where it saves some 150 MB of keys and values: (sequences - 1) * P * kv_heads * head_dim * 4 bytes. The results depend on the inputs and the device's SM count alone. */
 typedef struct augur_cuda_nvfp4_sm100_shared_prefix_attention_args_v1 {
     uint32_t abi_version;
     uint32_t struct_size;
